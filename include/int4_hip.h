@@ -301,6 +301,99 @@ int w4_silu_mul(const void* gate, const void* up, int dtype, int64_t count, void
 int w4_norm_head(const void* x, const void* delta, const void* norm_weight, float eps, const void* weight,
                  int dtype, int64_t N, int64_t K, void* y, void* stream);
 
+/*
+ * Key-value cache in pages, of one layer, for a batch of sequences (rows).
+ *   k, v    [pages, kv_heads, page_size, head_dim] bf16 / fp16, dense, 16-byte aligned;
+ *           keys are held rotated
+ *   weight  fp32 [pages, kv_heads, page_size], dense: the attention weight each token
+ *           has received from every later query of its head's group; NULL where the
+ *           caller does not keep it
+ *   table   int32 [rows, width], dense: page of slots i * page_size.. of a row; entries
+ *           past a row's tokens are not read.  A page may stand in several rows (a
+ *           shared prefix) where weight is NULL and neither row writes to it.
+ * head_dim 64 or 128; page_size a power of two from 8 to 1024; width * page_size below
+ * 2^30.  Page ids, slots, positions and lengths are device memory: what is out of range
+ * is found by the kernels, which read and write nothing through it.
+ * No counterpart in the reference, whose model is Hugging Face's with a contiguous
+ * static cache (benchmarks/eval_llama.py:112-183).
+ */
+typedef struct w4_paged_cache {
+  void* k;
+  void* v;
+  float* weight;
+  const int32_t* table;
+  int64_t pages;
+  int64_t kv_heads;
+  int64_t page_size;
+  int64_t head_dim;
+  int64_t rows;
+  int64_t width;
+} w4_paged_cache;
+
+/*
+ * Tokens written into the pages: key t (rotary embedding at positions[t]; fp32
+ * products rounded separately, one rounding to the dtype) and value t of
+ * k, v [tokens, kv_heads * head_dim] (row strides stride_k, stride_v, multiples of 8)
+ * at slot slots[t] of table row rows[t]; weight there becomes 0.  cos, sin: fp32
+ * [angles, head_dim / 2].  A token whose row, slot, page or position is out of range
+ * (any negative number) is left out.  Two tokens for one slot: one of them, not
+ * defined which.
+ */
+int w4_paged_append(const w4_paged_cache* cache, int dtype, const void* k, const void* v, int64_t stride_k,
+                    int64_t stride_v, int64_t tokens, const int32_t* rows, const int32_t* slots,
+                    const int32_t* positions, const float* cos, const float* sin, int64_t angles, void* stream);
+
+/*
+ * Attention of one new token of every row: its key and value are written to slot
+ * lengths[b] as by w4_paged_append, then out [rows, num_heads * head_dim] (dense) =
+ * softmax(rope(q) K / sqrt(head_dim)) V over slots 0..lengths[b], in fp32 from the
+ * cached 16-bit keys and values, rounded once.  With cache->weight every slot's
+ * weight grows by the probabilities that the heads of its group gave it (the new
+ * slot's is set to them); `scores` is then scratch of rows * num_heads * width *
+ * page_size floats, else NULL.  lengths[b] < 0: the row is idle, its out zero and
+ * nothing written.  A new slot past the table or a position outside the angles: out
+ * NaN and nothing written; a page of the row outside the pool: out NaN.  In both the
+ * row's weights stay as they were.  lengths is not changed.
+ * workspace: as for w4a16_gemm, w4_paged_attention_workspace_bytes long.  Results are
+ * bit-identical run to run.
+ */
+size_t w4_paged_attention_workspace_bytes(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim);
+int w4_paged_attention(const w4_paged_cache* cache, int dtype, const void* q, const void* k, const void* v,
+                       int64_t stride_q, int64_t stride_k, int64_t stride_v, int64_t num_heads,
+                       const int32_t* lengths, const int32_t* positions, const float* cos, const float* sin,
+                       int64_t angles, void* out, float* scores, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
+ * The tokens worth keeping, copied to new pages: of row b's n = lengths[b] tokens and
+ * for every key-value head apart, all where n <= keep, else the last `recent` (at most
+ * keep) and, of the others, the keep - recent of largest weight (the lower slot first
+ * among equals, NaN above every number).  They go to slots 0.. of row b of new_table
+ * [rows, new_width] in the order of their slots, with their weights; new_lengths[b] =
+ * min(n, keep) (-1 for an idle row, lengths[b] < 0).  `kept` [rows, kv_heads, keep]
+ * receives their old slots.  The pages of new_table must not be among those read, nor
+ * stand in it twice.  A row with n beyond the table is idle for this call, its new
+ * length -1; tokens on a page outside the pool are not copied.
+ */
+int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int32_t* lengths, const int32_t* new_table,
+                   int64_t new_width, int64_t keep, int64_t recent, int32_t* kept, int32_t* new_lengths,
+                   void* stream);
+
+/*
+ * Of every row of logits [rows, vocab] (bf16 / fp16 / fp32, row stride `stride`):
+ * logprob [rows] = log softmax at tokens[row] (NaN for a token outside the
+ * vocabulary; tokens and logprob may both be NULL), entropy [rows] of the
+ * distribution in nats, and the `top` (0..64, at most vocab) most likely tokens with
+ * their log probabilities, [rows, top] each, the lower index first among equal logits
+ * and a NaN above every number.  fp32 inside.  A row without a finite maximum (all
+ * -inf, a +inf or a NaN) has NaN log probabilities and entropy.
+ * workspace: as for w4a16_gemm, w4_token_logprobs_workspace_bytes long.
+ */
+size_t w4_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top);
+int w4_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
+                      const int64_t* tokens, int64_t top, float* logprob, float* entropy, float* top_logprob,
+                      int64_t* top_token, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

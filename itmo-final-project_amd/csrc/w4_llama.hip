@@ -15,7 +15,6 @@ constexpr int kAttnThreads = 256;
 constexpr int kAttnWaves = kAttnThreads / 64;
 constexpr int kAttnMaxChunks = 64;  // position chunks per key-value head
 constexpr int kAttnHeads = 4;       // query heads per workgroup
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnDecodeArgs {
   const uint16_t* q;  // [nh * D]
@@ -32,39 +31,6 @@ struct AttnDecodeArgs {
   float qscale;       // softmax scale * log2(e)
   int g, max_len, chunk, chunks;
 };
-
-// Rotates the pair (x1, x2) = (x[d], x[d + D/2]); products and sums rounded
-// separately, as the torch-op version does.
-__device__ __forceinline__ void rope_pair(float x1, float x2, float c, float s, float* r1, float* r2) {
-#pragma clang fp contract(off)
-  *r1 = x1 * c - x2 * s;
-  *r2 = x2 * c + x1 * s;
-}
-
-// Reductions over the 64 lanes (all active), the result in every lane: four DPP
-// steps within the rows of 16, then the four rows through scalar registers (a
-// shuffle through LDS per step is ten times the latency).
-template <int CTRL>
-__device__ __forceinline__ float lane_perm(float v) {
-  return __builtin_bit_cast(float, dpp_mov<CTRL>(__builtin_bit_cast(uint32_t, v)));
-}
-__device__ __forceinline__ float lane_read(float v, int lane) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
-}
-__device__ __forceinline__ float wave_max(float v) {
-  v = fmaxf(v, lane_perm<0xB1>(v));   // lane ^ 1
-  v = fmaxf(v, lane_perm<0x4E>(v));   // lane ^ 2
-  v = fmaxf(v, lane_perm<0x141>(v));  // half rows mirrored
-  v = fmaxf(v, lane_perm<0x140>(v));  // rows mirrored
-  return fmaxf(fmaxf(lane_read(v, 0), lane_read(v, 16)), fmaxf(lane_read(v, 32), lane_read(v, 48)));
-}
-__device__ __forceinline__ float wave_sum(float v) {
-  v += lane_perm<0xB1>(v);
-  v += lane_perm<0x4E>(v);
-  v += lane_perm<0x141>(v);
-  v += lane_perm<0x140>(v);
-  return (lane_read(v, 0) + lane_read(v, 16)) + (lane_read(v, 32) + lane_read(v, 48));
-}
 
 // One workgroup = one key-value head x one chunk of cache positions (a
 // multiple of 64) x up to four of its query heads (eight would need 256

@@ -10,7 +10,9 @@ from . import quantize  # callable: quantize(w, group_size) == quantize_int4(w, 
 from .quantize import (dequantize_int4, dequantize_int4_ref, quantize_int4, quantize_int4_grouped,
                        quantize_int4_ref, unpack_int4_ref)
 from .gemm import w4a16_matmul, w4a16_matmul_grouped, w16a16_matmul
+from .paged import paged_append, paged_attention, paged_evict
 from .qlinear import Int4Linear, quantize_model_linears
+from .scoring import TokenLogprobs, token_logprobs
 
 __all__ = [
     "quantize_int4",
@@ -26,4 +28,9 @@ __all__ = [
     "unpack_int4_ref",
     "w4a16_matmul_grouped",
     "quantize_int4_grouped",
+    "paged_append",
+    "paged_attention",
+    "paged_evict",
+    "token_logprobs",
+    "TokenLogprobs",
 ]

@@ -66,6 +66,23 @@ class QuantProblem(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of ``w4_paged_cache`` (include/int4_hip.h)."""
+
+    _fields_ = [
+        ("k", _c_vp),
+        ("v", _c_vp),
+        ("weight", _c_vp),
+        ("table", _c_vp),
+        ("pages", _c_i64),
+        ("kv_heads", _c_i64),
+        ("page_size", _c_i64),
+        ("head_dim", _c_i64),
+        ("rows", _c_i64),
+        ("width", _c_i64),
+    ]
+
+
 # symbol -> (restype, argtypes); exactly the functions include/int4_hip.h declares
 SIGNATURES = {
     "w4_abi_version": (_c_int, []),
@@ -91,6 +108,16 @@ SIGNATURES = {
     "w4_rmsnorm": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_i64, ctypes.c_float, _c_vp, _c_vp, _c_vp]),
     "w4_silu_mul": (_c_int, [_c_vp, _c_vp, _c_int, _c_i64, _c_vp, _c_vp]),
     "w4_norm_head": (_c_int, [_c_vp, _c_vp, _c_vp, ctypes.c_float, _c_vp, _c_int, _c_i64, _c_i64, _c_vp, _c_vp]),
+    "w4_paged_append": (_c_int, [ctypes.POINTER(PagedCache), _c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp,
+                                 _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
+    "w4_paged_attention_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64]),
+    "w4_paged_attention": (_c_int, [ctypes.POINTER(PagedCache), _c_int, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,
+                                    _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_sz, _c_vp]),
+    "w4_paged_evict": (_c_int, [ctypes.POINTER(PagedCache), _c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp,
+                                _c_vp]),
+    "w4_token_logprobs_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64]),
+    "w4_token_logprobs": (_c_int, [_c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp,
+                                   _c_vp, _c_sz, _c_vp]),
 }
 
 _lock = threading.Lock()
