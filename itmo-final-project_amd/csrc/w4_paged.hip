@@ -8,6 +8,8 @@
 namespace w4 {
 
 constexpr int kPagedThreads = 256;
+constexpr int kPagedBufFlags = 0x00020000;  // raw buffer: the range is checked in bytes
+constexpr int kPagedCoherentAux = 16;       // sc1: the cache policy of agent-scope atomic loads and stores
 
 struct PagedView {
   uint16_t* k;     // [pages, nkv, S, D]
@@ -76,114 +78,521 @@ struct PagedAttnArgs {
   const int32_t *lengths, *positions;
   const float *cos, *sin;
   uint16_t* out;  // [rows, nkv * g * D]
+  float* scores;  // [rows, nkv * g, width * page_size], of q K / sqrt(D); null without weights
+  float* stats;   // [rows, nkv * g, 2]: the scores' maximum in powers of two, and their sum relative to it
+  float* part;    // [items, part_stride]: outputs of a part, then (maximum, sum) of its heads
+  unsigned* cnt;  // one arrival counter per row and tile of heads
   float scale;    // 1 / sqrt(D)
-  int g;
+  int g, htiles, part_stride;
 };
 
-// One workgroup per row and key-value head, its query heads one after the other;
-// a thread holds the running maximum, sum and output of every 256th slot, joined at
-// the end of a head.  The weights' pass computes the scores again.
+// The work of one workgroup: a part of the slots of one row and one tile of its heads.
+struct AttnItem {
+  int b, tile, part, parts, first;  // first: the index of part 0
+};
+
+constexpr int kAttnItems = 1024;    // parts the tokens of a batch are cut into, about
+constexpr int kAttnMinUnits = 4;    // units of a part at least: one a wave
+constexpr int kPagedCounters = W4_WORKSPACE_COUNTER_BYTES / 4;
+
+// Inclusive sum over the lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // shifted right by 1, 2, 4, 8 in rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // rows 1, 3 take the last lane before them
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // rows 2, 3 take lane 31
+  return v;
+}
+
+// Which item this is, the same in every wave and launch.  The lengths lie on the GPU, so the split is made here:
+// every row is cut into equal parts of at most `per` units of UP slots, per = all units / kAttnItems, so that short
+// rows stay whole and long ones spread over the chip, whatever else is in the batch.  Rows that need no
+// attention (idle, refused) are one part.
+template <int UP>
+__device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __restrict__ lengths, int tiles, int item,
+                                          AttnItem* it) {
+  const int lane = threadIdx.x & 63;
+  auto units = [&](int row) {
+    const int len = row < c.rows ? lengths[row] : -1;
+    return len >= 0 && len < c.capacity() ? len / UP + 1 : 1;
+  };
+  float all = 0.f;
+  for (int r = 0; r < c.rows; r += 64) all += r + lane < c.rows ? (float)units(r + lane) : 0.f;
+  all = wave_sum(all);
+  int per = (int)fminf(ceilf(all * ((float)tiles / kAttnItems)), 1e9f);
+  per = max(per, kAttnMinUnits);
+  if ((int64_t)c.rows * tiles > kPagedCounters) per = 1 << 30;  // no counters for parts to meet at
+  int base = 0;
+  for (int r = 0; r < c.rows; r += 64) {
+    const int parts = r + lane < c.rows ? (units(r + lane) + per - 1) / per : 0;
+    const int upto = base + wave_scan(parts * tiles);
+    const int end = __builtin_amdgcn_readlane(upto, 63);
+    if (item < end) {
+      const int i = __popcll(__ballot(item >= upto));
+      it->parts = __builtin_amdgcn_readlane(parts, i);
+      const int rem = item - (__builtin_amdgcn_readlane(upto, i) - it->parts * tiles);
+      it->b = r + i;
+      it->tile = rem / it->parts;
+      it->part = rem - it->tile * it->parts;
+      it->first = item - it->part;
+      return true;
+    }
+    base = end;
+  }
+  return false;
+}
+
+// How an fp32 operand enters 16-bit matrix instructions: as the sum of its roundings.
+template <int DT> struct Split;
+template <> struct Split<W4_DTYPE_BF16> { static constexpr int N = 3; };  // 8 significant bits each: all 24
+template <> struct Split<W4_DTYPE_FP16> { static constexpr int N = 2; };  // 11 each: 22
+
+template <int DT>
+__device__ __forceinline__ void split8(const float v[8], int parts, u32x4* out) {
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = v[e];
+  for (int p = 0; p < parts; ++p) {
+    out[p] = pack8<DT>(r);
+    float t[8];
+    unpack8<DT>(out[p], t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] -= t[e];
+  }
+}
+
+// The D / 32 chunks of eight elements that lane group c holds of a head's D (chunk j: elements 32 j + 8 c..), rotated
+// and multiplied by `scale`.  A chunk's partner, D / 2 further on, is in the same lane.
 template <int DT, int D>
-__global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAttnArgs a) {
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int h = blockIdx.x, b = blockIdx.y;
-  __shared__ __attribute__((aligned(16))) float q_s[D];
-  __shared__ float red[4], o_s[4][D];
-  __shared__ int bad_s;
-  const int len = a.lengths[b], pos = a.positions[b];
-  uint16_t* const out = a.out + ((int64_t)b * a.c.nkv + h) * a.g * D;
-  const int n = len + 1;
-  if (tid == 0) bad_s = 0;
-  __syncthreads();
-  bool bad = len >= a.c.capacity() || (uint64_t)(int64_t)pos >= (uint64_t)a.angles;
-  if (len >= 0 && !bad) {
-    for (int p = tid; p <= (len >> a.c.log2s); p += kPagedThreads)
-      if (a.c.token(b, p << a.c.log2s, h) < 0) bad_s = 1;
-    const int64_t at = a.c.token(b, len, h);
-    if (at >= 0) {
-      if (tid < D / 2) {
-        const uint16_t* kp = a.k + b * a.stride_k + h * D + tid;
-        float r1, r2;
-        rope_pair(act_bits_to_float(kp[0], DT), act_bits_to_float(kp[D / 2], DT), a.cos[(int64_t)pos * (D / 2) + tid],
-                  a.sin[(int64_t)pos * (D / 2) + tid], &r1, &r2);
-        a.c.k[at * D + tid] = float_to_act_bits<DT>(r1);
-        a.c.k[at * D + tid + D / 2] = float_to_act_bits<DT>(r2);
-      } else if (tid >= 128 && tid < 128 + D) {
-        a.c.v[at * D + tid - 128] = a.v[b * a.stride_v + h * D + tid - 128];
-      }
+__device__ __forceinline__ void rope_chunks(const uint16_t* __restrict__ x, const float* __restrict__ cos,
+                                            const float* __restrict__ sin, int c, float scale, float (*out)[8]) {
+  constexpr int NJ = D / 32;
+  u32x4 raw[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) raw[j] = *reinterpret_cast<const u32x4*>(x + 32 * j + 8 * c);
+#pragma unroll
+  for (int j = 0; j < NJ / 2; ++j) {
+    float a[8], b[8];
+    unpack8<DT>(raw[j], a);
+    unpack8<DT>(raw[j + NJ / 2], b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float r1, r2;
+      rope_pair(a[e], b[e], cos[32 * j + 8 * c + e], sin[32 * j + 8 * c + e], &r1, &r2);
+      out[j][e] = r1 * scale;
+      out[j + NJ / 2][e] = r2 * scale;
     }
   }
-  __threadfence_block();
-  __syncthreads();
-  bad = bad || bad_s;
-  if (len < 0 || bad) {
+}
+
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.f : m; }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+// One workgroup = one part of one row's slots for up to 16 query heads of one key-value head; its four waves take
+// units of UP = 4096 / D slots in turn (16 KB of keys and values).
+//
+// Both products are 16x16x32 matrix instructions, transposed: scores S^T = K Q^T, slots by heads, then O^T = V^T P^T.
+// A tile's row r of keys is slot 8 (r / 4) + 4 t + r % 4 of its block of 32 (t: the first or second tile), so the
+// scores that a lane holds of one head are those of eight slots in a row: exactly its part of the second product's
+// operand, which never leaves its registers.  Keys go from memory to the operands; values go through LDS, which
+// transposes them on reading.  The running maximum of a head is only raised when a score passes it by 2^8 (its value
+// cancels in the end), so that most units need no exchange between lanes.
+template <int DT, int D>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(PagedAttnArgs a) {
+  constexpr int KB = 128 / D, UP = 32 * KB, NJ = D / 32, ND = D / 16, VR = 512 / D, NP = Split<DT>::N;
+  constexpr int ROW = D == 64 ? 72 : 144;  // halfwords of a value row in LDS: four rows on different banks
+  constexpr int OROW = D + 4;              // floats of an output row in LDS
+  constexpr int WAVE_H = UP * ROW;
+  static_assert(16 * OROW * 2 <= WAVE_H, "a wave's outputs take its values' place");
+  typedef typename Act<DT>::frag frag;
+  __shared__ __attribute__((aligned(16))) uint16_t v_s[4][WAVE_H];
+  __shared__ float m_s[4][16], l_s[4][16];
+  __shared__ int bad_s;
+  __shared__ unsigned arrived_s;
+
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, c = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  AttnItem it;
+  if (!find_item<UP>(a.c, a.lengths, a.c.nkv * a.htiles, blockIdx.x, &it)) return;
+  const int b = it.b, h = it.tile / a.htiles, ht = it.tile - h * a.htiles;
+  const int h0 = h * a.g + ht * 16, gh = min(a.g - ht * 16, 16);  // query heads of the row
+  const int nh = a.c.nkv * a.g;
+  const int len = a.lengths[b], pos = a.positions[b];
+  uint16_t* const out = a.out + ((int64_t)b * nh + h0) * D;
+  if (len < 0 || len >= a.c.capacity() || (uint64_t)(int64_t)pos >= (uint64_t)a.angles) {
     const uint16_t fill = len < 0 ? 0 : float_to_act_bits<DT>(__builtin_nanf(""));
-    for (int i = tid; i < a.g * D; i += kPagedThreads) out[i] = fill;
+    for (int i = tid; i < gh * D; i += kPagedThreads) out[i] = fill;
     return;
   }
-  auto score = [&](int j) {
-    const uint16_t* kp = a.c.k + a.c.token(b, j, h) * D;
-    float s = 0.f;
-    for (int d = 0; d < D; d += 8) {
-      float x[8];
-      unpack8<DT>(*reinterpret_cast<const u32x4*>(kp + d), x);
+  if (tid == 0) bad_s = 0;
+  const int nu = len / UP + 1;
+  const int u0 = (int)((int64_t)it.part * nu / it.parts), u1 = (int)((int64_t)(it.part + 1) * nu / it.parts);
+  const float* const cosr = a.cos + (int64_t)pos * (D / 2);
+  const float* const sinr = a.sin + (int64_t)pos * (D / 2);
+  const int32_t* const table = a.c.table + (int64_t)b * a.c.width;
+  const int smask = (1 << a.c.log2s) - 1;
+
+  // the query: heads past gh are zero
+  u32x4 qf[NJ][NP];
+  {
+    float x[NJ][8];
+    rope_chunks<DT, D>(a.q + b * a.stride_q + (int64_t)(h0 + min(l16, gh - 1)) * D, cosr, sinr, c, a.scale, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = __builtin_fmaf(q_s[d + e], x[e], s);
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[j][e] = l16 < gh ? x[j][e] : 0.f;
+      split8<DT>(x[j], NP, qf[j]);
     }
-    return s;
+  }
+
+  u32x4 kr[KB][2][NJ], vr[8];
+  bool bad = false;
+  // Lane i: the page of the unit's slots 8 i.. (past the row's end, its last page).
+  auto load_ids = [&](int u) {
+    const int slot = min(u * UP + 8 * min(lane, UP / 8 - 1), len);
+    return table[slot >> a.c.log2s];
   };
-  for (int hq = 0; hq < a.g; ++hq) {
-    __syncthreads();
-    if (tid < D / 2) {
-      const uint16_t* qp = a.q + b * a.stride_q + (int64_t)(h * a.g + hq) * D + tid;
-      float r1, r2;
-      rope_pair(act_bits_to_float(qp[0], DT), act_bits_to_float(qp[D / 2], DT), a.cos[(int64_t)pos * (D / 2) + tid],
-                a.sin[(int64_t)pos * (D / 2) + tid], &r1, &r2);
-      q_s[tid] = r1 * a.scale;
-      q_s[tid + D / 2] = r2 * a.scale;
+  auto load = [&](int u, int ids) {
+    const bool out_of_pool = (unsigned)ids >= (unsigned)a.c.pages;
+    bad = bad || __ballot(out_of_pool);
+    ids = out_of_pool ? 0 : ids;
+    const int base = u * UP;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int page = __shfl(ids, kb * 4 + (l16 >> 2));
+      const int slot = base + kb * 32 + 8 * (l16 >> 2) + (l16 & 3);
+      const uint16_t* kp =
+          a.c.k + (((((int64_t)page * a.c.nkv + h) << a.c.log2s) + (slot & smask)) * D + 8 * c);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) kr[kb][t][j] = *reinterpret_cast<const u32x4*>(kp + 4 * t * D + 32 * j);
     }
-    __syncthreads();
-    float m = -__builtin_inff(), l = 0.f, o[D];
 #pragma unroll
-    for (int d = 0; d < D; ++d) o[d] = 0.f;
-    for (int j = tid; j < n; j += kPagedThreads) {
-      const float s = score(j);
-      const float mn = fmaxf(m, s), base = mn == -__builtin_inff() ? 0.f : mn;
-      const float al = expf(m - base), p = expf(s - base);
-      const uint16_t* vp = a.c.v + a.c.token(b, j, h) * D;
-      l = l * al + p;
+    for (int i = 0; i < 8; ++i) {
+      const int page = __builtin_amdgcn_readlane(ids, i * VR / 8);
+      const int64_t at = (((int64_t)page * a.c.nkv + h) << a.c.log2s) + ((base + i * VR) & smask);
+      vr[i] = *reinterpret_cast<const u32x4*>(a.c.v + at * D + lane * 8);
+    }
+  };
+  uint16_t* const vw = v_s[wv];
+
+  float m, l;  // of head l16: the reference exponent and this lane's share of the sum
+  f32x4 o[ND];
+  bool precise = true;
+  for (;;) {
+    m = -__builtin_inff(), l = 0.f;
 #pragma unroll
-      for (int d = 0; d < D; d += 8) {
-        float x[8];
-        unpack8<DT>(*reinterpret_cast<const u32x4*>(vp + d), x);
+    for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int u = u0 + wv;
+    int ids = 0;
+    if (u < u1) {
+      load(u, load_ids(u));
+      ids = load_ids(min(u + 4, u1 - 1));
+    }
+    for (; u < u1; u += 4) {
+      const int base = u * UP;
+      const bool last = base + UP > len;  // the new token is in this unit, and what lies past it
+      if (last) {
+        const int at = len - base;
+        const uint16_t* kin = a.k + b * a.stride_k + h * D;
+        float x[NJ][8];
+        u32x4 kn[NJ];
+        rope_chunks<DT, D>(kin, cosr, sinr, c, 1.f, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[d + e] = __builtin_fmaf(p, x[e], o[d + e] * al);
+        for (int j = 0; j < NJ; ++j) kn[j] = pack8<DT>(x[j]);
+        const int page = table[len >> a.c.log2s];
+        const int64_t tok = (((int64_t)page * a.c.nkv + h) << a.c.log2s) + (len & smask);
+        const bool write = ht == 0 && precise && (unsigned)page < (unsigned)a.c.pages;
+        const bool mine = l16 == ((at & 31) >> 3) * 4 + (at & 3);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (at >> 5 == kb && ((at >> 2) & 1) == t)
+#pragma unroll
+              for (int j = 0; j < NJ; ++j) kr[kb][t][j] = mine ? kn[j] : kr[kb][t][j];
+        if (write && mine) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) *reinterpret_cast<u32x4*>(a.c.k + tok * D + 32 * j + 8 * c) = kn[j];
+        }
+        const int vrow = lane * 8 / D, vd = lane * 8 % D;
+        const u32x4 vn = *reinterpret_cast<const u32x4*>(a.v + b * a.stride_v + h * D + vd);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = i * VR + vrow;
+          vr[i] = row == at ? vn : row > at ? u32x4{0u, 0u, 0u, 0u} : vr[i];
+          if (write && row == at) *reinterpret_cast<u32x4*>(a.c.v + tok * D + vd) = vn;
+        }
       }
-      m = mn;
-    }
-    const float wm = wave_max(m);
-    if (lane == 0) red[wv] = wm;
-    __syncthreads();
-    const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), base = M == -__builtin_inff() ? 0.f : M;
-    const float al = expf(m - base);
-    __syncthreads();
-    const float wl = wave_sum(l * al);
-    if (lane == 0) red[wv] = wl;
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      const float t = wave_sum(l == 0.f ? 0.f : o[d] * al);
-      if (lane == 0) o_s[wv][d] = t;
-    }
-    __syncthreads();
-    const float L = (red[0] + red[1]) + (red[2] + red[3]);
-    if (tid < D)
-      out[hq * D + tid] = float_to_act_bits<DT>(((o_s[0][tid] + o_s[1][tid]) + (o_s[2][tid] + o_s[3][tid])) / L);
-    if (a.c.weight)
-      for (int j = tid; j < n; j += kPagedThreads) {
-        float* w = a.c.weight + a.c.token(b, j, h);
-        const float p = expf(score(j) - base) / L;
-        *w = j == len && hq == 0 ? p : *w + p;
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<u32x4*>(vw + (i * VR + lane * 8 / D) * ROW + lane * 8 % D) = vr[i];
+      f32x4 s[KB][2];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (precise) {  // the small parts first
+#pragma unroll
+            for (int p = NP - 1; p > 0; --p)
+#pragma unroll
+              for (int j = 0; j < NJ; ++j)
+                s[kb][t] = Mfma<DT>::m16(__builtin_bit_cast(frag, kr[kb][t][j]), __builtin_bit_cast(frag, qf[j][p]),
+                                         s[kb][t]);
+          }
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            s[kb][t] = Mfma<DT>::m16(__builtin_bit_cast(frag, kr[kb][t][j]), __builtin_bit_cast(frag, qf[j][0]),
+                                     s[kb][t]);
+        }
+      if (u + 4 < u1) {  // the next unit's loads travel under the rest
+        load(u + 4, ids);
+        ids = load_ids(min(u + 8, u1 - 1));
       }
+      if (last) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (base + kb * 32 + 8 * c + 4 * t + e > len) s[kb][t][e] = -__builtin_inff();
+      }
+      if (a.scores && l16 < gh) {
+        float* sp = a.scores + ((int64_t)b * nh + h0 + l16) * a.c.capacity() + base + 8 * c;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (base + kb * 32 + 8 * c + 4 * t <= len) *reinterpret_cast<f32x4*>(sp + kb * 32 + 4 * t) = s[kb][t];
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kb][t][e]);
+      top *= kLog2e;
+      if (__ballot(top > m + 8.f)) {
+        float mn = fmaxf(top, m);
+        mn = fmaxf(mn, __shfl_xor(mn, 16));
+        mn = fmaxf(mn, __shfl_xor(mn, 32));
+        const float al = __builtin_amdgcn_exp2f(m - finite_or_zero(mn));
+        l *= al;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][e] *= al;
+        m = mn;
+      }
+      const float mz = finite_or_zero(m);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3], kLog2e, -mz));
+          l += p[e];
+        }
+        u32x4 pf[2];
+        split8<DT>(p, 2, pf);  // 16 (22) bits: the output's one rounding stays the error
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const uint16_t* at = vw + (kb * 32 + 8 * c + (l16 >> 2)) * ROW + d * 16 + 4 * (l16 & 3);
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * ROW));
+          const u32x2 lw = __builtin_bit_cast(u32x2, lo), hw = __builtin_bit_cast(u32x2, hi);
+          const frag vf = __builtin_bit_cast(frag, u32x4{lw[0], lw[1], hw[0], hw[1]});
+          if (precise) o[d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[1]), o[d]);
+          o[d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[0]), o[d]);
+        }
+      }
+    }
+    // An infinity meets the small parts of an operand as inf * 0 or with the wrong sign.  Where something is not
+    // finite the part is computed again from the leading parts alone, whose zeros and signs are the operand's.
+    if (!precise) break;
+    float sum = l;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += __builtin_fabsf(o[d][e]);
+    if (!__ballot(l16 < gh && !(sum < __builtin_inff()))) break;
+    precise = false;
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+
+  // The waves' outputs meet in LDS.
+  float* const ow = reinterpret_cast<float*>(vw);
+  if (l16 < gh) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(ow + l16 * OROW + d * 16 + 4 * c) = o[d];
+    if (c == 0) m_s[wv][l16] = m, l_s[wv][l16] = l;
+  }
+  __syncthreads();
+  if (bad) bad_s = 1;  // (uniform in a wave; the barrier above has passed the zero)
+  __syncthreads();
+  const bool refused = bad_s;
+  const int quads = gh * (D / 4);
+  const int stride = a.part_stride;
+  const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(a.part + (int64_t)it.first * stride), (short)0, it.parts * stride * 4, kPagedBufFlags);
+  for (int i = tid; i < quads; i += kPagedThreads) {
+    const int hd = i / (D / 4), d = i % (D / 4) * 4;
+    const float M = fmaxf(fmaxf(m_s[0][hd], m_s[1][hd]), fmaxf(m_s[2][hd], m_s[3][hd])), mz = finite_or_zero(M);
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    float L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(m_s[w][hd] - mz);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v_s[w]) + hd * OROW + d);
+      L = __builtin_fmaf(f, l_s[w][hd], L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(f, x[e], t[e]);
+    }
+    if (it.parts == 1) {
+      const float inv = refused ? __builtin_nanf("") : 1.f / L;
+      u32x2 r;
+      r[0] = (uint32_t)float_to_act_bits<DT>(t[0] * inv) | ((uint32_t)float_to_act_bits<DT>(t[1] * inv) << 16);
+      r[1] = (uint32_t)float_to_act_bits<DT>(t[2] * inv) | ((uint32_t)float_to_act_bits<DT>(t[3] * inv) << 16);
+      *reinterpret_cast<u32x2*>(out + hd * D + d) = r;
+      if (a.scores && d == 0) {
+        a.stats[((int64_t)b * nh + h0 + hd) * 2] = refused ? __builtin_nanf("") : mz;
+        a.stats[((int64_t)b * nh + h0 + hd) * 2 + 1] = L;
+      }
+    } else {
+      const uint32_t at = (uint32_t)(it.part * stride) * 4u;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, t), rp, at + (uint32_t)i * 16u, 0,
+                                             kPagedCoherentAux);
+      if (d == 0) {
+        const f32x2 ml = {refused ? __builtin_nanf("") : M, L};
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, ml), rp, at + (uint32_t)quads * 16u + (uint32_t)hd * 8u, 0,
+                                              kPagedCoherentAux);
+      }
+    }
+  }
+  if (it.parts == 1) return;
+
+  // The last part of a row and tile to arrive joins them, in their order.
+  __builtin_amdgcn_s_waitcnt(0);  // the stores have reached the level all XCDs share
+  __syncthreads();
+  unsigned* const cnt = a.cnt + b * (a.c.nkv * a.htiles) + it.tile;
+  if (tid == 0) arrived_s = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived_s != (unsigned)(it.parts - 1)) return;
+  if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  auto stat = [&](int part, int hd) {
+    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(
+        rp, (uint32_t)(part * stride) * 4u + (uint32_t)quads * 16u + hd * 8u, 0, kPagedCoherentAux));
+  };
+  for (int hd = wv; hd < gh; hd += 4) {
+    float M = -__builtin_inff();
+    bool ref = false;
+    for (int p = lane; p < it.parts; p += 64) {
+      const float x = stat(p, hd)[0];
+      ref = ref || x != x;
+      M = fmaxf(M, x);
+    }
+    M = finite_or_zero(wave_max(M));
+    float L = 0.f;
+    for (int p = lane; p < it.parts; p += 64) {
+      const f32x2 x = stat(p, hd);
+      L = __builtin_fmaf(__builtin_amdgcn_exp2f(x[0] - M), x[1], L);
+    }
+    L = wave_sum(L);
+    const bool any = __ballot(ref) != 0;
+    if (lane == 0) m_s[0][hd] = any ? __builtin_nanf("") : M, l_s[0][hd] = L;
+  }
+  __syncthreads();
+  // threads: the quads of the output, and where those are few, several runs of parts beside each other
+  const int runs = max(1, kPagedThreads / quads);
+  f32x4* const red = reinterpret_cast<f32x4*>(&v_s[0][0]);
+  for (int i0 = 0; i0 < quads; i0 += kPagedThreads) {
+    const int run = runs > 1 ? tid / quads : 0, i = runs > 1 ? tid - run * quads : i0 + tid;
+    const bool on = run < runs && i < quads;
+    const int hd = on ? i / (D / 4) : 0;
+    const float M = m_s[0][hd];
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    if (on) {
+      for (int p0 = run; p0 < it.parts; p0 += runs * 8) {
+        f32x4 x[8];
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int p = min(p0 + k * runs, it.parts - 1);
+          x[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+              rp, (uint32_t)(p * stride) * 4u + (uint32_t)i * 16u, 0, kPagedCoherentAux));
+          f[k] = stat(p, hd)[0];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (p0 + k * runs < it.parts) {
+            const float w = __builtin_amdgcn_exp2f(f[k] - M);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(w, x[k][e], t[e]);
+          }
+      }
+    }
+    if (runs > 1) {
+      if (on) red[tid] = t;
+      __syncthreads();
+      if (run == 0 && on)
+        for (int r = 1; r < runs; ++r) {
+          const f32x4 x = red[r * quads + i];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] += x[e];
+        }
+    }
+    if (on && run == 0) {
+      const float inv = 1.f / l_s[0][hd];  // (a refused row's maximum, and so its sums, are NaN)
+      u32x2 r;
+      r[0] = (uint32_t)float_to_act_bits<DT>(t[0] * inv) | ((uint32_t)float_to_act_bits<DT>(t[1] * inv) << 16);
+      r[1] = (uint32_t)float_to_act_bits<DT>(t[2] * inv) | ((uint32_t)float_to_act_bits<DT>(t[3] * inv) << 16);
+      *reinterpret_cast<u32x2*>(out + i * 4) = r;
+      if (a.scores && i % (D / 4) == 0) {
+        a.stats[((int64_t)b * nh + h0 + hd) * 2] = M;
+        a.stats[((int64_t)b * nh + h0 + hd) * 2 + 1] = l_s[0][hd];
+      }
+    }
+  }
+}
+
+// Adds every slot's probabilities to its weight, from the scores, maxima and sums that the attention left: the same
+// parts of the rows, four slots a thread.
+template <int UP>
+__global__ __launch_bounds__(kPagedThreads) void paged_weight_kernel(PagedAttnArgs a) {
+  AttnItem it;
+  if (!find_item<UP>(a.c, a.lengths, a.c.nkv, blockIdx.x, &it)) return;
+  const int b = it.b, h = it.tile, len = a.lengths[b], pos = a.positions[b], nh = a.c.nkv * a.g;
+  if (len < 0 || len >= a.c.capacity() || (uint64_t)(int64_t)pos >= (uint64_t)a.angles) return;
+  const float* const st = a.stats + ((int64_t)b * nh + h * a.g) * 2;
+  if (st[0] != st[0]) return;  // a page outside the pool
+  const int nu = len / UP + 1;
+  const int s0 = (int)((int64_t)it.part * nu / it.parts) * UP;
+  const int s1 = min((int)((int64_t)(it.part + 1) * nu / it.parts) * UP, len + 1);
+  const int64_t cap = a.c.capacity();
+  for (int s = s0 + 4 * threadIdx.x; s < s1; s += 4 * kPagedThreads) {
+    float* const wp = a.c.weight + a.c.token(b, s, h);
+    f32x4 w = *reinterpret_cast<const f32x4*>(wp);
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    const float* sp = a.scores + ((int64_t)b * nh + h * a.g) * cap + s;
+    for (int g = 0; g < a.g; ++g) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(sp + g * cap);
+      const float M = st[2 * g], inv = 1.f / st[2 * g + 1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], kLog2e, -M)) * inv;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = s + e < len ? w[e] + t[e] : s + e == len ? t[e] : w[e];
+    *reinterpret_cast<f32x4*>(wp) = w;
   }
 }
 
@@ -354,10 +763,36 @@ extern "C" int w4_paged_append(const w4_paged_cache* cache, int dtype, const voi
   return check_launch("w4_paged_append");
 }
 
+namespace {
+
+struct PagedAttnPlan {
+  int64_t tiles, items, part_stride;  // tiles of up to 16 query heads a row, workgroups, floats of a part
+  size_t part_bytes, bytes;           // the parts' share of the workspace, and all of it
+};
+
+bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, PagedAttnPlan* p) {
+  if (rows < 0 || num_heads < 1 || kv_heads < 1 || num_heads % kv_heads) return false;
+  const int64_t g = num_heads / kv_heads;
+  p->tiles = kv_heads * ((g + 15) / 16);
+  p->items = w4::kAttnItems + rows * p->tiles + 1;
+  p->part_stride = (g < 16 ? g : 16) * (head_dim + 2) + 3 & ~int64_t(3);
+  const bool split = rows * p->tiles <= w4::kPagedCounters;
+  p->part_bytes = split ? (size_t)(p->items * p->part_stride) * 4 : 0;
+  p->bytes = W4_WORKSPACE_COUNTER_BYTES + p->part_bytes + (size_t)(rows * num_heads) * 8;
+  return true;
+}
+
+template <int DT, int D>
+void launch_paged_attention(const w4::PagedAttnArgs& a, int64_t items, hipStream_t st) {
+  w4::paged_attention_kernel<DT, D><<<dim3((unsigned)items), w4::kPagedThreads, 0, st>>>(a);
+}
+
+}  // namespace
+
 extern "C" size_t w4_paged_attention_workspace_bytes(int64_t rows, int64_t num_heads, int64_t kv_heads,
                                                      int64_t head_dim) {
-  (void)rows, (void)num_heads, (void)kv_heads, (void)head_dim;
-  return 0;
+  PagedAttnPlan p;
+  return rows > 0 && paged_attn_plan(rows, num_heads, kv_heads, head_dim, &p) ? p.bytes : 0;
 }
 
 extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const void* q, const void* k, const void* v,
@@ -366,17 +801,25 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
                                   const float* sin, int64_t angles, void* out, float* scores, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   clear_error();
-  (void)workspace, (void)workspace_bytes;
   if (const int rc = check_cache(cache, dtype, "w4_paged_attention")) return rc;
   if (num_heads < 1 || num_heads % cache->kv_heads || num_heads / cache->kv_heads > 1024 || angles < 1)
     return fail(W4_ERR_INVALID, "w4_paged_attention: %lld query heads on %lld key-value heads, %lld angles",
                 (long long)num_heads, (long long)cache->kv_heads, (long long)angles);
   if (cache->rows == 0) return W4_OK;
+  PagedAttnPlan p;
+  paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, &p);
+  // a launch of 2^32 threads, or more, is refused by HIP
+  if (p.items > 0xFFFFFFFFll / w4::kPagedThreads)
+    return fail(W4_ERR_UNSUPPORTED, "w4_paged_attention: %lld rows of %lld heads", (long long)cache->rows,
+                (long long)num_heads);
   if (!q || !k || !v || !lengths || !positions || !cos || !sin || !out || (cache->weight && !scores))
     return fail(W4_ERR_INVALID, "w4_paged_attention: null pointer");
   if (!rows_ok(q, stride_q) || !rows_ok(k, stride_k) || !rows_ok(v, stride_v) ||
-      ((uintptr_t)cos | (uintptr_t)sin | (uintptr_t)out | (uintptr_t)scores) % 16)
+      ((uintptr_t)cos | (uintptr_t)sin | (uintptr_t)out | (uintptr_t)scores | (uintptr_t)cache->weight) % 16)
     return fail(W4_ERR_INVALID, "w4_paged_attention: operands must be 16-byte aligned, row strides multiples of 8");
+  if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 256)
+    return fail(W4_ERR_WORKSPACE, "w4_paged_attention: needs a 256-byte aligned workspace of %zu bytes (got %zu)",
+                p.bytes, workspace_bytes);
   w4::PagedAttnArgs a{};
   a.c = view_of(cache);
   a.q = static_cast<const uint16_t*>(q);
@@ -385,20 +828,29 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   a.stride_q = stride_q, a.stride_k = stride_k, a.stride_v = stride_v, a.angles = angles;
   a.lengths = lengths, a.positions = positions, a.cos = cos, a.sin = sin;
   a.out = static_cast<uint16_t*>(out);
+  a.scores = cache->weight ? scores : nullptr;
+  char* const ws = static_cast<char*>(workspace);
+  a.cnt = reinterpret_cast<unsigned*>(ws);
+  a.part = reinterpret_cast<float*>(ws + W4_WORKSPACE_COUNTER_BYTES);
+  a.stats = reinterpret_cast<float*>(ws + W4_WORKSPACE_COUNTER_BYTES + p.part_bytes);
   a.scale = 1.f / sqrtf((float)cache->head_dim);
   a.g = (int)(num_heads / cache->kv_heads);
-  const dim3 grid((unsigned)cache->kv_heads, (unsigned)cache->rows);
+  a.htiles = (int)(p.tiles / cache->kv_heads);
+  a.part_stride = (int)p.part_stride;
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define W4_ATTN(DT, D) w4::paged_attention_kernel<DT, D><<<grid, w4::kPagedThreads, 0, st>>>(a)
   if (dtype == W4_DTYPE_BF16) {
-    if (cache->head_dim == 64) W4_ATTN(W4_DTYPE_BF16, 64);
-    else W4_ATTN(W4_DTYPE_BF16, 128);
+    if (cache->head_dim == 64) launch_paged_attention<W4_DTYPE_BF16, 64>(a, p.items, st);
+    else launch_paged_attention<W4_DTYPE_BF16, 128>(a, p.items, st);
   } else {
-    if (cache->head_dim == 64) W4_ATTN(W4_DTYPE_FP16, 64);
-    else W4_ATTN(W4_DTYPE_FP16, 128);
+    if (cache->head_dim == 64) launch_paged_attention<W4_DTYPE_FP16, 64>(a, p.items, st);
+    else launch_paged_attention<W4_DTYPE_FP16, 128>(a, p.items, st);
   }
-#undef W4_ATTN
-  return check_launch("w4_paged_attention");
+  if (const int rc = check_launch("w4_paged_attention")) return rc;
+  if (!cache->weight) return W4_OK;
+  const dim3 grid((unsigned)(w4::kAttnItems + cache->rows * cache->kv_heads + 1));
+  if (cache->head_dim == 64) w4::paged_weight_kernel<64><<<grid, w4::kPagedThreads, 0, st>>>(a);
+  else w4::paged_weight_kernel<32><<<grid, w4::kPagedThreads, 0, st>>>(a);
+  return check_launch("w4_paged_attention (weights)");
 }
 
 extern "C" int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int32_t* lengths,
