@@ -89,10 +89,12 @@ struct PagedAttnArgs {
 // The work of one workgroup: a part of the slots of one row and one tile of its heads.
 struct AttnItem {
   int b, tile, part, parts, first;  // first: the index of part 0
+  int len, pos;                     // of the row
 };
 
-constexpr int kAttnItems = 1024;    // parts the tokens of a batch are cut into, about
-constexpr int kAttnMinUnits = 4;    // units of a part at least: one a wave
+constexpr int kAttnWaves = 4;
+constexpr int kAttnItems = 256;     // parts the tokens of a batch are cut into, about
+constexpr int kAttnMinUnits = 16;   // units of a part at least
 constexpr int kPagedCounters = W4_WORKSPACE_COUNTER_BYTES / 4;
 
 // Inclusive sum over the lanes.
@@ -111,22 +113,22 @@ __device__ __forceinline__ int wave_scan(int v) {
 // rows stay whole and long ones spread over the chip, whatever else is in the batch.  Rows that need no
 // attention (idle, refused) are one part.
 template <int UP>
-__device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __restrict__ lengths, int tiles, int item,
-                                          AttnItem* it) {
+__device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __restrict__ lengths,
+                                          const int32_t* __restrict__ positions, int tiles, int item, AttnItem* it) {
   const int lane = threadIdx.x & 63;
-  auto units = [&](int row) {
-    const int len = row < c.rows ? lengths[row] : -1;
-    return len >= 0 && len < c.capacity() ? len / UP + 1 : 1;
-  };
-  float all = 0.f;
-  for (int r = 0; r < c.rows; r += 64) all += r + lane < c.rows ? (float)units(r + lane) : 0.f;
+  auto length = [&](int r) { return r + lane < c.rows ? lengths[r + lane] : -1; };
+  auto units = [&](int len) { return len >= 0 && len < c.capacity() ? len / UP + 1 : 1; };
+  int len = length(0), pos = lane < c.rows ? positions[lane] : 0;
+  float all = lane < c.rows ? (float)units(len) : 0.f;
+  for (int r = 64; r < c.rows; r += 64) all += r + lane < c.rows ? (float)units(length(r)) : 0.f;
   all = wave_sum(all);
   int per = (int)fminf(ceilf(all * ((float)tiles / kAttnItems)), 1e9f);
   per = max(per, kAttnMinUnits);
   if ((int64_t)c.rows * tiles > kPagedCounters) per = 1 << 30;  // no counters for parts to meet at
   int base = 0;
   for (int r = 0; r < c.rows; r += 64) {
-    const int parts = r + lane < c.rows ? (units(r + lane) + per - 1) / per : 0;
+    if (r) len = length(r), pos = r + lane < c.rows ? positions[r + lane] : 0;
+    const int parts = r + lane < c.rows ? (units(len) + per - 1) / per : 0;
     const int upto = base + wave_scan(parts * tiles);
     const int end = __builtin_amdgcn_readlane(upto, 63);
     if (item < end) {
@@ -137,6 +139,8 @@ __device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __r
       it->tile = rem / it->parts;
       it->part = rem - it->tile * it->parts;
       it->first = item - it->part;
+      it->len = __builtin_amdgcn_readlane(len, i);
+      it->pos = __builtin_amdgcn_readlane(pos, i);
       return true;
     }
     base = end;
@@ -163,27 +167,21 @@ __device__ __forceinline__ void split8(const float v[8], int parts, u32x4* out) 
   }
 }
 
-// The D / 32 chunks of eight elements that lane group c holds of a head's D (chunk j: elements 32 j + 8 c..), rotated
-// and multiplied by `scale`.  A chunk's partner, D / 2 further on, is in the same lane.
+// Lane group c holds D / 32 chunks of eight elements of a head's D (chunk j: elements 32 j + 8 c..).  Chunk j < D / 64
+// and its partner D / 2 further on, rotated and multiplied by `scale`.
 template <int DT, int D>
-__device__ __forceinline__ void rope_chunks(const uint16_t* __restrict__ x, const float* __restrict__ cos,
-                                            const float* __restrict__ sin, int c, float scale, float (*out)[8]) {
-  constexpr int NJ = D / 32;
-  u32x4 raw[NJ];
+__device__ __forceinline__ void rope_chunk(const uint16_t* __restrict__ x, const float* __restrict__ cos,
+                                           const float* __restrict__ sin, int j, int c, float scale, float lo[8],
+                                           float hi[8]) {
+  const int d = 32 * j + 8 * c;
+  unpack8<DT>(*reinterpret_cast<const u32x4*>(x + d), lo);
+  unpack8<DT>(*reinterpret_cast<const u32x4*>(x + d + D / 2), hi);
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) raw[j] = *reinterpret_cast<const u32x4*>(x + 32 * j + 8 * c);
-#pragma unroll
-  for (int j = 0; j < NJ / 2; ++j) {
-    float a[8], b[8];
-    unpack8<DT>(raw[j], a);
-    unpack8<DT>(raw[j + NJ / 2], b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float r1, r2;
-      rope_pair(a[e], b[e], cos[32 * j + 8 * c + e], sin[32 * j + 8 * c + e], &r1, &r2);
-      out[j][e] = r1 * scale;
-      out[j + NJ / 2][e] = r2 * scale;
-    }
+  for (int e = 0; e < 8; ++e) {
+    float r1, r2;
+    rope_pair(lo[e], hi[e], cos[d + e], sin[d + e], &r1, &r2);
+    lo[e] = r1 * scale;
+    hi[e] = r2 * scale;
   }
 }
 
@@ -203,33 +201,34 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 // transposes them on reading.  The running maximum of a head is only raised when a score passes it by 2^8 (its value
 // cancels in the end), so that most units need no exchange between lanes.
 template <int DT, int D>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int KB = 128 / D, UP = 32 * KB, NJ = D / 32, ND = D / 16, VR = 512 / D, NP = Split<DT>::N;
-  constexpr int ROW = D == 64 ? 72 : 144;  // halfwords of a value row in LDS: four rows on different banks
+  constexpr int KROW = D + 8;              // halfwords of a key row in LDS: sixteen rows on different banks
+  constexpr int VROW = D == 64 ? 72 : 144; // of a value row: four rows of 32 bytes on different banks
   constexpr int OROW = D + 4;              // floats of an output row in LDS
-  constexpr int WAVE_H = UP * ROW;
-  static_assert(16 * OROW * 2 <= WAVE_H, "a wave's outputs take its values' place");
+  constexpr int WAVE_H = UP * (KROW + VROW), kThreads = 64 * kAttnWaves;
+  static_assert(16 * OROW * 2 <= WAVE_H, "a wave's outputs take its tokens' place");
   typedef typename Act<DT>::frag frag;
-  __shared__ __attribute__((aligned(16))) uint16_t v_s[4][WAVE_H];
-  __shared__ float m_s[4][16], l_s[4][16];
-  __shared__ int bad_s;
+  __shared__ __attribute__((aligned(16))) uint16_t kv_s[kAttnWaves][WAVE_H];
+  __shared__ __attribute__((aligned(16))) uint16_t new_s[2][D];
+  __shared__ float m_s[kAttnWaves][16], l_s[kAttnWaves][16];
+  __shared__ int bad_s[kAttnWaves];
   __shared__ unsigned arrived_s;
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, c = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   AttnItem it;
-  if (!find_item<UP>(a.c, a.lengths, a.c.nkv * a.htiles, blockIdx.x, &it)) return;
+  if (!find_item<UP>(a.c, a.lengths, a.positions, a.c.nkv * a.htiles, blockIdx.x, &it)) return;
   const int b = it.b, h = it.tile / a.htiles, ht = it.tile - h * a.htiles;
   const int h0 = h * a.g + ht * 16, gh = min(a.g - ht * 16, 16);  // query heads of the row
   const int nh = a.c.nkv * a.g;
-  const int len = a.lengths[b], pos = a.positions[b];
+  const int len = it.len, pos = it.pos;
   uint16_t* const out = a.out + ((int64_t)b * nh + h0) * D;
   if (len < 0 || len >= a.c.capacity() || (uint64_t)(int64_t)pos >= (uint64_t)a.angles) {
     const uint16_t fill = len < 0 ? 0 : float_to_act_bits<DT>(__builtin_nanf(""));
-    for (int i = tid; i < gh * D; i += kPagedThreads) out[i] = fill;
+    for (int i = tid; i < gh * D; i += kThreads) out[i] = fill;
     return;
   }
-  if (tid == 0) bad_s = 0;
   const int nu = len / UP + 1;
   const int u0 = (int)((int64_t)it.part * nu / it.parts), u1 = (int)((int64_t)(it.part + 1) * nu / it.parts);
   const float* const cosr = a.cos + (int64_t)pos * (D / 2);
@@ -237,20 +236,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
   const int32_t* const table = a.c.table + (int64_t)b * a.c.width;
   const int smask = (1 << a.c.log2s) - 1;
 
-  // the query: heads past gh are zero
-  u32x4 qf[NJ][NP];
-  {
-    float x[NJ][8];
-    rope_chunks<DT, D>(a.q + b * a.stride_q + (int64_t)(h0 + min(l16, gh - 1)) * D, cosr, sinr, c, a.scale, x);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[j][e] = l16 < gh ? x[j][e] : 0.f;
-      split8<DT>(x[j], NP, qf[j]);
-    }
-  }
-
-  u32x4 kr[KB][2][NJ], vr[8];
+  u32x4 kr[8], vr[8];
   bool bad = false;
   // Lane i: the page of the unit's slots 8 i.. (past the row's end, its last page).
   auto load_ids = [&](int u) {
@@ -263,24 +249,65 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     ids = out_of_pool ? 0 : ids;
     const int base = u * UP;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      const int page = __shfl(ids, kb * 4 + (l16 >> 2));
-      const int slot = base + kb * 32 + 8 * (l16 >> 2) + (l16 & 3);
-      const uint16_t* kp =
-          a.c.k + (((((int64_t)page * a.c.nkv + h) << a.c.log2s) + (slot & smask)) * D + 8 * c);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) kr[kb][t][j] = *reinterpret_cast<const u32x4*>(kp + 4 * t * D + 32 * j);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i) {  // eight (D = 64) or four rows
       const int page = __builtin_amdgcn_readlane(ids, i * VR / 8);
-      const int64_t at = (((int64_t)page * a.c.nkv + h) << a.c.log2s) + ((base + i * VR) & smask);
-      vr[i] = *reinterpret_cast<const u32x4*>(a.c.v + at * D + lane * 8);
+      const int64_t at = ((((int64_t)page * a.c.nkv + h) << a.c.log2s) + ((base + i * VR) & smask)) * D + lane * 8;
+      kr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.c.k + at));
+      vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.c.v + at));
     }
   };
-  uint16_t* const vw = v_s[wv];
+  uint16_t* const kw = kv_s[wv];
+  uint16_t* const vw = kw + UP * KROW;
+  const int srow = lane * 8 / D, sd = lane * 8 % D;  // this lane's place in a load's rows
+  // A key lies in LDS in the order of the tiles' rows: slot 8 g + 4 t + e of a block at row 16 t + 4 g + e.
+  auto krow = [&](int i) {
+    return D == 64 ? (i >> 2) * 32 + (srow >> 2) * 16 + (i & 3) * 4 + (srow & 3) : (i & 1) * 16 + (i >> 1) * 4 + srow;
+  };
+  int u = u0 + wv, ids = 0;
+  if (u < u1) {  // on their way before the query is at hand
+    load(u, load_ids(u));
+    ids = load_ids(min(u + kAttnWaves, u1 - 1));
+  }
+
+  // the query: heads past gh copy another and count for nothing
+  u32x4 qf[NJ][NP];
+  {
+    const uint16_t* const qp = a.q + b * a.stride_q + (int64_t)(h0 + min(l16, gh - 1)) * D;
+    const float scale = l16 < gh ? a.scale : 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ / 2; ++j) {
+      float lo[8], hi[8];
+      rope_chunk<DT, D>(qp, cosr, sinr, j, c, scale, lo, hi);
+      split8<DT>(lo, NP, qf[j]);
+      split8<DT>(hi, NP, qf[j + NJ / 2]);
+    }
+  }
+  // The wave that takes the row's last unit rotates the new key, keeps it and the value at hand and writes them to
+  // the cache.
+  if (it.part == it.parts - 1 && wv == (nu - 1 - u0) % kAttnWaves) {
+    const uint16_t* const kin = a.k + b * a.stride_k + h * D;
+    float x[8], y[8];
+    unpack8<DT>(*reinterpret_cast<const u32x4*>(kin + sd), x);
+    unpack8<DT>(*reinterpret_cast<const u32x4*>(kin + (sd ^ (D / 2))), y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float cc = cosr[(sd & (D / 2 - 1)) + e], ss = sinr[(sd & (D / 2 - 1)) + e];
+      float r1, r2;
+      if (sd < D / 2) rope_pair(x[e], y[e], cc, ss, &r1, &r2), x[e] = r1;
+      else rope_pair(y[e], x[e], cc, ss, &r1, &r2), x[e] = r2;
+    }
+    const u32x4 kn = pack8<DT>(x), vn = *reinterpret_cast<const u32x4*>(a.v + b * a.stride_v + h * D + sd);
+    const int page = table[len >> a.c.log2s];
+    if (srow == 0) {
+      *reinterpret_cast<u32x4*>(&new_s[0][sd]) = kn;
+      *reinterpret_cast<u32x4*>(&new_s[1][sd]) = vn;
+      if (ht == 0 && (unsigned)page < (unsigned)a.c.pages) {
+        const int64_t tok = ((((int64_t)page * a.c.nkv + h) << a.c.log2s) + (len & smask)) * D + sd;
+        *reinterpret_cast<u32x4*>(a.c.k + tok) = kn;
+        *reinterpret_cast<u32x4*>(a.c.v + tok) = vn;
+      }
+    }
+  }
 
   float m, l;  // of head l16: the reference exponent and this lane's share of the sum
   f32x4 o[ND];
@@ -289,73 +316,48 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
     m = -__builtin_inff(), l = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int u = u0 + wv;
-    int ids = 0;
-    if (u < u1) {
-      load(u, load_ids(u));
-      ids = load_ids(min(u + 4, u1 - 1));
-    }
-    for (; u < u1; u += 4) {
+    for (; u < u1; u += kAttnWaves) {
       const int base = u * UP;
       const bool last = base + UP > len;  // the new token is in this unit, and what lies past it
       if (last) {
         const int at = len - base;
-        const uint16_t* kin = a.k + b * a.stride_k + h * D;
-        float x[NJ][8];
-        u32x4 kn[NJ];
-        rope_chunks<DT, D>(kin, cosr, sinr, c, 1.f, x);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) kn[j] = pack8<DT>(x[j]);
-        const int page = table[len >> a.c.log2s];
-        const int64_t tok = (((int64_t)page * a.c.nkv + h) << a.c.log2s) + (len & smask);
-        const bool write = ht == 0 && precise && (unsigned)page < (unsigned)a.c.pages;
-        const bool mine = l16 == ((at & 31) >> 3) * 4 + (at & 3);
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (at >> 5 == kb && ((at >> 2) & 1) == t)
-#pragma unroll
-              for (int j = 0; j < NJ; ++j) kr[kb][t][j] = mine ? kn[j] : kr[kb][t][j];
-        if (write && mine) {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) *reinterpret_cast<u32x4*>(a.c.k + tok * D + 32 * j + 8 * c) = kn[j];
-        }
-        const int vrow = lane * 8 / D, vd = lane * 8 % D;
-        const u32x4 vn = *reinterpret_cast<const u32x4*>(a.v + b * a.stride_v + h * D + vd);
+        const u32x4 kn = *reinterpret_cast<const u32x4*>(&new_s[0][sd]);
+        const u32x4 vn = *reinterpret_cast<const u32x4*>(&new_s[1][sd]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int row = i * VR + vrow;
+          const int row = i * VR + srow;
+          kr[i] = row == at ? kn : kr[i];
           vr[i] = row == at ? vn : row > at ? u32x4{0u, 0u, 0u, 0u} : vr[i];
-          if (write && row == at) *reinterpret_cast<u32x4*>(a.c.v + tok * D + vd) = vn;
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<u32x4*>(vw + (i * VR + lane * 8 / D) * ROW + lane * 8 % D) = vr[i];
+      for (int i = 0; i < 8; ++i) {
+        *reinterpret_cast<u32x4*>(kw + krow(i) * KROW + sd) = kr[i];
+        *reinterpret_cast<u32x4*>(vw + (i * VR + srow) * VROW + sd) = vr[i];
+      }
+      if (u + kAttnWaves < u1) {  // the next unit's loads travel under the rest
+        load(u + kAttnWaves, ids);
+        ids = load_ids(min(u + 2 * kAttnWaves, u1 - 1));
+      }
       f32x4 s[KB][2];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+          const uint16_t* const at = kw + (kb * 32 + t * 16 + l16) * KROW + 8 * c;
+          frag kf[NJ];
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const frag*>(at + 32 * j);
           s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
           if (precise) {  // the small parts first
 #pragma unroll
             for (int p = NP - 1; p > 0; --p)
 #pragma unroll
-              for (int j = 0; j < NJ; ++j)
-                s[kb][t] = Mfma<DT>::m16(__builtin_bit_cast(frag, kr[kb][t][j]), __builtin_bit_cast(frag, qf[j][p]),
-                                         s[kb][t]);
+              for (int j = 0; j < NJ; ++j) s[kb][t] = Mfma<DT>::m16(kf[j], __builtin_bit_cast(frag, qf[j][p]), s[kb][t]);
           }
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
-            s[kb][t] = Mfma<DT>::m16(__builtin_bit_cast(frag, kr[kb][t][j]), __builtin_bit_cast(frag, qf[j][0]),
-                                     s[kb][t]);
+          for (int j = 0; j < NJ; ++j) s[kb][t] = Mfma<DT>::m16(kf[j], __builtin_bit_cast(frag, qf[j][0]), s[kb][t]);
         }
-      if (u + 4 < u1) {  // the next unit's loads travel under the rest
-        load(u + 4, ids);
-        ids = load_ids(min(u + 8, u1 - 1));
-      }
       if (last) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -406,9 +408,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
         split8<DT>(p, 2, pf);  // 16 (22) bits: the output's one rounding stays the error
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-          const uint16_t* at = vw + (kb * 32 + 8 * c + (l16 >> 2)) * ROW + d * 16 + 4 * (l16 & 3);
+          const uint16_t* at = vw + (kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3);
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * ROW));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * VROW));
           const u32x2 lw = __builtin_bit_cast(u32x2, lo), hw = __builtin_bit_cast(u32x2, hi);
           const frag vf = __builtin_bit_cast(frag, u32x4{lw[0], lw[1], hw[0], hw[1]});
           if (precise) o[d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[1]), o[d]);
@@ -426,34 +428,41 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
       for (int e = 0; e < 4; ++e) sum += __builtin_fabsf(o[d][e]);
     if (!__ballot(l16 < gh && !(sum < __builtin_inff()))) break;
     precise = false;
+    u = u0 + wv;
+    load(u, load_ids(u));
+    ids = load_ids(min(u + kAttnWaves, u1 - 1));
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
 
   // The waves' outputs meet in LDS.
-  float* const ow = reinterpret_cast<float*>(vw);
+  float* const ow = reinterpret_cast<float*>(kw);
   if (l16 < gh) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(ow + l16 * OROW + d * 16 + 4 * c) = o[d];
     if (c == 0) m_s[wv][l16] = m, l_s[wv][l16] = l;
   }
+  if (lane == 0) bad_s[wv] = bad;
   __syncthreads();
-  if (bad) bad_s = 1;  // (uniform in a wave; the barrier above has passed the zero)
-  __syncthreads();
-  const bool refused = bad_s;
+  int refused = 0;
+#pragma unroll
+  for (int w = 0; w < kAttnWaves; ++w) refused |= bad_s[w];
   const int quads = gh * (D / 4);
   const int stride = a.part_stride;
   const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(a.part + (int64_t)it.first * stride), (short)0, it.parts * stride * 4, kPagedBufFlags);
-  for (int i = tid; i < quads; i += kPagedThreads) {
+  for (int i = tid; i < quads; i += kThreads) {
     const int hd = i / (D / 4), d = i % (D / 4) * 4;
-    const float M = fmaxf(fmaxf(m_s[0][hd], m_s[1][hd]), fmaxf(m_s[2][hd], m_s[3][hd])), mz = finite_or_zero(M);
+    float M = m_s[0][hd];
+#pragma unroll
+    for (int w = 1; w < kAttnWaves; ++w) M = fmaxf(M, m_s[w][hd]);
+    const float mz = finite_or_zero(M);
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
     float L = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kAttnWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(m_s[w][hd] - mz);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v_s[w]) + hd * OROW + d);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(kv_s[w]) + hd * OROW + d);
       L = __builtin_fmaf(f, l_s[w][hd], L);
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(f, x[e], t[e]);
@@ -489,77 +498,57 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
   __syncthreads();
   if (arrived_s != (unsigned)(it.parts - 1)) return;
   if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  auto stat = [&](int part, int hd) {
-    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(
-        rp, (uint32_t)(part * stride) * 4u + (uint32_t)quads * 16u + hd * 8u, 0, kPagedCoherentAux));
-  };
-  for (int hd = wv; hd < gh; hd += 4) {
-    float M = -__builtin_inff();
-    bool ref = false;
-    for (int p = lane; p < it.parts; p += 64) {
-      const float x = stat(p, hd)[0];
-      ref = ref || x != x;
-      M = fmaxf(M, x);
-    }
-    M = finite_or_zero(wave_max(M));
-    float L = 0.f;
-    for (int p = lane; p < it.parts; p += 64) {
-      const f32x2 x = stat(p, hd);
-      L = __builtin_fmaf(__builtin_amdgcn_exp2f(x[0] - M), x[1], L);
-    }
-    L = wave_sum(L);
-    const bool any = __ballot(ref) != 0;
-    if (lane == 0) m_s[0][hd] = any ? __builtin_nanf("") : M, l_s[0][hd] = L;
-  }
-  __syncthreads();
-  // threads: the quads of the output, and where those are few, several runs of parts beside each other
-  const int runs = max(1, kPagedThreads / quads);
-  f32x4* const red = reinterpret_cast<f32x4*>(&v_s[0][0]);
-  for (int i0 = 0; i0 < quads; i0 += kPagedThreads) {
+  // Threads: the quads of the output, and where those are few, several runs of parts beside each other.  Maxima,
+  // sums and outputs of eight parts travel together.
+  const int runs = max(1, kThreads / quads);
+  f32x4* const red = reinterpret_cast<f32x4*>(&kv_s[0][0]);
+  f32x2* const red_ml = reinterpret_cast<f32x2*>(red + kThreads);
+  for (int i0 = 0; i0 < quads; i0 += kThreads) {
     const int run = runs > 1 ? tid / quads : 0, i = runs > 1 ? tid - run * quads : i0 + tid;
     const bool on = run < runs && i < quads;
     const int hd = on ? i / (D / 4) : 0;
-    const float M = m_s[0][hd];
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    float M = -__builtin_inff(), L = 0.f;
+    auto add = [&](float m1, float l1, const f32x4& x) {  // one more share; a refused one's maximum is NaN
+      const float mn = M != M || m1 != m1 ? __builtin_nanf("") : fmaxf(M, m1), mz = finite_or_zero(mn);
+      const float w0 = __builtin_amdgcn_exp2f(M - mz), w1 = __builtin_amdgcn_exp2f(m1 - mz);
+      L = __builtin_fmaf(w1, l1, L * w0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(w1, x[e], t[e] * w0);
+      M = mn;
+    };
     if (on) {
       for (int p0 = run; p0 < it.parts; p0 += runs * 8) {
         f32x4 x[8];
-        float f[8];
+        f32x2 ml[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int p = min(p0 + k * runs, it.parts - 1);
-          x[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-              rp, (uint32_t)(p * stride) * 4u + (uint32_t)i * 16u, 0, kPagedCoherentAux));
-          f[k] = stat(p, hd)[0];
+          const uint32_t at = (uint32_t)(min(p0 + k * runs, it.parts - 1) * stride) * 4u;
+          x[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, at + (uint32_t)i * 16u, 0,
+                                                                                 kPagedCoherentAux));
+          ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(
+              rp, at + (uint32_t)quads * 16u + (uint32_t)hd * 8u, 0, kPagedCoherentAux));
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (p0 + k * runs < it.parts) {
-            const float w = __builtin_amdgcn_exp2f(f[k] - M);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(w, x[k][e], t[e]);
-          }
+          if (p0 + k * runs < it.parts) add(ml[k][0], ml[k][1], x[k]);
       }
     }
     if (runs > 1) {
-      if (on) red[tid] = t;
+      if (on) red[tid] = t, red_ml[tid] = f32x2{M, L};
       __syncthreads();
       if (run == 0 && on)
-        for (int r = 1; r < runs; ++r) {
-          const f32x4 x = red[r * quads + i];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] += x[e];
-        }
+        for (int r = 1; r < runs; ++r) add(red_ml[r * quads + i][0], red_ml[r * quads + i][1], red[r * quads + i]);
     }
     if (on && run == 0) {
-      const float inv = 1.f / l_s[0][hd];  // (a refused row's maximum, and so its sums, are NaN)
+      const float inv = 1.f / L;
       u32x2 r;
       r[0] = (uint32_t)float_to_act_bits<DT>(t[0] * inv) | ((uint32_t)float_to_act_bits<DT>(t[1] * inv) << 16);
       r[1] = (uint32_t)float_to_act_bits<DT>(t[2] * inv) | ((uint32_t)float_to_act_bits<DT>(t[3] * inv) << 16);
       *reinterpret_cast<u32x2*>(out + i * 4) = r;
       if (a.scores && i % (D / 4) == 0) {
-        a.stats[((int64_t)b * nh + h0 + hd) * 2] = M;
-        a.stats[((int64_t)b * nh + h0 + hd) * 2 + 1] = l_s[0][hd];
+        a.stats[((int64_t)b * nh + h0 + hd) * 2] = finite_or_zero(M);
+        a.stats[((int64_t)b * nh + h0 + hd) * 2 + 1] = L;
       }
     }
   }
@@ -570,8 +559,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_attention_kernel(Paged
 template <int UP>
 __global__ __launch_bounds__(kPagedThreads) void paged_weight_kernel(PagedAttnArgs a) {
   AttnItem it;
-  if (!find_item<UP>(a.c, a.lengths, a.c.nkv, blockIdx.x, &it)) return;
-  const int b = it.b, h = it.tile, len = a.lengths[b], pos = a.positions[b], nh = a.c.nkv * a.g;
+  if (!find_item<UP>(a.c, a.lengths, a.positions, a.c.nkv, blockIdx.x, &it)) return;
+  const int b = it.b, h = it.tile, len = it.len, pos = it.pos, nh = a.c.nkv * a.g;
   if (len < 0 || len >= a.c.capacity() || (uint64_t)(int64_t)pos >= (uint64_t)a.angles) return;
   const float* const st = a.stats + ((int64_t)b * nh + h * a.g) * 2;
   if (st[0] != st[0]) return;  // a page outside the pool
@@ -784,7 +773,7 @@ bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t 
 
 template <int DT, int D>
 void launch_paged_attention(const w4::PagedAttnArgs& a, int64_t items, hipStream_t st) {
-  w4::paged_attention_kernel<DT, D><<<dim3((unsigned)items), w4::kPagedThreads, 0, st>>>(a);
+  w4::paged_attention_kernel<DT, D><<<dim3((unsigned)items), 64 * w4::kAttnWaves, 0, st>>>(a);
 }
 
 }  // namespace
@@ -809,7 +798,7 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   PagedAttnPlan p;
   paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, &p);
   // a launch of 2^32 threads, or more, is refused by HIP
-  if (p.items > 0xFFFFFFFFll / w4::kPagedThreads)
+  if (p.items > 0xFFFFFFFFll / (64 * w4::kAttnWaves))
     return fail(W4_ERR_UNSUPPORTED, "w4_paged_attention: %lld rows of %lld heads", (long long)cache->rows,
                 (long long)num_heads);
   if (!q || !k || !v || !lengths || !positions || !cos || !sin || !out || (cache->weight && !scores))
