@@ -354,8 +354,8 @@ int w4_paged_append(const w4_paged_cache* cache, int dtype, const void* k, const
  * nothing written.  A new slot past the table or a position outside the angles: out
  * NaN and nothing written; a page of the row outside the pool: out NaN.  In both the
  * row's weights stay as they were.  lengths is not changed.
- * workspace: as for w4a16_gemm, w4_paged_attention_workspace_bytes long.  Results are
- * bit-identical run to run.
+ * num_heads: at most 256 for each key-value head.  workspace: as for w4a16_gemm,
+ * w4_paged_attention_workspace_bytes long.  Results are bit-identical run to run.
  */
 size_t w4_paged_attention_workspace_bytes(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim);
 int w4_paged_attention(const w4_paged_cache* cache, int dtype, const void* q, const void* k, const void* v,

@@ -79,11 +79,13 @@ struct PagedAttnArgs {
   const float *cos, *sin;
   uint16_t* out;  // [rows, nkv * g * D]
   float* scores;  // [rows, nkv * g, width * page_size], of q K / sqrt(D); null without weights
-  float* stats;   // [rows, nkv * g, 2]: the scores' maximum in powers of two, and their sum relative to it
-  float* part;    // [items, part_stride]: outputs of a part, then (maximum, sum) of its heads
+  float* part;    // [items, min(g, 16), D]: outputs of a part, where a row's slots are cut
+  float* stats;   // [items, 16, 2]: its heads' maxima of the scores, in powers of two, and sums relative to them
+  int* first;     // [rows, nkv * htiles, 2]: index of a row and tile's first part, and how many there are
   unsigned* cnt;  // one arrival counter per row and tile of heads
   float scale;    // 1 / sqrt(D)
-  int g, htiles, part_stride;
+  int g, htiles;
+  int later;      // the parts are joined by a launch of its own
 };
 
 // The work of one workgroup: a part of the slots of one row and one tile of its heads.
@@ -187,6 +189,27 @@ __device__ __forceinline__ void rope_chunk(const uint16_t* __restrict__ x, const
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.f : m; }
 
+// Softmax sums and a quad of outputs, relative to 2^M.  A refused part's maximum is NaN and stays.
+struct Share {
+  float M = -__builtin_inff(), L = 0.f;
+  f32x4 t = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float m, float l, const f32x4& x) {
+    const float mn = M != M || m != m ? __builtin_nanf("") : fmaxf(M, m), mz = finite_or_zero(mn);
+    const float w0 = __builtin_amdgcn_exp2f(M - mz), w1 = __builtin_amdgcn_exp2f(m - mz);
+    L = __builtin_fmaf(w1, l, L * w0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(w1, x[e], t[e] * w0);
+    M = mn;
+  }
+  template <int DT> __device__ __forceinline__ u32x2 out() const {
+    const float inv = 1.f / L;
+    u32x2 r;
+    r[0] = (uint32_t)float_to_act_bits<DT>(t[0] * inv) | ((uint32_t)float_to_act_bits<DT>(t[1] * inv) << 16);
+    r[1] = (uint32_t)float_to_act_bits<DT>(t[2] * inv) | ((uint32_t)float_to_act_bits<DT>(t[3] * inv) << 16);
+    return r;
+  }
+};
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
@@ -227,6 +250,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
   if (len < 0 || len >= a.c.capacity() || (uint64_t)(int64_t)pos >= (uint64_t)a.angles) {
     const uint16_t fill = len < 0 ? 0 : float_to_act_bits<DT>(__builtin_nanf(""));
     for (int i = tid; i < gh * D; i += kThreads) out[i] = fill;
+    if (a.later && tid == 0) a.first[(b * a.c.nkv * a.htiles + it.tile) * 2 + 1] = 1;
     return;
   }
   const int nu = len / UP + 1;
@@ -447,48 +471,34 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
   int refused = 0;
 #pragma unroll
   for (int w = 0; w < kAttnWaves; ++w) refused |= bad_s[w];
-  const int quads = gh * (D / 4);
-  const int stride = a.part_stride;
+  const int quads = gh * (D / 4), stride = min(a.g, 16) * D;
   const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(a.part + (int64_t)it.first * stride), (short)0, it.parts * stride * 4, kPagedBufFlags);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(a.stats + (int64_t)it.first * 32), (short)0, it.parts * 128, kPagedBufFlags);
+  if (a.later && it.part == 0 && tid == 0) {
+    int* const f = a.first + (b * a.c.nkv * a.htiles + it.tile) * 2;
+    f[0] = it.first;
+    f[1] = it.parts;
+  }
   for (int i = tid; i < quads; i += kThreads) {
     const int hd = i / (D / 4), d = i % (D / 4) * 4;
-    float M = m_s[0][hd];
+    Share x;
 #pragma unroll
-    for (int w = 1; w < kAttnWaves; ++w) M = fmaxf(M, m_s[w][hd]);
-    const float mz = finite_or_zero(M);
-    f32x4 t = {0.f, 0.f, 0.f, 0.f};
-    float L = 0.f;
-#pragma unroll
-    for (int w = 0; w < kAttnWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(m_s[w][hd] - mz);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(kv_s[w]) + hd * OROW + d);
-      L = __builtin_fmaf(f, l_s[w][hd], L);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(f, x[e], t[e]);
-    }
-    if (it.parts == 1) {
-      const float inv = refused ? __builtin_nanf("") : 1.f / L;
-      u32x2 r;
-      r[0] = (uint32_t)float_to_act_bits<DT>(t[0] * inv) | ((uint32_t)float_to_act_bits<DT>(t[1] * inv) << 16);
-      r[1] = (uint32_t)float_to_act_bits<DT>(t[2] * inv) | ((uint32_t)float_to_act_bits<DT>(t[3] * inv) << 16);
-      *reinterpret_cast<u32x2*>(out + hd * D + d) = r;
-      if (a.scores && d == 0) {
-        a.stats[((int64_t)b * nh + h0 + hd) * 2] = refused ? __builtin_nanf("") : mz;
-        a.stats[((int64_t)b * nh + h0 + hd) * 2 + 1] = L;
-      }
-    } else {
-      const uint32_t at = (uint32_t)(it.part * stride) * 4u;
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, t), rp, at + (uint32_t)i * 16u, 0,
-                                             kPagedCoherentAux);
-      if (d == 0) {
-        const f32x2 ml = {refused ? __builtin_nanf("") : M, L};
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, ml), rp, at + (uint32_t)quads * 16u + (uint32_t)hd * 8u, 0,
-                                              kPagedCoherentAux);
-      }
-    }
+    for (int w = 0; w < kAttnWaves; ++w)
+      x.add(m_s[w][hd], l_s[w][hd],
+            *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(kv_s[w]) + hd * OROW + d));
+    if (refused) x.M = x.L = __builtin_nanf("");
+    if (it.parts == 1)
+      *reinterpret_cast<u32x2*>(out + hd * D + d) = x.template out<DT>();
+    else
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x.t), rp,
+                                             (uint32_t)(it.part * stride + i * 4) * 4u, 0, kPagedCoherentAux);
+    if (d == 0 && (it.parts > 1 || a.later))
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{x.M, x.L}), rs,
+                                            (uint32_t)(it.part * 16 + hd) * 8u, 0, kPagedCoherentAux);
   }
-  if (it.parts == 1) return;
+  if (it.parts == 1 || a.later) return;
 
   // The last part of a row and tile to arrive joins them, in their order.
   __builtin_amdgcn_s_waitcnt(0);  // the stores have reached the level all XCDs share
@@ -498,87 +508,117 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
   __syncthreads();
   if (arrived_s != (unsigned)(it.parts - 1)) return;
   if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // Threads: the quads of the output, and where those are few, several runs of parts beside each other.  Maxima,
-  // sums and outputs of eight parts travel together.
-  const int runs = max(1, kThreads / quads);
+  // Threads: the quads of the output (no more than there are threads), and several runs of parts beside each other.
+  // Maxima, sums and outputs of eight parts travel together.
+  const int runs = kThreads / quads, run = tid / quads, i = tid - run * quads, hd = i / (D / 4);
   f32x4* const red = reinterpret_cast<f32x4*>(&kv_s[0][0]);
   f32x2* const red_ml = reinterpret_cast<f32x2*>(red + kThreads);
-  for (int i0 = 0; i0 < quads; i0 += kThreads) {
-    const int run = runs > 1 ? tid / quads : 0, i = runs > 1 ? tid - run * quads : i0 + tid;
-    const bool on = run < runs && i < quads;
-    const int hd = on ? i / (D / 4) : 0;
-    f32x4 t = {0.f, 0.f, 0.f, 0.f};
-    float M = -__builtin_inff(), L = 0.f;
-    auto add = [&](float m1, float l1, const f32x4& x) {  // one more share; a refused one's maximum is NaN
-      const float mn = M != M || m1 != m1 ? __builtin_nanf("") : fmaxf(M, m1), mz = finite_or_zero(mn);
-      const float w0 = __builtin_amdgcn_exp2f(M - mz), w1 = __builtin_amdgcn_exp2f(m1 - mz);
-      L = __builtin_fmaf(w1, l1, L * w0);
+  Share x;
+  if (run < runs) {
+    for (int p0 = run; p0 < it.parts; p0 += runs * 8) {
+      f32x4 t[8];
+      f32x2 ml[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(w1, x[e], t[e] * w0);
-      M = mn;
-    };
-    if (on) {
-      for (int p0 = run; p0 < it.parts; p0 += runs * 8) {
-        f32x4 x[8];
-        f32x2 ml[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t at = (uint32_t)(min(p0 + k * runs, it.parts - 1) * stride) * 4u;
-          x[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, at + (uint32_t)i * 16u, 0,
-                                                                                 kPagedCoherentAux));
-          ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(
-              rp, at + (uint32_t)quads * 16u + (uint32_t)hd * 8u, 0, kPagedCoherentAux));
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (p0 + k * runs < it.parts) add(ml[k][0], ml[k][1], x[k]);
+      for (int k = 0; k < 8; ++k) {
+        const int p = min(p0 + k * runs, it.parts - 1);
+        t[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (uint32_t)(p * stride + i * 4) * 4u,
+                                                                               0, kPagedCoherentAux));
+        ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, (uint32_t)(p * 16 + hd) * 8u, 0,
+                                                                               kPagedCoherentAux));
       }
-    }
-    if (runs > 1) {
-      if (on) red[tid] = t, red_ml[tid] = f32x2{M, L};
-      __syncthreads();
-      if (run == 0 && on)
-        for (int r = 1; r < runs; ++r) add(red_ml[r * quads + i][0], red_ml[r * quads + i][1], red[r * quads + i]);
-    }
-    if (on && run == 0) {
-      const float inv = 1.f / L;
-      u32x2 r;
-      r[0] = (uint32_t)float_to_act_bits<DT>(t[0] * inv) | ((uint32_t)float_to_act_bits<DT>(t[1] * inv) << 16);
-      r[1] = (uint32_t)float_to_act_bits<DT>(t[2] * inv) | ((uint32_t)float_to_act_bits<DT>(t[3] * inv) << 16);
-      *reinterpret_cast<u32x2*>(out + i * 4) = r;
-      if (a.scores && i % (D / 4) == 0) {
-        a.stats[((int64_t)b * nh + h0 + hd) * 2] = finite_or_zero(M);
-        a.stats[((int64_t)b * nh + h0 + hd) * 2 + 1] = L;
-      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (p0 + k * runs < it.parts) x.add(ml[k][0], ml[k][1], t[k]);
     }
   }
+  if (runs > 1) {
+    if (run < runs) red[tid] = x.t, red_ml[tid] = f32x2{x.M, x.L};
+    __syncthreads();
+    if (run == 0)
+      for (int r = 1; r < runs; ++r) x.add(red_ml[r * quads + i][0], red_ml[r * quads + i][1], red[r * quads + i]);
+  }
+  if (run == 0) *reinterpret_cast<u32x2*>(out + i * 4) = x.template out<DT>();
 }
 
-// Adds every slot's probabilities to its weight, from the scores, maxima and sums that the attention left: the same
-// parts of the rows, four slots a thread.
-template <int UP>
-__global__ __launch_bounds__(kPagedThreads) void paged_weight_kernel(PagedAttnArgs a) {
+// What the attention leaves to a second launch.  Workgroups [0, rows * heads): the parts of one row and query head
+// joined (a wide group's by the last part alone would be one CU's traffic with memory).  The others add every
+// slot's probabilities to its weight, from the scores, maxima and sums: the parts of the rows again, four slots
+// a thread.
+template <int DT, int D>
+__global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnArgs a) {
+  constexpr int UP = 4096 / D, QUADS = D / 4, RUNS = kPagedThreads / QUADS;
+  __shared__ f32x4 red[kPagedThreads];
+  __shared__ f32x2 red_ml[kPagedThreads];
+  const int tid = threadIdx.x, nh = a.c.nkv * a.g;
+  auto parts_of = [&](int b, int h, int g) { return a.first + ((b * a.c.nkv + h) * a.htiles + g / 16) * 2; };
+  if (blockIdx.x < (unsigned)(a.c.rows * nh)) {
+    const int b = blockIdx.x / nh, head = blockIdx.x - b * nh, h = head / a.g, g = head - h * a.g;
+    const int* const f = parts_of(b, h, g);
+    const int first = f[0], parts = f[1];
+    if (parts == 1) return;
+    const int stride = min(a.g, 16) * D, run = tid / QUADS, i = tid % QUADS;
+    const float* const part = a.part + (int64_t)first * stride + (g & 15) * D + i * 4;
+    const float* const st = a.stats + ((int64_t)first * 16 + (g & 15)) * 2;
+    Share x;
+    for (int p0 = run; p0 < parts; p0 += RUNS * 4) {
+      f32x4 t[4];
+      f32x2 ml[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t p = min(p0 + k * RUNS, parts - 1);
+        t[k] = *reinterpret_cast<const f32x4*>(part + p * stride);
+        ml[k] = *reinterpret_cast<const f32x2*>(st + p * 32);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (p0 + k * RUNS < parts) x.add(ml[k][0], ml[k][1], t[k]);
+    }
+    red[tid] = x.t;
+    red_ml[tid] = f32x2{x.M, x.L};
+    __syncthreads();
+    if (run > 0) return;
+    for (int r = 1; r < min(RUNS, parts); ++r)
+      x.add(red_ml[r * QUADS + i][0], red_ml[r * QUADS + i][1], red[r * QUADS + i]);
+    *reinterpret_cast<u32x2*>(a.out + ((int64_t)b * nh + head) * D + i * 4) = x.template out<DT>();
+    return;
+  }
   AttnItem it;
-  if (!find_item<UP>(a.c, a.lengths, a.positions, a.c.nkv, blockIdx.x, &it)) return;
-  const int b = it.b, h = it.tile, len = it.len, pos = it.pos, nh = a.c.nkv * a.g;
+  if (!find_item<UP>(a.c, a.lengths, a.positions, a.c.nkv, blockIdx.x - a.c.rows * nh, &it)) return;
+  const int b = it.b, h = it.tile, len = it.len, pos = it.pos;
   if (len < 0 || len >= a.c.capacity() || (uint64_t)(int64_t)pos >= (uint64_t)a.angles) return;
-  const float* const st = a.stats + ((int64_t)b * nh + h * a.g) * 2;
-  if (st[0] != st[0]) return;  // a page outside the pool
   const int nu = len / UP + 1;
   const int s0 = (int)((int64_t)it.part * nu / it.parts) * UP;
   const int s1 = min((int)((int64_t)(it.part + 1) * nu / it.parts) * UP, len + 1);
   const int64_t cap = a.c.capacity();
-  for (int s = s0 + 4 * threadIdx.x; s < s1; s += 4 * kPagedThreads) {
-    float* const wp = a.c.weight + a.c.token(b, s, h);
-    f32x4 w = *reinterpret_cast<const f32x4*>(wp);
+  // the heads' maxima and sums: several threads a head, each some of its parts
+  const int runs = kPagedThreads / a.g, run = tid / a.g, g = tid - run * a.g;
+  const int* const f = parts_of(b, h, g);
+  const int parts = f[1];  // (the same for all tiles of a row)
+  Share x;
+  if (run < runs) {
+    const float* const st = a.stats + ((int64_t)f[0] * 16 + (g & 15)) * 2;
+    for (int p = run; p < parts; p += runs) x.add(st[p * 32], st[p * 32 + 1], f32x4{0.f, 0.f, 0.f, 0.f});
+    red_ml[tid] = f32x2{x.M, x.L};
+  }
+  __syncthreads();
+  if (run == 0) {
+    for (int r = 1; r < min(runs, parts); ++r)
+      x.add(red_ml[r * a.g + g][0], red_ml[r * a.g + g][1], f32x4{0.f, 0.f, 0.f, 0.f});
+    red[g] = f32x4{finite_or_zero(x.M), 1.f / x.L, 0.f, 0.f};
+  }
+  __syncthreads();
+  if (red[0][0] != red[0][0]) return;  // a page outside the pool (in all heads alike)
+  for (int s = s0 + 4 * tid; s < s1; s += 4 * kPagedThreads) {
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
     const float* sp = a.scores + ((int64_t)b * nh + h * a.g) * cap + s;
-    for (int g = 0; g < a.g; ++g) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(sp + g * cap);
-      const float M = st[2 * g], inv = 1.f / st[2 * g + 1];
+    for (int e0 = 0; e0 < a.g; ++e0) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(sp + e0 * cap);
+      const float M = red[e0][0], inv = red[e0][1];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], kLog2e, -M)) * inv;
+      for (int e = 0; e < 4; ++e) t[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(y[e], kLog2e, -M)) * inv;
     }
+    float* const wp = a.c.weight + a.c.token(b, s, h);
+    f32x4 w = *reinterpret_cast<const f32x4*>(wp);
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = s + e < len ? w[e] + t[e] : s + e == len ? t[e] : w[e];
     *reinterpret_cast<f32x4*>(wp) = w;
@@ -754,9 +794,11 @@ extern "C" int w4_paged_append(const w4_paged_cache* cache, int dtype, const voi
 
 namespace {
 
+constexpr int kLaterFloats = 1024;
+
 struct PagedAttnPlan {
-  int64_t tiles, items, part_stride;  // tiles of up to 16 query heads a row, workgroups, floats of a part
-  size_t part_bytes, bytes;           // the parts' share of the workspace, and all of it
+  int64_t tiles, items;         // tiles of up to 16 query heads a row, workgroups
+  size_t part, first, bytes;    // offsets of PagedAttnArgs' part and first in the workspace, and all of it
 };
 
 bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, PagedAttnPlan* p) {
@@ -764,16 +806,22 @@ bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t 
   const int64_t g = num_heads / kv_heads;
   p->tiles = kv_heads * ((g + 15) / 16);
   p->items = w4::kAttnItems + rows * p->tiles + 1;
-  p->part_stride = (g < 16 ? g : 16) * (head_dim + 2) + 3 & ~int64_t(3);
-  const bool split = rows * p->tiles <= w4::kPagedCounters;
-  p->part_bytes = split ? (size_t)(p->items * p->part_stride) * 4 : 0;
-  p->bytes = W4_WORKSPACE_COUNTER_BYTES + p->part_bytes + (size_t)(rows * num_heads) * 8;
+  if (p->items >= (1 << 22)) return false;
+  p->part = W4_WORKSPACE_COUNTER_BYTES + (size_t)p->items * 128;
+  p->first = p->part;
+  if (rows * p->tiles <= w4::kPagedCounters) p->first += (size_t)(p->items * (g < 16 ? g : 16) * head_dim) * 4;
+  p->bytes = p->first + (size_t)(rows * p->tiles) * 8;
   return true;
 }
 
 template <int DT, int D>
-void launch_paged_attention(const w4::PagedAttnArgs& a, int64_t items, hipStream_t st) {
+int launch_paged_attention(const w4::PagedAttnArgs& a, int64_t items, hipStream_t st) {
   w4::paged_attention_kernel<DT, D><<<dim3((unsigned)items), 64 * w4::kAttnWaves, 0, st>>>(a);
+  if (const int rc = check_launch("w4_paged_attention")) return rc;
+  if (!a.later) return W4_OK;
+  const int64_t more = a.scores ? w4::kAttnItems + (int64_t)a.c.rows * a.c.nkv + 1 : 0;
+  w4::paged_finish_kernel<DT, D><<<dim3((unsigned)((int64_t)a.c.rows * a.c.nkv * a.g + more)), w4::kPagedThreads, 0, st>>>(a);
+  return check_launch("w4_paged_attention (finish)");
 }
 
 }  // namespace
@@ -791,14 +839,13 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
                                   size_t workspace_bytes, void* stream) {
   clear_error();
   if (const int rc = check_cache(cache, dtype, "w4_paged_attention")) return rc;
-  if (num_heads < 1 || num_heads % cache->kv_heads || num_heads / cache->kv_heads > 1024 || angles < 1)
+  if (num_heads < 1 || num_heads % cache->kv_heads || num_heads / cache->kv_heads > 256 || angles < 1)
     return fail(W4_ERR_INVALID, "w4_paged_attention: %lld query heads on %lld key-value heads, %lld angles",
                 (long long)num_heads, (long long)cache->kv_heads, (long long)angles);
   if (cache->rows == 0) return W4_OK;
   PagedAttnPlan p;
-  paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, &p);
-  // a launch of 2^32 threads, or more, is refused by HIP
-  if (p.items > 0xFFFFFFFFll / (64 * w4::kAttnWaves))
+  if (!paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, &p) ||
+      cache->rows * num_heads >= (1 << 23))
     return fail(W4_ERR_UNSUPPORTED, "w4_paged_attention: %lld rows of %lld heads", (long long)cache->rows,
                 (long long)num_heads);
   if (!q || !k || !v || !lengths || !positions || !cos || !sin || !out || (cache->weight && !scores))
@@ -820,26 +867,21 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   a.scores = cache->weight ? scores : nullptr;
   char* const ws = static_cast<char*>(workspace);
   a.cnt = reinterpret_cast<unsigned*>(ws);
-  a.part = reinterpret_cast<float*>(ws + W4_WORKSPACE_COUNTER_BYTES);
-  a.stats = reinterpret_cast<float*>(ws + W4_WORKSPACE_COUNTER_BYTES + p.part_bytes);
+  a.stats = reinterpret_cast<float*>(ws + W4_WORKSPACE_COUNTER_BYTES);
+  a.part = reinterpret_cast<float*>(ws + p.part);
+  a.first = reinterpret_cast<int*>(ws + p.first);
   a.scale = 1.f / sqrtf((float)cache->head_dim);
   a.g = (int)(num_heads / cache->kv_heads);
   a.htiles = (int)(p.tiles / cache->kv_heads);
-  a.part_stride = (int)p.part_stride;
+  // The weights need a launch behind the attention anyway; without them the last part joins, unless
+  // a tile's outputs are more than one quad a thread.
+  a.later = a.scores || (a.g < 16 ? a.g : 16) * cache->head_dim > kLaterFloats;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == W4_DTYPE_BF16) {
-    if (cache->head_dim == 64) launch_paged_attention<W4_DTYPE_BF16, 64>(a, p.items, st);
-    else launch_paged_attention<W4_DTYPE_BF16, 128>(a, p.items, st);
-  } else {
-    if (cache->head_dim == 64) launch_paged_attention<W4_DTYPE_FP16, 64>(a, p.items, st);
-    else launch_paged_attention<W4_DTYPE_FP16, 128>(a, p.items, st);
-  }
-  if (const int rc = check_launch("w4_paged_attention")) return rc;
-  if (!cache->weight) return W4_OK;
-  const dim3 grid((unsigned)(w4::kAttnItems + cache->rows * cache->kv_heads + 1));
-  if (cache->head_dim == 64) w4::paged_weight_kernel<64><<<grid, w4::kPagedThreads, 0, st>>>(a);
-  else w4::paged_weight_kernel<32><<<grid, w4::kPagedThreads, 0, st>>>(a);
-  return check_launch("w4_paged_attention (weights)");
+  if (dtype == W4_DTYPE_BF16)
+    return cache->head_dim == 64 ? launch_paged_attention<W4_DTYPE_BF16, 64>(a, p.items, st)
+                                 : launch_paged_attention<W4_DTYPE_BF16, 128>(a, p.items, st);
+  return cache->head_dim == 64 ? launch_paged_attention<W4_DTYPE_FP16, 64>(a, p.items, st)
+                               : launch_paged_attention<W4_DTYPE_FP16, 128>(a, p.items, st);
 }
 
 extern "C" int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int32_t* lengths,
