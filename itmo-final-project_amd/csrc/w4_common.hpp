@@ -106,6 +106,17 @@ __device__ __forceinline__ float wave_sum(float v) {
   return (lane_read(v, 0) + lane_read(v, 16)) + (lane_read(v, 32) + lane_read(v, 48));
 }
 
+// Inclusive sum over the lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // shifted right by 1, 2, 4, 8 in rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // rows 1, 3 take the last lane before them
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // rows 2, 3 take lane 31
+  return v;
+}
+
 // A key whose unsigned order is the order of the values, equal zeros equal, NaN above all.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.f);

@@ -8,14 +8,37 @@ namespace w4 {
 
 constexpr int kLogThreads = 256;
 constexpr int kMaxTop = 64;
+constexpr int kLogBlock = 8192;                 // logits a workgroup reads in a step: 32 a thread
+constexpr int kLogGroups = kLogBlock / 128;     // groups of 128 logits in it, a quad of lanes each
+constexpr int kLogMaxGroups = 192;              // groups that may hold alternatives: under 2 top + kLogGroups
+constexpr int kLogSpare = 16;                   // groups too many, before the range of their maxima is narrowed again
+constexpr int kLogList = 512;
+constexpr int kLogBins = 2048;
+constexpr int64_t kLogMaxVocab = 1 << 22;
+constexpr int kLogBufFlags = 0x00020000;        // raw buffer: the range is checked in bytes
+constexpr int kLogCoherentAux = 16;             // sc1: the cache policy of agent-scope atomic loads and stores
 
 struct LogprobArgs {
   const void* x;
   const int64_t* tokens;
   float *logprob, *entropy, *top_logprob;
   int64_t* top_token;
-  int64_t vocab, stride;
-  int top;
+  unsigned* cnt;     // one arrival counter a row
+  uint32_t* scratch; // of a row: (maximum, sum, weighted sum, -) of every part, then the keys of its groups' maxima
+  int64_t stride;
+  int vocab, top, parts, blocks, row_words;
+};
+
+template <int DT> struct Logits {  // 16 bytes of them
+  static constexpr int N = 8;
+  typedef uint16_t scalar;
+  // (rows need not start on 16 bytes: a vocabulary may be odd)
+  typedef u32x4 vec __attribute__((aligned(2)));
+};
+template <> struct Logits<W4_DTYPE_FP32> {
+  static constexpr int N = 4;
+  typedef float scalar;
+  typedef u32x4 vec __attribute__((aligned(4)));
 };
 
 template <int DT>
@@ -24,60 +47,292 @@ __device__ __forceinline__ float logit_at(const void* x, int64_t i) {
   else return act_bits_to_float(static_cast<const uint16_t*>(x)[i], DT);
 }
 
-// One workgroup a row: the maximum, the sums, then the alternatives one after the
-// other, each the largest (key, lowest index) below the one before.
+// Sum of e^(x - m) and of e^(x - m) (x - m) over some logits.  The reference m starts at the lowest finite number, so
+// that rows of -inf meet no difference of infinities.
+struct LogSum {
+  float m = -3.402823466e38f, s = 0.f, t = 0.f;
+  __device__ __forceinline__ void rebase(float to) {  // to >= m
+    const float d = m - to, f = __builtin_amdgcn_exp2f(d * kLog2e);
+    // (a distance beyond all exponents: nothing is left of the sums, whatever the product)
+    t = s == 0.f ? t * f : f * __builtin_fmaf(fmaxf(d, -1e4f), s, t);
+    s *= f;
+    m = to;
+  }
+  __device__ __forceinline__ void add(float m1, float s1, float t1) {
+    LogSum o;
+    o.m = m1, o.s = s1, o.t = t1;
+    const float to = fmaxf(m, m1);
+    rebase(to), o.rebase(to);
+    s += o.s, t += o.t;
+  }
+};
+
+// Values of `each` between lo and hi (those above are kept, `wanted` of the `count` between are), narrowed eleven bits
+// at a time until no more than `stop` are left or lo == hi; the number above grows with them.
+template <typename Each>
+__device__ __forceinline__ void narrow(const Each& each, uint64_t& lo, uint64_t& hi, int& wanted, int& above,
+                                       int& count, int stop, int* hist, int* wave_s, int* found_s) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  constexpr int PER = kLogBins / kLogThreads;
+  while (count > stop && lo < hi) {
+    const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);
+    for (int i = tid; i < kLogBins; i += kLogThreads) hist[i] = 0;
+    __syncthreads();
+    each([&](uint64_t v) {
+      if (v >= lo && v <= hi) atomicAdd(&hist[(int)((v - lo) >> shift)], 1);
+    });
+    __syncthreads();
+    const int top = kLogBins - PER - PER * tid;  // from the top
+    int mine = 0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) mine += hist[top + e];
+    const int upto = wave_scan(mine);
+    if (lane == 63) wave_s[wv] = upto;
+    __syncthreads();
+    int over = upto - mine;
+    for (int w = 0; w < wv; ++w) over += wave_s[w];
+    if (over < wanted && over + mine >= wanted) {
+      int e = PER - 1;
+      while (over + hist[top + e] < wanted) over += hist[top + e--];
+      found_s[0] = top + e;
+      found_s[1] = over;
+      found_s[2] = hist[top + e];
+    }
+    __syncthreads();
+    lo += (uint64_t)found_s[0] << shift;
+    const uint64_t end = lo + ((1ull << shift) - 1ull);
+    hi = end < hi ? end : hi;
+    wanted -= found_s[1];
+    above += found_s[1];
+    count = found_s[2];
+  }
+}
+
+// One workgroup = one row and part of its blocks.  Everything of a logit is done when it is read: the sums of the softmax and
+// the entropy, relative to the lane's own maximum so far, and the maximum of its group of 128.  The last part of a row
+// to arrive joins the sums, in their order, and finds the alternatives: as many groups reach the top-th largest of the
+// groups' maxima as there are alternatives (or more, where they are equal), and no alternative lies outside of
+// them, so only those groups' logits are read again.
 template <int DT>
 __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
+  typedef Logits<DT> T;
+  constexpr int NV = 32 / T::N, PIECE = 64 * T::N;  // loads of a thread in a block, logits of a wave's load
+  __shared__ f32x4 sum_s[kLogThreads / 64];
+  __shared__ int hist[kLogBins];
+  __shared__ __attribute__((aligned(16))) uint64_t list[kLogList];
+  __shared__ int groups_s[kLogMaxGroups + kLogGroups];
+  __shared__ int wave_s[kLogThreads / 64], found_s[3];
+  __shared__ unsigned arrived_s;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int64_t row = blockIdx.x, base = row * a.stride;
-  __shared__ float red[4], red2[4];
-  __shared__ uint64_t best_s[4];
-  float m = -__builtin_inff();
-  for (int64_t i = tid; i < a.vocab; i += kLogThreads) m = fmaxf(m, logit_at<DT>(a.x, base + i));
-  m = wave_max(m);
-  if (lane == 0) red[wv] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  __syncthreads();
-  float s = 0.f, t = 0.f;
-  for (int64_t i = tid; i < a.vocab; i += kLogThreads) {
-    const float y = logit_at<DT>(a.x, base + i) - m, e = expf(y);
-    s += e;
-    t += y == -__builtin_inff() ? 0.f : e * y;
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  const int b0 = (int)((int64_t)part * a.blocks / a.parts), b1 = (int)((int64_t)(part + 1) * a.blocks / a.parts);
+  const typename T::scalar* const x = static_cast<const typename T::scalar*>(a.x) + row * a.stride;
+  uint32_t* const scratch = a.scratch + (int64_t)row * a.row_words;
+  const __amdgpu_buffer_rsrc_t rp =
+      __builtin_amdgcn_make_buffer_rsrc((void*)scratch, (short)0, a.row_words * 4, kLogBufFlags);
+
+  u32x4 raw[NV];
+  auto load = [&](int blk) {
+    const int i0 = blk * kLogBlock + wv * 2048 + lane * T::N;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = i0 + j * PIECE;
+      if (i + T::N <= a.vocab) {
+        raw[j] = *reinterpret_cast<const typename T::vec*>(x + i);
+      } else {  // past the row: -inf
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (DT == W4_DTYPE_FP32) {
+            w[e] = i + e < a.vocab ? __builtin_bit_cast(uint32_t, x[i + e]) : 0xFF800000u;
+          } else {
+            const uint32_t none = DT == W4_DTYPE_BF16 ? 0xFF80u : 0xFC00u;
+            const uint32_t l = i + 2 * e < a.vocab ? x[i + 2 * e] : none;
+            const uint32_t h = i + 2 * e + 1 < a.vocab ? x[i + 2 * e + 1] : none;
+            w[e] = l | h << 16;
+          }
+        }
+        raw[j] = u32x4{w[0], w[1], w[2], w[3]};
+      }
+    }
+  };
+  LogSum sum;
+  load(b0);
+  for (int blk = b0; blk < b1; ++blk) {
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if constexpr (DT == W4_DTYPE_FP32) {
+        const f32x4 f = __builtin_bit_cast(f32x4, raw[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * j + e] = f[e];
+      } else {
+        unpack8<DT>(raw[j], v + 8 * j);
+      }
+    }
+    if (blk + 1 < b1) load(blk + 1);  // on its way under this one's arithmetic
+    float top = v[0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) top = fmaxf(top, v[e]);
+    sum.rebase(fmaxf(sum.m, top));
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const float y = v[e] - sum.m, p = __builtin_amdgcn_exp2f(y * kLog2e);
+      s += p;
+      t = __builtin_fmaf(p, fmaxf(y, -1e4f), t);  // p = 0 counts nothing, at -inf too
+    }
+    sum.s += s;
+    sum.t += t;
+    if (a.top) {
+      if (__ballot(s != s)) {  // a NaN (or a +inf) among them: NaN is above every number
+#pragma unroll
+        for (int e = 0; e < 32; ++e) top = v[e] != v[e] ? v[e] : top;
+      }
+      uint32_t key = order_key(top);
+      key = max(key, dpp_mov<0xB1>(key));  // lane ^ 1
+      key = max(key, dpp_mov<0x4E>(key));  // lane ^ 2
+      if ((lane & 3) == 0)
+        __builtin_amdgcn_raw_buffer_store_b32(
+            key, rp, (uint32_t)(a.parts * 4 + blk * kLogGroups + wv * 16 + lane / 4) * 4u, 0, kLogCoherentAux);
+    }
   }
-  s = wave_sum(s), t = wave_sum(t);
-  if (lane == 0) red[wv] = s, red2[wv] = t;
+  {
+    LogSum w = sum;
+    w.rebase(wave_max(sum.m));
+    w.s = wave_sum(w.s), w.t = wave_sum(w.t);
+    if (lane == 0) sum_s[wv] = f32x4{w.m, w.s, w.t, 0.f};
+  }
   __syncthreads();
-  s = (red[0] + red[1]) + (red[2] + red[3]);
-  t = (red2[0] + red2[1]) + (red2[2] + red2[3]);
-  const float ls = logf(s);
+  sum = LogSum();
+  for (int w = 0; w < kLogThreads / 64; ++w) sum.add(sum_s[w][0], sum_s[w][1], sum_s[w][2]);
+  if (a.parts > 1) {
+    if (tid == 0)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{sum.m, sum.s, sum.t, 0.f}), rp,
+                                             (uint32_t)part * 16u, 0, kLogCoherentAux);
+    __builtin_amdgcn_s_waitcnt(0);  // the stores have reached the level all XCDs share
+    __syncthreads();
+    if (tid == 0) arrived_s = __hip_atomic_fetch_add(a.cnt + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived_s != (unsigned)(a.parts - 1)) return;
+    if (tid == 0) __hip_atomic_store(a.cnt + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sum = LogSum();
+    for (int p = 0; p < a.parts; ++p) {
+      const f32x4 o = __builtin_bit_cast(
+          f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (uint32_t)p * 16u, 0, kLogCoherentAux));
+      sum.add(o[0], o[1], o[2]);
+    }
+  } else {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+  const float logz = logf(sum.s);
   if (tid == 0) {
-    a.entropy[row] = ls - t / s;
+    a.entropy[row] = logz - sum.t / sum.s;
     if (a.tokens) {
       const int64_t tok = a.tokens[row];
-      a.logprob[row] = (uint64_t)tok < (uint64_t)a.vocab ? (logit_at<DT>(a.x, base + tok) - m) - ls : __builtin_nanf("");
+      a.logprob[row] =
+          (uint64_t)tok < (uint64_t)a.vocab ? (logit_at<DT>(x, tok) - sum.m) - logz : __builtin_nanf("");
     }
   }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < a.top; ++k) {
-    uint64_t best = 0;
-    for (int64_t i = tid; i < a.vocab; i += kLogThreads) {
-      const uint64_t key = ((uint64_t)order_key(logit_at<DT>(a.x, base + i)) << 32) | (uint32_t)(~(uint32_t)i);
-      if (key < last && key > best) best = key;
+  if (a.top == 0) return;
+
+  // The groups that may hold alternatives.
+  const int groups = a.blocks * kLogGroups;
+  auto group_key = [&](int g) {
+    return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rp, (uint32_t)(a.parts * 4 + g) * 4u, 0, kLogCoherentAux);
+  };
+  uint64_t lo = 0, hi = 0xFFFFFFFFull;
+  int wanted = min(a.top, groups), above = 0, count = groups;
+  narrow([&](auto f) {
+    for (int g = tid; g < groups; g += 4 * kLogThreads) {
+      uint32_t k[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = group_key(min(g + i * kLogThreads, groups - 1));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (g + i * kLogThreads < groups) f((uint64_t)k[i]);
     }
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint64_t o = __shfl_xor((unsigned long long)best, d);
-      best = o > best ? o : best;
+  }, lo, hi, wanted, above, count, kLogSpare, hist, wave_s, found_s);
+  // More equal maxima than fit: those of the first blocks, until there is one for every alternative (a block is a
+  // run of logits, so its equal logits come before all later ones).
+  const bool few = above + count <= kLogMaxGroups;
+  int equal = 0, held = 0;
+  for (int g0 = 0; g0 < groups; g0 += kLogThreads) {
+    const int g = g0 + tid;
+    const uint32_t k = g < groups ? group_key(g) : 0u;
+    const bool same = g < groups && k == lo && !few;
+    const uint64_t m_same = __ballot(same);
+    __syncthreads();
+    if (lane == 0) wave_s[wv] = __popcll(m_same);
+    __syncthreads();
+    int before = equal;  // of the blocks in front (a wave has one block)
+    for (int w = 0; w < kLogThreads / 64; ++w) {
+      before += w < wv ? wave_s[w] : 0;
+      equal += wave_s[w];
     }
+    const bool take = g < groups && (few ? k >= lo : k > lo || (same && before < a.top));
+    const uint64_t m_take = __ballot(take);
     __syncthreads();
-    if (lane == 0) best_s[wv] = best;
+    if (lane == 0) wave_s[wv] = __popcll(m_take);
     __syncthreads();
-    for (int w = 0; w < 4; ++w) best = best_s[w] > best ? best_s[w] : best;
-    last = best;
-    if (tid == 0) {
-      const int64_t tok = (int64_t)(uint32_t)~(uint32_t)best;
-      a.top_token[row * a.top + k] = tok;
-      a.top_logprob[row * a.top + k] = (logit_at<DT>(a.x, base + tok) - m) - ls;
+    int at = held + __popcll(m_take & ((1ull << lane) - 1));
+    for (int w = 0; w < kLogThreads / 64; ++w) {
+      at += w < wv ? wave_s[w] : 0;
+      held += wave_s[w];
+    }
+    if (take) groups_s[at] = g;
+  }
+  __syncthreads();
+
+  // Their logits: (key, lower index first) in one number.
+  auto members = [&](auto f) {
+    for (int i = tid >> 7; i < held; i += 8) {
+      uint64_t k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int g = groups_s[min(i + 2 * u, held - 1)], e = tid & 127;
+        const int at = (g / kLogGroups) * kLogBlock + (g / 16 % 4) * 2048 + e / (4 * T::N) * PIECE + g % 16 * (4 * T::N) +
+                       e % (4 * T::N);
+        k[u] = at < a.vocab ? (uint64_t)order_key(logit_at<DT>(x, at)) << 32 | (uint32_t)~at : 0ull;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + 2 * u < held) f(k[u]);
+    }
+  };
+  uint64_t from = lo << 32;
+  auto collect = [&] {
+    if (tid == 0) found_s[0] = 0;
+    __syncthreads();
+    members([&](uint64_t v) {
+      if (v >= from && v != 0) {
+        const int at = atomicAdd(&found_s[0], 1);
+        if (at < kLogList) list[at] = v;
+      }
+    });
+    __syncthreads();
+    return found_s[0];
+  };
+  int n = collect();
+  if (n > kLogList) {  // many equal or neighbouring logits: up to the threshold among the members themselves
+    uint64_t to = ~0ull;
+    int want = a.top, over = 0;
+    __syncthreads();
+    narrow(members, from, to, want, over, n, kLogList - kMaxTop, hist, wave_s, found_s);
+    __syncthreads();
+    n = collect();
+  }
+  for (int i = tid; i < n; i += kLogThreads) {
+    const uint64_t v = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > v;
+    if (rank < a.top) {
+      const uint32_t key = (uint32_t)(v >> 32);
+      const float l = key == 0xFFFFFFFFu ? __builtin_nanf("")
+                                         : __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
+      a.top_token[(int64_t)row * a.top + rank] = (int64_t)(uint32_t)~(uint32_t)v;
+      a.top_logprob[(int64_t)row * a.top + rank] = (l - sum.m) - logz;
     }
   }
 }
@@ -87,9 +342,35 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
 // ---------------------------------------------------------------- host side
 using namespace w4host;
 
+namespace {
+
+struct LogprobPlan {
+  int blocks, parts;
+  int64_t row_words, slice;  // words of scratch a row, rows of a launch
+};
+
+// A row is cut into parts of whole blocks while the launch has fewer than eight workgroups a CU.
+LogprobPlan logprob_plan(int64_t rows, int64_t vocab) {
+  LogprobPlan p;
+  p.blocks = (int)((vocab + w4::kLogBlock - 1) / w4::kLogBlock);
+  const int64_t most = 8 * device_cu_count();
+  p.parts = (int)(rows >= most ? 1 : most / rows < p.blocks ? most / rows : p.blocks);
+  p.row_words = p.parts * 4 + (int64_t)p.blocks * w4::kLogGroups;
+  // arrival counters, and no more than 64 MiB of scratch
+  p.slice = W4_WORKSPACE_COUNTER_BYTES / 4;
+  const int64_t fit = (64 << 20) / (p.row_words * 4);
+  if (p.slice > fit) p.slice = fit;
+  if (p.slice > rows) p.slice = rows;
+  return p;
+}
+
+}  // namespace
+
 extern "C" size_t w4_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top) {
-  (void)rows, (void)vocab, (void)top;
-  return 0;
+  (void)top;
+  if (rows < 1 || vocab < 1 || vocab > w4::kLogMaxVocab) return 0;
+  const LogprobPlan p = logprob_plan(rows, vocab);
+  return W4_WORKSPACE_COUNTER_BYTES + (size_t)(p.slice * p.row_words) * 4;
 }
 
 extern "C" int w4_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
@@ -97,21 +378,47 @@ extern "C" int w4_token_logprobs(const void* logits, int dtype, int64_t rows, in
                                  float* top_logprob, int64_t* top_token, void* workspace, size_t workspace_bytes,
                                  void* stream) {
   clear_error();
-  (void)workspace, (void)workspace_bytes;
   if (dtype != W4_DTYPE_BF16 && dtype != W4_DTYPE_FP16 && dtype != W4_DTYPE_FP32)
     return fail(W4_ERR_INVALID, "w4_token_logprobs: dtype must be bf16, fp16 or fp32 (got code %d)", dtype);
   if (rows < 0 || vocab < 1 || vocab >= (1ll << 31) || stride < 0 || top < 0 || top > w4::kMaxTop || top > vocab)
     return fail(W4_ERR_INVALID, "w4_token_logprobs: %lld rows of %lld logits, the top %lld (at most %d)",
                 (long long)rows, (long long)vocab, (long long)top, w4::kMaxTop);
-  if (rows >= (1ll << 24)) return fail(W4_ERR_UNSUPPORTED, "w4_token_logprobs: %lld rows", (long long)rows);
+  if (rows >= (1ll << 24) || vocab > w4::kLogMaxVocab)
+    return fail(W4_ERR_UNSUPPORTED, "w4_token_logprobs: %lld rows of %lld logits", (long long)rows, (long long)vocab);
   if (rows == 0) return W4_OK;
   if (!logits || !entropy || (!tokens != !logprob) || (top && (!top_logprob || !top_token)))
     return fail(W4_ERR_INVALID, "w4_token_logprobs: null pointer");
-  w4::LogprobArgs a{logits, tokens, logprob, entropy, top_logprob, top_token, vocab, stride, (int)top};
+  if ((uintptr_t)logits % (dtype == W4_DTYPE_FP32 ? 4 : 2))
+    return fail(W4_ERR_INVALID, "w4_token_logprobs: logits must be aligned to their size");
+  const size_t need = w4_token_logprobs_workspace_bytes(rows, vocab, top);
+  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)
+    return fail(W4_ERR_WORKSPACE, "w4_token_logprobs: needs a 256-byte aligned workspace of %zu bytes (got %zu)", need,
+                workspace_bytes);
+  const LogprobPlan p = logprob_plan(rows, vocab);
+  const int64_t bytes = dtype == W4_DTYPE_FP32 ? 4 : 2;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)rows);
-  if (dtype == W4_DTYPE_BF16) w4::logprob_kernel<W4_DTYPE_BF16><<<grid, w4::kLogThreads, 0, st>>>(a);
-  else if (dtype == W4_DTYPE_FP16) w4::logprob_kernel<W4_DTYPE_FP16><<<grid, w4::kLogThreads, 0, st>>>(a);
-  else w4::logprob_kernel<W4_DTYPE_FP32><<<grid, w4::kLogThreads, 0, st>>>(a);
-  return check_launch("w4_token_logprobs");
+  for (int64_t r = 0; r < rows; r += p.slice) {
+    const int64_t n = rows - r < p.slice ? rows - r : p.slice;
+    w4::LogprobArgs a{};
+    a.x = static_cast<const char*>(logits) + r * stride * bytes;
+    a.tokens = tokens ? tokens + r : nullptr;
+    a.logprob = logprob ? logprob + r : nullptr;
+    a.entropy = entropy + r;
+    a.top_logprob = top_logprob ? top_logprob + r * top : nullptr;
+    a.top_token = top_token ? top_token + r * top : nullptr;
+    a.cnt = static_cast<unsigned*>(workspace);
+    a.scratch = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + W4_WORKSPACE_COUNTER_BYTES);
+    a.stride = stride;
+    a.vocab = (int)vocab;
+    a.top = (int)top;
+    a.parts = p.parts;
+    a.blocks = p.blocks;
+    a.row_words = (int)p.row_words;
+    const dim3 grid((unsigned)(n * p.parts));
+    if (dtype == W4_DTYPE_BF16) w4::logprob_kernel<W4_DTYPE_BF16><<<grid, w4::kLogThreads, 0, st>>>(a);
+    else if (dtype == W4_DTYPE_FP16) w4::logprob_kernel<W4_DTYPE_FP16><<<grid, w4::kLogThreads, 0, st>>>(a);
+    else w4::logprob_kernel<W4_DTYPE_FP32><<<grid, w4::kLogThreads, 0, st>>>(a);
+    if (const int rc = check_launch("w4_token_logprobs")) return rc;
+  }
+  return W4_OK;
 }

@@ -99,17 +99,6 @@ constexpr int kAttnItems = 256;     // parts the tokens of a batch are cut into,
 constexpr int kAttnMinUnits = 16;   // units of a part at least
 constexpr int kPagedCounters = W4_WORKSPACE_COUNTER_BYTES / 4;
 
-// Inclusive sum over the lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // shifted right by 1, 2, 4, 8 in rows of 16
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // rows 1, 3 take the last lane before them
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // rows 2, 3 take lane 31
-  return v;
-}
-
 // Which item this is, the same in every wave and launch.  The lengths lie on the GPU, so the split is made here:
 // every row is cut into equal parts of at most `per` units of UP slots, per = all units / kAttnItems, so that short
 // rows stay whole and long ones spread over the chip, whatever else is in the batch.  Rows that need no
@@ -635,82 +624,200 @@ struct EvictArgs {
   int new_width, keep, recent;
 };
 
-// One workgroup per row and key-value head finds the slots to keep: the key of the
-// last one by bisection, then its equals counted from the front.
-__global__ __launch_bounds__(kPagedThreads) void paged_select_kernel(EvictArgs a) {
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectBins = 4096;
+constexpr int kSelectList = 256;  // keys few enough to be ranked against each other
+
+// One workgroup per row and key-value head finds the slots to keep.  The key of the last one (its weight's place in
+// the order of all weights) lies in a range that a histogram of 4096 bins narrows twelve bits at a time until no more
+// than 256 keys are in it, which are then ranked one against all: at most three histograms, one as a rule.  A last
+// pass gives every kept slot its place, counting the larger keys and the equal ones in front of it.
+__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a) {
+  constexpr int WAVES = kSelectThreads / 64, STEP = 4 * kSelectThreads;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = blockIdx.x, b = blockIdx.y;
-  __shared__ int red[4];
+  __shared__ int hist[kSelectBins];
+  __shared__ __attribute__((aligned(16))) uint32_t list[kSelectList];
+  __shared__ int wave_s[WAVES], found_s[3];
+  __shared__ uint32_t edge_s;
   int n = a.lengths[b];
   if (n > a.c.capacity()) n = -1;
   if (h == 0 && tid == 0) a.new_lengths[b] = n < 0 ? -1 : min(n, a.keep);
-  if (n < 0) return;
+  if (n <= a.keep) return;  // idle, or all of it kept: the copy needs no list
   int32_t* const kept = a.kept + ((int64_t)b * a.c.nkv + h) * a.keep;
-  if (n <= a.keep) {
-    for (int j = tid; j < n; j += kPagedThreads) kept[j] = j;
-    return;
+  const int early = n - a.recent;
+  int want = a.keep - a.recent;
+  for (int j = tid; j < a.recent; j += kSelectThreads) kept[want + j] = early + j;
+  if (want == 0) return;
+  // f(slot, key) for every early slot, four slots in a row a thread, in the order of the threads
+  auto keys_of = [&](int s, uint32_t k[4]) {
+    const int64_t at = s < early ? a.c.token(b, s, h) : -1;  // (four slots never straddle a page)
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    if (at >= 0) w = *reinterpret_cast<const f32x4*>(a.c.weight + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) k[e] = at < 0 ? 0u : order_key(w[e]);
+  };
+
+  uint32_t lo = 0, hi = 0xFFFFFFFFu;
+  int count = early, wanted = want;  // keys in the range, and how many of them are kept
+  while (count > kSelectList && lo < hi) {
+    const int shift = max(0, 32 - __builtin_clz(hi - lo) - 12);
+    for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
+    __syncthreads();
+    for (int s0 = 4 * tid; s0 < early; s0 += 2 * STEP) {
+      uint32_t k[2][4];
+      keys_of(s0, k[0]);
+      keys_of(s0 + STEP, k[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (s0 + i * STEP + e < early && k[i][e] >= lo && k[i][e] <= hi) atomicAdd(&hist[(k[i][e] - lo) >> shift], 1);
+    }
+    __syncthreads();
+    // from the top: thread t has the bins 4 (1023 - t)..
+    const int top = kSelectBins - 4 - 4 * tid;
+    const int mine = hist[top] + hist[top + 1] + hist[top + 2] + hist[top + 3];
+    const int upto = wave_scan(mine);
+    if (lane == 63) wave_s[wv] = upto;
+    __syncthreads();
+    int above = upto - mine;
+    for (int w = 0; w < wv; ++w) above += wave_s[w];
+    if (above < wanted && above + mine >= wanted) {
+      int e = 3;
+      while (above + hist[top + e] < wanted) above += hist[top + e--];
+      found_s[0] = top + e;
+      found_s[1] = above;
+      found_s[2] = hist[top + e];
+    }
+    __syncthreads();
+    lo += (uint32_t)found_s[0] << shift;
+    hi = min(hi, lo + ((1u << shift) - 1u));
+    wanted -= found_s[1];
+    count = found_s[2];
   }
-  const int early = n - a.recent, want = a.keep - a.recent;
-  auto key = [&](int j) {
-    const int64_t at = a.c.token(b, j, h);
-    return at < 0 ? 0u : order_key(a.c.weight[at]);
-  };
-  auto total = [&](int x) {  // of the workgroup
-    for (int s = 1; s < 64; s <<= 1) x += __shfl_xor(x, s);
+  uint32_t edge = lo;
+  if (lo < hi) {
     __syncthreads();
-    if (lane == 0) red[wv] = x;
+    if (tid == 0) found_s[0] = 0;
+    if (tid < kSelectList) list[tid] = 0;
     __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
-  };
-  uint32_t edge = 0;  // the largest key that at least `want` slots reach
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t t = edge | (1u << bit);
+    for (int s0 = 4 * tid; s0 < early; s0 += 2 * STEP) {
+      uint32_t k[2][4];
+      keys_of(s0, k[0]);
+      keys_of(s0 + STEP, k[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (s0 + i * STEP + e < early && k[i][e] >= lo && k[i][e] <= hi) {
+            const int at = atomicAdd(&found_s[0], 1);
+            if (at < kSelectList) list[at] = k[i][e];  // (weights that change under the call stay in bounds)
+          }
+    }
+    __syncthreads();
+    if (tid < count) {
+      const uint32_t k = list[tid];
+      int more = 0, same = 0;
+      for (int i = 0; i < count; i += 4) {  // (what lies past the list is zero, or its count is taken off below)
+        const u32x4 x = *reinterpret_cast<const u32x4*>(&list[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) more += x[e] > k, same += x[e] == k;
+      }
+      if (k == 0) same -= (-count) & 3;
+      if (more < wanted && more + same >= wanted) edge_s = k;  // (every equal key says the same)
+    }
+    __syncthreads();
+    edge = edge_s;
+  }
+
+  // A kept slot's place: the larger keys in front of it, and the equal ones as far as they are kept.
+  int larger = 0, equal = 0;  // in front of this step
+  int ties = want;            // equal keys kept: want less all larger ones, counted first
+  {
     int x = 0;
-    for (int j = tid; j < early; j += kPagedThreads) x += key(j) >= t;
-    if (total(x) >= want) edge = t;
+    for (int s0 = 4 * tid; s0 < early; s0 += 2 * STEP) {
+      uint32_t k[2][4];
+      keys_of(s0, k[0]);
+      keys_of(s0 + STEP, k[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x += s0 + i * STEP + e < early && k[i][e] > edge;
+    }
+    x = wave_scan(x);
+    __syncthreads();
+    if (lane == 63) wave_s[wv] = x;
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) ties -= wave_s[w];
   }
-  int above = 0;
-  for (int j = tid; j < early; j += kPagedThreads) above += key(j) > edge;
-  const int ties = want - total(above);
-  int done = 0, equal = 0;
-  for (int j0 = 0; j0 < early; j0 += kPagedThreads) {
-    const int j = j0 + tid;
-    const uint32_t k = j < early ? key(j) : 0u;
-    auto before = [&](bool f, int* all) {  // of the threads in front of this one
-      const uint64_t m = __ballot(f);
-      __syncthreads();
-      if (lane == 0) red[wv] = __popcll(m);
-      __syncthreads();
-      int x = __popcll(m & ((1ull << lane) - 1));
-      for (int w = 0; w < wv; ++w) x += red[w];
-      *all = red[0] + red[1] + red[2] + red[3];
-      return x;
-    };
-    int all;
-    const bool tie = j < early && k == edge;
-    const int rank = equal + before(tie, &all);
-    equal += all;
-    const bool take = j < early && (k > edge || (tie && rank < ties));
-    const int at = done + before(take, &all);
-    done += all;
-    if (take) kept[at] = j;
+  for (int s0 = 0; s0 < early; s0 += STEP) {
+    const int s = s0 + 4 * tid;
+    uint32_t k[4];
+    keys_of(s, k);
+    int x = 0;  // larger keys in the low half, equal ones in the high half (at most 4096 of either a step)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (s + e < early) x += k[e] > edge ? 1 : k[e] == edge ? 1 << 16 : 0;
+    const int upto = wave_scan(x);
+    __syncthreads();
+    if (lane == 63) wave_s[wv] = upto;
+    __syncthreads();
+    int before = upto - x, all = 0;
+    for (int w = 0; w < WAVES; ++w) {
+      before += w < wv ? wave_s[w] : 0;
+      all += wave_s[w];
+    }
+    int l = larger + (before & 0xFFFF), q = equal + (before >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (s + e < early) {
+        const int at = l + min(q, ties);
+        if ((k[e] > edge || (k[e] == edge && q < ties)) && at < want) kept[at] = s + e;
+        l += k[e] > edge;
+        q += k[e] == edge;
+      }
+    larger += all & 0xFFFF;
+    equal += all >> 16;
   }
-  for (int j = tid; j < a.recent; j += kPagedThreads) kept[want + j] = early + j;
 }
 
-// Sixteen bytes of a kept token's key and value a thread.
+// Sixteen bytes of a kept token's key and value a thread, of four tokens in turn.
 template <int D>
 __global__ __launch_bounds__(kPagedThreads) void paged_copy_kernel(EvictArgs a) {
-  constexpr int CH = D / 8, TOK = kPagedThreads / CH;
-  const int h = blockIdx.y, b = blockIdx.z, c = threadIdx.x % CH;
-  const int j = blockIdx.x * TOK + threadIdx.x / CH, n = a.new_lengths[b];
-  if (j >= n) return;
-  const int64_t src = a.c.token(b, a.kept[((int64_t)b * a.c.nkv + h) * a.keep + j], h);
-  const int64_t page = a.new_table[(int64_t)b * a.new_width + (j >> a.c.log2s)];
-  if (src < 0 || (uint64_t)page >= (uint64_t)a.c.pages) return;
-  const int64_t dst = ((page * a.c.nkv + h) << a.c.log2s) + (j & ((1 << a.c.log2s) - 1));
-  *reinterpret_cast<u32x4*>(a.c.k + dst * D + c * 8) = *reinterpret_cast<const u32x4*>(a.c.k + src * D + c * 8);
-  *reinterpret_cast<u32x4*>(a.c.v + dst * D + c * 8) = *reinterpret_cast<const u32x4*>(a.c.v + src * D + c * 8);
-  if (c == 0) a.c.weight[dst] = a.c.weight[src];
+  constexpr int CH = D / 8, TOK = kPagedThreads / CH, PER = 4;
+  const int h = blockIdx.y, b = blockIdx.z, c = threadIdx.x % CH, n = a.new_lengths[b];
+  const int j0 = blockIdx.x * (TOK * PER) + threadIdx.x / CH;
+  if (j0 >= n) return;
+  const bool all = a.lengths[b] <= a.keep;
+  int64_t src[PER], dst[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = min(j0 + i * TOK, n - 1);
+    src[i] = all ? j : a.kept[((int64_t)b * a.c.nkv + h) * a.keep + j];
+    dst[i] = a.new_table[(int64_t)b * a.new_width + (j >> a.c.log2s)];
+  }
+  u32x4 k[PER], v[PER];
+  float w[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = min(j0 + i * TOK, n - 1);
+    const int64_t page = dst[i];
+    src[i] = a.c.token(b, (int)src[i], h);
+    const bool ok = src[i] >= 0 && (uint64_t)page < (uint64_t)a.c.pages && j0 + i * TOK < n;
+    dst[i] = ok ? ((page * a.c.nkv + h) << a.c.log2s) + (j & ((1 << a.c.log2s) - 1)) : -1;
+    if (ok) {
+      k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.c.k + src[i] * D + c * 8));
+      v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.c.v + src[i] * D + c * 8));
+      w[i] = a.c.weight[src[i]];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (dst[i] >= 0) {
+      *reinterpret_cast<u32x4*>(a.c.k + dst[i] * D + c * 8) = k[i];
+      *reinterpret_cast<u32x4*>(a.c.v + dst[i] * D + c * 8) = v[i];
+      if (c == 0) a.c.weight[dst[i]] = w[i];
+    }
 }
 
 }  // namespace w4
@@ -896,11 +1003,12 @@ extern "C" int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int3
   if (cache->rows == 0) return W4_OK;
   if (!cache->weight || !lengths || !new_table || !kept || !new_lengths)
     return fail(W4_ERR_INVALID, "w4_paged_evict: null pointer");
+  if ((uintptr_t)cache->weight % 16) return fail(W4_ERR_INVALID, "w4_paged_evict: weight must be 16-byte aligned");
   w4::EvictArgs a{view_of(cache), lengths, new_table, kept, new_lengths, (int)new_width, (int)keep, (int)recent};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  w4::paged_select_kernel<<<dim3((unsigned)cache->kv_heads, (unsigned)cache->rows), w4::kPagedThreads, 0, st>>>(a);
+  w4::paged_select_kernel<<<dim3((unsigned)cache->kv_heads, (unsigned)cache->rows), w4::kSelectThreads, 0, st>>>(a);
   if (const int rc = check_launch("w4_paged_evict (select)")) return rc;
-  const int tok = w4::kPagedThreads / (int)(cache->head_dim / 8);
+  const int tok = 4 * w4::kPagedThreads / (int)(cache->head_dim / 8);
   const dim3 grid((unsigned)((keep + tok - 1) / tok), (unsigned)cache->kv_heads, (unsigned)cache->rows);
   if (cache->head_dim == 64) w4::paged_copy_kernel<64><<<grid, w4::kPagedThreads, 0, st>>>(a);
   else w4::paged_copy_kernel<128><<<grid, w4::kPagedThreads, 0, st>>>(a);
