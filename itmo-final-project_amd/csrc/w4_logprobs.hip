@@ -47,14 +47,23 @@ __device__ __forceinline__ float logit_at(const void* x, int64_t i) {
   else return act_bits_to_float(static_cast<const uint16_t*>(x)[i], DT);
 }
 
-// Sum of e^(x - m) and of e^(x - m) (x - m) over some logits.  The reference m starts at the lowest finite number, so
-// that rows of -inf meet no difference of infinities.
+// Sums over some logits x of 2^y and 2^y y with y = x log2(e) - ref(m).  The reference m is their maximum; it starts at
+// the lowest finite number, so that rows of -inf meet no difference of infinities.
 struct LogSum {
   float m = -3.402823466e38f, s = 0.f, t = 0.f;
+  static __device__ __forceinline__ bool plain(float m) { return __builtin_fabsf(m) < 1e38f; }  // m log2(e) is finite
+  // ref(m) is m log2(e) rounded, which y's one fma subtracts exactly; what the rounding left out comes off the
+  // logarithm at the end.
+  static __device__ __forceinline__ float left(float m) {
+    return plain(m) ? __builtin_fmaf(m, kLog2e, -(m * kLog2e)) : 0.f;
+  }
   __device__ __forceinline__ void rebase(float to) {  // to >= m
-    const float d = m - to, f = __builtin_amdgcn_exp2f(d * kLog2e);
+#pragma clang fp contract(off)
+    const float a = m * kLog2e, b = to * kLog2e;
+    const float d = plain(m) && plain(to) ? a - b : (m - to) * kLog2e;
+    const float f = __builtin_amdgcn_exp2f(d);
     // (a distance beyond all exponents: nothing is left of the sums, whatever the product)
-    t = s == 0.f ? t * f : f * __builtin_fmaf(fmaxf(d, -1e4f), s, t);
+    t = s == 0.f ? t * f : f * (fmaxf(d, -1e4f) * s + t);
     s *= f;
     m = to;
   }
@@ -131,29 +140,41 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   const __amdgpu_buffer_rsrc_t rp =
       __builtin_amdgcn_make_buffer_rsrc((void*)scratch, (short)0, a.row_words * 4, kLogBufFlags);
 
-  u32x4 raw[NV];
-  auto load = [&](int blk) {
-    const int i0 = blk * kLogBlock + wv * 2048 + lane * T::N;
+  // The N logits from i on; past the row: -inf.
+  auto load_at = [&](int i) __attribute__((always_inline)) -> u32x4 {
+    if (i + T::N <= a.vocab) return *reinterpret_cast<const typename T::vec*>(x + i);
+    uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int i = i0 + j * PIECE;
-      if (i + T::N <= a.vocab) {
-        raw[j] = *reinterpret_cast<const typename T::vec*>(x + i);
-      } else {  // past the row: -inf
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (DT == W4_DTYPE_FP32) {
-            w[e] = i + e < a.vocab ? __builtin_bit_cast(uint32_t, x[i + e]) : 0xFF800000u;
-          } else {
-            const uint32_t none = DT == W4_DTYPE_BF16 ? 0xFF80u : 0xFC00u;
-            const uint32_t l = i + 2 * e < a.vocab ? x[i + 2 * e] : none;
-            const uint32_t h = i + 2 * e + 1 < a.vocab ? x[i + 2 * e + 1] : none;
-            w[e] = l | h << 16;
-          }
-        }
-        raw[j] = u32x4{w[0], w[1], w[2], w[3]};
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == W4_DTYPE_FP32) {
+        w[e] = i + e < a.vocab ? __builtin_bit_cast(uint32_t, x[i + e]) : 0xFF800000u;
+      } else {
+        const uint32_t none = DT == W4_DTYPE_BF16 ? 0xFF80u : 0xFC00u;
+        const uint32_t l = i + 2 * e < a.vocab ? x[i + 2 * e] : none;
+        const uint32_t h = i + 2 * e + 1 < a.vocab ? x[i + 2 * e + 1] : none;
+        w[e] = l | h << 16;
       }
+    }
+    return u32x4{w[0], w[1], w[2], w[3]};
+  };
+  auto unpack = [&](const u32x4& r, float* v) __attribute__((always_inline)) {
+    if constexpr (DT == W4_DTYPE_FP32) {
+      const f32x4 f = __builtin_bit_cast(f32x4, r);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = f[e];
+    } else {
+      unpack8<DT>(r, v);
+    }
+  };
+  u32x4 raw[NV];
+  auto load = [&](int blk) __attribute__((always_inline)) {
+    const int i0 = blk * kLogBlock + wv * 2048 + lane * T::N;
+    if ((blk + 1) * kLogBlock <= a.vocab) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) raw[j] = *reinterpret_cast<const typename T::vec*>(x + i0 + j * PIECE);
+    } else {  // the row's last block
+#pragma unroll
+      for (int j = 0; j < NV; ++j) raw[j] = load_at(i0 + j * PIECE);
     }
   };
   LogSum sum;
@@ -161,26 +182,31 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   for (int blk = b0; blk < b1; ++blk) {
     float v[32];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if constexpr (DT == W4_DTYPE_FP32) {
-        const f32x4 f = __builtin_bit_cast(f32x4, raw[j]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * j + e] = f[e];
-      } else {
-        unpack8<DT>(raw[j], v + 8 * j);
-      }
-    }
+    for (int j = 0; j < NV; ++j) unpack(raw[j], v + T::N * j);
     if (blk + 1 < b1) load(blk + 1);  // on its way under this one's arithmetic
     float top = v[0];
 #pragma unroll
     for (int e = 1; e < 32; ++e) top = fmaxf(top, v[e]);
     sum.rebase(fmaxf(sum.m, top));
     float s = 0.f, t = 0.f;
+    const float ref = sum.m * kLog2e;
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
-      const float y = v[e] - sum.m, p = __builtin_amdgcn_exp2f(y * kLog2e);
+      const float y = __builtin_fmaf(v[e], kLog2e, -ref), p = __builtin_amdgcn_exp2f(y);
       s += p;
-      t = __builtin_fmaf(p, fmaxf(y, -1e4f), t);  // p = 0 counts nothing, at -inf too
+      t = __builtin_fmaf(p, y, t);
+    }
+    // -inf among them (0 * -inf; it counts nothing), numbers near the range's ends, infinities and NaN
+    if (__ballot(t != t || !LogSum::plain(sum.m))) {
+      s = t = 0.f;
+      const bool plain = LogSum::plain(sum.m);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const float y = plain ? __builtin_fmaf(v[e], kLog2e, -ref) : (v[e] - sum.m) * kLog2e;
+        const float p = __builtin_amdgcn_exp2f(y);
+        s += p;
+        t = __builtin_fmaf(p, fmaxf(y, -1e4f), t);
+      }
     }
     sum.s += s;
     sum.t += t;
@@ -217,18 +243,20 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     if (arrived_s != (unsigned)(a.parts - 1)) return;
     if (tid == 0) __hip_atomic_store(a.cnt + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     sum = LogSum();
-    for (int p = 0; p < a.parts; ++p) {
+    for (int p = lane; p < a.parts; p += 64) {
       const f32x4 o = __builtin_bit_cast(
           f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (uint32_t)p * 16u, 0, kLogCoherentAux));
       sum.add(o[0], o[1], o[2]);
     }
+    sum.rebase(wave_max(sum.m));
+    sum.s = wave_sum(sum.s), sum.t = wave_sum(sum.t);
   } else {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   }
-  const float logz = logf(sum.s);
+  const float ln2 = 0.6931471805599453f, logs = logf(sum.s), logz = __builtin_fmaf(-LogSum::left(sum.m), ln2, logs);
   if (tid == 0) {
-    a.entropy[row] = logz - sum.t / sum.s;
+    a.entropy[row] = __builtin_fmaf(-ln2, sum.t / sum.s, logs);
     if (a.tokens) {
       const int64_t tok = a.tokens[row];
       a.logprob[row] =
@@ -242,63 +270,91 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   auto group_key = [&](int g) {
     return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rp, (uint32_t)(a.parts * 4 + g) * 4u, 0, kLogCoherentAux);
   };
-  uint64_t lo = 0, hi = 0xFFFFFFFFull;
-  int wanted = min(a.top, groups), above = 0, count = groups;
-  narrow([&](auto f) {
-    for (int g = tid; g < groups; g += 4 * kLogThreads) {
-      uint32_t k[4];
+  uint32_t gk[4];  // of the first 1024 groups, this thread's
 #pragma unroll
-      for (int i = 0; i < 4; ++i) k[i] = group_key(min(g + i * kLogThreads, groups - 1));
+  for (int i = 0; i < 4; ++i) gk[i] = group_key(min(tid + i * kLogThreads, groups - 1));
+  auto each_group = [&](auto f) {  // f(group, key)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (g + i * kLogThreads < groups) f((uint64_t)k[i]);
+    for (int i = 0; i < 4; ++i)
+      if (tid + i * kLogThreads < groups) f(tid + i * kLogThreads, gk[i]);
+    for (int g = tid + 4 * kLogThreads; g < groups; g += kLogThreads) f(g, group_key(g));
+  };
+  uint32_t low = 0xFFFFFFFFu, high = 0;
+  each_group([&](int, uint32_t k) { low = min(low, k), high = max(high, k); });
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) low = min(low, (uint32_t)__shfl_xor((int)low, d)), high = max(high, (uint32_t)__shfl_xor((int)high, d));
+  if (lane == 0) wave_s[wv] = (int)low, groups_s[wv] = (int)high;
+  if (tid == 0) found_s[0] = 0;
+  __syncthreads();
+  for (int w = 0; w < kLogThreads / 64; ++w) low = min(low, (uint32_t)wave_s[w]), high = max(high, (uint32_t)groups_s[w]);
+  uint64_t lo = low, hi = high;
+  int wanted = a.top, above = 0, count = groups;  // (there are at least 64)
+  __syncthreads();
+  narrow([&](auto f) { each_group([&](int, uint32_t k) { f((uint64_t)k); }); }, lo, hi, wanted, above, count, kLogSpare,
+         hist, wave_s, found_s);
+  __syncthreads();
+  int held = 0;
+  if (above + count <= kLogMaxGroups) {  // in any order
+    if (tid == 0) found_s[0] = 0;
+    __syncthreads();
+    each_group([&](int g, uint32_t k) {
+      if (k >= lo) groups_s[atomicAdd(&found_s[0], 1)] = g;
+    });
+    __syncthreads();
+    held = found_s[0];
+  } else {
+    // More equal maxima than fit: those of the first blocks, until there is one for every alternative (a block is a
+    // run of logits, so its equal logits come before all later ones).
+    int equal = 0;
+    for (int g0 = 0; g0 < groups; g0 += kLogThreads) {
+      const int g = g0 + tid;
+      const uint32_t k = g < groups ? group_key(g) : 0u;
+      const bool same = g < groups && k == lo;
+      const uint64_t m_same = __ballot(same);
+      __syncthreads();
+      if (lane == 0) wave_s[wv] = __popcll(m_same);
+      __syncthreads();
+      int before = equal;  // of the blocks in front (a wave has one block)
+      for (int w = 0; w < kLogThreads / 64; ++w) {
+        before += w < wv ? wave_s[w] : 0;
+        equal += wave_s[w];
+      }
+      const bool take = g < groups && (k > lo || (same && before < a.top));
+      const uint64_t m_take = __ballot(take);
+      __syncthreads();
+      if (lane == 0) wave_s[wv] = __popcll(m_take);
+      __syncthreads();
+      int at = held + __popcll(m_take & ((1ull << lane) - 1));
+      for (int w = 0; w < kLogThreads / 64; ++w) {
+        at += w < wv ? wave_s[w] : 0;
+        held += wave_s[w];
+      }
+      if (take) groups_s[at] = g;
     }
-  }, lo, hi, wanted, above, count, kLogSpare, hist, wave_s, found_s);
-  // More equal maxima than fit: those of the first blocks, until there is one for every alternative (a block is a
-  // run of logits, so its equal logits come before all later ones).
-  const bool few = above + count <= kLogMaxGroups;
-  int equal = 0, held = 0;
-  for (int g0 = 0; g0 < groups; g0 += kLogThreads) {
-    const int g = g0 + tid;
-    const uint32_t k = g < groups ? group_key(g) : 0u;
-    const bool same = g < groups && k == lo && !few;
-    const uint64_t m_same = __ballot(same);
-    __syncthreads();
-    if (lane == 0) wave_s[wv] = __popcll(m_same);
-    __syncthreads();
-    int before = equal;  // of the blocks in front (a wave has one block)
-    for (int w = 0; w < kLogThreads / 64; ++w) {
-      before += w < wv ? wave_s[w] : 0;
-      equal += wave_s[w];
-    }
-    const bool take = g < groups && (few ? k >= lo : k > lo || (same && before < a.top));
-    const uint64_t m_take = __ballot(take);
-    __syncthreads();
-    if (lane == 0) wave_s[wv] = __popcll(m_take);
-    __syncthreads();
-    int at = held + __popcll(m_take & ((1ull << lane) - 1));
-    for (int w = 0; w < kLogThreads / 64; ++w) {
-      at += w < wv ? wave_s[w] : 0;
-      held += wave_s[w];
-    }
-    if (take) groups_s[at] = g;
   }
   __syncthreads();
 
   // Their logits: (key, lower index first) in one number.
-  auto members = [&](auto f) {
-    for (int i = tid >> 7; i < held; i += 8) {
-      uint64_t k[4];
+  auto members = [&](auto f) __attribute__((always_inline)) {
+    constexpr int VECS = 128 / T::N, STEP = kLogThreads / VECS, U = 4;  // loads of a group, groups of a step
+    const int vec = tid % VECS;
+    for (int i = tid / VECS; i < held; i += U * STEP) {
+      int at[U];
+      u32x4 r[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int g = groups_s[min(i + 2 * u, held - 1)], e = tid & 127;
-        const int at = (g / kLogGroups) * kLogBlock + (g / 16 % 4) * 2048 + e / (4 * T::N) * PIECE + g % 16 * (4 * T::N) +
-                       e % (4 * T::N);
-        k[u] = at < a.vocab ? (uint64_t)order_key(logit_at<DT>(x, at)) << 32 | (uint32_t)~at : 0ull;
+      for (int u = 0; u < U; ++u) {
+        const int g = groups_s[min(i + u * STEP, held - 1)];
+        at[u] = (g / kLogGroups) * kLogBlock + (g / 16 % 4) * 2048 + vec / 4 * PIECE + (g % 16 * 4 + vec % 4) * T::N;
+        r[u] = load_at(at[u]);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (i + 2 * u < held) f(k[u]);
+      for (int u = 0; u < U; ++u) {
+        float v[T::N];
+        unpack(r[u], v);
+#pragma unroll
+        for (int e = 0; e < T::N; ++e)
+          if (i + u * STEP < held && at[u] + e < a.vocab) f((uint64_t)order_key(v[e]) << 32 | (uint32_t)~(at[u] + e));
+      }
     }
   };
   uint64_t from = lo << 32;
@@ -306,7 +362,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     if (tid == 0) found_s[0] = 0;
     __syncthreads();
     members([&](uint64_t v) {
-      if (v >= from && v != 0) {
+      if (v >= from) {
         const int at = atomicAdd(&found_s[0], 1);
         if (at < kLogList) list[at] = v;
       }
@@ -326,6 +382,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   for (int i = tid; i < n; i += kLogThreads) {
     const uint64_t v = list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += list[j] > v;
     if (rank < a.top) {
       const uint32_t key = (uint32_t)(v >> 32);
@@ -353,7 +410,7 @@ struct LogprobPlan {
 LogprobPlan logprob_plan(int64_t rows, int64_t vocab) {
   LogprobPlan p;
   p.blocks = (int)((vocab + w4::kLogBlock - 1) / w4::kLogBlock);
-  const int64_t most = 8 * device_cu_count();
+  const int64_t most = 3 * device_cu_count();
   p.parts = (int)(rows >= most ? 1 : most / rows < p.blocks ? most / rows : p.blocks);
   p.row_words = p.parts * 4 + (int64_t)p.blocks * w4::kLogGroups;
   // arrival counters, and no more than 64 MiB of scratch

@@ -628,16 +628,24 @@ constexpr int kSelectThreads = 1024;
 constexpr int kSelectBins = 4096;
 constexpr int kSelectList = 256;  // keys few enough to be ranked against each other
 
+constexpr int kSelectRun = 32768;  // keys that LDS holds
+
 // One workgroup per row and key-value head finds the slots to keep.  The key of the last one (its weight's place in
 // the order of all weights) lies in a range that a histogram of 4096 bins narrows twelve bits at a time until no more
-// than 256 keys are in it, which are then ranked one against all: at most three histograms, one as a rule.  A last
-// pass gives every kept slot its place, counting the larger keys and the equal ones in front of it.
+// than 256 keys are in it, which are then ranked one against all: at most three histograms, one as a rule.  Then
+// every kept slot gets its place, the larger keys in front of it and the equal ones as far as they are kept: a wave
+// holds a run of slots, so that after one exchange of counts each goes through its own.
+//
+// What bounds it is the latency of its steps, so the keys are read from memory once and stay in LDS (of more than
+// 32768 early slots, a run at a time in every step).
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a) {
-  constexpr int WAVES = kSelectThreads / 64, STEP = 4 * kSelectThreads;
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = blockIdx.x, b = blockIdx.y;
+  constexpr int WAVES = kSelectThreads / 64, RUN = kSelectRun, Q = RUN / (4 * kSelectThreads);
+  const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x, b = blockIdx.y;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ __attribute__((aligned(16))) uint32_t key_s[RUN];
   __shared__ int hist[kSelectBins];
   __shared__ __attribute__((aligned(16))) uint32_t list[kSelectList];
-  __shared__ int wave_s[WAVES], found_s[3];
+  __shared__ int wave_s[2][WAVES], found_s[3];
   __shared__ uint32_t edge_s;
   int n = a.lengths[b];
   if (n > a.c.capacity()) n = -1;
@@ -645,16 +653,43 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
   if (n <= a.keep) return;  // idle, or all of it kept: the copy needs no list
   int32_t* const kept = a.kept + ((int64_t)b * a.c.nkv + h) * a.keep;
   const int early = n - a.recent;
-  int want = a.keep - a.recent;
+  const int want = a.keep - a.recent;
   for (int j = tid; j < a.recent; j += kSelectThreads) kept[want + j] = early + j;
   if (want == 0) return;
-  // f(slot, key) for every early slot, four slots in a row a thread, in the order of the threads
-  auto keys_of = [&](int s, uint32_t k[4]) {
-    const int64_t at = s < early ? a.c.token(b, s, h) : -1;  // (four slots never straddle a page)
-    f32x4 w = {0.f, 0.f, 0.f, 0.f};
-    if (at >= 0) w = *reinterpret_cast<const f32x4*>(a.c.weight + at);
+
+  // Quad q of a thread: four slots of a run from at(q) on; a wave's quads are `quads` * 256 slots in a row.
+  const int quads = min(Q, (early + 4 * kSelectThreads - 1) / (4 * kSelectThreads));
+  auto at = [&](int q) { return (wv * quads + q) * 256 + 4 * lane; };
+  auto load = [&](int run) __attribute__((always_inline)) {
+    int64_t tok[Q];
+    f32x4 w[Q];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) k[e] = at < 0 ? 0u : order_key(w[e]);
+    for (int q = 0; q < Q; ++q) tok[q] = q < quads && run + at(q) < early ? a.c.token(b, run + at(q), h) : -1;
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (tok[q] >= 0) w[q] = *reinterpret_cast<const f32x4*>(a.c.weight + tok[q]);
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (q < quads) {
+        u32x4 x = {0u, 0u, 0u, 0u};  // on a page outside the pool: below all
+        if (tok[q] >= 0) x = u32x4{order_key(w[q][0]), order_key(w[q][1]), order_key(w[q][2]), order_key(w[q][3])};
+        *reinterpret_cast<u32x4*>(&key_s[at(q)]) = x;
+      }
+  };
+  const bool once = early <= RUN;
+  if (once) load(0);  // (a thread reads back what it wrote itself)
+  auto quad = [&](int q) { return *reinterpret_cast<const u32x4*>(&key_s[at(q)]); };
+  // f(key) for every early slot
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    for (int run = 0; run < early; run += RUN) {
+      if (!once) load(run);
+      for (int q = 0; q < quads; ++q) {
+        const u32x4 k = quad(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (run + at(q) + e < early) f((uint32_t)k[e]);
+      }
+    }
   };
 
   uint32_t lo = 0, hi = 0xFFFFFFFFu;
@@ -663,25 +698,18 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
     const int shift = max(0, 32 - __builtin_clz(hi - lo) - 12);
     for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
     __syncthreads();
-    for (int s0 = 4 * tid; s0 < early; s0 += 2 * STEP) {
-      uint32_t k[2][4];
-      keys_of(s0, k[0]);
-      keys_of(s0 + STEP, k[1]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (s0 + i * STEP + e < early && k[i][e] >= lo && k[i][e] <= hi) atomicAdd(&hist[(k[i][e] - lo) >> shift], 1);
-    }
+    each([&](uint32_t key) {
+      if (key >= lo && key <= hi) atomicAdd(&hist[(key - lo) >> shift], 1);
+    });
     __syncthreads();
     // from the top: thread t has the bins 4 (1023 - t)..
     const int top = kSelectBins - 4 - 4 * tid;
     const int mine = hist[top] + hist[top + 1] + hist[top + 2] + hist[top + 3];
     const int upto = wave_scan(mine);
-    if (lane == 63) wave_s[wv] = upto;
+    if (lane == 63) wave_s[0][wv] = upto;
     __syncthreads();
     int above = upto - mine;
-    for (int w = 0; w < wv; ++w) above += wave_s[w];
+    for (int w = 0; w < wv; ++w) above += wave_s[0][w];
     if (above < wanted && above + mine >= wanted) {
       int e = 3;
       while (above + hist[top + e] < wanted) above += hist[top + e--];
@@ -701,83 +729,87 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
     if (tid == 0) found_s[0] = 0;
     if (tid < kSelectList) list[tid] = 0;
     __syncthreads();
-    for (int s0 = 4 * tid; s0 < early; s0 += 2 * STEP) {
-      uint32_t k[2][4];
-      keys_of(s0, k[0]);
-      keys_of(s0 + STEP, k[1]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (s0 + i * STEP + e < early && k[i][e] >= lo && k[i][e] <= hi) {
-            const int at = atomicAdd(&found_s[0], 1);
-            if (at < kSelectList) list[at] = k[i][e];  // (weights that change under the call stay in bounds)
-          }
-    }
+    each([&](uint32_t key) {
+      if (key >= lo && key <= hi) {
+        const int at = atomicAdd(&found_s[0], 1);
+        if (at < kSelectList) list[at] = key;  // (weights that change under the call stay in bounds)
+      }
+    });
     __syncthreads();
     if (tid < count) {
-      const uint32_t k = list[tid];
+      const uint32_t key = list[tid];
       int more = 0, same = 0;
+#pragma unroll 4
       for (int i = 0; i < count; i += 4) {  // (what lies past the list is zero, or its count is taken off below)
         const u32x4 x = *reinterpret_cast<const u32x4*>(&list[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) more += x[e] > k, same += x[e] == k;
+        for (int e = 0; e < 4; ++e) more += x[e] > key, same += x[e] == key;
       }
-      if (k == 0) same -= (-count) & 3;
-      if (more < wanted && more + same >= wanted) edge_s = k;  // (every equal key says the same)
+      if (key == 0) same -= (-count) & 3;
+      if (more < wanted && more + same >= wanted) edge_s = key;  // (every equal key says the same)
     }
     __syncthreads();
     edge = edge_s;
   }
 
-  // A kept slot's place: the larger keys in front of it, and the equal ones as far as they are kept.
-  int larger = 0, equal = 0;  // in front of this step
-  int ties = want;            // equal keys kept: want less all larger ones, counted first
-  {
-    int x = 0;
-    for (int s0 = 4 * tid; s0 < early; s0 += 2 * STEP) {
-      uint32_t k[2][4];
-      keys_of(s0, k[0]);
-      keys_of(s0 + STEP, k[1]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x += s0 + i * STEP + e < early && k[i][e] > edge;
-    }
-    x = wave_scan(x);
-    __syncthreads();
-    if (lane == 63) wave_s[wv] = x;
-    __syncthreads();
-    for (int w = 0; w < WAVES; ++w) ties -= wave_s[w];
+  // Of every run, the larger and the equal keys of each wave; `ties` equal ones are kept, what all larger ones leave.
+  int larger = 0, equal = 0;
+  each([&](uint32_t key) { larger += key > edge, equal += key == edge; });
+  int ties = want, l0 = 0, q0 = 0;  // (of a single run: the same counts say where a wave begins)
+  larger = __builtin_amdgcn_readlane(wave_scan(larger), 63);
+  equal = __builtin_amdgcn_readlane(wave_scan(equal), 63);
+  __syncthreads();
+  if (lane == 0) wave_s[0][wv] = larger, wave_s[1][wv] = equal;
+  __syncthreads();
+  for (int w = 0; w < WAVES; ++w) {
+    ties -= wave_s[0][w];
+    l0 += w < wv ? wave_s[0][w] : 0;
+    q0 += w < wv ? wave_s[1][w] : 0;
   }
-  for (int s0 = 0; s0 < early; s0 += STEP) {
-    const int s = s0 + 4 * tid;
-    uint32_t k[4];
-    keys_of(s, k);
-    int x = 0;  // larger keys in the low half, equal ones in the high half (at most 4096 of either a step)
+  int l_run = 0, q_run = 0;  // in front of the run
+  for (int run = 0; run < early; run += RUN) {
+    if (!once) {
+      load(run);
+      larger = equal = 0;
+      for (int q = 0; q < quads; ++q) {
+        const u32x4 k = quad(q);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (s + e < early) x += k[e] > edge ? 1 : k[e] == edge ? 1 << 16 : 0;
-    const int upto = wave_scan(x);
-    __syncthreads();
-    if (lane == 63) wave_s[wv] = upto;
-    __syncthreads();
-    int before = upto - x, all = 0;
-    for (int w = 0; w < WAVES; ++w) {
-      before += w < wv ? wave_s[w] : 0;
-      all += wave_s[w];
-    }
-    int l = larger + (before & 0xFFFF), q = equal + (before >> 16);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (s + e < early) {
-        const int at = l + min(q, ties);
-        if ((k[e] > edge || (k[e] == edge && q < ties)) && at < want) kept[at] = s + e;
-        l += k[e] > edge;
-        q += k[e] == edge;
+        for (int e = 0; e < 4; ++e)
+          if (run + at(q) + e < early) larger += k[e] > edge, equal += k[e] == edge;
       }
-    larger += all & 0xFFFF;
-    equal += all >> 16;
+      larger = __builtin_amdgcn_readlane(wave_scan(larger), 63);
+      equal = __builtin_amdgcn_readlane(wave_scan(equal), 63);
+      __syncthreads();
+      if (lane == 0) wave_s[0][wv] = larger, wave_s[1][wv] = equal;
+      __syncthreads();
+      l0 = l_run, q0 = q_run;
+      for (int w = 0; w < WAVES; ++w) {
+        l_run += wave_s[0][w];
+        q_run += wave_s[1][w];
+        l0 += w < wv ? wave_s[0][w] : 0;
+        q0 += w < wv ? wave_s[1][w] : 0;
+      }
+    }
+    for (int q = 0; q < quads; ++q) {
+      const int s = run + at(q);
+      const u32x4 k = quad(q);
+      int x = 0;  // larger keys in the low half, equal ones in the high half
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (s + e < early) x += k[e] > edge ? 1 : k[e] == edge ? 1 << 16 : 0;
+      const int upto = wave_scan(x), all = __builtin_amdgcn_readlane(upto, 63);
+      int l = l0 + ((upto - x) & 0xFFFF), t = q0 + ((upto - x) >> 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (s + e < early) {
+          const int to = l + min(t, ties);
+          if ((k[e] > edge || (k[e] == edge && t < ties)) && to < want) kept[to] = s + e;
+          l += k[e] > edge;
+          t += k[e] == edge;
+        }
+      l0 += all & 0xFFFF;
+      q0 += all >> 16;
+    }
   }
 }
 
