@@ -106,6 +106,15 @@ __device__ __forceinline__ float wave_sum(float v) {
   return (lane_read(v, 0) + lane_read(v, 16)) + (lane_read(v, 32) + lane_read(v, 48));
 }
 
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+  v = max(v, dpp_mov<0xB1>(v));
+  v = max(v, dpp_mov<0x4E>(v));
+  v = max(v, dpp_mov<0x141>(v));
+  v = max(v, dpp_mov<0x140>(v));
+  const auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+  return max(max(at(0), at(16)), max(at(32), at(48)));
+}
+
 // Inclusive sum over the lanes.
 __device__ __forceinline__ int wave_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // shifted right by 1, 2, 4, 8 in rows of 16

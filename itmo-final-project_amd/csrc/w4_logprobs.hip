@@ -11,10 +11,13 @@ constexpr int kMaxTop = 64;
 constexpr int kLogBlock = 8192;                 // logits a workgroup reads in a step: 32 a thread
 constexpr int kLogGroups = kLogBlock / 128;     // groups of 128 logits in it, a quad of lanes each
 constexpr int kLogMaxGroups = 192;              // groups that may hold alternatives: under 2 top + kLogGroups
+constexpr int kLogNear = 1024;                  // groups whose maxima LDS holds, of a row in one part
 constexpr int kLogSpare = 16;                   // groups too many, before the range of their maxima is narrowed again
 constexpr int kLogList = 512;
 constexpr int kLogBins = 2048;
 constexpr int64_t kLogMaxVocab = 1 << 22;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kLogBufFlags = 0x00020000;        // raw buffer: the range is checked in bytes
 constexpr int kLogCoherentAux = 16;             // sc1: the cache policy of agent-scope atomic loads and stores
 
@@ -77,7 +80,8 @@ struct LogSum {
 };
 
 // Values of `each` between lo and hi (those above are kept, `wanted` of the `count` between are), narrowed eleven bits
-// at a time until no more than `stop` are left or lo == hi; the number above grows with them.
+// at a time until no more than `stop` are left or lo == hi; the number above grows with them.  hist is zero before and
+// after.
 template <typename Each>
 __device__ __forceinline__ void narrow(const Each& each, uint64_t& lo, uint64_t& hi, int& wanted, int& above,
                                        int& count, int stop, int* hist, int* wave_s, int* found_s) {
@@ -85,27 +89,37 @@ __device__ __forceinline__ void narrow(const Each& each, uint64_t& lo, uint64_t&
   constexpr int PER = kLogBins / kLogThreads;
   while (count > stop && lo < hi) {
     const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);
-    for (int i = tid; i < kLogBins; i += kLogThreads) hist[i] = 0;
-    __syncthreads();
-    each([&](uint64_t v) {
+    each([&](uint64_t v) __attribute__((always_inline)) {
       if (v >= lo && v <= hi) atomicAdd(&hist[(int)((v - lo) >> shift)], 1);
     });
     __syncthreads();
     const int top = kLogBins - PER - PER * tid;  // from the top
+    i32x4 bins[PER / 4];
     int mine = 0;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) mine += hist[top + e];
+    for (int e = 0; e < PER / 4; ++e) {
+      bins[e] = *reinterpret_cast<const i32x4*>(&hist[top + 4 * e]);
+      *reinterpret_cast<i32x4*>(&hist[top + 4 * e]) = i32x4{0, 0, 0, 0};
+      mine += bins[e][0] + bins[e][1] + bins[e][2] + bins[e][3];
+    }
     const int upto = wave_scan(mine);
     if (lane == 63) wave_s[wv] = upto;
     __syncthreads();
     int over = upto - mine;
     for (int w = 0; w < wv; ++w) over += wave_s[w];
     if (over < wanted && over + mine >= wanted) {
-      int e = PER - 1;
-      while (over + hist[top + e] < wanted) over += hist[top + e--];
-      found_s[0] = top + e;
-      found_s[1] = over;
-      found_s[2] = hist[top + e];
+      bool found = false;
+#pragma unroll
+      for (int e = PER - 1; e >= 0; --e) {
+        const int in = bins[e / 4][e % 4];
+        if (!found && over + in >= wanted) {
+          found = true;
+          found_s[0] = top + e;
+          found_s[1] = over;
+          found_s[2] = in;
+        }
+        over += in;
+      }
     }
     __syncthreads();
     lo += (uint64_t)found_s[0] << shift;
@@ -127,7 +141,8 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   typedef Logits<DT> T;
   constexpr int NV = 32 / T::N, PIECE = 64 * T::N;  // loads of a thread in a block, logits of a wave's load
   __shared__ f32x4 sum_s[kLogThreads / 64];
-  __shared__ int hist[kLogBins];
+  __shared__ __attribute__((aligned(16))) int hist[kLogBins];
+  __shared__ uint32_t key_s[kLogNear];
   __shared__ __attribute__((aligned(16))) uint64_t list[kLogList];
   __shared__ int groups_s[kLogMaxGroups + kLogGroups];
   __shared__ int wave_s[kLogThreads / 64], found_s[3];
@@ -177,8 +192,11 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
       for (int j = 0; j < NV; ++j) raw[j] = load_at(i0 + j * PIECE);
     }
   };
+  const int groups = a.blocks * kLogGroups;
+  const bool near = a.parts == 1 && groups <= kLogNear;
   LogSum sum;
   load(b0);
+  for (int i = tid; i < kLogBins; i += kLogThreads) hist[i] = 0;
   for (int blk = b0; blk < b1; ++blk) {
     float v[32];
 #pragma unroll
@@ -195,17 +213,21 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
       const float y = __builtin_fmaf(v[e], kLog2e, -ref), p = __builtin_amdgcn_exp2f(y);
       s += p;
       t = __builtin_fmaf(p, y, t);
+      if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (all at once would cost a wave a SIMD)
     }
     // -inf among them (0 * -inf; it counts nothing), numbers near the range's ends, infinities and NaN
     if (__ballot(t != t || !LogSum::plain(sum.m))) {
       s = t = 0.f;
       const bool plain = LogSum::plain(sum.m);
+      float again = ref;
+      asm volatile("" : "+v"(again));  // (else the exponents above would be kept in registers for here)
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
-        const float y = plain ? __builtin_fmaf(v[e], kLog2e, -ref) : (v[e] - sum.m) * kLog2e;
+        const float y = plain ? __builtin_fmaf(v[e], kLog2e, -again) : (v[e] - sum.m) * kLog2e;
         const float p = __builtin_amdgcn_exp2f(y);
         s += p;
         t = __builtin_fmaf(p, fmaxf(y, -1e4f), t);
+        if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);
       }
     }
     sum.s += s;
@@ -218,9 +240,11 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
       uint32_t key = order_key(top);
       key = max(key, dpp_mov<0xB1>(key));  // lane ^ 1
       key = max(key, dpp_mov<0x4E>(key));  // lane ^ 2
-      if ((lane & 3) == 0)
-        __builtin_amdgcn_raw_buffer_store_b32(
-            key, rp, (uint32_t)(a.parts * 4 + blk * kLogGroups + wv * 16 + lane / 4) * 4u, 0, kLogCoherentAux);
+      const int g = blk * kLogGroups + wv * 16 + lane / 4;
+      if ((lane & 3) == 0) {
+        if (near) key_s[g] = key;
+        else __builtin_amdgcn_raw_buffer_store_b32(key, rp, (uint32_t)(a.parts * 4 + g) * 4u, 0, kLogCoherentAux);
+      }
     }
   }
   {
@@ -242,6 +266,20 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     __syncthreads();
     if (arrived_s != (unsigned)(a.parts - 1)) return;
     if (tid == 0) __hip_atomic_store(a.cnt + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  } else {
+    if (!near) __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+  auto group_key = [&](int g) __attribute__((always_inline)) {
+    return near ? key_s[g]
+                : (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rp, (uint32_t)(a.parts * 4 + g) * 4u, 0, kLogCoherentAux);
+  };
+  uint32_t gk[4];  // of the first 1024 groups, this thread's
+  if (a.top) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) gk[i] = group_key(min(tid + i * kLogThreads, groups - 1));
+  }
+  if (a.parts > 1) {
     sum = LogSum();
     for (int p = lane; p < a.parts; p += 64) {
       const f32x4 o = __builtin_bit_cast(
@@ -250,9 +288,6 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     }
     sum.rebase(wave_max(sum.m));
     sum.s = wave_sum(sum.s), sum.t = wave_sum(sum.t);
-  } else {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
   }
   const float ln2 = 0.6931471805599453f, logs = logf(sum.s), logz = __builtin_fmaf(-LogSum::left(sum.m), ln2, logs);
   if (tid == 0) {
@@ -266,14 +301,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   if (a.top == 0) return;
 
   // The groups that may hold alternatives.
-  const int groups = a.blocks * kLogGroups;
-  auto group_key = [&](int g) {
-    return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rp, (uint32_t)(a.parts * 4 + g) * 4u, 0, kLogCoherentAux);
-  };
-  uint32_t gk[4];  // of the first 1024 groups, this thread's
-#pragma unroll
-  for (int i = 0; i < 4; ++i) gk[i] = group_key(min(tid + i * kLogThreads, groups - 1));
-  auto each_group = [&](auto f) {  // f(group, key)
+  auto each_group = [&](auto f) __attribute__((always_inline)) {  // f(group, key)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (tid + i * kLogThreads < groups) f(tid + i * kLogThreads, gk[i]);
@@ -281,8 +309,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   };
   uint32_t low = 0xFFFFFFFFu, high = 0;
   each_group([&](int, uint32_t k) { low = min(low, k), high = max(high, k); });
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) low = min(low, (uint32_t)__shfl_xor((int)low, d)), high = max(high, (uint32_t)__shfl_xor((int)high, d));
+  low = ~wave_umax(~low), high = wave_umax(high);
   if (lane == 0) wave_s[wv] = (int)low, groups_s[wv] = (int)high;
   if (tid == 0) found_s[0] = 0;
   __syncthreads();
@@ -354,30 +381,30 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
 #pragma unroll
         for (int e = 0; e < T::N; ++e)
           if (i + u * STEP < held && at[u] + e < a.vocab) f((uint64_t)order_key(v[e]) << 32 | (uint32_t)~(at[u] + e));
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
   uint64_t from = lo << 32;
-  auto collect = [&] {
+  int n;
+  for (;;) {
     if (tid == 0) found_s[0] = 0;
     __syncthreads();
-    members([&](uint64_t v) {
+    members([&](uint64_t v) __attribute__((always_inline)) {
       if (v >= from) {
         const int at = atomicAdd(&found_s[0], 1);
         if (at < kLogList) list[at] = v;
       }
     });
     __syncthreads();
-    return found_s[0];
-  };
-  int n = collect();
-  if (n > kLogList) {  // many equal or neighbouring logits: up to the threshold among the members themselves
+    n = found_s[0];
+    if (n <= kLogList) break;
+    // many equal or neighbouring logits: the threshold is sought among the members themselves, which are all different
     uint64_t to = ~0ull;
     int want = a.top, over = 0;
     __syncthreads();
     narrow(members, from, to, want, over, n, kLogList - kMaxTop, hist, wave_s, found_s);
     __syncthreads();
-    n = collect();
   }
   for (int i = tid; i < n; i += kLogThreads) {
     const uint64_t v = list[i];
