@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     const int i0 = blk * kLogBlock + wv * 2048 + lane * T::N;
     if ((blk + 1) * kLogBlock <= a.vocab) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) raw[j] = *reinterpret_cast<const typename T::vec*>(x + i0 + j * PIECE);
+      for (int j = 0; j < NV; ++j) raw[j] = __builtin_nontemporal_load(reinterpret_cast<const typename T::vec*>(x + i0 + j * PIECE));
     } else {  // the row's last block
 #pragma unroll
       for (int j = 0; j < NV; ++j) raw[j] = load_at(i0 + j * PIECE);
