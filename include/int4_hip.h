@@ -370,13 +370,14 @@ int w4_paged_attention(const w4_paged_cache* cache, int dtype, const void* q, co
  * keep) and, of the others, the keep - recent of largest weight (the lower slot first
  * among equals, NaN above every number).  They go to slots 0.. of row b of new_table
  * [rows, new_width] in the order of their slots, with their weights; new_lengths[b] =
- * min(n, keep) (-1 for an idle row, lengths[b] < 0).  `kept` [rows, kv_heads, keep]
- * receives their old slots.  The pages of new_table must not be among those read, nor
- * stand in it twice.  A row with n beyond the table is idle for this call, its new
- * length -1; tokens on a page outside the pool are not copied.
+ * min(n, keep) (-1 for an idle row, lengths[b] < 0).  The pages of new_table must not be
+ * among those read, nor stand in it twice.  A row with n beyond the table is idle for
+ * this call, its new length -1; tokens on a page outside the pool, or that would go to
+ * one, are not copied.  scratch: w4_paged_evict_scratch_words int32 words.
  */
+size_t w4_paged_evict_scratch_words(const w4_paged_cache* cache, int64_t keep);
 int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int32_t* lengths, const int32_t* new_table,
-                   int64_t new_width, int64_t keep, int64_t recent, int32_t* kept, int32_t* new_lengths,
+                   int64_t new_width, int64_t keep, int64_t recent, int32_t* scratch, int32_t* new_lengths,
                    void* stream);
 
 /*

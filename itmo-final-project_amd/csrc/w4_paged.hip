@@ -619,22 +619,30 @@ struct EvictArgs {
   PagedView c;
   const int32_t* lengths;
   const int32_t* new_table;  // [rows, new_width]
-  int32_t* kept;             // [rows, nkv, keep]
+  int32_t* scratch;          // of a row and head: select_words(), see below
   int32_t* new_lengths;
   int new_width, keep, recent;
 };
 
+// What the selection leaves of a row and head: the key of the last kept token, how many equal keys are kept, and of
+// every 256 slots the number of larger (low half) and of equal keys; then the kept slots.
+constexpr int kSelectBlock = 256;
+__host__ __device__ constexpr int64_t select_words(int64_t capacity, int64_t keep) {
+  return 2 + (capacity + kSelectBlock - 1) / kSelectBlock + keep;
+}
+
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectBins = 4096;
-constexpr int kSelectList = 256;  // keys few enough to be ranked against each other
+constexpr int kSelectList = 2048;  // keys few enough to be put aside
+constexpr int kSelectRank = 256;   // and to be ranked against each other
 
 constexpr int kSelectRun = 32768;  // keys that LDS holds
 
 // One workgroup per row and key-value head finds the slots to keep.  The key of the last one (its weight's place in
-// the order of all weights) lies in a range that a histogram of 4096 bins narrows twelve bits at a time until no more
-// than 256 keys are in it, which are then ranked one against all: at most three histograms, one as a rule.  Then
-// every kept slot gets its place, the larger keys in front of it and the equal ones as far as they are kept: a wave
-// holds a run of slots, so that after one exchange of counts each goes through its own.
+// the order of all weights) lies in a range that a histogram of 4096 bins narrows twelve bits at a time; once no more
+// than 2048 keys are in it they are put aside and narrowed alone, and the last 256 are ranked one against all.  The
+// larger and equal keys of every 256 slots are counted, from which a launch that has all of the chip finds the slots'
+// places (here that took 8 us of 28, for 32768 slots).
 //
 // What bounds it is the latency of its steps, so the keys are read from memory once and stay in LDS (of more than
 // 32768 early slots, a run at a time in every step).
@@ -646,16 +654,15 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
   __shared__ int hist[kSelectBins];
   __shared__ __attribute__((aligned(16))) uint32_t list[kSelectList];
   __shared__ int wave_s[2][WAVES], found_s[3];
+  __shared__ __attribute__((aligned(16))) uint32_t rank_s[kSelectRank];
   __shared__ uint32_t edge_s;
-  int n = a.lengths[b];
-  if (n > a.c.capacity()) n = -1;
-  if (h == 0 && tid == 0) a.new_lengths[b] = n < 0 ? -1 : min(n, a.keep);
-  if (n <= a.keep) return;  // idle, or all of it kept: the copy needs no list
-  int32_t* const kept = a.kept + ((int64_t)b * a.c.nkv + h) * a.keep;
+  __shared__ int ties_s;
+  const int n = a.lengths[b];
+  if (n <= a.keep || n > a.c.capacity()) return;  // idle, or all of it kept
   const int early = n - a.recent;
   const int want = a.keep - a.recent;
-  for (int j = tid; j < a.recent; j += kSelectThreads) kept[want + j] = early + j;
-  if (want == 0) return;
+  if (want == 0) return;  // the last ones alone
+  int32_t* const scratch = a.scratch + ((int64_t)b * a.c.nkv + h) * select_words(a.c.capacity(), a.keep);
 
   // Quad q of a thread: four slots of a run from at(q) on; a wave's quads are `quads` * 256 slots in a row.
   const int quads = min(Q, (early + 4 * kSelectThreads - 1) / (4 * kSelectThreads));
@@ -677,7 +684,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
       }
   };
   const bool once = early <= RUN;
-  if (once) load(0);  // (a thread reads back what it wrote itself)
+  if (once) load(0);  // (a wave reads back what it wrote itself)
   auto quad = [&](int q) { return *reinterpret_cast<const u32x4*>(&key_s[at(q)]); };
   // f(key) for every early slot
   auto each = [&](auto f) __attribute__((always_inline)) {
@@ -685,147 +692,185 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
       if (!once) load(run);
       for (int q = 0; q < quads; ++q) {
         const u32x4 k = quad(q);
+        if (run + (wv * quads + q + 1) * 256 <= early) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (run + at(q) + e < early) f((uint32_t)k[e]);
+          for (int e = 0; e < 4; ++e) f((uint32_t)k[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (run + at(q) + e < early) f((uint32_t)k[e]);
+        }
       }
     }
   };
 
   uint32_t lo = 0, hi = 0xFFFFFFFFu;
   int count = early, wanted = want;  // keys in the range, and how many of them are kept
-  while (count > kSelectList && lo < hi) {
-    const int shift = max(0, 32 - __builtin_clz(hi - lo) - 12);
-    for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
-    __syncthreads();
-    each([&](uint32_t key) {
-      if (key >= lo && key <= hi) atomicAdd(&hist[(key - lo) >> shift], 1);
-    });
-    __syncthreads();
-    // from the top: thread t has the bins 4 (1023 - t)..
-    const int top = kSelectBins - 4 - 4 * tid;
-    const int mine = hist[top] + hist[top + 1] + hist[top + 2] + hist[top + 3];
-    const int upto = wave_scan(mine);
-    if (lane == 63) wave_s[0][wv] = upto;
-    __syncthreads();
-    int above = upto - mine;
-    for (int w = 0; w < wv; ++w) above += wave_s[0][w];
-    if (above < wanted && above + mine >= wanted) {
-      int e = 3;
-      while (above + hist[top + e] < wanted) above += hist[top + e--];
-      found_s[0] = top + e;
-      found_s[1] = above;
-      found_s[2] = hist[top + e];
+  auto narrow = [&](auto keys, int stop) __attribute__((always_inline)) {
+    while (count > stop && lo < hi) {
+      const int shift = max(0, 32 - __builtin_clz(hi - lo) - 12);
+      for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
+      __syncthreads();
+      keys([&](uint32_t key) __attribute__((always_inline)) {
+        if (key >= lo && key <= hi) atomicAdd(&hist[(key - lo) >> shift], 1);
+      });
+      __syncthreads();
+      // from the top: thread t has the bins 4 (1023 - t)..
+      const int top = kSelectBins - 4 - 4 * tid;
+      const int mine = hist[top] + hist[top + 1] + hist[top + 2] + hist[top + 3];
+      const int upto = wave_scan(mine);
+      if (lane == 63) wave_s[0][wv] = upto;
+      __syncthreads();
+      int above = upto - mine;
+      for (int w = 0; w < wv; ++w) above += wave_s[0][w];
+      if (above < wanted && above + mine >= wanted) {
+        int e = 3;
+        while (above + hist[top + e] < wanted) above += hist[top + e--];
+        found_s[0] = top + e;
+        found_s[1] = above;
+        found_s[2] = hist[top + e];
+      }
+      __syncthreads();
+      lo += (uint32_t)found_s[0] << shift;
+      hi = min(hi, lo + ((1u << shift) - 1u));
+      wanted -= found_s[1];
+      count = found_s[2];
     }
-    __syncthreads();
-    lo += (uint32_t)found_s[0] << shift;
-    hi = min(hi, lo + ((1u << shift) - 1u));
-    wanted -= found_s[1];
-    count = found_s[2];
-  }
+  };
+  narrow(each, kSelectList);
   uint32_t edge = lo;
+  int ties = wanted;  // keys equal to the edge that are kept
   if (lo < hi) {
     __syncthreads();
     if (tid == 0) found_s[0] = 0;
-    if (tid < kSelectList) list[tid] = 0;
     __syncthreads();
-    each([&](uint32_t key) {
+    each([&](uint32_t key) __attribute__((always_inline)) {
       if (key >= lo && key <= hi) {
-        const int at = atomicAdd(&found_s[0], 1);
-        if (at < kSelectList) list[at] = key;  // (weights that change under the call stay in bounds)
+        const int to = atomicAdd(&found_s[0], 1);
+        if (to < kSelectList) list[to] = key;  // (weights that change under the call stay in bounds)
       }
     });
     __syncthreads();
-    if (tid < count) {
-      const uint32_t key = list[tid];
-      int more = 0, same = 0;
+    const int held = min(count, kSelectList);
+    narrow([&](auto f) __attribute__((always_inline)) {
+      for (int i = tid; i < held; i += kSelectThreads) f(list[i]);
+    }, kSelectRank);
+    if (lo < hi) {
+      // of the keys in the range (a thread has at most two): how many are larger, how many equal
+      __syncthreads();
+      if (tid < kSelectRank) rank_s[tid] = 0;
+      if (tid == 0) found_s[0] = 0;
+      __syncthreads();
+      for (int i = tid; i < held; i += kSelectThreads)
+        if (list[i] >= lo && list[i] <= hi) rank_s[min(atomicAdd(&found_s[0], 1), kSelectRank - 1)] = list[i];
+      __syncthreads();
+      if (tid < count) {
+        const uint32_t key = rank_s[tid];
+        int more = 0, same = 0;
 #pragma unroll 4
-      for (int i = 0; i < count; i += 4) {  // (what lies past the list is zero, or its count is taken off below)
-        const u32x4 x = *reinterpret_cast<const u32x4*>(&list[i]);
+        for (int i = 0; i < count; i += 4) {  // (what lies past them is zero; its count is taken off below)
+          const u32x4 x = *reinterpret_cast<const u32x4*>(&rank_s[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) more += x[e] > key, same += x[e] == key;
+          for (int e = 0; e < 4; ++e) more += x[e] > key, same += x[e] == key;
+        }
+        if (key == 0) same -= (-count) & 3;
+        if (more < wanted && more + same >= wanted) edge_s = key, ties_s = wanted - more;  // (all equal keys say the same)
       }
-      if (key == 0) same -= (-count) & 3;
-      if (more < wanted && more + same >= wanted) edge_s = key;  // (every equal key says the same)
+      __syncthreads();
+      edge = edge_s;
+      ties = ties_s;
+    } else {
+      edge = lo;
+      ties = wanted;
     }
-    __syncthreads();
-    edge = edge_s;
   }
 
-  // Of every run, the larger and the equal keys of each wave; `ties` equal ones are kept, what all larger ones leave.
-  int larger = 0, equal = 0;
-  each([&](uint32_t key) { larger += key > edge, equal += key == edge; });
-  int ties = want, l0 = 0, q0 = 0;  // (of a single run: the same counts say where a wave begins)
-  larger = __builtin_amdgcn_readlane(wave_scan(larger), 63);
-  equal = __builtin_amdgcn_readlane(wave_scan(equal), 63);
-  __syncthreads();
-  if (lane == 0) wave_s[0][wv] = larger, wave_s[1][wv] = equal;
-  __syncthreads();
-  for (int w = 0; w < WAVES; ++w) {
-    ties -= wave_s[0][w];
-    l0 += w < wv ? wave_s[0][w] : 0;
-    q0 += w < wv ? wave_s[1][w] : 0;
-  }
-  int l_run = 0, q_run = 0;  // in front of the run
+  if (tid == 0) scratch[0] = (int)edge, scratch[1] = ties;
   for (int run = 0; run < early; run += RUN) {
-    if (!once) {
-      load(run);
-      larger = equal = 0;
-      for (int q = 0; q < quads; ++q) {
-        const u32x4 k = quad(q);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (run + at(q) + e < early) larger += k[e] > edge, equal += k[e] == edge;
-      }
-      larger = __builtin_amdgcn_readlane(wave_scan(larger), 63);
-      equal = __builtin_amdgcn_readlane(wave_scan(equal), 63);
-      __syncthreads();
-      if (lane == 0) wave_s[0][wv] = larger, wave_s[1][wv] = equal;
-      __syncthreads();
-      l0 = l_run, q0 = q_run;
-      for (int w = 0; w < WAVES; ++w) {
-        l_run += wave_s[0][w];
-        q_run += wave_s[1][w];
-        l0 += w < wv ? wave_s[0][w] : 0;
-        q0 += w < wv ? wave_s[1][w] : 0;
-      }
-    }
+    if (!once) load(run);
     for (int q = 0; q < quads; ++q) {
-      const int s = run + at(q);
+      const int s0 = run + (wv * quads + q) * 256;
+      if (s0 >= early) break;
       const u32x4 k = quad(q);
-      int x = 0;  // larger keys in the low half, equal ones in the high half
+      int x = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (s + e < early) x += k[e] > edge ? 1 : k[e] == edge ? 1 << 16 : 0;
-      const int upto = wave_scan(x), all = __builtin_amdgcn_readlane(upto, 63);
-      int l = l0 + ((upto - x) & 0xFFFF), t = q0 + ((upto - x) >> 16);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (s + e < early) {
-          const int to = l + min(t, ties);
-          if ((k[e] > edge || (k[e] == edge && t < ties)) && to < want) kept[to] = s + e;
-          l += k[e] > edge;
-          t += k[e] == edge;
-        }
-      l0 += all & 0xFFFF;
-      q0 += all >> 16;
+        if (run + at(q) + e < early) x += k[e] > edge ? 1 : k[e] == edge ? 1 << 16 : 0;
+      x = __builtin_amdgcn_readlane(wave_scan(x), 63);
+      if (lane == 0) scratch[2 + s0 / kSelectBlock] = x;
     }
   }
 }
 
-// Sixteen bytes of a kept token's key and value a thread, of four tokens in turn.
+// One workgroup per 1024 slots of a row and head: the kept slots in their order.  A slot's place is the number of
+// larger keys in front of it, and of equal ones as far as they are kept; the last `recent` come behind all.
+constexpr int kPlaceSlots = 4 * kPagedThreads;
+
+__global__ __launch_bounds__(kPagedThreads) void paged_place_kernel(EvictArgs a) {
+  constexpr int WAVES = kPagedThreads / 64;
+  __shared__ int front_s[2][WAVES], own_s[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, h = blockIdx.y, b = blockIdx.z;
+  const int s0 = blockIdx.x * kPlaceSlots, s = s0 + 4 * tid, n = a.lengths[b];
+  if (n <= a.keep || n > a.c.capacity() || s0 >= n) return;  // idle, or all of it kept: no list
+  const int early = n - a.recent, want = a.keep - a.recent;
+  const int32_t* const scratch = a.scratch + ((int64_t)b * a.c.nkv + h) * select_words(a.c.capacity(), a.keep);
+  int32_t* const kept =
+      a.scratch + ((int64_t)b * a.c.nkv + h + 1) * select_words(a.c.capacity(), a.keep) - a.keep;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (s + e >= early && s + e < n) kept[want + s + e - early] = s + e;
+  if (want == 0 || s0 >= early) return;
+  const uint32_t edge = (uint32_t)scratch[0];
+  const int ties = scratch[1];
+  int larger = 0, equal = 0;  // in front of this workgroup
+  for (int i = tid; i < s0 / kSelectBlock; i += kPagedThreads) {
+    const int x = scratch[2 + i];
+    larger += x & 0xFFFF, equal += x >> 16;
+  }
+  uint32_t key[4] = {0u, 0u, 0u, 0u};
+  const int64_t at = s < early ? a.c.token(b, s, h) : -1;
+  if (at >= 0) {
+    const f32x4 w = *reinterpret_cast<const f32x4*>(a.c.weight + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) key[e] = order_key(w[e]);
+  }
+  int x = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (s + e < early) x += key[e] > edge ? 1 : key[e] == edge ? 1 << 16 : 0;
+  const int upto = wave_scan(x);
+  larger = wave_scan(larger), equal = wave_scan(equal);
+  if (lane == 63) front_s[0][wv] = larger, front_s[1][wv] = equal, own_s[wv] = upto;
+  __syncthreads();
+  int l = (upto - x) & 0xFFFF, t = (upto - x) >> 16;
+  for (int w = 0; w < WAVES; ++w) l += front_s[0][w], t += front_s[1][w];
+  for (int w = 0; w < wv; ++w) l += own_s[w] & 0xFFFF, t += own_s[w] >> 16;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool g = s + e < early && key[e] > edge, q = s + e < early && key[e] == edge;
+    const int to = l + min(t, ties);
+    if ((g || (q && t < ties)) && to < want) kept[to] = s + e;  // (in bounds too if weights change under the call)
+    l += g, t += q;
+  }
+}
+
+// Sixteen bytes of a kept token's key and value a thread, of four tokens at a time.
 template <int D>
 __global__ __launch_bounds__(kPagedThreads) void paged_copy_kernel(EvictArgs a) {
   constexpr int CH = D / 8, TOK = kPagedThreads / CH, PER = 4;
-  const int h = blockIdx.y, b = blockIdx.z, c = threadIdx.x % CH, n = a.new_lengths[b];
+  const int h = blockIdx.y, b = blockIdx.z, c = threadIdx.x % CH;
+  const int len = a.lengths[b], n = len > a.c.capacity() ? -1 : min(len, a.keep);
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.new_lengths[b] = n < 0 ? -1 : n;
   const int j0 = blockIdx.x * (TOK * PER) + threadIdx.x / CH;
   if (j0 >= n) return;
-  const bool all = a.lengths[b] <= a.keep;
+  const int32_t* const kept =
+      a.scratch + ((int64_t)b * a.c.nkv + h + 1) * select_words(a.c.capacity(), a.keep) - a.keep;
+  const bool all = len <= a.keep;
   int64_t src[PER], dst[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int j = min(j0 + i * TOK, n - 1);
-    src[i] = all ? j : a.kept[((int64_t)b * a.c.nkv + h) * a.keep + j];
+    src[i] = all ? j : min((unsigned)kept[j], (unsigned)len - 1u);
     dst[i] = a.new_table[(int64_t)b * a.new_width + (j >> a.c.log2s)];
   }
   u32x4 k[PER], v[PER];
@@ -1023,9 +1068,14 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
                                : launch_paged_attention<W4_DTYPE_FP16, 128>(a, p.items, st);
 }
 
+extern "C" size_t w4_paged_evict_scratch_words(const w4_paged_cache* cache, int64_t keep) {
+  if (!cache || cache->rows < 1 || cache->kv_heads < 1 || cache->width < 1 || cache->page_size < 1 || keep < 1) return 0;
+  return (size_t)(cache->rows * cache->kv_heads * w4::select_words(cache->width * cache->page_size, keep));
+}
+
 extern "C" int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int32_t* lengths,
                               const int32_t* new_table, int64_t new_width, int64_t keep, int64_t recent,
-                              int32_t* kept, int32_t* new_lengths, void* stream) {
+                              int32_t* scratch, int32_t* new_lengths, void* stream) {
   clear_error();
   if (const int rc = check_cache(cache, dtype, "w4_paged_evict")) return rc;
   if (keep < 1 || recent < 0 || recent > keep || new_width < 1 || new_width > (1ll << 30) ||
@@ -1033,15 +1083,24 @@ extern "C" int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int3
     return fail(W4_ERR_INVALID, "w4_paged_evict: keep %lld with the last %lld in %lld pages of %lld", (long long)keep,
                 (long long)recent, (long long)new_width, (long long)cache->page_size);
   if (cache->rows == 0) return W4_OK;
-  if (!cache->weight || !lengths || !new_table || !kept || !new_lengths)
+  if (!cache->weight || !lengths || !new_table || !scratch || !new_lengths)
     return fail(W4_ERR_INVALID, "w4_paged_evict: null pointer");
   if ((uintptr_t)cache->weight % 16) return fail(W4_ERR_INVALID, "w4_paged_evict: weight must be 16-byte aligned");
-  w4::EvictArgs a{view_of(cache), lengths, new_table, kept, new_lengths, (int)new_width, (int)keep, (int)recent};
+  w4::EvictArgs a{view_of(cache), lengths, new_table, scratch, new_lengths, (int)new_width, (int)keep, (int)recent};
+  const int64_t slots = cache->width * cache->page_size;
+  const unsigned heads = (unsigned)cache->kv_heads, rows = (unsigned)cache->rows;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  w4::paged_select_kernel<<<dim3((unsigned)cache->kv_heads, (unsigned)cache->rows), w4::kSelectThreads, 0, st>>>(a);
-  if (const int rc = check_launch("w4_paged_evict (select)")) return rc;
-  const int tok = 4 * w4::kPagedThreads / (int)(cache->head_dim / 8);
-  const dim3 grid((unsigned)((keep + tok - 1) / tok), (unsigned)cache->kv_heads, (unsigned)cache->rows);
+  if (slots > keep) {  // (else no row has more than it keeps)
+    if (recent < keep) {
+      w4::paged_select_kernel<<<dim3(heads, rows), w4::kSelectThreads, 0, st>>>(a);
+      if (const int rc = check_launch("w4_paged_evict (select)")) return rc;
+    }
+    w4::paged_place_kernel<<<dim3((unsigned)((slots + w4::kPlaceSlots - 1) / w4::kPlaceSlots), heads, rows),
+                             w4::kPagedThreads, 0, st>>>(a);
+    if (const int rc = check_launch("w4_paged_evict (place)")) return rc;
+  }
+  const int64_t tok = 4 * w4::kPagedThreads / (cache->head_dim / 8);
+  const dim3 grid((unsigned)((keep + tok - 1) / tok), heads, rows);
   if (cache->head_dim == 64) w4::paged_copy_kernel<64><<<grid, w4::kPagedThreads, 0, st>>>(a);
   else w4::paged_copy_kernel<128><<<grid, w4::kPagedThreads, 0, st>>>(a);
   return check_launch("w4_paged_evict (copy)");

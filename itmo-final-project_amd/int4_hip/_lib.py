@@ -113,6 +113,7 @@ SIGNATURES = {
     "w4_paged_attention_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "w4_paged_attention": (_c_int, [ctypes.POINTER(PagedCache), _c_int, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,
                                     _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_sz, _c_vp]),
+    "w4_paged_evict_scratch_words": (_c_sz, [ctypes.POINTER(PagedCache), _c_i64]),
     "w4_paged_evict": (_c_int, [ctypes.POINTER(PagedCache), _c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp,
                                 _c_vp]),
     "w4_token_logprobs_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64]),

@@ -155,12 +155,12 @@ def paged_evict(k_pages, v_pages, weight, table, lengths, new_table, keep: int, 
     assert new_table.dtype == torch.int32 and new_table.dim() == 2 and new_table.shape[0] == B
     assert new_table.is_contiguous() and new_table.device == dev
     assert 0 <= recent <= keep and 1 <= keep <= new_table.shape[1] * c.page_size, (keep, recent, new_table.shape)
-    kept = torch.empty((B, c.kv_heads, keep), dtype=torch.int32, device=dev)
     n = torch.empty(B, dtype=torch.int32, device=dev)
     lib = _lib.load()
+    scratch = torch.empty(lib.w4_paged_evict_scratch_words(c, keep), dtype=torch.int32, device=dev)
     rc = _on(dev, lambda st: lib.w4_paged_evict(
         c, DTYPES[k_pages.dtype], lengths.data_ptr(), new_table.data_ptr(), new_table.shape[1], keep, recent,
-        kept.data_ptr(), n.data_ptr(), st))
+        scratch.data_ptr(), n.data_ptr(), st))
     if rc:
         _lib.check(rc, "w4_paged_evict")
     return n

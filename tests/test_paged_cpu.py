@@ -42,8 +42,8 @@ def _attention(lib, c, dtype=0, q=FAKE, stride=256, heads=4, angles=10, scores=F
                                   scores, *ws, None)
 
 
-def _evict(lib, c, dtype=0, keep=10, recent=2, width=1, kept=FAKE):
-    return lib.w4_paged_evict(c, dtype, FAKE, FAKE, width, keep, recent, kept, FAKE, None)
+def _evict(lib, c, dtype=0, keep=10, recent=2, width=1, scratch=FAKE):
+    return lib.w4_paged_evict(c, dtype, FAKE, FAKE, width, keep, recent, scratch, FAKE, None)
 
 
 @pytest.mark.parametrize("change,code,word", BAD_CACHES)
@@ -74,7 +74,7 @@ def test_c_abi_rejects_bad_arguments(lib):
     assert _evict(lib, ok, keep=3, recent=4) == _lib.ERR_INVALID
     assert _evict(lib, ok, recent=-1) == _lib.ERR_INVALID
     assert _evict(lib, ok, keep=17) == _lib.ERR_INVALID
-    assert _evict(lib, ok, kept=None) == _lib.ERR_INVALID
+    assert _evict(lib, ok, scratch=None) == _lib.ERR_INVALID
     assert _evict(lib, _cache(weight=None)) == _lib.ERR_INVALID and b"null" in lib.w4_last_error()
     assert _evict(lib, _cache(rows=0)) == _lib.OK
 
