@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -38,6 +39,13 @@ struct Api {
   decltype(&w4_quantize_grouped) quantize_grouped;
   decltype(&w4_quantize) quantize;
   decltype(&w4_dequantize) dequantize;
+  decltype(&w4_paged_append) paged_append;
+  decltype(&w4_paged_attention_workspace_bytes) paged_attention_workspace_bytes;
+  decltype(&w4_paged_attention) paged_attention;
+  decltype(&w4_paged_evict_scratch_words) paged_evict_scratch_words;
+  decltype(&w4_paged_evict) paged_evict;
+  decltype(&w4_token_logprobs_workspace_bytes) token_logprobs_workspace_bytes;
+  decltype(&w4_token_logprobs) token_logprobs;
 };
 Api api{};
 PyObject* py_workspace = nullptr;  // (device index, stream, bytes) -> (address, bytes)
@@ -361,6 +369,224 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- paged cache and log probabilities
+// Each takes the arguments of the Python function of its name, all of them by position.
+
+bool tracked(const at::Tensor* t) { return t->requires_grad() && c10::GradMode::is_enabled(); }
+
+// The cache of plain, dense tensors; false: not plain.
+struct Cache {
+  const at::Tensor *k, *v, *weight, *table;
+  w4_paged_cache c;
+};
+bool cache_of(PyObject* k, PyObject* v, PyObject* table, PyObject* weight, Cache* out) {
+  out->k = plain(k);
+  out->v = plain(v);
+  out->table = plain(table);
+  out->weight = nullptr;
+  if (!out->k || !out->v || !out->table) return false;
+  if (weight != Py_None && !(out->weight = plain(weight))) return false;
+  const at::Tensor &kt = *out->k, &vt = *out->v, &tt = *out->table;
+  const c10::Device dev = kt.device();
+  if (act_code(kt.scalar_type()) < 0 || kt.dim() != 4 || vt.scalar_type() != kt.scalar_type() ||
+      vt.sizes() != kt.sizes() || vt.device() != dev || !kt.is_contiguous() || !vt.is_contiguous() || tracked(&kt) ||
+      tracked(&vt))
+    return false;
+  if (tt.scalar_type() != at::kInt || tt.dim() != 2 || tt.device() != dev || !tt.is_contiguous() || tt.size(1) < 1)
+    return false;
+  if (out->weight) {
+    const at::Tensor& w = *out->weight;
+    if (w.scalar_type() != at::kFloat || w.dim() != 3 || w.sizes() != kt.sizes().slice(0, 3) || w.device() != dev ||
+        !w.is_contiguous() || tracked(&w))
+      return false;
+  }
+  out->c = w4_paged_cache{kt.mutable_data_ptr(),
+                          vt.mutable_data_ptr(),
+                          out->weight ? static_cast<float*>(out->weight->mutable_data_ptr()) : nullptr,
+                          static_cast<const int32_t*>(tt.const_data_ptr()),
+                          kt.size(0),
+                          kt.size(1),
+                          kt.size(2),
+                          kt.size(3),
+                          tt.size(0),
+                          tt.size(1)};
+  return (out->c.head_dim == 64 || out->c.head_dim == 128) && current(dev);
+}
+
+// [n, width] like the cache, rows dense and 16-byte aligned.
+bool rows_fit(const at::Tensor* t, int64_t n, int64_t width, const at::Tensor& like) {
+  return t && t->dim() == 2 && t->size(0) == n && t->size(1) == width && t->scalar_type() == like.scalar_type() &&
+         t->device() == like.device() && t->stride(1) == 1 && t->stride(0) % 8 == 0 &&
+         (uintptr_t)t->const_data_ptr() % 16 == 0 && !tracked(t);
+}
+
+bool index_fit(const at::Tensor* t, int64_t n, c10::Device dev) {
+  return t && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && t->device() == dev &&
+         t->is_contiguous();
+}
+
+bool angles_fit(const at::Tensor* cos, const at::Tensor* sin, int64_t d, c10::Device dev) {
+  for (const at::Tensor* t : {cos, sin})
+    if (!t || t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(1) != d / 2 || t->size(0) < 1 ||
+        t->device() != dev || !t->is_contiguous() || (uintptr_t)t->const_data_ptr() % 16 != 0)
+      return false;
+  return cos->size(0) == sin->size(0);
+}
+
+const int32_t* ints(const at::Tensor* t) { return static_cast<const int32_t*>(t->const_data_ptr()); }
+const float* floats(const at::Tensor* t) { return static_cast<const float*>(t->const_data_ptr()); }
+
+// (k, v, cos, sin, k_pages, v_pages, table, rows, slots, positions, weight) -> True
+PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Cache p;
+  if (n != 11 || !api.paged_append || !quiet() || !cache_of(args[4], args[5], args[6], args[10], &p)) Py_RETURN_NONE;
+  const at::Tensor *k = plain(args[0]), *v = plain(args[1]), *cos = plain(args[2]), *sin = plain(args[3]);
+  const at::Tensor *rows = plain(args[7]), *slots = plain(args[8]), *positions = plain(args[9]);
+  if (!k || k->dim() != 2) Py_RETURN_NONE;
+  const int64_t T = k->size(0), width = p.c.kv_heads * p.c.head_dim;
+  const c10::Device dev = p.k->device();
+  if (!rows_fit(k, T, width, *p.k) || !rows_fit(v, T, width, *p.k) || !angles_fit(cos, sin, p.c.head_dim, dev) ||
+      !index_fit(rows, T, dev) || !index_fit(slots, T, dev) || !index_fit(positions, T, dev))
+    Py_RETURN_NONE;
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.paged_append(&p.c, act_code(p.k->scalar_type()), k->const_data_ptr(), v->const_data_ptr(), k->stride(0),
+                        v->stride(0), T, ints(rows), ints(slots), ints(positions), floats(cos), floats(sin),
+                        cos->size(0), stream);
+  Py_END_ALLOW_THREADS
+  if (!check(rc, "w4_paged_append")) return nullptr;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k, v, cos, sin, k_pages, v_pages, table, lengths, positions, weight) -> out
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Cache p;
+  if (n != 11 || !api.paged_attention || !quiet() || !cache_of(args[5], args[6], args[7], args[10], &p)) Py_RETURN_NONE;
+  const at::Tensor *q = plain(args[0]), *k = plain(args[1]), *v = plain(args[2]), *cos = plain(args[3]),
+                   *sin = plain(args[4]), *lengths = plain(args[8]), *positions = plain(args[9]);
+  if (!q || q->dim() != 2) Py_RETURN_NONE;
+  const int64_t B = p.c.rows, d = p.c.head_dim, width = p.c.kv_heads * d;
+  const c10::Device dev = p.k->device();
+  if (q->size(1) < 1 || q->size(1) % width != 0 || !rows_fit(q, B, q->size(1), *p.k) ||
+      !rows_fit(k, B, width, *p.k) || !rows_fit(v, B, width, *p.k) || !angles_fit(cos, sin, d, dev) ||
+      !index_fit(lengths, B, dev) || !index_fit(positions, B, dev) || B < 1)
+    Py_RETURN_NONE;
+  const int64_t heads = q->size(1) / d;
+  at::Tensor out = empty({B, q->size(1)}, p.k->scalar_type(), dev), scores;
+  if (p.weight) scores = empty({B * heads * p.c.width * p.c.page_size}, at::kFloat, dev);
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  void* ws;
+  size_t ws_bytes;
+  if (!workspace(dev, stream, api.paged_attention_workspace_bytes(B, heads, p.c.kv_heads, d), &ws, &ws_bytes))
+    return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.paged_attention(&p.c, act_code(p.k->scalar_type()), q->const_data_ptr(), k->const_data_ptr(),
+                           v->const_data_ptr(), q->stride(0), k->stride(0), v->stride(0), heads, ints(lengths),
+                           ints(positions), floats(cos), floats(sin), cos->size(0), out.mutable_data_ptr(),
+                           scores.defined() ? static_cast<float*>(scores.mutable_data_ptr()) : nullptr, ws, ws_bytes,
+                           stream);
+  Py_END_ALLOW_THREADS
+  if (!check(rc, "w4_paged_attention")) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A Python int that fits; else -1.
+int64_t count_arg(PyObject* o) {
+  if (!PyLong_CheckExact(o)) return -1;
+  int overflow = 0;
+  const long long v = PyLong_AsLongLongAndOverflow(o, &overflow);
+  return overflow || v < 0 ? -1 : v;
+}
+
+// (k_pages, v_pages, weight, table, lengths, new_table, keep, recent) -> new lengths
+PyObject* paged_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Cache p;
+  if (n != 8 || !api.paged_evict || !quiet() || args[2] == Py_None ||
+      !cache_of(args[0], args[1], args[3], args[2], &p))
+    Py_RETURN_NONE;
+  const at::Tensor *lengths = plain(args[4]), *to = plain(args[5]);
+  const int64_t keep = count_arg(args[6]), recent = count_arg(args[7]), B = p.c.rows;
+  const c10::Device dev = p.k->device();
+  if (!index_fit(lengths, B, dev) || !to || to->scalar_type() != at::kInt || to->dim() != 2 || to->size(0) != B ||
+      to->device() != dev || !to->is_contiguous() || keep < 1 || recent < 0 || recent > keep || B < 1 ||
+      keep > to->size(1) * p.c.page_size)
+    Py_RETURN_NONE;
+  at::Tensor lens = empty({B}, at::kInt, dev),
+             scratch = empty({(int64_t)api.paged_evict_scratch_words(&p.c, keep)}, at::kInt, dev);
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.paged_evict(&p.c, act_code(p.k->scalar_type()), ints(lengths), ints(to), to->size(1), keep, recent,
+                       static_cast<int32_t*>(scratch.mutable_data_ptr()),
+                       static_cast<int32_t*>(lens.mutable_data_ptr()), stream);
+  Py_END_ALLOW_THREADS
+  if (!check(rc, "w4_paged_evict")) return nullptr;
+  return THPVariable_Wrap(std::move(lens));
+  END_HANDLE_TH_ERRORS
+}
+
+// (logits, tokens or None, top) -> (logprob or None, entropy, top_logprob, top_token)
+PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3 || !api.token_logprobs || !quiet()) Py_RETURN_NONE;
+  const at::Tensor* x = plain(args[0]);
+  if (!x || x->dim() != 2 || tracked(x)) Py_RETURN_NONE;
+  const int dt = x->scalar_type() == at::kFloat ? W4_DTYPE_FP32 : act_code(x->scalar_type());
+  const int64_t R = x->size(0), V = x->size(1), top = count_arg(args[2]);
+  const c10::Device dev = x->device();
+  if (dt < 0 || R < 1 || V < 1 || top < 0 || top > 64 || top > V || x->stride(1) != 1 || x->stride(0) < 0 ||
+      !current(dev))
+    Py_RETURN_NONE;
+  const at::Tensor* tokens = args[1] == Py_None ? nullptr : plain(args[1]);
+  if (args[1] != Py_None && (!tokens || tokens->scalar_type() != at::kLong || tokens->dim() != 1 ||
+                             tokens->size(0) != R || tokens->device() != dev || !tokens->is_contiguous()))
+    Py_RETURN_NONE;
+  at::Tensor logprob, entropy = empty({R}, at::kFloat, dev), top_logprob = empty({R, top}, at::kFloat, dev),
+             top_token = empty({R, top}, at::kLong, dev);
+  if (tokens) logprob = empty({R}, at::kFloat, dev);
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  void* ws;
+  size_t ws_bytes;
+  if (!workspace(dev, stream, api.token_logprobs_workspace_bytes(R, V, top), &ws, &ws_bytes)) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.token_logprobs(x->const_data_ptr(), dt, R, V, x->stride(0),
+                          tokens ? static_cast<const int64_t*>(tokens->const_data_ptr()) : nullptr, top,
+                          logprob.defined() ? static_cast<float*>(logprob.mutable_data_ptr()) : nullptr,
+                          static_cast<float*>(entropy.mutable_data_ptr()),
+                          static_cast<float*>(top_logprob.mutable_data_ptr()),
+                          static_cast<int64_t*>(top_token.mutable_data_ptr()), ws, ws_bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (!check(rc, "w4_token_logprobs")) return nullptr;
+  PyObject* first = Py_None;
+  if (logprob.defined()) first = THPVariable_Wrap(std::move(logprob));
+  else Py_INCREF(first);
+  return Py_BuildValue("(NNNN)", first, THPVariable_Wrap(std::move(entropy)), THPVariable_Wrap(std::move(top_logprob)),
+                       THPVariable_Wrap(std::move(top_token)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (addresses of the paged cache's and the log probabilities' C-ABI functions in Api's order)
+PyObject* init_paged(PyObject*, PyObject* args) {
+  unsigned long long p[7];
+  if (!PyArg_ParseTuple(args, "(KKKKKKK)", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6])) return nullptr;
+  api.paged_append = reinterpret_cast<decltype(api.paged_append)>(p[0]);
+  api.paged_attention_workspace_bytes = reinterpret_cast<decltype(api.paged_attention_workspace_bytes)>(p[1]);
+  api.paged_attention = reinterpret_cast<decltype(api.paged_attention)>(p[2]);
+  api.paged_evict_scratch_words = reinterpret_cast<decltype(api.paged_evict_scratch_words)>(p[3]);
+  api.paged_evict = reinterpret_cast<decltype(api.paged_evict)>(p[4]);
+  api.token_logprobs_workspace_bytes = reinterpret_cast<decltype(api.token_logprobs_workspace_bytes)>(p[5]);
+  api.token_logprobs = reinterpret_cast<decltype(api.token_logprobs)>(p[6]);
+  Py_RETURN_NONE;
+}
+
 // (addresses of the C-ABI functions in Api's order, workspace, check)
 PyObject* init(PyObject*, PyObject* args) {
   unsigned long long p[7];
@@ -384,6 +610,11 @@ PyObject* init(PyObject*, PyObject* args) {
 
 #define W4_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"init", init, METH_VARARGS, nullptr},
+                         {"init_paged", init_paged, METH_VARARGS, nullptr},
+                         W4_FAST(paged_append),
+                         W4_FAST(paged_attention),
+                         W4_FAST(paged_evict),
+                         W4_FAST(token_logprobs),
                          W4_FAST(matmul),
                          W4_FAST(matmul_grouped),
                          W4_FAST(quantize),

@@ -147,6 +147,10 @@ def _load_ext(lib, workspace=None):
              "w4_quantize_grouped", "w4_quantize", "w4_dequantize")
     _int4_torch.init(tuple(ctypes.cast(getattr(lib, n), _c_vp).value for n in names),
                      workspace or gemm._workspace_address, check)
+    names = ("w4_paged_append", "w4_paged_attention_workspace_bytes", "w4_paged_attention",
+             "w4_paged_evict_scratch_words", "w4_paged_evict", "w4_token_logprobs_workspace_bytes",
+             "w4_token_logprobs")
+    _int4_torch.init_paged(tuple(ctypes.cast(getattr(lib, n), _c_vp).value for n in names))
     return _int4_torch
 
 

@@ -83,6 +83,9 @@ def paged_append(k, v, cos, sin, k_pages, v_pages, table, rows, slots, positions
     A token whose row, slot, page or position is out of range (any negative number:
     padding) is left out.
     """
+    if _lib.ext is not None and _lib.ext.paged_append(k, v, cos, sin, k_pages, v_pages, table, rows, slots, positions,
+                                                      weight):
+        return  # plain operands: the same call without Python's share of its cost
     _no_grad(k, v, k_pages, v_pages, weight)
     c = _cache(k_pages, v_pages, table, weight)
     dev, T = k_pages.device, k.shape[0]
@@ -113,6 +116,10 @@ def paged_attention(q, k, v, cos, sin, k_pages, v_pages, table, lengths, positio
     table, a page outside the pool or a position outside the tables: the row's output
     is NaN.
     """
+    if _lib.ext is not None:
+        out = _lib.ext.paged_attention(q, k, v, cos, sin, k_pages, v_pages, table, lengths, positions, weight)
+        if out is not None:
+            return out
     _no_grad(q, k, v, k_pages, v_pages, weight)
     c = _cache(k_pages, v_pages, table, weight)
     dev, dtype, B = k_pages.device, k_pages.dtype, table.shape[0]
@@ -147,6 +154,10 @@ def paged_evict(k_pages, v_pages, weight, table, lengths, new_table, keep: int, 
     left whole; the pages of ``new_table`` must not be among them, nor stand in it twice.
     A row of length < 0, or longer than its table, is left alone (-1).
     """
+    if _lib.ext is not None:
+        n = _lib.ext.paged_evict(k_pages, v_pages, weight, table, lengths, new_table, keep, recent)
+        if n is not None:
+            return n
     _no_grad(k_pages, v_pages, weight)
     assert weight is not None
     c = _cache(k_pages, v_pages, table, weight)

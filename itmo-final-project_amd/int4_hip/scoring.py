@@ -31,6 +31,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
     finite maximum (all -inf, a +inf or a NaN among its logits).  Launches on the current
     stream; no part in autograd.
     """
+    if _lib.ext is not None:  # plain operands: the same call without Python's share of its cost
+        r = _lib.ext.token_logprobs(logits, tokens, top)
+        if r is not None:
+            return TokenLogprobs(*r)
     assert logits.dtype in DTYPES and logits.dim() == 2 and logits.is_cuda, (logits.dtype, logits.shape)
     assert not (torch.is_grad_enabled() and logits.requires_grad), \
         "token_logprobs has no backward pass: call it under torch.no_grad()"
