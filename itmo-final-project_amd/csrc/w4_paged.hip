@@ -111,36 +111,53 @@ __device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __r
                                           AttnItem* it) {
   const int lane = threadIdx.x & 63;
   auto length = [&](int r) { return r + lane < c.rows ? lengths[r + lane] : -1; };
-  auto units = [&](int len) { return len >= 0 && len < c.capacity() ? len / UP + 1 : 1; };
-  int len = length(0), pos = lane < c.rows ? positions[lane] : 0;
-  float all = lane < c.rows ? (float)units(len) : 0.f;
-  for (int r = 64; r < c.rows; r += 64) all += r + lane < c.rows ? (float)units(length(r)) : 0.f;
+  auto position = [&](int r) { return r + lane < c.rows ? positions[r + lane] : 0; };
+  auto units = [&](int r, int len) {
+    return r + lane >= c.rows ? 0 : len >= 0 && len < c.capacity() ? len / UP + 1 : 1;
+  };
+  // the first 128 rows' stay in registers
+  const int len0 = length(0), pos0 = position(0), len1 = length(64), pos1 = position(64);
+  const float nu0 = (float)units(0, len0), nu1 = (float)units(64, len1);
+  float all = nu0 + nu1;
+  for (int r = 128; r < c.rows; r += 64) all += (float)units(r, length(r));
   all = wave_sum(all);
   int per = (int)fminf(ceilf(all * ((float)tiles / kAttnItems)), 1e9f);
   per = max(per, kAttnMinUnits);
   if ((int64_t)c.rows * tiles > kPagedCounters) per = 1 << 30;  // no counters for parts to meet at
   int base = 0;
-  for (int r = 0; r < c.rows; r += 64) {
-    if (r) len = length(r), pos = r + lane < c.rows ? positions[r + lane] : 0;
-    const int nu = units(len);
+  // The rows r.. whose parts are of the size class asked for: whether the item is among them.
+  auto among = [&](int r, int len, int pos, int size, float quarter) __attribute__((always_inline)) {
+    const int nu = units(r, len);
     const int of = max(per, min((nu + at_once - 1) / at_once, 2 * kAttnMinUnits));
-    const int parts = r + lane < c.rows ? (nu + of - 1) / of : 0;
+    int parts = (nu + of - 1) / of;
+    if (quarter > 0.f && min((int)((float)nu / (float)max(parts, 1) * quarter), 3) != size) parts = 0;
     const int upto = base + wave_scan(parts * tiles);
     const int end = __builtin_amdgcn_readlane(upto, 63);
-    if (item < end) {
-      const int i = __popcll(__ballot(item >= upto));
-      it->parts = __builtin_amdgcn_readlane(parts, i);
-      const int rem = item - (__builtin_amdgcn_readlane(upto, i) - it->parts * tiles);
-      it->b = r + i;
-      it->tile = rem / it->parts;
-      it->part = rem - it->tile * it->parts;
-      it->first = item - it->part;
-      it->len = __builtin_amdgcn_readlane(len, i);
-      it->pos = __builtin_amdgcn_readlane(pos, i);
-      return true;
+    if (item >= end) {
+      base = end;
+      return false;
     }
-    base = end;
+    const int i = __popcll(__ballot(item >= upto));
+    it->parts = __builtin_amdgcn_readlane(parts, i);
+    const int rem = item - (__builtin_amdgcn_readlane(upto, i) - it->parts * tiles);
+    it->b = r + i;
+    it->tile = rem / it->parts;
+    it->part = rem - it->tile * it->parts;
+    it->first = item - it->part;
+    it->len = __builtin_amdgcn_readlane(len, i);
+    it->pos = __builtin_amdgcn_readlane(pos, i);
+    return true;
+  };
+  // Where the chip is full, the rows with the longest parts first, by quarters of the longest: the short ones fill the
+  // gaps at the end (32 rows of up to 4000 slots 31.1 us instead of 32.6, 20 of up to 9000 40.4 instead of 43.1).
+  const bool ordered = c.rows >= 8 && c.rows <= 128 && per > kAttnMinUnits;
+  const float quarter = ordered ? 4.f / fminf(wave_max(fmaxf(nu0, nu1)), (float)per) : 0.f;
+  for (int size = ordered ? 3 : 0; size >= 0; --size) {
+    if (among(0, len0, pos0, size, quarter)) return true;
+    if (c.rows > 64 && among(64, len1, pos1, size, quarter)) return true;
   }
+  for (int r = 128; r < c.rows; r += 64)
+    if (among(r, length(r), position(r), 0, 0.f)) return true;
   return false;
 }
 
