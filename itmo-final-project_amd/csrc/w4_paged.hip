@@ -3,6 +3,8 @@
 // them, and eviction by accumulated attention weight.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "w4_common.hpp"
 
 namespace w4 {
@@ -571,17 +573,17 @@ __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnAr
     const float* const part = a.part + (int64_t)first * stride + (g & 15) * D + i * 4;
     const float* const st = a.stats + ((int64_t)first * 16 + (g & 15)) * 2;
     Share x;
-    for (int p0 = run; p0 < parts; p0 += RUNS * 4) {
-      f32x4 t[4];
-      f32x2 ml[4];
+    for (int p0 = run; p0 < parts; p0 += RUNS * 8) {
+      f32x4 t[8];
+      f32x2 ml[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 8; ++k) {
         const int64_t p = min(p0 + k * RUNS, parts - 1);
         t[k] = *reinterpret_cast<const f32x4*>(part + p * stride);
         ml[k] = *reinterpret_cast<const f32x2*>(st + p * 32);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 8; ++k)
         if (p0 + k * RUNS < parts) x.add(ml[k][0], ml[k][1], t[k]);
     }
     red[tid] = x.t;
@@ -1000,8 +1002,6 @@ extern "C" int w4_paged_append(const w4_paged_cache* cache, int dtype, const voi
 
 namespace {
 
-constexpr int kLaterFloats = 1024;
-
 struct PagedAttnPlan {
   int64_t tiles, items;         // tiles of up to 16 query heads a row, workgroups
   size_t part, first, bytes;    // offsets of PagedAttnArgs' part and first in the workspace, and all of it
@@ -1079,11 +1079,15 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   a.scale = 1.f / sqrtf((float)cache->head_dim);
   a.g = (int)(num_heads / cache->kv_heads);
   a.htiles = (int)(p.tiles / cache->kv_heads);
-  // The weights need a launch behind the attention anyway; without them the last part joins, unless
-  // a tile's outputs are more than one quad a thread.
-  a.later = a.scores || (a.g < 16 ? a.g : 16) * cache->head_dim > kLaterFloats;
-  const int quads = (a.g < 16 ? a.g : 16) * (int)cache->head_dim / 4;
-  a.at_once = a.later ? 1 << 20 : 8 * (64 * w4::kAttnWaves / quads);
+  // The weights need a launch behind the attention anyway.  Without them the last part joins, unless a tile's outputs
+  // are more than a quad a thread, or its parts may be more than the joining reads in two goes (24 heads of 64 on
+  // one key-value head, 131000 slots in 128 parts: 36 us, with a launch of its own 20).
+  const int quads = (a.g < 16 ? a.g : 16) * (int)cache->head_dim / 4, threads = 64 * w4::kAttnWaves;
+  a.at_once = quads <= threads ? 8 * (threads / quads) : 0;
+  const int64_t units = cache->width * cache->page_size * cache->head_dim / 4096 + 1;
+  const int64_t parts = std::min(w4::kAttnItems / (cache->rows * p.tiles) + 1, units / w4::kAttnMinUnits + 1);
+  a.later = a.scores || quads > threads || parts > 2 * a.at_once + 1;
+  if (a.later) a.at_once = 1 << 20;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == W4_DTYPE_BF16)
     return cache->head_dim == 64 ? launch_paged_attention<W4_DTYPE_BF16, 64>(a, p.items, st)
