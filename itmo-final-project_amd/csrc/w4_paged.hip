@@ -97,17 +97,18 @@ struct AttnItem {
   int len, pos;                     // of the row
 };
 
-constexpr int kAttnWaves = 4;
-constexpr int kAttnItems = 256;     // parts the tokens of a batch are cut into, about
-constexpr int kAttnMinUnits = 4;    // units of a part at least: one a wave
+// Workgroups of four waves, the tokens of a batch cut into about 256 parts; of one wave and 1024 parts where there are
+// many rows of a bounded length (see paged_attn_plan).  Parts have four units of slots at least.
+constexpr int kAttnWaves = 4, kAttnItems = 256, kAttnOneWaveItems = 1024;
+constexpr int kAttnMinUnits = 4;
 constexpr int kPagedCounters = W4_WORKSPACE_COUNTER_BYTES / 4;
 
 // Which item this is, the same in every wave and launch.  The lengths lie on the GPU, so the split is made here:
-// every row is cut into equal parts of at most `per` units of UP slots, per = all units / kAttnItems, so that short
+// every row is cut into equal parts of at most `per` units of UP slots, per = all units / ITEMS, so that short
 // rows stay whole and long ones spread over the chip, whatever else is in the batch.  Rows that need no
 // attention (idle, refused) are one part.  `at_once`: the parts that the joining reads together; a row has more only if
 // its parts would be longer than twice the least (4000 slots of 32 / 8 heads of 128: 16 parts 13.1 us, 32 14.6).
-template <int UP>
+template <int UP, int ITEMS>
 __device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __restrict__ lengths,
                                           const int32_t* __restrict__ positions, int tiles, int at_once, int item,
                                           AttnItem* it) {
@@ -123,7 +124,7 @@ __device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __r
   float all = nu0 + nu1;
   for (int r = 128; r < c.rows; r += 64) all += (float)units(r, length(r));
   all = wave_sum(all);
-  int per = (int)fminf(ceilf(all * ((float)tiles / kAttnItems)), 1e9f);
+  int per = (int)fminf(ceilf(all * ((float)tiles / ITEMS)), 1e9f);
   per = max(per, kAttnMinUnits);
   if ((int64_t)c.rows * tiles > kPagedCounters) per = 1 << 30;  // no counters for parts to meet at
   int base = 0;
@@ -227,7 +228,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-// One workgroup = one part of one row's slots for up to 16 query heads of one key-value head; its four waves take
+// One workgroup = one part of one row's slots for up to 16 query heads of one key-value head; its waves take
 // units of UP = 4096 / D slots in turn (16 KB of keys and values).
 //
 // Both products are 16x16x32 matrix instructions, transposed: scores S^T = K Q^T, slots by heads, then O^T = V^T P^T.
@@ -236,25 +237,25 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 // operand, which never leaves its registers.  Keys go from memory to the operands; values go through LDS, which
 // transposes them on reading.  The running maximum of a head is only raised when a score passes it by 2^8 (its value
 // cancels in the end), so that most units need no exchange between lanes.
-template <int DT, int D>
-__global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(PagedAttnArgs a) {
+template <int DT, int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int KB = 128 / D, UP = 32 * KB, NJ = D / 32, ND = D / 16, VR = 512 / D, NP = Split<DT>::N;
   constexpr int KROW = D + 8;              // halfwords of a key row in LDS: sixteen rows on different banks
   constexpr int VROW = D == 64 ? 72 : 144; // of a value row: four rows of 32 bytes on different banks
   constexpr int OROW = D + 4;              // floats of an output row in LDS
-  constexpr int WAVE_H = UP * (KROW + VROW), kThreads = 64 * kAttnWaves;
+  constexpr int WAVE_H = UP * (KROW + VROW), ITEMS = W == 1 ? kAttnOneWaveItems : kAttnItems, kThreads = 64 * W;
   static_assert(16 * OROW * 2 <= WAVE_H, "a wave's outputs take its tokens' place");
   typedef typename Act<DT>::frag frag;
-  __shared__ __attribute__((aligned(16))) uint16_t kv_s[kAttnWaves][WAVE_H];
+  __shared__ __attribute__((aligned(16))) uint16_t kv_s[W][WAVE_H];
   __shared__ __attribute__((aligned(16))) uint16_t new_s[2][D];
-  __shared__ float m_s[kAttnWaves][16], l_s[kAttnWaves][16];
-  __shared__ int bad_s[kAttnWaves];
+  __shared__ float m_s[W][16], l_s[W][16];
+  __shared__ int bad_s[W];
   __shared__ unsigned arrived_s;
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, c = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   AttnItem it;
-  if (!find_item<UP>(a.c, a.lengths, a.positions, a.c.nkv * a.htiles, a.at_once, blockIdx.x, &it)) return;
+  if (!find_item<UP, ITEMS>(a.c, a.lengths, a.positions, a.c.nkv * a.htiles, a.at_once, blockIdx.x, &it)) return;
   const int b = it.b, h = it.tile / a.htiles, ht = it.tile - h * a.htiles;
   const int h0 = h * a.g + ht * 16, gh = min(a.g - ht * 16, 16);  // query heads of the row
   const int nh = a.c.nkv * a.g;
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
   int u = u0 + wv, ids = 0;
   if (u < u1) {  // on their way before the query is at hand
     load(u, load_ids(u));
-    ids = load_ids(min(u + kAttnWaves, u1 - 1));
+    ids = load_ids(min(u + W, u1 - 1));
   }
 
   // the query: heads past gh copy another and count for nothing
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
   }
   // The wave that takes the row's last unit rotates the new key, keeps it and the value at hand and writes them to
   // the cache.
-  if (it.part == it.parts - 1 && wv == (nu - 1 - u0) % kAttnWaves) {
+  if (it.part == it.parts - 1 && wv == (nu - 1 - u0) % W) {
     const uint16_t* const kin = a.k + b * a.stride_k + h * D;
     float x[8], y[8];
     unpack8<DT>(*reinterpret_cast<const u32x4*>(kin + sd), x);
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
     m = -__builtin_inff(), l = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (; u < u1; u += kAttnWaves) {
+    for (; u < u1; u += W) {
       const int base = u * UP;
       const bool last = base + UP > len;  // the new token is in this unit, and what lies past it
       if (last) {
@@ -372,9 +373,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
         *reinterpret_cast<u32x4*>(kw + krow(i) * KROW + sd) = kr[i];
         *reinterpret_cast<u32x4*>(vw + (i * VR + srow) * VROW + sd) = vr[i];
       }
-      if (u + kAttnWaves < u1) {  // the next unit's loads travel under the rest
-        load(u + kAttnWaves, ids);
-        ids = load_ids(min(u + 2 * kAttnWaves, u1 - 1));
+      if (u + W < u1) {  // the next unit's loads travel under the rest
+        load(u + W, ids);
+        ids = load_ids(min(u + 2 * W, u1 - 1));
       }
       f32x4 s[KB][2];
 #pragma unroll
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
     precise = false;
     u = u0 + wv;
     load(u, load_ids(u));
-    ids = load_ids(min(u + kAttnWaves, u1 - 1));
+    ids = load_ids(min(u + W, u1 - 1));
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -483,7 +484,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
   __syncthreads();
   int refused = 0;
 #pragma unroll
-  for (int w = 0; w < kAttnWaves; ++w) refused |= bad_s[w];
+  for (int w = 0; w < W; ++w) refused |= bad_s[w];
   const int quads = gh * (D / 4), stride = min(a.g, 16) * D;
   const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(a.part + (int64_t)it.first * stride), (short)0, it.parts * stride * 4, kPagedBufFlags);
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
     const int hd = i / (D / 4), d = i % (D / 4) * 4;
     Share x;
 #pragma unroll
-    for (int w = 0; w < kAttnWaves; ++w)
+    for (int w = 0; w < W; ++w)
       x.add(m_s[w][hd], l_s[w][hd],
             *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(kv_s[w]) + hd * OROW + d));
     if (refused) x.M = x.L = __builtin_nanf("");
@@ -521,36 +522,39 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void paged_attention_kernel(Pag
   __syncthreads();
   if (arrived_s != (unsigned)(it.parts - 1)) return;
   if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // Threads: the quads of the output (no more than there are threads), and several runs of parts beside each other.
+  // Threads: the quads of the output, and several runs of parts beside each other (or several goes, of a single wave).
   // Maxima, sums and outputs of eight parts travel together.
-  const int runs = kThreads / quads, run = tid / quads, i = tid - run * quads, hd = i / (D / 4);
+  const int runs = max(1, kThreads / quads), run = min(tid / quads, runs);
   f32x4* const red = reinterpret_cast<f32x4*>(&kv_s[0][0]);
   f32x2* const red_ml = reinterpret_cast<f32x2*>(red + kThreads);
-  Share x;
-  if (run < runs) {
-    for (int p0 = run; p0 < it.parts; p0 += runs * 8) {
-      f32x4 t[8];
-      f32x2 ml[8];
+  for (int i = tid - run * quads; i < quads; i += kThreads) {
+    const int hd = i / (D / 4);
+    Share x;
+    if (run < runs) {
+      for (int p0 = run; p0 < it.parts; p0 += runs * 8) {
+        f32x4 t[8];
+        f32x2 ml[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int p = min(p0 + k * runs, it.parts - 1);
-        t[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (uint32_t)(p * stride + i * 4) * 4u,
-                                                                               0, kPagedCoherentAux));
-        ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, (uint32_t)(p * 16 + hd) * 8u, 0,
-                                                                               kPagedCoherentAux));
+        for (int k = 0; k < 8; ++k) {
+          const int p = min(p0 + k * runs, it.parts - 1);
+          t[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                               rp, (uint32_t)(p * stride + i * 4) * 4u, 0, kPagedCoherentAux));
+          ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, (uint32_t)(p * 16 + hd) * 8u, 0,
+                                                                                 kPagedCoherentAux));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (p0 + k * runs < it.parts) x.add(ml[k][0], ml[k][1], t[k]);
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (p0 + k * runs < it.parts) x.add(ml[k][0], ml[k][1], t[k]);
     }
+    if (runs > 1) {  // (then this is the only go, of all threads)
+      if (run < runs) red[tid] = x.t, red_ml[tid] = f32x2{x.M, x.L};
+      __syncthreads();
+      if (run == 0)
+        for (int r = 1; r < runs; ++r) x.add(red_ml[r * quads + i][0], red_ml[r * quads + i][1], red[r * quads + i]);
+    }
+    if (run == 0) *reinterpret_cast<u32x2*>(out + i * 4) = x.template out<DT>();
   }
-  if (runs > 1) {
-    if (run < runs) red[tid] = x.t, red_ml[tid] = f32x2{x.M, x.L};
-    __syncthreads();
-    if (run == 0)
-      for (int r = 1; r < runs; ++r) x.add(red_ml[r * quads + i][0], red_ml[r * quads + i][1], red[r * quads + i]);
-  }
-  if (run == 0) *reinterpret_cast<u32x2*>(out + i * 4) = x.template out<DT>();
 }
 
 // What the attention leaves to a second launch.  Workgroups [0, rows * heads): the parts of one row and query head
@@ -596,7 +600,8 @@ __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnAr
     return;
   }
   AttnItem it;
-  if (!find_item<UP>(a.c, a.lengths, a.positions, a.c.nkv, a.at_once, blockIdx.x - a.c.rows * nh, &it)) return;
+  const int item = blockIdx.x - a.c.rows * nh;
+  if (!find_item<UP, kAttnItems>(a.c, a.lengths, a.positions, a.c.nkv, a.at_once, item, &it)) return;
   const int b = it.b, h = it.tile, len = it.len, pos = it.pos;
   if (len < 0 || len >= a.c.capacity() || (uint64_t)(int64_t)pos >= (uint64_t)a.angles) return;
   const int nu = len / UP + 1;
@@ -1004,14 +1009,22 @@ namespace {
 
 struct PagedAttnPlan {
   int64_t tiles, items;         // tiles of up to 16 query heads a row, workgroups
+  bool one_wave;                // those of one wave each
   size_t part, first, bytes;    // offsets of PagedAttnArgs' part and first in the workspace, and all of it
 };
 
-bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, PagedAttnPlan* p) {
+// `units` of slots that a row has at most.  More rows and tiles than the chip holds workgroups of four waves (two a CU:
+// LDS) are faster a wave each, four or eight to a CU: of 32 / 8 heads of 64, 500 rows of up to 100 slots 29.9 us
+// instead of 73.2, 96 of them 9.9 instead of 14.5, 200 of up to 1000 46.6 instead of 51.0.  Long rows are not:
+// their units follow each other in one wave (64 of 4000 87.8 instead of 82.7; one of 131000 among 31 short ones 69
+// instead of 49).
+bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, int64_t units,
+                     PagedAttnPlan* p) {
   if (rows < 0 || num_heads < 1 || kv_heads < 1 || num_heads % kv_heads) return false;
   const int64_t g = num_heads / kv_heads;
   p->tiles = kv_heads * ((g + 15) / 16);
-  p->items = w4::kAttnItems + rows * p->tiles + 1;
+  p->one_wave = rows * p->tiles > 2 * device_cu_count() && units <= 128;
+  p->items = (p->one_wave ? w4::kAttnOneWaveItems : w4::kAttnItems) + rows * p->tiles + 1;
   if (p->items >= (1 << 22)) return false;
   p->part = W4_WORKSPACE_COUNTER_BYTES + (size_t)p->items * 128;
   p->first = p->part;
@@ -1021,8 +1034,10 @@ bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t 
 }
 
 template <int DT, int D>
-int launch_paged_attention(const w4::PagedAttnArgs& a, int64_t items, hipStream_t st) {
-  w4::paged_attention_kernel<DT, D><<<dim3((unsigned)items), 64 * w4::kAttnWaves, 0, st>>>(a);
+int launch_paged_attention(const w4::PagedAttnArgs& a, const PagedAttnPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)p.items);
+  if (p.one_wave) w4::paged_attention_kernel<DT, D, 1><<<grid, 64, 0, st>>>(a);
+  else w4::paged_attention_kernel<DT, D, w4::kAttnWaves><<<grid, 64 * w4::kAttnWaves, 0, st>>>(a);
   if (const int rc = check_launch("w4_paged_attention")) return rc;
   if (!a.later) return W4_OK;
   const int64_t more = a.scores ? w4::kAttnItems + (int64_t)a.c.rows * a.c.nkv + 1 : 0;
@@ -1035,7 +1050,7 @@ int launch_paged_attention(const w4::PagedAttnArgs& a, int64_t items, hipStream_
 extern "C" size_t w4_paged_attention_workspace_bytes(int64_t rows, int64_t num_heads, int64_t kv_heads,
                                                      int64_t head_dim) {
   PagedAttnPlan p;
-  return rows > 0 && paged_attn_plan(rows, num_heads, kv_heads, head_dim, &p) ? p.bytes : 0;
+  return rows > 0 && paged_attn_plan(rows, num_heads, kv_heads, head_dim, 1, &p) ? p.bytes : 0;
 }
 
 extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const void* q, const void* k, const void* v,
@@ -1049,8 +1064,9 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
     return fail(W4_ERR_INVALID, "w4_paged_attention: %lld query heads on %lld key-value heads, %lld angles",
                 (long long)num_heads, (long long)cache->kv_heads, (long long)angles);
   if (cache->rows == 0) return W4_OK;
+  const int64_t units = cache->width * cache->page_size * cache->head_dim / 4096 + 1;
   PagedAttnPlan p;
-  if (!paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, &p) ||
+  if (!paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, units, &p) ||
       cache->rows * num_heads >= (1 << 23))
     return fail(W4_ERR_UNSUPPORTED, "w4_paged_attention: %lld rows of %lld heads", (long long)cache->rows,
                 (long long)num_heads);
@@ -1082,18 +1098,17 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   // The weights need a launch behind the attention anyway.  Without them the last part joins, unless a tile's outputs
   // are more than a quad a thread, or its parts may be more than the joining reads in two goes (24 heads of 64 on
   // one key-value head, 131000 slots in 128 parts: 36 us, with a launch of its own 20).
-  const int quads = (a.g < 16 ? a.g : 16) * (int)cache->head_dim / 4, threads = 64 * w4::kAttnWaves;
-  a.at_once = quads <= threads ? 8 * (threads / quads) : 0;
-  const int64_t units = cache->width * cache->page_size * cache->head_dim / 4096 + 1;
-  const int64_t parts = std::min(w4::kAttnItems / (cache->rows * p.tiles) + 1, units / w4::kAttnMinUnits + 1);
-  a.later = a.scores || quads > threads || parts > 2 * a.at_once + 1;
+  const int quads = (a.g < 16 ? a.g : 16) * (int)cache->head_dim / 4, threads = p.one_wave ? 64 : 64 * w4::kAttnWaves;
+  a.at_once = 8 * std::max(threads / quads, 1);
+  const int64_t parts = std::min(p.items / (cache->rows * p.tiles), units / w4::kAttnMinUnits + 1);
+  a.later = a.scores || quads > (p.one_wave ? 2 : 1) * threads || parts > 2 * a.at_once + 1;
   if (a.later) a.at_once = 1 << 20;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == W4_DTYPE_BF16)
-    return cache->head_dim == 64 ? launch_paged_attention<W4_DTYPE_BF16, 64>(a, p.items, st)
-                                 : launch_paged_attention<W4_DTYPE_BF16, 128>(a, p.items, st);
-  return cache->head_dim == 64 ? launch_paged_attention<W4_DTYPE_FP16, 64>(a, p.items, st)
-                               : launch_paged_attention<W4_DTYPE_FP16, 128>(a, p.items, st);
+    return cache->head_dim == 64 ? launch_paged_attention<W4_DTYPE_BF16, 64>(a, p, st)
+                                 : launch_paged_attention<W4_DTYPE_BF16, 128>(a, p, st);
+  return cache->head_dim == 64 ? launch_paged_attention<W4_DTYPE_FP16, 64>(a, p, st)
+                               : launch_paged_attention<W4_DTYPE_FP16, 128>(a, p, st);
 }
 
 extern "C" size_t w4_paged_evict_scratch_words(const w4_paged_cache* cache, int64_t keep) {

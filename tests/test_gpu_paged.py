@@ -92,6 +92,26 @@ def test_attention_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("nh,nkv,d", [(8, 4, 64), (16, 4, 128), (36, 4, 64)])
+def test_attention_more_rows_than_the_chip_holds(dtype, nh, nkv, d):
+    """Workgroups of one wave; two rows long enough that several share them, one of them with a page outside the pool."""
+    lens = [(13 * i) % 71 - 1 for i in range(140)]
+    lens[3], lens[70], lens[139] = 1500, 129, 4000 * 64 // d
+    print(f"[paged attention] {dtype} 140 rows of {nh}/{nkv}x{d}", flush=True)
+    for weights in (True, False):
+        c = R.attention_case(lens, nh, nkv, d, 32, dtype, seed=nh, weights=weights)
+        c["table"][139, 17] = c["k_pages"].shape[0]
+        c["v_pages"][c["table"][3, 30], 1, 3, 5] = math.inf
+        out = int4_hip.paged_attention(**_to(c))
+        want, mass, reach, _ = R.attention(**c)
+        rest = torch.arange(140) != 3
+        _check(out.cpu()[rest], want[rest], mass[rest], dtype)
+        # beside an infinity as in test_attention_not_finite
+        prob = (2.0 ** -8 * (1 + reach[3].clamp(max=40).max())).item()
+        _check(out[3], want[3], mass[3].nan_to_num(0, 0, 0), dtype, prob)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 def test_attention_steps_accumulate(dtype):
     """Several steps, lengths growing across a page's end: every step's state feeds the next."""
     lens = [14, 0, 30]
