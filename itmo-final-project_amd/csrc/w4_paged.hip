@@ -878,7 +878,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_place_kernel(EvictArgs a)
   for (int e = 0; e < 4; ++e) {
     const bool g = s + e < early && key[e] > edge, q = s + e < early && key[e] == edge;
     const int to = l + min(t, ties);
-    if ((g || (q && t < ties)) && to < want) kept[to] = s + e;  // (in bounds too if weights change under the call)
+    if ((g || (q && t < ties)) && (unsigned)to < (unsigned)want) kept[to] = s + e;  // (whatever the scratch holds)
     l += g, t += q;
   }
 }
