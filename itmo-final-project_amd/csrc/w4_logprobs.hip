@@ -14,6 +14,7 @@ constexpr int kLogMaxGroups = 192;              // groups that may hold alternat
 constexpr int kLogNear = 1024;                  // groups whose maxima LDS holds, of a row in one part
 constexpr int kLogSpare = 16;                   // groups too many, before the range of their maxima is narrowed again
 constexpr int kLogList = 512;
+constexpr int kLogRank = 128;                   // numbers ranked against each other
 constexpr int kLogBins = 2048;
 constexpr int64_t kLogMaxVocab = 1 << 22;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -131,11 +132,16 @@ __device__ __forceinline__ void narrow(const Each& each, uint64_t& lo, uint64_t&
   }
 }
 
-// One workgroup = one row and part of its blocks.  Everything of a logit is done when it is read: the sums of the softmax and
-// the entropy, relative to the lane's own maximum so far, and the maximum of its group of 128.  The last part of a row
-// to arrive joins the sums, in their order, and finds the alternatives: as many groups reach the top-th largest of the
-// groups' maxima as there are alternatives (or more, where they are equal), and no alternative lies outside of
-// them, so only those groups' logits are read again.
+// One workgroup = one row and part of its blocks.  Everything of a logit is done when it is read: the sums of the
+// softmax and the entropy, relative to the lane's own maximum so far, and the maximum of its group of 128.  The last
+// part of a row to arrive joins the sums, in their order, and finds the alternatives: as many groups reach the top-th
+// largest of the groups' maxima as there are alternatives (or more, where they are equal), and no alternative lies
+// outside of them, so only those groups' logits are read again.
+//
+// Bound by memory where there are many rows: 500 x 128256 bf16 with 20 alternatives in 31.5 us, 128 MB at 4.1 TB/s
+// (five operations and an exponential a logit beside it), 1000 x 32001 fp32 without in 24.0, 128 MB at 5.3 TB/s.  A
+// few rows are a chain of latencies, 8 with 5 alternatives 11.6 us; so are many short ones, a dozen barriers each and
+// four workgroups on a CU: 2000 x 1000 fp32 with 20 in 36 us.
 template <int DT>
 __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   typedef Logits<DT> T;
@@ -186,7 +192,8 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     const int i0 = blk * kLogBlock + wv * 2048 + lane * T::N;
     if ((blk + 1) * kLogBlock <= a.vocab) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) raw[j] = __builtin_nontemporal_load(reinterpret_cast<const typename T::vec*>(x + i0 + j * PIECE));
+      for (int j = 0; j < NV; ++j)
+        raw[j] = __builtin_nontemporal_load(reinterpret_cast<const typename T::vec*>(x + i0 + j * PIECE));
     } else {  // the row's last block
 #pragma unroll
       for (int j = 0; j < NV; ++j) raw[j] = load_at(i0 + j * PIECE);
@@ -271,8 +278,8 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     __syncthreads();
   }
   auto group_key = [&](int g) __attribute__((always_inline)) {
-    return near ? key_s[g]
-                : (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rp, (uint32_t)(a.parts * 4 + g) * 4u, 0, kLogCoherentAux);
+    if (near) return key_s[g];
+    return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rp, (uint32_t)(a.parts * 4 + g) * 4u, 0, kLogCoherentAux);
   };
   uint32_t gk[4];  // of the first 1024 groups, this thread's
   if (a.top) {
@@ -313,15 +320,21 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   if (lane == 0) wave_s[wv] = (int)low, groups_s[wv] = (int)high;
   if (tid == 0) found_s[0] = 0;
   __syncthreads();
-  for (int w = 0; w < kLogThreads / 64; ++w) low = min(low, (uint32_t)wave_s[w]), high = max(high, (uint32_t)groups_s[w]);
+  for (int w = 0; w < kLogThreads / 64; ++w)
+    low = min(low, (uint32_t)wave_s[w]), high = max(high, (uint32_t)groups_s[w]);
   uint64_t lo = low, hi = high;
   int wanted = a.top, above = 0, count = groups;  // (there are at least 64)
+  const int used = (a.vocab + 2047) / 2048 * 16;  // groups that hold any logits: the first ones
   __syncthreads();
-  narrow([&](auto f) { each_group([&](int, uint32_t k) { f((uint64_t)k); }); }, lo, hi, wanted, above, count, kLogSpare,
-         hist, wave_s, found_s);
+  if (used > a.top)
+    narrow([&](auto f) { each_group([&](int, uint32_t k) { f((uint64_t)k); }); }, lo, hi, wanted, above, count,
+           kLogSpare, hist, wave_s, found_s);
   __syncthreads();
   int held = 0;
-  if (above + count <= kLogMaxGroups) {  // in any order
+  if (used <= a.top) {  // all of them (no more than one block's; no alternative lies below the least maximum)
+    if (tid < used) groups_s[tid] = tid;
+    held = used;
+  } else if (above + count <= kLogMaxGroups) {  // in any order
     if (tid == 0) found_s[0] = 0;
     __syncthreads();
     each_group([&](int g, uint32_t k) {
@@ -385,6 +398,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
       }
     }
   };
+  const uint64_t most = (uint64_t)high << 32 | 0xFFFFFFFFu;
   uint64_t from = lo << 32;
   int n;
   for (;;) {
@@ -400,17 +414,36 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     n = found_s[0];
     if (n <= kLogList) break;
     // many equal or neighbouring logits: the threshold is sought among the members themselves, which are all different
-    uint64_t to = ~0ull;
+    uint64_t to = most;
     int want = a.top, over = 0;
     __syncthreads();
     narrow(members, from, to, want, over, n, kLogList - kMaxTop, hist, wave_s, found_s);
     __syncthreads();
   }
+  // Ranked one against all; of many, those that come into question (2000 x 1000 with 20: 36 us, 51 without this and
+  // the shorter way above).
+  const uint64_t* ranked = list;
+  if (n > kLogRank) {
+    uint64_t to = most;
+    int want = a.top, over = 0, left = n;
+    narrow([&](auto f) __attribute__((always_inline)) {
+      for (int i = tid; i < n; i += kLogThreads) f(list[i]);
+    }, from, to, want, over, left, kLogRank - kMaxTop, hist, wave_s, found_s);
+    __syncthreads();
+    if (tid == 0) found_s[0] = 0;
+    __syncthreads();
+    uint64_t* const some = reinterpret_cast<uint64_t*>(hist);
+    for (int i = tid; i < n; i += kLogThreads)
+      if (list[i] >= from) some[atomicAdd(&found_s[0], 1)] = list[i];
+    __syncthreads();
+    n = found_s[0];
+    ranked = some;
+  }
   for (int i = tid; i < n; i += kLogThreads) {
-    const uint64_t v = list[i];
+    const uint64_t v = ranked[i];
     int rank = 0;
 #pragma unroll 8
-    for (int j = 0; j < n; ++j) rank += list[j] > v;
+    for (int j = 0; j < n; ++j) rank += ranked[j] > v;
     if (rank < a.top) {
       const uint32_t key = (uint32_t)(v >> 32);
       const float l = key == 0xFFFFFFFFu ? __builtin_nanf("")
@@ -433,7 +466,8 @@ struct LogprobPlan {
   int64_t row_words, slice;  // words of scratch a row, rows of a launch
 };
 
-// A row is cut into parts of whole blocks while the launch has fewer than eight workgroups a CU.
+// A row is cut into parts of whole blocks while the launch has fewer than three workgroups a CU; more of them are no
+// faster.
 LogprobPlan logprob_plan(int64_t rows, int64_t vocab) {
   LogprobPlan p;
   p.blocks = (int)((vocab + w4::kLogBlock - 1) / w4::kLogBlock);
