@@ -109,8 +109,9 @@ def paged_attention(q, k, v, cos, sin, k_pages, v_pages, table, lengths, positio
     int32 [rows]: the tokens a row has in the cache, ``positions`` int32 [rows]: the new
     tokens' positions.  The new key and value go to slot ``lengths[b]``, then the row's
     query attends to slots 0..lengths[b] in fp32; with ``weight`` each of them is
-    credited the probabilities its head's group gave it.  ``lengths`` is left as it is
-    (all layers of a model share it).
+    credited the probabilities its head's group gave it; the call then holds rows * heads
+    * width * page_size fp32 scores, so a table is best passed no wider than its longest
+    row needs.  ``lengths`` is left as it is (all layers of a model share it).
 
     ``lengths[b] < 0``: an idle row, its output zero, nothing written.  A slot past the
     table, a page outside the pool or a position outside the tables: the row's output

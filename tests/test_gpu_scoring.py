@@ -75,6 +75,18 @@ def test_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("R,V,top", [(3, 8192, 64), (2, 6145, 64), (50, 1000, 20), (4, 300, 20), (3, 2048, 16),
+                                     (3, 2049, 32), (2, 8193, 64), (2, 20000, 64)])
+def test_alternatives_of_small_vocabularies(dtype, R, V, top):
+    """Every group holds alternatives, or nearly every one; many candidates for few places."""
+    print(f"[logprobs] {dtype} {R}x{V} top {top}", flush=True)
+    x = randn((R, V), R * V, sigma=3.0, dtype=dtype)
+    x[0, V // 3:] = x[0, V // 3].clone()
+    x[1, ::3] = -math.inf
+    _check(x, torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(V)) // 3 * 3 + 1 - V % 2, top)
+
+
+@pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("V", [100, 5000, 128256])
 def test_equal_logits(dtype, V):
     """Ties everywhere: the lowest indices, in their order."""
