@@ -410,7 +410,8 @@ bool cache_of(PyObject* k, PyObject* v, PyObject* table, PyObject* weight, Cache
                           kt.size(3),
                           tt.size(0),
                           tt.size(1)};
-  return (out->c.head_dim == 64 || out->c.head_dim == 128) && current(dev);
+  const int64_t d = out->c.head_dim, S = out->c.page_size;
+  return (d == 64 || d == 128) && S >= 8 && S <= 1024 && (S & (S - 1)) == 0 && current(dev);
 }
 
 // [n, width] like the cache, rows dense and 16-byte aligned.

@@ -491,6 +491,21 @@ def test_attention_refuses(change):
         int4_hip.paged_attention(**dict(_to(c), q=c["q"]))
 
 
+@pytest.mark.parametrize("S,d", [(24, 64), (4, 64), (2048, 64), (16, 32), (16, 96)])
+def test_caches_of_other_forms_are_refused(S, d):
+    """By every operator as a caller's mistake, before anything is launched."""
+    z = lambda *shape, dtype=torch.bfloat16: torch.zeros(shape, dtype=dtype, device=DEV)
+    i = z(2, dtype=torch.int32)
+    pages, table, w = [z(4, 2, S, d), z(4, 2, S, d)], z(2, 2, dtype=torch.int32), z(4, 2, S, dtype=torch.float32)
+    cos = z(9, d // 2, dtype=torch.float32)
+    with pytest.raises(AssertionError):
+        int4_hip.paged_append(z(2, 2 * d), z(2, 2 * d), cos, cos, *pages, table, i, i, i)
+    with pytest.raises(AssertionError):
+        int4_hip.paged_attention(z(2, 4 * d), z(2, 2 * d), z(2, 2 * d), cos, cos, *pages, table, i, i, w)
+    with pytest.raises(AssertionError):
+        int4_hip.paged_evict(*pages, w, table, i, table, 4, 1)
+
+
 def test_append_and_evict_refuse():
     c = _to(R.attention_case([5, 2], 4, 2, 64, 16, torch.bfloat16, seed=1))
     i = torch.zeros(2, dtype=torch.int32, device=DEV)
