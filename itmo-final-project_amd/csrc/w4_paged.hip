@@ -686,7 +686,11 @@ constexpr int kSelectRun = 32768;  // keys that LDS holds
 // What bounds it is the latency of its steps on the one CU that has the row and head, so the keys are read from
 // memory once and stay in LDS (of more than 32768 early slots, a run at a time in every step).  32768 slots: 20.1 us,
 // of them 4.1 for the keys, 4.0 for the first histogram, 3.3 for the list, 2.8 for the counts; 576 slots 5.8; 100000
-// slots 65.5.
+// slots 55.1.
+//
+// ONCE: no row is longer than LDS holds (a kernel that may have to load again is slower for the others: 32768 slots 21.8
+// us instead of 20.2, 576 slots 6.2 instead of 5.7).
+template <bool ONCE>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a) {
   constexpr int WAVES = kSelectThreads / 64, RUN = kSelectRun, Q = RUN / (4 * kSelectThreads);
   const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x, b = blockIdx.y;
@@ -694,6 +698,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
   __shared__ __attribute__((aligned(16))) uint32_t key_s[RUN];
   __shared__ int hist[kSelectBins];
   __shared__ __attribute__((aligned(16))) uint32_t list[kSelectList];
+  __shared__ uint16_t from_s[kSelectList];  // the 256 slots that a key of the list is from
   __shared__ int wave_s[2][WAVES], found_s[3];
   __shared__ __attribute__((aligned(16))) uint32_t rank_s[kSelectRank];
   __shared__ uint32_t edge_s;
@@ -724,25 +729,31 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
         *reinterpret_cast<u32x4*>(&key_s[at(q)]) = x;
       }
   };
-  const bool once = early <= RUN;
+  const bool once = ONCE || early <= RUN;
   if (once) load(0);  // (a wave reads back what it wrote itself)
   auto quad = [&](int q) { return *reinterpret_cast<const u32x4*>(&key_s[at(q)]); };
-  // f(key) for every early slot
-  auto each = [&](auto f) __attribute__((always_inline)) {
+  // f(s0, keys, valid) for every 256 early slots from s0 on, a quad of keys a lane, the first `valid` of them early.
+  auto each_quad = [&](auto f) __attribute__((always_inline)) {
     for (int run = 0; run < early; run += RUN) {
       if (!once) load(run);
       for (int q = 0; q < quads; ++q) {
-        const u32x4 k = quad(q);
-        if (run + (wv * quads + q + 1) * 256 <= early) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) f((uint32_t)k[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (run + at(q) + e < early) f((uint32_t)k[e]);
-        }
+        const int s0 = run + (wv * quads + q) * 256;
+        if (s0 >= early) break;
+        f(s0, quad(q), early - s0 - 4 * lane);
       }
     }
+  };
+  auto each = [&](auto f) __attribute__((always_inline)) {  // f(key)
+    each_quad([&](int s0, const u32x4& k, int valid) __attribute__((always_inline)) {
+      if (s0 + 256 <= early) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f((uint32_t)k[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < valid) f((uint32_t)k[e]);
+      }
+    });
   };
 
   uint32_t lo = 0, hi = 0xFFFFFFFFu;
@@ -781,18 +792,30 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
   narrow(each, kSelectList);
   uint32_t edge = lo;
   int ties = wanted;  // keys equal to the edge that are kept
+  // Where a look at the keys is a pass over memory, the larger ones are counted while the list is made (100000 slots
+  // 55.1 us instead of 65.5; 32768 in LDS gain nothing by it).
+  const bool count_here = !once && lo < hi && early <= kSelectBlock << 16;
+  int held = 0;  // keys put aside
   if (lo < hi) {
     __syncthreads();
     if (tid == 0) found_s[0] = 0;
     __syncthreads();
-    each([&](uint32_t key) __attribute__((always_inline)) {
-      if (key >= lo && key <= hi) {
-        const int to = atomicAdd(&found_s[0], 1);
-        if (to < kSelectList) list[to] = key;  // (weights that change under the call stay in bounds)
+    each_quad([&](int s0, const u32x4& k, int valid) __attribute__((always_inline)) {
+      int larger = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (count_here) larger += __popcll(__ballot(e < valid && k[e] > hi));
+        if (e < valid && k[e] >= lo && k[e] <= hi) {
+          const int to = atomicAdd(&found_s[0], 1);
+          if (to < kSelectList)  // (weights that change under the call stay in bounds)
+            list[to] = k[e], from_s[to] = (uint16_t)(s0 / kSelectBlock);
+        }
       }
+      if (count_here && lane == 0) scratch[2 + s0 / kSelectBlock] = larger;
     });
+    __builtin_amdgcn_s_waitcnt(0);  // the counts are where others will add to them
     __syncthreads();
-    const int held = min(count, kSelectList);
+    held = min(found_s[0], kSelectList);
     narrow([&](auto f) __attribute__((always_inline)) {
       for (int i = tid; i < held; i += kSelectThreads) f(list[i]);
     }, kSelectRank);
@@ -828,20 +851,19 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
   }
 
   if (tid == 0) scratch[0] = (int)edge, scratch[1] = ties;
-  for (int run = 0; run < early; run += RUN) {
-    if (!once) load(run);
-    for (int q = 0; q < quads; ++q) {
-      const int s0 = run + (wv * quads + q) * 256;
-      if (s0 >= early) break;
-      const u32x4 k = quad(q);
-      int x = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (run + at(q) + e < early) x += k[e] > edge ? 1 : k[e] == edge ? 1 << 16 : 0;
-      x = __builtin_amdgcn_readlane(wave_scan(x), 63);
-      if (lane == 0) scratch[2 + s0 / kSelectBlock] = x;
-    }
+  if (count_here) {
+    for (int i = tid; i < held; i += kSelectThreads)
+      if (list[i] >= edge) atomicAdd(&scratch[2 + from_s[i]], list[i] > edge ? 1 : 1 << 16);
+    return;
   }
+  each_quad([&](int s0, const u32x4& k, int valid) __attribute__((always_inline)) {
+    int x = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < valid) x += k[e] > edge ? 1 : k[e] == edge ? 1 << 16 : 0;
+    x = __builtin_amdgcn_readlane(wave_scan(x), 63);
+    if (lane == 0) scratch[2 + s0 / kSelectBlock] = x;
+  });
 }
 
 // One workgroup per 1024 slots of a row and head: the kept slots in their order.  A slot's place is the number of
@@ -1153,7 +1175,9 @@ extern "C" int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int3
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (slots > keep) {  // (else no row has more than it keeps)
     if (recent < keep) {
-      w4::paged_select_kernel<<<dim3(heads, rows), w4::kSelectThreads, 0, st>>>(a);
+      if (slots - recent <= w4::kSelectRun)
+        w4::paged_select_kernel<true><<<dim3(heads, rows), w4::kSelectThreads, 0, st>>>(a);
+      else w4::paged_select_kernel<false><<<dim3(heads, rows), w4::kSelectThreads, 0, st>>>(a);
       if (const int rc = check_launch("w4_paged_evict (select)")) return rc;
     }
     w4::paged_place_kernel<<<dim3((unsigned)((slots + w4::kPlaceSlots - 1) / w4::kPlaceSlots), heads, rows),

@@ -391,6 +391,17 @@ def _evict(lens, nkv, d, S, keep, recent, dtype, seed, fix=None):
         assert _same(a, b)
 
 
+@pytest.mark.parametrize("keep,recent,levels", [(40000, 500, 0), (100, 0, 0), (69900, 100, 0), (33000, 0, 7),
+                                                (20000, 1000, 1), (30000, 11, 30000)])
+def test_evict_rows_longer_than_the_selection_holds(keep, recent, levels):
+    """Keys read in several runs; with `levels` the weights are of so many values only."""
+    def fix(w):
+        if levels:
+            w.copy_((w * levels).floor().clamp(max=levels - 1))
+    print(f"[paged eviction] 70001, keep {keep} / {recent}, {levels} levels", flush=True)
+    _evict([70001, 33000 + recent, 32768 + recent], 2, 64, 256, keep, recent, torch.bfloat16, seed=keep, fix=fix)
+
+
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("lens,nkv,d,S,keep,recent", [
     ([1], 1, 64, 8, 1, 0), ([5, 0, -1, 9], 2, 64, 8, 4, 2), ([64, 65, 63], 2, 128, 16, 64, 64),
