@@ -83,12 +83,12 @@ struct PagedAttnArgs {
   const float *cos, *sin;
   uint16_t* out;  // [rows, nkv * g * D]
   float* scores;  // [rows, nkv * g, width * page_size], of q K / sqrt(D); null without weights
-  float* part;    // [items, min(g, 16), D]: outputs of a part, where a row's slots are cut
-  float* stats;   // [items, 16, 2]: its heads' maxima of the scores, in powers of two, and sums relative to them
+  float* part;    // [items, min(g, tile), D]: outputs of a part, where a row's slots are cut
+  float* stats;   // [items, tile, 2]: its heads' maxima of the scores, in powers of two, and sums relative to them
   int* first;     // [rows, nkv * htiles, 2]: index of a row and tile's first part, and how many there are
   unsigned* cnt;  // one arrival counter per row and tile of heads
   float scale;    // 1 / sqrt(D)
-  int g, htiles;
+  int g, tile, htiles;  // query heads a key-value head, of them in a tile, tiles
   int later;      // the parts are joined by a launch of its own
   int at_once;    // parts that the joining reads together
 };
@@ -230,32 +230,33 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-// One workgroup = one part of one row's slots for up to 16 query heads of one key-value head; its waves take
-// units of UP = 4096 / D slots in turn (16 KB of keys and values).
+// One workgroup = one part of one row's slots for up to 16 HT query heads of one key-value head; its waves take units of
+// UP = 4096 / D slots in turn (16 KB of keys and values).
 //
 // Both products are 16x16x32 matrix instructions, transposed: scores S^T = K Q^T, slots by heads, then O^T = V^T P^T.
 // A tile's row r of keys is slot 8 (r / 4) + 4 t + r % 4 of its block of 32 (t: the first or second tile), so the
 // scores that a lane holds of one head are those of eight slots in a row: exactly its part of the second product's
-// operand, which never leaves its registers.  Keys go from memory to the operands; values go through LDS, which
-// transposes them on reading.  The running maximum of a head is only raised when a score passes it by 2^8 (its value
+// operand, which never leaves its registers.  Keys and values come in whole lines and go through a wave's own LDS, which
+// puts the keys into the tiles' order and transposes the values on reading.  The running maximum of a head is only raised when a score passes it by 2^8 (its value
 // cancels in the end), so that most units need no exchange between lanes.
 //
 // Bound by memory where there is enough of it: 131000 slots of 32 / 8 heads of 128 in 91.6 us, 537 MB at 5.9 TB/s; 16
 // rows of 3001 with the weights' scores (203 MB) in 39.8; 32 rows of up to 4000 of 64 in 31.7, 123 MB at 3.9 TB/s,
 // whose unequal parts leave CUs idle at the end.  A short row is a chain of latencies (lengths, page, tokens, sums,
 // output): 100 slots 7.2 us.
-template <int DT, int D, int W>
+template <int DT, int D, int W, int HT>
 __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int KB = 128 / D, UP = 32 * KB, NJ = D / 32, ND = D / 16, VR = 512 / D, NP = Split<DT>::N;
   constexpr int KROW = D + 8;              // halfwords of a key row in LDS: sixteen rows on different banks
   constexpr int VROW = D == 64 ? 72 : 144; // of a value row: four rows of 32 bytes on different banks
   constexpr int OROW = D + 4;              // floats of an output row in LDS
   constexpr int WAVE_H = UP * (KROW + VROW), ITEMS = W == 1 ? kAttnOneWaveItems : kAttnItems, kThreads = 64 * W;
-  static_assert(16 * OROW * 2 <= WAVE_H, "a wave's outputs take its tokens' place");
+  constexpr int HEADS = 16 * HT;
+  static_assert(HEADS * OROW * 2 <= WAVE_H, "a wave's outputs take its tokens' place");
   typedef typename Act<DT>::frag frag;
   __shared__ __attribute__((aligned(16))) uint16_t kv_s[W][WAVE_H];
   __shared__ __attribute__((aligned(16))) uint16_t new_s[2][D];
-  __shared__ float m_s[W][16], l_s[W][16];
+  __shared__ float m_s[W][HEADS], l_s[W][HEADS];
   __shared__ int bad_s[W];
   __shared__ unsigned arrived_s;
 
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
   AttnItem it;
   if (!find_item<UP, ITEMS>(a.c, a.lengths, a.positions, a.c.nkv * a.htiles, a.at_once, blockIdx.x, &it)) return;
   const int b = it.b, h = it.tile / a.htiles, ht = it.tile - h * a.htiles;
-  const int h0 = h * a.g + ht * 16, gh = min(a.g - ht * 16, 16);  // query heads of the row
+  const int h0 = h * a.g + ht * HEADS, gh = min(a.g - ht * HEADS, HEADS);  // query heads of the row
   const int nh = a.c.nkv * a.g;
   const int len = it.len, pos = it.pos;
   uint16_t* const out = a.out + ((int64_t)b * nh + h0) * D;
@@ -315,16 +316,18 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
   }
 
   // the query: heads past gh copy another and count for nothing
-  u32x4 qf[NJ][NP];
-  {
-    const uint16_t* const qp = a.q + b * a.stride_q + (int64_t)(h0 + min(l16, gh - 1)) * D;
-    const float scale = l16 < gh ? a.scale : 0.f;
+  u32x4 qf[HT][NJ][NP];
+#pragma unroll
+  for (int ht0 = 0; ht0 < HT; ++ht0) {
+    const int hd = ht0 * 16 + l16;
+    const uint16_t* const qp = a.q + b * a.stride_q + (int64_t)(h0 + min(hd, gh - 1)) * D;
+    const float scale = hd < gh ? a.scale : 0.f;
 #pragma unroll
     for (int j = 0; j < NJ / 2; ++j) {
       float lo[8], hi[8];
       rope_chunk<DT, D>(qp, cosr, sinr, j, c, scale, lo, hi);
-      split8<DT>(lo, NP, qf[j]);
-      split8<DT>(hi, NP, qf[j + NJ / 2]);
+      split8<DT>(lo, NP, qf[ht0][j]);
+      split8<DT>(hi, NP, qf[ht0][j + NJ / 2]);
     }
   }
   // The wave that takes the row's last unit rotates the new key, keeps it and the value at hand and writes them to
@@ -354,13 +357,16 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
     }
   }
 
-  float m, l;  // of head l16: the reference exponent and this lane's share of the sum
-  f32x4 o[ND];
+  float m[HT], l[HT];  // of head l16 of a tile: the reference exponent and this lane's share of the sum
+  f32x4 o[HT][ND];
   bool precise = true;
   for (;;) {
-    m = -__builtin_inff(), l = 0.f;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < HT; ++i) {
+      m[i] = -__builtin_inff(), l[i] = 0.f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     for (; u < u1; u += W) {
       const int base = u * UP;
       const bool last = base + UP > len;  // the new token is in this unit, and what lies past it
@@ -384,120 +390,133 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
         load(u + W, ids);
         ids = load_ids(min(u + 2 * W, u1 - 1));
       }
-      f32x4 s[KB][2];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+      for (int i = 0; i < HT; ++i) {
+        f32x4 s[KB][2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint16_t* const at = kw + (kb * 32 + t * 16 + l16) * KROW + 8 * c;
-          frag kf[NJ];
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const frag*>(at + 32 * j);
-          s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (precise) {  // the small parts first
+          for (int t = 0; t < 2; ++t) {
+            const uint16_t* const at = kw + (kb * 32 + t * 16 + l16) * KROW + 8 * c;
+            frag kf[NJ];
 #pragma unroll
-            for (int p = NP - 1; p > 0; --p)
+            for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const frag*>(at + 32 * j);
+            s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (precise) {  // the small parts first
 #pragma unroll
-              for (int j = 0; j < NJ; ++j)
-                s[kb][t] = Mfma<DT>::m16(kf[j], __builtin_bit_cast(frag, qf[j][p]), s[kb][t]);
+              for (int p = NP - 1; p > 0; --p)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                  s[kb][t] = Mfma<DT>::m16(kf[j], __builtin_bit_cast(frag, qf[i][j][p]), s[kb][t]);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+              s[kb][t] = Mfma<DT>::m16(kf[j], __builtin_bit_cast(frag, qf[i][j][0]), s[kb][t]);
           }
+        if (last) {
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) s[kb][t] = Mfma<DT>::m16(kf[j], __builtin_bit_cast(frag, qf[j][0]), s[kb][t]);
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (base + kb * 32 + 8 * c + 4 * t + e > len) s[kb][t][e] = -__builtin_inff();
         }
-      if (last) {
+        if (a.scores && i * 16 + l16 < gh) {
+          float* sp = a.scores + ((int64_t)b * nh + h0 + i * 16 + l16) * a.c.capacity() + base + 8 * c;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (base + kb * 32 + 8 * c + 4 * t <= len) *reinterpret_cast<f32x4*>(sp + kb * 32 + 4 * t) = s[kb][t];
+        }
+        float top = -__builtin_inff();
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (base + kb * 32 + 8 * c + 4 * t + e > len) s[kb][t][e] = -__builtin_inff();
-      }
-      if (a.scores && l16 < gh) {
-        float* sp = a.scores + ((int64_t)b * nh + h0 + l16) * a.c.capacity() + base + 8 * c;
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kb][t][e]);
+        top *= kLog2e;
+        if (__ballot(top > m[i] + 8.f)) {
+          float mn = fmaxf(top, m[i]);
+          mn = fmaxf(mn, __shfl_xor(mn, 16));
+          mn = fmaxf(mn, __shfl_xor(mn, 32));
+          const float al = __builtin_amdgcn_exp2f(m[i] - finite_or_zero(mn));
+          l[i] *= al;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+          for (int d = 0; d < ND; ++d)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (base + kb * 32 + 8 * c + 4 * t <= len) *reinterpret_cast<f32x4*>(sp + kb * 32 + 4 * t) = s[kb][t];
-      }
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kb][t][e]);
-      top *= kLog2e;
-      if (__ballot(top > m + 8.f)) {
-        float mn = fmaxf(top, m);
-        mn = fmaxf(mn, __shfl_xor(mn, 16));
-        mn = fmaxf(mn, __shfl_xor(mn, 32));
-        const float al = __builtin_amdgcn_exp2f(m - finite_or_zero(mn));
-        l *= al;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[d][e] *= al;
-        m = mn;
-      }
-      const float mz = finite_or_zero(m);
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3], kLog2e, -mz));
-          l += p[e];
+            for (int e = 0; e < 4; ++e) o[i][d][e] *= al;
+          m[i] = mn;
         }
-        u32x4 pf[2];
-        split8<DT>(p, 2, pf);  // 16 (22) bits: the output's one rounding stays the error
+        const float mz = finite_or_zero(m[i]);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const uint16_t* at = vw + (kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3);
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * VROW));
-          const u32x2 lw = __builtin_bit_cast(u32x2, lo), hw = __builtin_bit_cast(u32x2, hi);
-          const frag vf = __builtin_bit_cast(frag, u32x4{lw[0], lw[1], hw[0], hw[1]});
-          if (precise) o[d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[1]), o[d]);
-          o[d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[0]), o[d]);
+        for (int kb = 0; kb < KB; ++kb) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3], kLog2e, -mz));
+            l[i] += p[e];
+          }
+          u32x4 pf[2];
+          split8<DT>(p, 2, pf);  // 16 (22) bits: the output's one rounding stays the error
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            const uint16_t* at = vw + (kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * VROW));
+            const u32x2 lw = __builtin_bit_cast(u32x2, lo), hw = __builtin_bit_cast(u32x2, hi);
+            const frag vf = __builtin_bit_cast(frag, u32x4{lw[0], lw[1], hw[0], hw[1]});
+            if (precise) o[i][d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[1]), o[i][d]);
+            o[i][d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[0]), o[i][d]);
+          }
         }
       }
     }
     // An infinity meets the small parts of an operand as inf * 0 or with the wrong sign.  Where something is not
     // finite the part is computed again from the leading parts alone, whose zeros and signs are the operand's.
     if (!precise) break;
-    float sum = l;
+    bool finite = true;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int i = 0; i < HT; ++i) {
+      float sum = l[i];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum += __builtin_fabsf(o[d][e]);
-    if (!__ballot(l16 < gh && !(sum < __builtin_inff()))) break;
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += __builtin_fabsf(o[i][d][e]);
+      finite = finite && !__ballot(i * 16 + l16 < gh && !(sum < __builtin_inff()));
+    }
+    if (finite) break;
     precise = false;
     u = u0 + wv;
     load(u, load_ids(u));
     ids = load_ids(min(u + W, u1 - 1));
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
 
   // The waves' outputs meet in LDS.
   float* const ow = reinterpret_cast<float*>(kw);
-  if (l16 < gh) {
 #pragma unroll
-    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(ow + l16 * OROW + d * 16 + 4 * c) = o[d];
-    if (c == 0) m_s[wv][l16] = m, l_s[wv][l16] = l;
+  for (int i = 0; i < HT; ++i) {
+    const int hd = i * 16 + l16;
+    l[i] += __shfl_xor(l[i], 16);
+    l[i] += __shfl_xor(l[i], 32);
+    if (hd < gh) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(ow + hd * OROW + d * 16 + 4 * c) = o[i][d];
+      if (c == 0) m_s[wv][hd] = m[i], l_s[wv][hd] = l[i];
+    }
   }
   if (lane == 0) bad_s[wv] = bad;
   __syncthreads();
   int refused = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) refused |= bad_s[w];
-  const int quads = gh * (D / 4), stride = min(a.g, 16) * D;
+  const int quads = gh * (D / 4), stride = min(a.g, HEADS) * D;
   const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(a.part + (int64_t)it.first * stride), (short)0, it.parts * stride * 4, kPagedBufFlags);
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(a.stats + (int64_t)it.first * 32), (short)0, it.parts * 128, kPagedBufFlags);
+      (void*)(a.stats + (int64_t)it.first * (2 * HEADS)), (short)0, it.parts * HEADS * 8, kPagedBufFlags);
   if (a.later && it.part == 0 && tid == 0) {
     int* const f = a.first + (b * a.c.nkv * a.htiles + it.tile) * 2;
     f[0] = it.first;
@@ -518,7 +537,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
                                              (uint32_t)(it.part * stride + i * 4) * 4u, 0, kPagedCoherentAux);
     if (d == 0 && (it.parts > 1 || a.later))
       __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{x.M, x.L}), rs,
-                                            (uint32_t)(it.part * 16 + hd) * 8u, 0, kPagedCoherentAux);
+                                            (uint32_t)(it.part * HEADS + hd) * 8u, 0, kPagedCoherentAux);
   }
   if (it.parts == 1 || a.later) return;
 
@@ -547,7 +566,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
           const int p = min(p0 + k * runs, it.parts - 1);
           t[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                                rp, (uint32_t)(p * stride + i * 4) * 4u, 0, kPagedCoherentAux));
-          ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, (uint32_t)(p * 16 + hd) * 8u, 0,
+          ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, (uint32_t)(p * HEADS + hd) * 8u, 0,
                                                                                  kPagedCoherentAux));
         }
 #pragma unroll
@@ -577,15 +596,15 @@ __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnAr
   __shared__ f32x4 red[kPagedThreads];
   __shared__ f32x2 red_ml[kPagedThreads];
   const int tid = threadIdx.x, nh = a.c.nkv * a.g;
-  auto parts_of = [&](int b, int h, int g) { return a.first + ((b * a.c.nkv + h) * a.htiles + g / 16) * 2; };
+  auto parts_of = [&](int b, int h, int g) { return a.first + ((b * a.c.nkv + h) * a.htiles + g / a.tile) * 2; };
   if (blockIdx.x < (unsigned)(a.c.rows * nh)) {
     const int b = blockIdx.x / nh, head = blockIdx.x - b * nh, h = head / a.g, g = head - h * a.g;
     const int* const f = parts_of(b, h, g);
     const int first = f[0], parts = f[1];
     if (parts == 1) return;
-    const int stride = min(a.g, 16) * D, run = tid / QUADS, i = tid % QUADS;
-    const float* const part = a.part + (int64_t)first * stride + (g & 15) * D + i * 4;
-    const float* const st = a.stats + ((int64_t)first * 16 + (g & 15)) * 2;
+    const int stride = min(a.g, a.tile) * D, run = tid / QUADS, i = tid % QUADS;
+    const float* const part = a.part + (int64_t)first * stride + g % a.tile * D + i * 4;
+    const float* const st = a.stats + ((int64_t)first * a.tile + g % a.tile) * 2;
     Share x;
     for (int p0 = run; p0 < parts; p0 += RUNS * 8) {
       f32x4 t[8];
@@ -594,7 +613,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnAr
       for (int k = 0; k < 8; ++k) {
         const int64_t p = min(p0 + k * RUNS, parts - 1);
         t[k] = *reinterpret_cast<const f32x4*>(part + p * stride);
-        ml[k] = *reinterpret_cast<const f32x2*>(st + p * 32);
+        ml[k] = *reinterpret_cast<const f32x2*>(st + p * (2 * a.tile));
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -624,8 +643,11 @@ __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnAr
   const int parts = f[1];  // (the same for all tiles of a row)
   Share x;
   if (run < runs) {
-    const float* const st = a.stats + ((int64_t)f[0] * 16 + (g & 15)) * 2;
-    for (int p = run; p < parts; p += runs) x.add(st[p * 32], st[p * 32 + 1], f32x4{0.f, 0.f, 0.f, 0.f});
+    const float* const st = a.stats + ((int64_t)f[0] * a.tile + g % a.tile) * 2;
+    for (int p = run; p < parts; p += runs) {
+      const float* const sp = st + p * (2 * a.tile);
+      x.add(sp[0], sp[1], f32x4{0.f, 0.f, 0.f, 0.f});
+    }
     red_ml[tid] = f32x2{x.M, x.L};
   }
   __syncthreads();
@@ -688,8 +710,8 @@ constexpr int kSelectRun = 32768;  // keys that LDS holds
 // of them 4.1 for the keys, 4.0 for the first histogram, 3.3 for the list, 2.8 for the counts; 576 slots 5.8; 100000
 // slots 55.1.
 //
-// ONCE: no row is longer than LDS holds (a kernel that may have to load again is slower for the others: 32768 slots 21.8
-// us instead of 20.2, 576 slots 6.2 instead of 5.7).
+// ONCE: no row is longer than LDS holds (a kernel that may have to load again is slower for the others: 32768 slots
+// 21.8 us instead of 20.2, 576 slots 6.2 instead of 5.7).
 template <bool ONCE>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a) {
   constexpr int WAVES = kSelectThreads / 64, RUN = kSelectRun, Q = RUN / (4 * kSelectThreads);
@@ -1046,7 +1068,7 @@ extern "C" int w4_paged_append(const w4_paged_cache* cache, int dtype, const voi
 namespace {
 
 struct PagedAttnPlan {
-  int64_t tiles, items;         // tiles of up to 16 query heads a row, workgroups
+  int64_t tile, tiles, items;   // query heads of a tile, tiles a row, workgroups
   bool one_wave;                // those of one wave each
   size_t part, first, bytes;    // offsets of PagedAttnArgs' part and first in the workspace, and all of it
 };
@@ -1056,26 +1078,37 @@ struct PagedAttnPlan {
 // instead of 73.2, 96 of them 9.9 instead of 14.5, 200 of up to 1000 46.6 instead of 51.0.  Long rows are not:
 // their units follow each other in one wave (64 of 4000 87.8 instead of 82.7; one of 131000 among 31 short ones 69
 // instead of 49).
+//
+// More than sixteen query heads a key-value head of 64 share their slots' loads in tiles of 32, where the parts are
+// long enough for it: 24 / 1 heads, 10 rows of 107000 slots with weights 109 us instead of 170, 6 of up to 117000 26.7
+// instead of 49.1; 16 of up to 2000 would take 14.2 instead of 11.1.  (Heads of 128 have no registers for two tiles.)
 bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, int64_t units,
                      PagedAttnPlan* p) {
   if (rows < 0 || num_heads < 1 || kv_heads < 1 || num_heads % kv_heads) return false;
   const int64_t g = num_heads / kv_heads;
-  p->tiles = kv_heads * ((g + 15) / 16);
+  p->tile = g > 16 && head_dim == 64 && rows * kv_heads * units >= 8 * w4::kAttnItems ? 32 : 16;
+  p->tiles = kv_heads * ((g + p->tile - 1) / p->tile);
   p->one_wave = rows * p->tiles > 2 * device_cu_count() && units <= 128;
   p->items = (p->one_wave ? w4::kAttnOneWaveItems : w4::kAttnItems) + rows * p->tiles + 1;
   if (p->items >= (1 << 22)) return false;
-  p->part = W4_WORKSPACE_COUNTER_BYTES + (size_t)p->items * 128;
+  p->part = W4_WORKSPACE_COUNTER_BYTES + (size_t)(p->items * p->tile) * 8;
   p->first = p->part;
-  if (rows * p->tiles <= w4::kPagedCounters) p->first += (size_t)(p->items * (g < 16 ? g : 16) * head_dim) * 4;
+  if (rows * p->tiles <= w4::kPagedCounters) p->first += (size_t)(p->items * std::min(g, p->tile) * head_dim) * 4;
   p->bytes = p->first + (size_t)(rows * p->tiles) * 8;
   return true;
 }
 
 template <int DT, int D>
 int launch_paged_attention(const w4::PagedAttnArgs& a, const PagedAttnPlan& p, hipStream_t st) {
-  const dim3 grid((unsigned)p.items);
-  if (p.one_wave) w4::paged_attention_kernel<DT, D, 1><<<grid, 64, 0, st>>>(a);
-  else w4::paged_attention_kernel<DT, D, w4::kAttnWaves><<<grid, 64 * w4::kAttnWaves, 0, st>>>(a);
+  const dim3 grid((unsigned)p.items), threads(p.one_wave ? 64 : 64 * w4::kAttnWaves);
+  auto run = [&](auto kernel) { kernel<<<grid, threads, 0, st>>>(a); };
+  if (p.tile == 16) {
+    if (p.one_wave) run(w4::paged_attention_kernel<DT, D, 1, 1>);
+    else run(w4::paged_attention_kernel<DT, D, w4::kAttnWaves, 1>);
+  } else if constexpr (D == 64) {
+    if (p.one_wave) run(w4::paged_attention_kernel<DT, D, 1, 2>);
+    else run(w4::paged_attention_kernel<DT, D, w4::kAttnWaves, 2>);
+  }
   if (const int rc = check_launch("w4_paged_attention")) return rc;
   if (!a.later) return W4_OK;
   const int64_t more = a.scores ? w4::kAttnItems + (int64_t)a.c.rows * a.c.nkv + 1 : 0;
@@ -1088,8 +1121,12 @@ int launch_paged_attention(const w4::PagedAttnArgs& a, const PagedAttnPlan& p, h
 
 extern "C" size_t w4_paged_attention_workspace_bytes(int64_t rows, int64_t num_heads, int64_t kv_heads,
                                                      int64_t head_dim) {
-  PagedAttnPlan p;
-  return rows > 0 && paged_attn_plan(rows, num_heads, kv_heads, head_dim, 1, &p) ? p.bytes : 0;
+  size_t bytes = 0;  // of tables of any width
+  for (const int64_t units : {1, 128, 129, 1 << 30}) {
+    PagedAttnPlan p;
+    if (rows > 0 && paged_attn_plan(rows, num_heads, kv_heads, head_dim, units, &p)) bytes = std::max(bytes, p.bytes);
+  }
+  return bytes;
 }
 
 extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const void* q, const void* k, const void* v,
@@ -1135,12 +1172,14 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   a.g = (int)(num_heads / cache->kv_heads);
   a.htiles = (int)(p.tiles / cache->kv_heads);
   // The weights need a launch behind the attention anyway.  Without them the last part joins, unless a tile's outputs
-  // are more than a quad a thread, or its parts may be more than the joining reads in two goes (24 heads of 64 on
-  // one key-value head, 131000 slots in 128 parts: 36 us, with a launch of its own 20).
-  const int quads = (a.g < 16 ? a.g : 16) * (int)cache->head_dim / 4, threads = p.one_wave ? 64 : 64 * w4::kAttnWaves;
+  // are more than two quads a thread (four of a lone wave, whose rows have few parts), or its parts may be more than
+  // the joining reads in two goes (24 heads of 64 on one key-value head, 131000 slots in 128 parts: 36 us, with a
+  // launch of its own 20).
+  a.tile = (int)p.tile;
+  const int quads = std::min(a.g, a.tile) * (int)cache->head_dim / 4, threads = p.one_wave ? 64 : 64 * w4::kAttnWaves;
   a.at_once = 8 * std::max(threads / quads, 1);
   const int64_t parts = std::min(p.items / (cache->rows * p.tiles), units / w4::kAttnMinUnits + 1);
-  a.later = a.scores || quads > (p.one_wave ? 2 : 1) * threads || parts > 2 * a.at_once + 1;
+  a.later = a.scores || quads > (p.one_wave ? 4 : 2) * threads || parts > 2 * a.at_once + 1;
   if (a.later) a.at_once = 1 << 20;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == W4_DTYPE_BF16)

@@ -112,6 +112,19 @@ def test_attention_more_rows_than_the_chip_holds(dtype, nh, nkv, d):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("lens,nh,nkv", [([0, 5, -1, 64], 17, 1), ([3000, 129, 1], 32, 1), ([5000, 255], 33, 1),
+                                         ([700, 9000], 80, 2), ([20, 66] * 40 + [2000], 100, 5),
+                                         ([20, 66] * 60 + [2000], 100, 5)])
+def test_attention_many_query_heads_a_key_head(dtype, lens, nh, nkv):
+    print(f"[paged attention] {dtype} {len(lens)} rows of {nh}/{nkv}x64", flush=True)
+    for weights in (True, False):
+        c = R.attention_case(lens, nh, nkv, 64, 64, dtype, seed=nh, weights=weights)
+        if len(lens) == 4:
+            c["table"][3, 0] = -1
+        _run(c, dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 def test_attention_steps_accumulate(dtype):
     """Several steps, lengths growing across a page's end: every step's state feeds the next."""
     lens = [14, 0, 30]
