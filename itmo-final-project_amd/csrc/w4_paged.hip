@@ -230,15 +230,36 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-// One workgroup = one part of one row's slots for up to 16 HT query heads of one key-value head; its waves take units of
-// UP = 4096 / D slots in turn (16 KB of keys and values).
+// The probabilities of slots s.. s + 3 added to their weights (the new token's, slot `len`, set); head(g): the maximum
+// (not -inf) and reciprocal sum of a key-value head's query head.
+template <typename Head>
+__device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h, int s, int len, const Head& head) {
+  const int64_t cap = a.c.capacity();
+  const float* const sp = a.scores + ((int64_t)b * a.c.nkv + h) * a.g * cap + s;
+  f32x4 t = {0.f, 0.f, 0.f, 0.f};
+  for (int g = 0; g < a.g; ++g) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(sp + g * cap);
+    const f32x2 ml = head(g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(y[e], kLog2e, -ml[0])) * ml[1];
+  }
+  float* const wp = a.c.weight + a.c.token(b, s, h);
+  f32x4 w = *reinterpret_cast<const f32x4*>(wp);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = s + e < len ? w[e] + t[e] : s + e == len ? t[e] : w[e];
+  *reinterpret_cast<f32x4*>(wp) = w;
+}
+
+// One workgroup = one part of one row's slots for up to 16 HT query heads of one key-value head; its waves take units
+// of UP = 4096 / D slots in turn (16 KB of keys and values).
 //
 // Both products are 16x16x32 matrix instructions, transposed: scores S^T = K Q^T, slots by heads, then O^T = V^T P^T.
 // A tile's row r of keys is slot 8 (r / 4) + 4 t + r % 4 of its block of 32 (t: the first or second tile), so the
 // scores that a lane holds of one head are those of eight slots in a row: exactly its part of the second product's
-// operand, which never leaves its registers.  Keys and values come in whole lines and go through a wave's own LDS, which
-// puts the keys into the tiles' order and transposes the values on reading.  The running maximum of a head is only raised when a score passes it by 2^8 (its value
-// cancels in the end), so that most units need no exchange between lanes.
+// operand, which never leaves its registers.  Keys and values come in whole lines and go through a wave's own LDS,
+// which puts the keys into the tiles' order and transposes the values on reading.  The running maximum of a head is
+// only raised when a score passes it by 2^8 (its value cancels in the end), so that most units need no exchange
+// between lanes.
 //
 // Bound by memory where there is enough of it: 131000 slots of 32 / 8 heads of 128 in 91.6 us, 537 MB at 5.9 TB/s; 16
 // rows of 3001 with the weights' scores (203 MB) in 39.8; 32 rows of up to 4000 of 64 in 31.7, 123 MB at 3.9 TB/s,
@@ -257,6 +278,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
   __shared__ __attribute__((aligned(16))) uint16_t kv_s[W][WAVE_H];
   __shared__ __attribute__((aligned(16))) uint16_t new_s[2][D];
   __shared__ float m_s[W][HEADS], l_s[W][HEADS];
+  __shared__ f32x2 head_s[HEADS];
   __shared__ int bad_s[W];
   __shared__ unsigned arrived_s;
 
@@ -530,6 +552,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
       x.add(m_s[w][hd], l_s[w][hd],
             *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(kv_s[w]) + hd * OROW + d));
     if (refused) x.M = x.L = __builtin_nanf("");
+    if (d == 0) head_s[hd] = f32x2{finite_or_zero(x.M), 1.f / x.L};
     if (it.parts == 1)
       *reinterpret_cast<u32x2*>(out + hd * D + d) = x.template out<DT>();
     else
@@ -539,7 +562,16 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
       __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{x.M, x.L}), rs,
                                             (uint32_t)(it.part * HEADS + hd) * 8u, 0, kPagedCoherentAux);
   }
-  if (it.parts == 1 || a.later) return;
+  if (a.later) return;
+  if (it.parts == 1) {
+    if (a.scores && !refused) {  // no row of the call has more parts, nor a head tiles
+      __builtin_amdgcn_s_waitcnt(0);  // the scores have left this wave
+      __syncthreads();
+      for (int s = 4 * tid; s <= len; s += 4 * kThreads)
+        add_weights(a, b, h, s, len, [&](int g) { return head_s[g]; });
+    }
+    return;
+  }
 
   // The last part of a row and tile to arrive joins them, in their order.
   __builtin_amdgcn_s_waitcnt(0);  // the stores have reached the level all XCDs share
@@ -636,7 +668,6 @@ __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnAr
   const int nu = len / UP + 1;
   const int s0 = (int)((int64_t)it.part * nu / it.parts) * UP;
   const int s1 = min((int)((int64_t)(it.part + 1) * nu / it.parts) * UP, len + 1);
-  const int64_t cap = a.c.capacity();
   // the heads' maxima and sums: several threads a head, each some of its parts
   const int runs = kPagedThreads / a.g, run = tid / a.g, g = tid - run * a.g;
   const int* const f = parts_of(b, h, g);
@@ -658,21 +689,8 @@ __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnAr
   }
   __syncthreads();
   if (red[0][0] != red[0][0]) return;  // a page outside the pool (in all heads alike)
-  for (int s = s0 + 4 * tid; s < s1; s += 4 * kPagedThreads) {
-    f32x4 t = {0.f, 0.f, 0.f, 0.f};
-    const float* sp = a.scores + ((int64_t)b * nh + h * a.g) * cap + s;
-    for (int e0 = 0; e0 < a.g; ++e0) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(sp + e0 * cap);
-      const float M = red[e0][0], inv = red[e0][1];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(y[e], kLog2e, -M)) * inv;
-    }
-    float* const wp = a.c.weight + a.c.token(b, s, h);
-    f32x4 w = *reinterpret_cast<const f32x4*>(wp);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = s + e < len ? w[e] + t[e] : s + e == len ? t[e] : w[e];
-    *reinterpret_cast<f32x4*>(wp) = w;
-  }
+  for (int s = s0 + 4 * tid; s < s1; s += 4 * kPagedThreads)
+    add_weights(a, b, h, s, len, [&](int e0) { return f32x2{red[e0][0], red[e0][1]}; });
 }
 
 // ---------------------------------------------------------------- eviction
@@ -1140,7 +1158,7 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
     return fail(W4_ERR_INVALID, "w4_paged_attention: %lld query heads on %lld key-value heads, %lld angles",
                 (long long)num_heads, (long long)cache->kv_heads, (long long)angles);
   if (cache->rows == 0) return W4_OK;
-  const int64_t units = cache->width * cache->page_size * cache->head_dim / 4096 + 1;
+  const int64_t units = (cache->width * cache->page_size * cache->head_dim + 4095) / 4096;
   PagedAttnPlan p;
   if (!paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, units, &p) ||
       cache->rows * num_heads >= (1 << 23))
@@ -1171,15 +1189,17 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   a.scale = 1.f / sqrtf((float)cache->head_dim);
   a.g = (int)(num_heads / cache->kv_heads);
   a.htiles = (int)(p.tiles / cache->kv_heads);
-  // The weights need a launch behind the attention anyway.  Without them the last part joins, unless a tile's outputs
-  // are more than two quads a thread (four of a lone wave, whose rows have few parts), or its parts may be more than
-  // the joining reads in two goes (24 heads of 64 on one key-value head, 131000 slots in 128 parts: 36 us, with a
-  // launch of its own 20).
+  // The weights need a launch behind the attention, but where every row is a workgroup's alone (1 row of 100 slots of
+  // 32 / 8 heads of 128 9.2 us instead of 8.2 and 4.6, 250 of them 31.5 instead of 30.0 and 15.8).  Without them the
+  // last part joins, unless a tile's outputs are more than two quads a thread (four of a lone wave, whose rows have few
+  // parts), or its parts may be more than the joining reads in two goes (24 heads of 64 on one key-value head, 131000
+  // slots in 128 parts: 36 us, with a launch of its own 20).
   a.tile = (int)p.tile;
   const int quads = std::min(a.g, a.tile) * (int)cache->head_dim / 4, threads = p.one_wave ? 64 : 64 * w4::kAttnWaves;
   a.at_once = 8 * std::max(threads / quads, 1);
   const int64_t parts = std::min(p.items / (cache->rows * p.tiles), units / w4::kAttnMinUnits + 1);
-  a.later = a.scores || quads > (p.one_wave ? 4 : 2) * threads || parts > 2 * a.at_once + 1;
+  const bool whole = units <= w4::kAttnMinUnits && a.htiles == 1;  // no row of the table has a second part
+  a.later = (a.scores && !whole) || quads > (p.one_wave ? 4 : 2) * threads || parts > 2 * a.at_once + 1;
   if (a.later) a.at_once = 1 << 20;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == W4_DTYPE_BF16)

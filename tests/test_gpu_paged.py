@@ -125,6 +125,22 @@ def test_attention_many_query_heads_a_key_head(dtype, lens, nh, nkv):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("B,nh,nkv,d,S,width", [(5, 8, 2, 64, 64, 4), (5, 8, 2, 64, 64, 5), (5, 8, 1, 128, 32, 4),
+                                                (5, 8, 1, 128, 128, 1), (5, 24, 1, 64, 8, 3), (5, 24, 1, 128, 64, 2),
+                                                (150, 4, 4, 64, 16, 16), (150, 8, 4, 128, 8, 16)])
+def test_attention_weights_of_narrow_tables(dtype, B, nh, nkv, d, S, width):
+    """Rows up to the last slot of tables that one workgroup has whole, and of tables just wider."""
+    cap = width * S
+    lens = [[cap - 1, 0, -1, cap // 2, 3, cap - 2, 7][i % 7] for i in range(B)]
+    print(f"[paged attention] {dtype} {B} rows of {width}x{S}, {nh}/{nkv}x{d}", flush=True)
+    c = R.attention_case(lens, nh, nkv, d, S, dtype, seed=B + width, weights=True, width=width)
+    c["table"] = c["table"][:, :width].contiguous()
+    c["table"][3, 0] = -1
+    c["positions"][4] = len(c["cos"])
+    _run(c, dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 def test_attention_steps_accumulate(dtype):
     """Several steps, lengths growing across a page's end: every step's state feeds the next."""
     lens = [14, 0, 30]
