@@ -716,6 +716,7 @@ constexpr int kSelectList = 2048;  // keys few enough to be put aside
 constexpr int kSelectRank = 256;   // and to be ranked against each other
 
 constexpr int kSelectRun = 32768;  // keys that LDS holds
+constexpr int kSelectPlace = 16384;  // early slots that the selection lists itself
 
 // One workgroup per row and key-value head finds the slots to keep.  The key of the last one (its weight's place in
 // the order of all weights) lies in a range that a histogram of 4096 bins narrows twelve bits at a time; once no more
@@ -729,8 +730,10 @@ constexpr int kSelectRun = 32768;  // keys that LDS holds
 // slots 55.1.
 //
 // ONCE: no row is longer than LDS holds (a kernel that may have to load again is slower for the others: 32768 slots
-// 21.8 us instead of 20.2, 576 slots 6.2 instead of 5.7).
-template <bool ONCE>
+// 21.8 us instead of 20.2, 576 slots 6.2 instead of 5.7).  PLACE: the rows are short enough that the kept slots are
+// best listed here (576 slots 6.5 us instead of 5.7 and 3.4 for a launch that places them, 16000 16.6 instead of 13.4
+// and 5.0, 32768 26.0 instead of 20.2 and 5.1).
+template <bool ONCE, bool PLACE>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a) {
   constexpr int WAVES = kSelectThreads / 64, RUN = kSelectRun, Q = RUN / (4 * kSelectThreads);
   const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x, b = blockIdx.y;
@@ -890,6 +893,37 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
     }
   }
 
+  if constexpr (PLACE) {
+    int32_t* const kept = scratch + (select_words(a.c.capacity(), a.keep) - a.keep);
+    // 1 for a larger key, 1 << 16 for an equal one
+    auto weigh = [&](uint32_t key, bool valid) { return !valid ? 0 : key > edge ? 1 : key == edge ? 1 << 16 : 0; };
+    int mine = 0;
+    each_quad([&](int, const u32x4& k, int valid) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine += weigh(k[e], e < valid);
+    });
+    mine = __builtin_amdgcn_readlane(wave_scan(mine), 63);
+    if (lane == 0) wave_s[1][wv] = mine;
+    __syncthreads();
+    int front = 0;
+    for (int w = 0; w < wv; ++w) front += wave_s[1][w];
+    each_quad([&](int s0, const u32x4& k, int valid) __attribute__((always_inline)) {
+      int x = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x += weigh(k[e], e < valid);
+      const int upto = front + wave_scan(x);
+      x = upto - x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int y = weigh(k[e], e < valid), to = (x & 0xFFFF) + min(x >> 16, ties);
+        if ((y == 1 || (y && x >> 16 < ties)) && (unsigned)to < (unsigned)want) kept[to] = s0 + 4 * lane + e;
+        x += y;
+      }
+      front = __builtin_amdgcn_readlane(upto, 63);
+    });
+    for (int i = tid; i < a.recent; i += kSelectThreads) kept[want + i] = early + i;
+    return;
+  }
   if (tid == 0) scratch[0] = (int)edge, scratch[1] = ties;
   if (count_here) {
     for (int i = tid; i < held; i += kSelectThreads)
@@ -1233,15 +1267,20 @@ extern "C" int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int3
   const unsigned heads = (unsigned)cache->kv_heads, rows = (unsigned)cache->rows;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (slots > keep) {  // (else no row has more than it keeps)
+    const bool place = recent < keep && slots - recent <= w4::kSelectPlace;
     if (recent < keep) {
-      if (slots - recent <= w4::kSelectRun)
-        w4::paged_select_kernel<true><<<dim3(heads, rows), w4::kSelectThreads, 0, st>>>(a);
-      else w4::paged_select_kernel<false><<<dim3(heads, rows), w4::kSelectThreads, 0, st>>>(a);
+      const dim3 grid(heads, rows);
+      if (place) w4::paged_select_kernel<true, true><<<grid, w4::kSelectThreads, 0, st>>>(a);
+      else if (slots - recent <= w4::kSelectRun)
+        w4::paged_select_kernel<true, false><<<grid, w4::kSelectThreads, 0, st>>>(a);
+      else w4::paged_select_kernel<false, false><<<grid, w4::kSelectThreads, 0, st>>>(a);
       if (const int rc = check_launch("w4_paged_evict (select)")) return rc;
     }
-    w4::paged_place_kernel<<<dim3((unsigned)((slots + w4::kPlaceSlots - 1) / w4::kPlaceSlots), heads, rows),
-                             w4::kPagedThreads, 0, st>>>(a);
-    if (const int rc = check_launch("w4_paged_evict (place)")) return rc;
+    if (!place) {
+      const dim3 grid((unsigned)((slots + w4::kPlaceSlots - 1) / w4::kPlaceSlots), heads, rows);
+      w4::paged_place_kernel<<<grid, w4::kPagedThreads, 0, st>>>(a);
+      if (const int rc = check_launch("w4_paged_evict (place)")) return rc;
+    }
   }
   const int64_t tok = 4 * w4::kPagedThreads / (cache->head_dim / 8);
   const dim3 grid((unsigned)((keep + tok - 1) / tok), heads, rows);

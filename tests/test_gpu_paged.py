@@ -402,9 +402,9 @@ def test_append_skips_pages_outside_the_pool_and_takes_strided_rows():
 
 
 # ---------------------------------------------------------------- eviction
-def _evict(lens, nkv, d, S, keep, recent, dtype, seed, fix=None):
+def _evict(lens, nkv, d, S, keep, recent, dtype, seed, fix=None, width=None):
     B = len(lens)
-    P, both = R.pages_for([max(n, 0) for n in lens] + [keep] * B, S, seed)
+    P, both = R.pages_for([max(n, 0) for n in lens] + [keep] * B, S, seed, width=width)
     table = both[:B].contiguous()
     new = both[B:, :-(-keep // S)].contiguous()
     kp, vp = (randn((P, nkv, S, d), seed + i, dtype=dtype) for i in (1, 2))
@@ -418,6 +418,16 @@ def _evict(lens, nkv, d, S, keep, recent, dtype, seed, fix=None):
     assert torch.equal(n.cpu(), want)
     for a, b in zip(g, (kp, vp, w)):
         assert _same(a, b)
+
+
+@pytest.mark.parametrize("width,S", [(20000, 8), (300, 64), (130, 128), (40, 1024), (513, 64), (2100, 8)])
+@pytest.mark.parametrize("lens,nkv,keep,recent", [([1], 1, 1, 0), ([5, 0, -1, 9], 2, 4, 2), ([64, 65, 63], 2, 64, 64),
+                                                  ([300, 299, 12, 301], 3, 299, 10), ([1000, 1025, 2048], 2, 77, 0),
+                                                  ([2000, 4099], 2, 1025, 1024), ([15000, 8193], 1, 6001, 300)])
+def test_evict_from_wide_tables(width, S, lens, nkv, keep, recent):
+    """Short rows of tables of every width: what is launched follows the table."""
+    print(f"[paged eviction] {lens} of {width}x{S}, keep {keep} / {recent}", flush=True)
+    _evict(lens, nkv, 64, S, keep, recent, torch.float16, seed=width, width=width)
 
 
 @pytest.mark.parametrize("keep,recent,levels", [(40000, 500, 0), (100, 0, 0), (69900, 100, 0), (33000, 0, 7),
