@@ -722,12 +722,11 @@ constexpr int kSelectPlace = 16384;  // early slots that the selection lists its
 // the order of all weights) lies in a range that a histogram of 4096 bins narrows twelve bits at a time; once no more
 // than 2048 keys are in it they are put aside and narrowed alone, and the last 256 are ranked one against all.  The
 // larger and equal keys of every 256 slots are counted, from which a launch that has all of the chip finds the slots'
-// places (here that took 8 us of 28, for 32768 slots).
+// places.
 //
 // What bounds it is the latency of its steps on the one CU that has the row and head, so the keys are read from
 // memory once and stay in LDS (of more than 32768 early slots, a run at a time in every step).  32768 slots: 20.1 us,
-// of them 4.1 for the keys, 4.0 for the first histogram, 3.3 for the list, 2.8 for the counts; 576 slots 5.8; 100000
-// slots 55.1.
+// of them 4.1 for the keys, 4.0 for the first histogram, 3.3 for the list, 2.8 for the counts; 100000 slots 55.1.
 //
 // ONCE: no row is longer than LDS holds (a kernel that may have to load again is slower for the others: 32768 slots
 // 21.8 us instead of 20.2, 576 slots 6.2 instead of 5.7).  PLACE: the rows are short enough that the kept slots are
