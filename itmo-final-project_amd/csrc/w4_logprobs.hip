@@ -141,7 +141,7 @@ __device__ __forceinline__ void narrow(const Each& each, uint64_t& lo, uint64_t&
 // Bound by memory where there are many rows: 500 x 128256 bf16 with 20 alternatives in 31.5 us, 128 MB at 4.1 TB/s
 // (five operations and an exponential a logit beside it), 1000 x 32001 fp32 without in 24.0, 128 MB at 5.3 TB/s.  A
 // few rows are a chain of latencies, 8 with 5 alternatives 11.6 us; so are many short ones, a dozen barriers each and
-// four workgroups on a CU: 2000 x 1000 fp32 with 20 in 36 us.
+// four workgroups on a CU: 2000 x 1000 fp32 with 20 in 30 us.
 template <int DT>
 __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   typedef Logits<DT> T;
@@ -400,8 +400,16 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   };
   const uint64_t most = (uint64_t)high << 32 | 0xFFFFFFFFu;
   uint64_t from = lo << 32;
-  int n;
+  int n = used <= a.top ? a.vocab : 0;  // as far as it is known
   for (;;) {
+    if (n > kLogList) {
+      // many equal or neighbouring logits: the threshold is sought among the members themselves, which are all different
+      uint64_t to = most;
+      int want = a.top, over = 0;
+      __syncthreads();
+      narrow(members, from, to, want, over, n, kLogList - kMaxTop, hist, wave_s, found_s);
+      __syncthreads();
+    }
     if (tid == 0) found_s[0] = 0;
     __syncthreads();
     members([&](uint64_t v) __attribute__((always_inline)) {
@@ -413,15 +421,9 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
     __syncthreads();
     n = found_s[0];
     if (n <= kLogList) break;
-    // many equal or neighbouring logits: the threshold is sought among the members themselves, which are all different
-    uint64_t to = most;
-    int want = a.top, over = 0;
-    __syncthreads();
-    narrow(members, from, to, want, over, n, kLogList - kMaxTop, hist, wave_s, found_s);
-    __syncthreads();
   }
-  // Ranked one against all; of many, those that come into question (2000 x 1000 with 20: 36 us, 51 without this and
-  // the shorter way above).
+  // Ranked one against all; of many, those that come into question (2000 x 1000 with 20: 30 us, 51 without this and
+  // the shorter ways above).
   const uint64_t* ranked = list;
   if (n > kLogRank) {
     uint64_t to = most;
