@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(LogprobArgs a) {
   int n = used <= a.top ? a.vocab : 0;  // as far as it is known
   for (;;) {
     if (n > kLogList) {
-      // many equal or neighbouring logits: the threshold is sought among the members themselves, which are all different
+      // many equal or neighbouring logits: the threshold is sought among the members, which are all different
       uint64_t to = most;
       int want = a.top, over = 0;
       __syncthreads();

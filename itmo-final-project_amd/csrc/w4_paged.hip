@@ -1131,13 +1131,16 @@ struct PagedAttnPlan {
 // instead of 49).
 //
 // More than sixteen query heads a key-value head of 64 share their slots' loads in tiles of 32, where the parts are
-// long enough for it: 24 / 1 heads, 10 rows of 107000 slots with weights 109 us instead of 170, 6 of up to 117000 26.7
-// instead of 49.1; 16 of up to 2000 would take 14.2 instead of 11.1.  (Heads of 128 have no registers for two tiles.)
-bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, int64_t units,
+// long enough for it: 24 / 1 heads, 10 rows of 107000 slots with weights 109 us instead of 170, 6 of up to 117000
+// 26.7 instead of 49.1; 16 of up to 2000 would take 14.2 instead of 11.1.  So they do where the weights then need no
+// second launch (7 of 15 11.8 us instead of 8.4 and 5.8, 300 of 120 17.7 instead of 15.9 and 12.7).  (Heads of 128
+// have no registers for two tiles.)
+bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, int64_t units, bool weights,
                      PagedAttnPlan* p) {
   if (rows < 0 || num_heads < 1 || kv_heads < 1 || num_heads % kv_heads) return false;
   const int64_t g = num_heads / kv_heads;
-  p->tile = g > 16 && head_dim == 64 && rows * kv_heads * units >= 8 * w4::kAttnItems ? 32 : 16;
+  const bool alone = weights && units <= w4::kAttnMinUnits && g <= 32;
+  p->tile = g > 16 && head_dim == 64 && (alone || rows * kv_heads * units >= 8 * w4::kAttnItems) ? 32 : 16;
   p->tiles = kv_heads * ((g + p->tile - 1) / p->tile);
   p->one_wave = rows * p->tiles > 2 * device_cu_count() && units <= 128;
   p->items = (p->one_wave ? w4::kAttnOneWaveItems : w4::kAttnItems) + rows * p->tiles + 1;
@@ -1173,10 +1176,12 @@ int launch_paged_attention(const w4::PagedAttnArgs& a, const PagedAttnPlan& p, h
 extern "C" size_t w4_paged_attention_workspace_bytes(int64_t rows, int64_t num_heads, int64_t kv_heads,
                                                      int64_t head_dim) {
   size_t bytes = 0;  // of tables of any width
-  for (const int64_t units : {1, 128, 129, 1 << 30}) {
-    PagedAttnPlan p;
-    if (rows > 0 && paged_attn_plan(rows, num_heads, kv_heads, head_dim, units, &p)) bytes = std::max(bytes, p.bytes);
-  }
+  for (const int64_t units : {1, 128, 129, 1 << 30})
+    for (const bool weights : {false, true}) {
+      PagedAttnPlan p;
+      if (rows > 0 && paged_attn_plan(rows, num_heads, kv_heads, head_dim, units, weights, &p))
+        bytes = std::max(bytes, p.bytes);
+    }
   return bytes;
 }
 
@@ -1193,7 +1198,7 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   if (cache->rows == 0) return W4_OK;
   const int64_t units = (cache->width * cache->page_size * cache->head_dim + 4095) / 4096;
   PagedAttnPlan p;
-  if (!paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, units, &p) ||
+  if (!paged_attn_plan(cache->rows, num_heads, cache->kv_heads, cache->head_dim, units, cache->weight, &p) ||
       cache->rows * num_heads >= (1 << 23))
     return fail(W4_ERR_UNSUPPORTED, "w4_paged_attention: %lld rows of %lld heads", (long long)cache->rows,
                 (long long)num_heads);
@@ -1231,8 +1236,9 @@ extern "C" int w4_paged_attention(const w4_paged_cache* cache, int dtype, const 
   const int quads = std::min(a.g, a.tile) * (int)cache->head_dim / 4, threads = p.one_wave ? 64 : 64 * w4::kAttnWaves;
   a.at_once = 8 * std::max(threads / quads, 1);
   const int64_t parts = std::min(p.items / (cache->rows * p.tiles), units / w4::kAttnMinUnits + 1);
-  const bool whole = units <= w4::kAttnMinUnits && a.htiles == 1;  // no row of the table has a second part
-  a.later = (a.scores && !whole) || quads > (p.one_wave ? 4 : 2) * threads || parts > 2 * a.at_once + 1;
+  const bool whole = units <= w4::kAttnMinUnits;  // no row of the table has a second part
+  a.later = a.scores ? !whole || a.htiles > 1
+                     : !whole && (quads > (p.one_wave ? 4 : 2) * threads || parts > 2 * a.at_once + 1);
   if (a.later) a.at_once = 1 << 20;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == W4_DTYPE_BF16)

@@ -141,6 +141,13 @@ def test_attention_weights_of_narrow_tables(dtype, B, nh, nkv, d, S, width):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("B,nh,nkv,S,width", [(6, 17, 1, 64, 4), (6, 33, 1, 64, 4), (150, 100, 5, 16, 16),
+                                              (150, 132, 4, 32, 2), (600, 24, 1, 8, 9), (9, 64, 2, 256, 1)])
+def test_attention_weights_of_narrow_tables_and_wide_groups(dtype, B, nh, nkv, S, width):
+    test_attention_weights_of_narrow_tables(dtype, B, nh, nkv, 64, S, width)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 def test_attention_steps_accumulate(dtype):
     """Several steps, lengths growing across a page's end: every step's state feeds the next."""
     lens = [14, 0, 30]
