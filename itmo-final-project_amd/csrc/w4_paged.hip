@@ -84,7 +84,7 @@ struct PagedAttnArgs {
   uint16_t* out;  // [rows, nkv * g * D]
   float* scores;  // [rows, nkv * g, width * page_size], of q K / sqrt(D); null without weights
   float* part;    // [items, min(g, tile), D]: outputs of a part, where a row's slots are cut
-  float* stats;   // [items, tile, 2]: its heads' maxima of the scores, in powers of two, and sums relative to them
+  float* stats;   // [items, tile, 2]: its heads' references, in powers of two, and sums relative to them
   int* first;     // [rows, nkv * htiles, 2]: index of a row and tile's first part, and how many there are
   unsigned* cnt;  // one arrival counter per row and tile of heads
   float scale;    // 1 / sqrt(D)
@@ -170,6 +170,15 @@ __device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __r
 template <int DT> struct Split;
 template <> struct Split<W4_DTYPE_BF16> { static constexpr int N = 3; };  // 8 significant bits each: all 24
 template <> struct Split<W4_DTYPE_FP16> { static constexpr int N = 2; };  // 11 each: 22
+
+// The range of the probabilities, powers of two relative to a head's reference: when it is raised it is put `above`
+// under the largest score, and raised again only once a score passes that by `lag`.  bf16 has fp32's exponents.  fp16
+// ends at 65504, so the largest probability is kept between 2^13 and 2^15: both parts of one 2^25 times smaller are then
+// still numbers, and what is lost of any is 2^-38 of the largest.  (With the largest at 1, the tail of a row that one
+// token dominates by e^17 would be lost, while its sum counts it.)
+template <int DT> struct Probs;
+template <> struct Probs<W4_DTYPE_BF16> { static constexpr float above = 0.f, lag = 8.f; };
+template <> struct Probs<W4_DTYPE_FP16> { static constexpr float above = 13.f, lag = 2.f; };
 
 template <int DT>
 __device__ __forceinline__ void split8(const float v[8], int parts, u32x4* out) {
@@ -257,9 +266,8 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
 // A tile's row r of keys is slot 8 (r / 4) + 4 t + r % 4 of its block of 32 (t: the first or second tile), so the
 // scores that a lane holds of one head are those of eight slots in a row: exactly its part of the second product's
 // operand, which never leaves its registers.  Keys and values come in whole lines and go through a wave's own LDS,
-// which puts the keys into the tiles' order and transposes the values on reading.  The running maximum of a head is
-// only raised when a score passes it by 2^8 (its value cancels in the end), so that most units need no exchange
-// between lanes.
+// which puts the keys into the tiles' order and transposes the values on reading.  A head's reference follows the
+// running maximum with a lag (Probs; its value cancels in the end), so that most units need no exchange between lanes.
 //
 // Bound by memory where there is enough of it: 131000 slots of 32 / 8 heads of 128 in 91.6 us, 537 MB at 5.9 TB/s; 16
 // rows of 3001 with the weights' scores (203 MB) in 39.8; 32 rows of up to 4000 of 64 in 31.7, 123 MB at 3.9 TB/s,
@@ -275,6 +283,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
   constexpr int HEADS = 16 * HT;
   static_assert(HEADS * OROW * 2 <= WAVE_H, "a wave's outputs take its tokens' place");
   typedef typename Act<DT>::frag frag;
+  typedef Probs<DT> P;
   __shared__ __attribute__((aligned(16))) uint16_t kv_s[W][WAVE_H];
   __shared__ __attribute__((aligned(16))) uint16_t new_s[2][D];
   __shared__ float m_s[W][HEADS], l_s[W][HEADS];
@@ -379,7 +388,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
     }
   }
 
-  float m[HT], l[HT];  // of head l16 of a tile: the reference exponent and this lane's share of the sum
+  float m[HT], l[HT];  // of head l16 of a tile: the reference and this lane's share of the sum
   f32x4 o[HT][ND];
   bool precise = true;
   for (;;) {
@@ -460,8 +469,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kb][t][e]);
         top *= kLog2e;
-        if (__ballot(top > m[i] + 8.f)) {
-          float mn = fmaxf(top, m[i]);
+        if (__ballot(top > m[i] + (P::above + P::lag))) {
+          float mn = fmaxf(top - P::above, m[i]);
           mn = fmaxf(mn, __shfl_xor(mn, 16));
           mn = fmaxf(mn, __shfl_xor(mn, 32));
           const float al = __builtin_amdgcn_exp2f(m[i] - finite_or_zero(mn));
@@ -482,7 +491,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
             l[i] += p[e];
           }
           u32x4 pf[2];
-          split8<DT>(p, 2, pf);  // 16 (22) bits: the output's one rounding stays the error
+          split8<DT>(p, 2, pf);  // 16 (22) bits of each
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
             const uint16_t* at = vw + (kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3);

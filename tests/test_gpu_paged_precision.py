@@ -1,0 +1,65 @@
+"""GPU: what the paged attention (int4_hip/paged.py) keeps of its operands' bits, where
+it shows: rows that one token dominates, queries of every scale, results beside
+infinities."""
+import pytest
+import torch
+
+import _paged_ref as R
+import int4_hip
+from test_gpu_paged import BOTH, DEV, _check, _run, _to
+
+pytestmark = pytest.mark.gpu
+
+
+def _sink(lens, nh, nkv, d, S, dtype, gap, seed, slot=0, equal=False, weights=False):
+    """Rows whose slot ``slot`` scores ``gap`` above the mean of the others (of spread 1,
+    or all equal) in every head and has the value 0: the output is the others' alone."""
+    c = R.attention_case(lens, nh, nkv, d, S, dtype, seed=seed, weights=weights)
+    c["positions"][:] = 0  # no rotation
+    B = len(lens)
+    c["q"].view(B, nh, d)[:, :, 0] = 4.0
+    c["k"].view(B, nkv, d)[:, :, 0] = 0.0
+    c["k_pages"][..., 0] = torch.where(c["k_pages"][..., 0].isnan(), c["k_pages"][..., 0], 0.0)
+    c["v"] += 1.0
+    c["v_pages"] += 1.0
+    if equal:
+        c["k"].zero_()
+        c["k_pages"].mul_(0.0)  # (NaN stays)
+    for b, n in enumerate(lens):
+        if n <= slot:
+            continue
+        p = int(c["table"][b, slot // S])
+        c["k_pages"][p, :, slot % S] = 0.0
+        c["k_pages"][p, :, slot % S, 0] = gap * d ** 0.5 / 4.0
+        c["v_pages"][p, :, slot % S] = 0.0
+    return c
+
+
+# A probability enters the product in two 16-bit parts.  bf16 has fp32's range.  fp16 ends
+# at 2^-24, with the largest probability of a wave's slots at 2^13 or more: what is lost of
+# any other is 2^-25, a part 2^-38 of the largest, which at a gap of 18 (26 powers of two) is
+# 2^-12 of the others' own, and as good as random where they differ.  So the bounds of
+# rows without such a token hold: the rounding to the type, 2e-5 of the terms.
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("gap", [10.0, 14.0, 16.0, 18.0])
+@pytest.mark.parametrize("lens,nh,nkv,d,S", [([300, 63, 1], 8, 2, 64, 16), ([4000], 8, 2, 64, 64),
+                                             ([9000, 700], 6, 1, 128, 32), ([5000, 900], 24, 1, 64, 128)])
+def test_attention_beside_a_dominant_token(dtype, gap, lens, nh, nkv, d, S):
+    print(f"[paged attention] {dtype} {lens} {nh}/{nkv}x{d}, one token {gap} above", flush=True)
+    for slot, equal in ((0, False), (lens[-1] // 2, False), (0, True)):
+        _run(_sink(lens, nh, nkv, d, S, dtype, min(gap, 17.0) if equal else gap, seed=nh, slot=slot, equal=equal,
+                   weights=slot == 0), dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("gap", [14.0, 18.0])
+@pytest.mark.parametrize("nh,nkv,d", [(8, 4, 64), (16, 4, 128), (36, 4, 64)])
+def test_attention_beside_a_dominant_token_many_rows(dtype, gap, nh, nkv, d):
+    """Workgroups of one wave, whose slots all share the largest probability."""
+    lens = [(13 * i) % 71 for i in range(140)]
+    lens[3], lens[139] = 1500, 4000 * 64 // d
+    print(f"[paged attention] {dtype} 140 rows of {nh}/{nkv}x{d}, one token {gap} above", flush=True)
+    c = _sink(lens, nh, nkv, d, 32, dtype, gap, seed=nh)
+    out = int4_hip.paged_attention(**_to(c))
+    want, mass, _, _ = R.attention(**c)
+    _check(out, want, mass, dtype)
