@@ -180,6 +180,28 @@ template <int DT> struct Probs;
 template <> struct Probs<W4_DTYPE_BF16> { static constexpr float above = 0.f, lag = 8.f; };
 template <> struct Probs<W4_DTYPE_FP16> { static constexpr float above = 13.f, lag = 2.f; };
 
+// What a head's query is multiplied by before it is split, a power of two.  Its scores carry it until they become
+// exponents (or are stored).  bf16: nothing.  fp16: its largest element gets to 2^13 or more, so that the parts of one 2^38
+// times smaller are still numbers, whatever the scale of queries and keys.
+template <int DT> struct QueryScale {
+  __device__ __forceinline__ float set(float) { return 1.f; }
+  __device__ __forceinline__ float back() const { return 1.f; }
+};
+template <> struct QueryScale<W4_DTYPE_FP16> {
+  float b = 1.f;
+  // The factor, from the largest magnitude of this lane's elements of the head (its four lanes take part).
+  __device__ __forceinline__ float set(float largest) {
+    largest = fmaxf(largest, __shfl_xor(largest, 16));
+    largest = fmaxf(largest, __shfl_xor(largest, 32));
+    // the exponent field; 2^13 / 2^e and back are numbers for any that fp16 elements and their rotations have
+    const uint32_t e = max(__builtin_bit_cast(uint32_t, largest) >> 23, 64u);
+    if (largest == 0.f || e == 255u) return 1.f;  // nothing to scale, or an infinity
+    b = __builtin_bit_cast(float, (e - 13u) << 23);
+    return __builtin_bit_cast(float, (267u - e) << 23);
+  }
+  __device__ __forceinline__ float back() const { return b; }
+};
+
 template <int DT>
 __device__ __forceinline__ void split8(const float v[8], int parts, u32x4* out) {
   float r[8];
@@ -348,17 +370,26 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
 
   // the query: heads past gh copy another and count for nothing
   u32x4 qf[HT][NJ][NP];
+  QueryScale<DT> qs[HT];
 #pragma unroll
   for (int ht0 = 0; ht0 < HT; ++ht0) {
     const int hd = ht0 * 16 + l16;
     const uint16_t* const qp = a.q + b * a.stride_q + (int64_t)(h0 + min(hd, gh - 1)) * D;
     const float scale = hd < gh ? a.scale : 0.f;
+    float lo[NJ / 2][8], hi[NJ / 2][8], largest = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ / 2; ++j) {
-      float lo[8], hi[8];
-      rope_chunk<DT, D>(qp, cosr, sinr, j, c, scale, lo, hi);
-      split8<DT>(lo, NP, qf[ht0][j]);
-      split8<DT>(hi, NP, qf[ht0][j + NJ / 2]);
+      rope_chunk<DT, D>(qp, cosr, sinr, j, c, scale, lo[j], hi[j]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fmaxf(__builtin_fabsf(lo[j][e]), __builtin_fabsf(hi[j][e])));
+    }
+    const float f = qs[ht0].set(largest);
+#pragma unroll
+    for (int j = 0; j < NJ / 2; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lo[j][e] *= f, hi[j][e] *= f;
+      split8<DT>(lo[j], NP, qf[ht0][j]);
+      split8<DT>(hi[j], NP, qf[ht0][j + NJ / 2]);
     }
   }
   // The wave that takes the row's last unit rotates the new key, keeps it and the value at hand and writes them to
@@ -459,7 +490,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-              if (base + kb * 32 + 8 * c + 4 * t <= len) *reinterpret_cast<f32x4*>(sp + kb * 32 + 4 * t) = s[kb][t];
+              if (base + kb * 32 + 8 * c + 4 * t <= len)
+                *reinterpret_cast<f32x4*>(sp + kb * 32 + 4 * t) = s[kb][t] * qs[i].back();
         }
         float top = -__builtin_inff();
 #pragma unroll
@@ -468,7 +500,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kb][t][e]);
-        top *= kLog2e;
+        const float log2e = kLog2e * qs[i].back();
+        top *= log2e;
         if (__ballot(top > m[i] + (P::above + P::lag))) {
           float mn = fmaxf(top - P::above, m[i]);
           mn = fmaxf(mn, __shfl_xor(mn, 16));
@@ -487,7 +520,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
           float p[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3], kLog2e, -mz));
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3], log2e, -mz));
             l[i] += p[e];
           }
           u32x4 pf[2];

@@ -63,3 +63,23 @@ def test_attention_beside_a_dominant_token_many_rows(dtype, gap, nh, nkv, d):
     out = int4_hip.paged_attention(**_to(c))
     want, mass, _, _ = R.attention(**c)
     _check(out, want, mass, dtype)
+
+
+# A score is a sum of d products of a query and a key of 16 bits, in 22 bits of the query and
+# more: relative to |q||k| it is off by as much at every scale of the two, 2^-22, and the
+# bounds of test_gpu_paged.py hold (|q||k| / sqrt(d) below 40 here too).
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("power", [-15, -8, 9, 13])
+@pytest.mark.parametrize("lens,nh,nkv,d,S", [([50, 3, 700], 8, 2, 64, 16), ([900], 20, 2, 128, 64),
+                                             ([5000], 24, 1, 64, 128)])
+def test_attention_of_small_and_large_queries(dtype, power, lens, nh, nkv, d, S):
+    """Queries of 2^power against keys of 2^-power; every other head's are 2^-4 of that."""
+    print(f"[paged attention] {dtype} {lens} {nh}/{nkv}x{d}, queries of 2^{power}", flush=True)
+    c = R.attention_case(lens, nh, nkv, d, S, dtype, seed=nh + power)
+    B = len(lens)
+    c["q"].clamp_(-3, 3).mul_(2.0 ** power).view(B, nh, d)[:, 1::2].mul_(2.0 ** -4)
+    for name in ("k", "k_pages"):
+        # (what fp16 holds, once rotated)
+        c[name] = torch.where(c[name].isnan(), c[name], c[name].clamp(-1.3, 1.3)) * 2.0 ** -power
+        c[name] = c[name].to(dtype)
+    _run(c, dtype)
