@@ -523,8 +523,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
             p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3], log2e, -mz));
             l[i] += p[e];
           }
-          u32x4 pf[2];
-          split8<DT>(p, 2, pf);  // 16 (22) bits of each
+          u32x4 pf[NP];
+          split8<DT>(p, NP, pf);
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
             const uint16_t* at = vw + (kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3);
@@ -532,7 +532,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * VROW));
             const u32x2 lw = __builtin_bit_cast(u32x2, lo), hw = __builtin_bit_cast(u32x2, hi);
             const frag vf = __builtin_bit_cast(frag, u32x4{lw[0], lw[1], hw[0], hw[1]});
-            if (precise) o[i][d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[1]), o[i][d]);
+            if (precise) {
+#pragma unroll
+              for (int p = NP - 1; p > 0; --p) o[i][d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[p]), o[i][d]);
+            }
             o[i][d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[0]), o[i][d]);
           }
         }
