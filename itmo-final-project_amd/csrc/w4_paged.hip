@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "w4_common.hpp"
 
@@ -202,18 +203,33 @@ template <> struct QueryScale<W4_DTYPE_FP16> {
   __device__ __forceinline__ float back() const { return b; }
 };
 
-template <int DT>
-__device__ __forceinline__ void split8(const float v[8], int parts, u32x4* out) {
+// QUERY: an infinity or NaN has no small parts.  (A probability is no infinity, and beside a NaN all of its head's are.)
+template <int DT, bool QUERY>
+__device__ __forceinline__ void split8(const float v[8], u32x4* out) {
   float r[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = v[e];
-  for (int p = 0; p < parts; ++p) {
+#pragma unroll
+  for (int p = 0; p < Split<DT>::N; ++p) {
     out[p] = pack8<DT>(r);
     float t[8];
     unpack8<DT>(out[p], t);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] -= t[e];
+    for (int e = 0; e < 8; ++e) r[e] = QUERY && !(__builtin_fabsf(t[e]) < __builtin_inff()) ? 0.f : r[e] - t[e];
   }
+}
+
+// Eight elements with zeros in the place of infinities and NaN.
+template <int DT>
+__device__ __forceinline__ typename Act<DT>::frag finite_part(const typename Act<DT>::frag& f) {
+  constexpr uint32_t TOP = DT == W4_DTYPE_BF16 ? 0x7F80u : 0x7C00u;  // all ones: not finite
+  u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if ((w[e] & TOP) == TOP) w[e] &= 0xFFFF0000u;
+    if ((w[e] & (TOP << 16)) == (TOP << 16)) w[e] &= 0xFFFFu;
+  }
+  return __builtin_bit_cast(typename Act<DT>::frag, w);
 }
 
 // Lane group c holds D / 32 chunks of eight elements of a head's D (chunk j: elements 32 j + 8 c..).  Chunk j < D / 64
@@ -388,8 +404,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
     for (int j = 0; j < NJ / 2; ++j) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) lo[j][e] *= f, hi[j][e] *= f;
-      split8<DT>(lo[j], NP, qf[ht0][j]);
-      split8<DT>(hi[j], NP, qf[ht0][j + NJ / 2]);
+      split8<DT, true>(lo[j], qf[ht0][j]);
+      split8<DT, true>(hi[j], qf[ht0][j + NJ / 2]);
     }
   }
   // The wave that takes the row's last unit rotates the new key, keeps it and the value at hand and writes them to
@@ -421,8 +437,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
 
   float m[HT], l[HT];  // of head l16 of a tile: the reference and this lane's share of the sum
   f32x4 o[HT][ND];
-  bool precise = true;
-  for (;;) {
+  // The part's units; careful: infinities and NaN are looked for.
+  auto attend = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < HT; ++i) {
       m[i] = -__builtin_inff(), l[i] = 0.f;
@@ -454,6 +470,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
       }
 #pragma unroll
       for (int i = 0; i < HT; ++i) {
+        if constexpr (HT > 1) asm volatile("" ::: "memory");  // (keys held for both tiles would be spilled)
         f32x4 s[KB][2];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -464,13 +481,15 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
 #pragma unroll
             for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const frag*>(at + 32 * j);
             s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (precise) {  // the small parts first
+            auto small = [&](auto f) __attribute__((always_inline)) {  // the small parts first
 #pragma unroll
               for (int p = NP - 1; p > 0; --p)
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
-                  s[kb][t] = Mfma<DT>::m16(kf[j], __builtin_bit_cast(frag, qf[i][j][p]), s[kb][t]);
-            }
+                  s[kb][t] = Mfma<DT>::m16(f(kf[j]), __builtin_bit_cast(frag, qf[i][j][p]), s[kb][t]);
+            };
+            if (careful) small(finite_part<DT>);
+            else small([](const frag& k) { return k; });
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
               s[kb][t] = Mfma<DT>::m16(kf[j], __builtin_bit_cast(frag, qf[i][j][0]), s[kb][t]);
@@ -524,7 +543,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
             l[i] += p[e];
           }
           u32x4 pf[NP];
-          split8<DT>(p, NP, pf);
+          split8<DT, false>(p, pf);
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
             const uint16_t* at = vw + (kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3);
@@ -532,19 +551,17 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * VROW));
             const u32x2 lw = __builtin_bit_cast(u32x2, lo), hw = __builtin_bit_cast(u32x2, hi);
             const frag vf = __builtin_bit_cast(frag, u32x4{lw[0], lw[1], hw[0], hw[1]});
-            if (precise) {
+            const frag vs = careful ? finite_part<DT>(vf) : vf;
 #pragma unroll
-              for (int p = NP - 1; p > 0; --p) o[i][d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[p]), o[i][d]);
-            }
+            for (int p = NP - 1; p > 0; --p) o[i][d] = Mfma<DT>::m16(vs, __builtin_bit_cast(frag, pf[p]), o[i][d]);
             o[i][d] = Mfma<DT>::m16(vf, __builtin_bit_cast(frag, pf[0]), o[i][d]);
           }
         }
       }
     }
-    // An infinity meets the small parts of an operand as inf * 0 or with the wrong sign.  Where something is not
-    // finite the part is computed again from the leading parts alone, whose zeros and signs are the operand's.
-    if (!precise) break;
-    bool finite = true;
+  };
+  auto all_finite = [&]() __attribute__((always_inline)) {
+    bool yes = true;
 #pragma unroll
     for (int i = 0; i < HT; ++i) {
       float sum = l[i];
@@ -552,14 +569,21 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum += __builtin_fabsf(o[i][d][e]);
-      finite = finite && !__ballot(i * 16 + l16 < gh && !(sum < __builtin_inff()));
+      yes = yes && !__ballot(i * 16 + l16 < gh && !(sum < __builtin_inff()));
     }
-    if (finite) break;
-    precise = false;
+    return yes;
+  };
+  auto rewind = [&]() __attribute__((always_inline)) {
     u = u0 + wv;
     load(u, load_ids(u));
     ids = load_ids(min(u + W, u1 - 1));
-  }
+  };
+  // An infinity would meet the small parts of the other operand as inf * 0 or with the wrong sign, so it is to meet the
+  // leading one alone, whose zeros and signs are the operand's.  Where a head's sums are not finite the part is done again
+  // with keys and values that are not finite left out of the products with the small parts (a query's own have none,
+  // split8).  What is finite keeps its bits.
+  attend(std::false_type{});
+  if (!all_finite()) rewind(), attend(std::true_type{});
 
   // The waves' outputs meet in LDS.
   float* const ow = reinterpret_cast<float*>(kw);

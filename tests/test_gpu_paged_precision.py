@@ -6,7 +6,7 @@ import torch
 
 import _paged_ref as R
 import int4_hip
-from test_gpu_paged import BOTH, DEV, _check, _run, _to
+from test_gpu_paged import BOTH, PROB, _check, _run, _to
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,46 @@ def test_attention_outputs_are_rounded_once():
         differ += (out != want).sum().item()
         count += want.numel()
     assert differ <= 7e-4 * count, (differ, count)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("where", ["value", "key", "query", "new value", "two of them"])
+@pytest.mark.parametrize("nh,nkv,d", [(8, 2, 64), (20, 2, 128), (48, 2, 64)])
+def test_attention_beside_infinities(dtype, where, nh, nkv, d):
+    """What is finite beside infinities and NaN, in other heads and channels and of other
+    slots' weights, is as near as without them: the bounds of test_gpu_paged.py."""
+    print(f"[paged attention] {dtype} {nh}/{nkv}x{d}, {where}", flush=True)
+    c = R.attention_case([50, 50, 700, 50], nh, nkv, d, 16, dtype, seed=nh)
+    c["q"] *= 3
+    for b, bad in enumerate((float("inf"), -float("inf"), float("inf"), float("nan"))):
+        p, s = int(c["table"][b, 1]), 5
+        if where == "query":
+            c["q"][b, 7] = bad
+        elif where == "new value":
+            c["v"][b, 3] = bad
+        elif where == "two of them":
+            c["v_pages"][p, 0, s, 40], c["v_pages"][p, 0, s + 1, 40] = bad, -bad
+            c["v_pages"][p, 1, s, 11] = bad
+        else:
+            (c["v_pages"] if where == "value" else c["k_pages"])[p, 1, s, 9] = bad
+    g = _to(c)
+    out = int4_hip.paged_attention(**g)
+    want, mass, _, grown = R.attention(**c)
+    assert want.isfinite().any(-1).all()
+    _check(out, want, mass.nan_to_num(0, 0, 0), dtype)
+    got = g["weight"].double().cpu()
+    assert torch.equal(got.isnan(), grown.isnan())
+    ok = grown.isfinite()
+    assert ((got - grown).abs()[ok] <= (PROB * nh / nkv + 2.0 ** -23 * grown.abs())[ok]).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_attention_beside_a_key_of_minus_infinity(dtype):
+    """A slot that scores -inf in every head weighs nothing, and costs the others nothing."""
+    c = R.attention_case([900], 8, 2, 64, 64, dtype, seed=21)
+    c["positions"][:] = 0  # no rotation
+    c["q"] *= 3
+    c["q"].view(1, 8, 64)[:, :, 5] = c["q"].view(1, 8, 64)[:, :, 5].abs() + 0.25
+    for i, s in ((0, 3), (7, 60), (13, 0)):
+        c["k_pages"][int(c["table"][0, i]), :, s, 5] = -float("inf")
+    _run(c, dtype)
