@@ -273,6 +273,13 @@ struct Share {
   }
 };
 
+// Between LDS accesses of one wave whose lanes write what others read: the LDS takes a wave's accesses in their order, and
+// the compiler is to leave them in it.  No instruction.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
@@ -448,6 +455,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
     for (; u < u1; u += W) {
       const int base = u * UP;
       const bool last = base + UP > len;  // the new token is in this unit, and what lies past it
+      wave_lds_order();  // the new token is there, the unit before has been read
       if (last) {
         const int at = len - base;
         const u32x4 kn = *reinterpret_cast<const u32x4*>(&new_s[0][sd]);
@@ -464,13 +472,14 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
         *reinterpret_cast<u32x4*>(kw + krow(i) * KROW + sd) = kr[i];
         *reinterpret_cast<u32x4*>(vw + (i * VR + srow) * VROW + sd) = vr[i];
       }
+      wave_lds_order();
       if (u + W < u1) {  // the next unit's loads travel under the rest
         load(u + W, ids);
         ids = load_ids(min(u + 2 * W, u1 - 1));
       }
 #pragma unroll
       for (int i = 0; i < HT; ++i) {
-        if constexpr (HT > 1) asm volatile("" ::: "memory");  // (keys held for both tiles would be spilled)
+        if constexpr (HT > 1) wave_lds_order();  // (keys held for both tiles would be spilled)
         f32x4 s[KB][2];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -586,6 +595,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
   if (!all_finite()) rewind(), attend(std::true_type{});
 
   // The waves' outputs meet in LDS.
+  wave_lds_order();
   float* const ow = reinterpret_cast<float*>(kw);
 #pragma unroll
   for (int i = 0; i < HT; ++i) {
