@@ -372,7 +372,10 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // ---------------------------------------------------------------- paged cache and log probabilities
 // Each takes the arguments of the Python function of its name, all of them by position.
 
-bool tracked(const at::Tensor* t) { return t->requires_grad() && c10::GradMode::is_enabled(); }
+// A derivative is asked for: gradients are recorded, or the tensor holds a tangent.
+bool tracked(const at::Tensor* t) {
+  return (t->requires_grad() && c10::GradMode::is_enabled()) || t->_fw_grad(/*level=*/0).defined();
+}
 
 // The cache of plain, dense tensors; false: not plain.
 struct Cache {
@@ -429,7 +432,7 @@ bool index_fit(const at::Tensor* t, int64_t n, c10::Device dev) {
 bool angles_fit(const at::Tensor* cos, const at::Tensor* sin, int64_t d, c10::Device dev) {
   for (const at::Tensor* t : {cos, sin})
     if (!t || t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(1) != d / 2 || t->size(0) < 1 ||
-        t->device() != dev || !t->is_contiguous() || (uintptr_t)t->const_data_ptr() % 16 != 0)
+        t->device() != dev || !t->is_contiguous() || (uintptr_t)t->const_data_ptr() % 16 != 0 || tracked(t))
       return false;
   return cos->size(0) == sin->size(0);
 }

@@ -38,6 +38,14 @@ def fusable(*tensors: torch.Tensor) -> bool:
     return True
 
 
+def underived(*tensors: torch.Tensor | None) -> bool:
+    """No derivative of what is read or written is asked for: none of the tensors records
+    gradients or holds a tangent, which a call on raw pointers would drop."""
+    grad, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    return not any(t is not None and ((grad and t.requires_grad) or
+                                      (dual and forward_ad.unpack_dual(t).tangent is not None)) for t in tensors)
+
+
 def _on(device: torch.device, call) -> int:
     """``call(stream)`` on the current stream of ``device``, made current."""
     if _C._cuda_getDevice() == device.index:

@@ -28,14 +28,14 @@ import torch
 
 from . import _lib
 from .gemm import _with_workspace
-from .llama_ops import DTYPES, _on
+from .llama_ops import DTYPES, _on, underived
 
 HEAD_DIMS = (64, 128)
 
 
 def _no_grad(*tensors):
-    assert not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)), \
-        "the paged cache's operators have no backward pass: call them under torch.no_grad()"
+    assert underived(*tensors), \
+        "the paged cache's operators have no derivatives: call them under torch.no_grad(), on tensors without tangents"
 
 
 def _cache(k_pages, v_pages, table, weight):
@@ -86,7 +86,7 @@ def paged_append(k, v, cos, sin, k_pages, v_pages, table, rows, slots, positions
     if _lib.ext is not None and _lib.ext.paged_append(k, v, cos, sin, k_pages, v_pages, table, rows, slots, positions,
                                                       weight):
         return  # plain operands: the same call without Python's share of its cost
-    _no_grad(k, v, k_pages, v_pages, weight)
+    _no_grad(k, v, cos, sin, k_pages, v_pages, weight)
     c = _cache(k_pages, v_pages, table, weight)
     dev, T = k_pages.device, k.shape[0]
     nkv, d = c.kv_heads, c.head_dim
@@ -121,7 +121,7 @@ def paged_attention(q, k, v, cos, sin, k_pages, v_pages, table, lengths, positio
         out = _lib.ext.paged_attention(q, k, v, cos, sin, k_pages, v_pages, table, lengths, positions, weight)
         if out is not None:
             return out
-    _no_grad(q, k, v, k_pages, v_pages, weight)
+    _no_grad(q, k, v, cos, sin, k_pages, v_pages, weight)
     c = _cache(k_pages, v_pages, table, weight)
     dev, dtype, B = k_pages.device, k_pages.dtype, table.shape[0]
     nkv, d = c.kv_heads, c.head_dim

@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 from .gemm import _with_workspace
-from .llama_ops import _on
+from .llama_ops import _on, underived
 
 DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
 MAX_TOP = 64
@@ -36,8 +36,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
         if r is not None:
             return TokenLogprobs(*r)
     assert logits.dtype in DTYPES and logits.dim() == 2 and logits.is_cuda, (logits.dtype, logits.shape)
-    assert not (torch.is_grad_enabled() and logits.requires_grad), \
-        "token_logprobs has no backward pass: call it under torch.no_grad()"
+    assert underived(logits), \
+        "token_logprobs has no derivatives: call it under torch.no_grad(), on logits without tangents"
     R, V = logits.shape
     dev = logits.device
     assert V >= 1 and 0 <= top <= min(MAX_TOP, V), (V, top)

@@ -1,0 +1,44 @@
+"""GPU: what the paged cache's operators and token_logprobs would lose of their operands
+is refused: gradients, tangents."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import _paged_ref as R
+import int4_hip
+from test_gpu_paged import DEV, _to
+
+pytestmark = pytest.mark.gpu
+
+
+def _calls(dtype=torch.float16):
+    """(function, arguments by name) of one call of each operator, every argument plain."""
+    c = _to(R.attention_case([5, 2], 4, 2, 64, 16, dtype, seed=1))
+    i = torch.zeros(2, dtype=torch.int32, device=DEV)
+    append = {n: c[n] for n in ("k", "v", "cos", "sin", "k_pages", "v_pages", "table", "weight")}
+    append.update(rows=i, slots=i + 1, positions=i)
+    evict = {n: c[n] for n in ("k_pages", "v_pages", "weight", "table", "lengths")}
+    evict.update(new_table=torch.tensor([[2], [3]], dtype=torch.int32, device=DEV), keep=4, recent=1)
+    x = torch.randn(3, 40, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    score = dict(logits=x, tokens=torch.tensor([1, 0, 39], device=DEV), top=3)
+    return {"attention": (int4_hip.paged_attention, c), "append": (int4_hip.paged_append, append),
+            "evict": (int4_hip.paged_evict, evict), "logprobs": (int4_hip.token_logprobs, score)}
+
+
+FLOATS = [("attention", n) for n in ("q", "k", "v", "cos", "sin", "k_pages", "v_pages", "weight")] + \
+         [("append", n) for n in ("k", "v", "cos", "sin", "k_pages", "v_pages", "weight")] + \
+         [("evict", n) for n in ("k_pages", "v_pages", "weight")] + [("logprobs", "logits")]
+
+
+@pytest.mark.parametrize("op,name", FLOATS)
+def test_gradients_and_tangents_are_refused(op, name):
+    f, c = _calls()[op]
+    f(**c)
+    with pytest.raises(AssertionError, match="no_grad"):
+        f(**dict(c, **{name: c[name].clone().requires_grad_()}))
+    with torch.no_grad():
+        f(**dict(c, **{name: c[name].clone().requires_grad_()}))
+    with forward_ad.dual_level():
+        f(**c)  # no tangent among them
+        with torch.no_grad(), pytest.raises(AssertionError, match="tangent"):
+            f(**dict(c, **{name: forward_ad.make_dual(c[name].clone(), torch.ones_like(c[name]))}))
