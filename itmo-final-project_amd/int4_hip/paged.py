@@ -47,6 +47,7 @@ def _cache(k_pages, v_pages, table, weight):
     dev = k_pages.device
     assert k_pages.is_cuda and v_pages.device == table.device == dev
     assert k_pages.is_contiguous() and v_pages.is_contiguous()
+    assert not any(t is not None and t.is_neg() for t in (k_pages, v_pages, table, weight))
     assert table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous() and table.shape[1] >= 1
     if weight is not None:
         assert weight.dtype == torch.float32 and weight.shape == (P, nkv, S) and weight.is_contiguous()
@@ -58,6 +59,7 @@ def _cache(k_pages, v_pages, table, weight):
 def _angles(cos, sin, d, dev):
     assert cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape
     assert cos.shape[1] == d // 2 and cos.shape[0] >= 1 and cos.device == sin.device == dev
+    cos, sin = cos.resolve_neg(), sin.resolve_neg()
     return tuple(t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
                  for t in (cos, sin))
 
@@ -65,6 +67,7 @@ def _angles(cos, sin, d, dev):
 def _rows(t, n, width, dtype, dev):
     """``t`` [n, width] with dense, 16-byte aligned rows, copied where it has none."""
     assert t.dtype == dtype and t.device == dev and t.shape == (n, width), (t.dtype, t.shape, (n, width))
+    t = t.resolve_neg()
     if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
@@ -72,7 +75,7 @@ def _rows(t, n, width, dtype, dev):
 
 def _index(t, n, dev):
     assert t.dtype == torch.int32 and t.shape == (n,) and t.device == dev, (t.dtype, t.shape, n)
-    return t.contiguous()
+    return t.resolve_neg().contiguous()
 
 
 def paged_append(k, v, cos, sin, k_pages, v_pages, table, rows, slots, positions, weight=None) -> None:
@@ -165,7 +168,7 @@ def paged_evict(k_pages, v_pages, weight, table, lengths, new_table, keep: int, 
     dev, B = k_pages.device, table.shape[0]
     lengths = _index(lengths, B, dev)
     assert new_table.dtype == torch.int32 and new_table.dim() == 2 and new_table.shape[0] == B
-    assert new_table.is_contiguous() and new_table.device == dev
+    assert new_table.is_contiguous() and new_table.device == dev and not new_table.is_neg()
     assert 0 <= recent <= keep and 1 <= keep <= new_table.shape[1] * c.page_size, (keep, recent, new_table.shape)
     n = torch.empty(B, dtype=torch.int32, device=dev)
     lib = _lib.load()

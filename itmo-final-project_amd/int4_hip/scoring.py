@@ -38,6 +38,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
     assert logits.dtype in DTYPES and logits.dim() == 2 and logits.is_cuda, (logits.dtype, logits.shape)
     assert underived(logits), \
         "token_logprobs has no derivatives: call it under torch.no_grad(), on logits without tangents"
+    logits = logits.resolve_neg()
     R, V = logits.shape
     dev = logits.device
     assert V >= 1 and 0 <= top <= min(MAX_TOP, V), (V, top)
@@ -46,7 +47,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
     logprob = None
     if tokens is not None:
         assert tokens.dtype == torch.int64 and tokens.shape == (R,) and tokens.device == dev, tokens.shape
-        tokens = tokens.contiguous()
+        tokens = tokens.resolve_neg().contiguous()
         logprob = torch.empty(R, device=dev)
     entropy = torch.empty(R, device=dev)
     top_logprob = torch.empty((R, top), device=dev)

@@ -1,5 +1,5 @@
 """GPU: what the paged cache's operators and token_logprobs would lose of their operands
-is refused: gradients, tangents."""
+is refused or resolved: gradients, tangents, negated views."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -42,3 +42,31 @@ def test_gradients_and_tangents_are_refused(op, name):
         f(**c)  # no tangent among them
         with torch.no_grad(), pytest.raises(AssertionError, match="tangent"):
             f(**dict(c, **{name: forward_ad.make_dual(c[name].clone(), torch.ones_like(c[name]))}))
+
+
+@pytest.mark.parametrize("op,name", FLOATS + [("attention", "lengths"), ("attention", "positions"), ("append", "rows"),
+                                              ("append", "slots"), ("evict", "lengths"), ("logprobs", "tokens")])
+def test_negated_views_are_resolved_or_refused(op, name):
+    """An operand whose memory holds the negative of its values; what is written to is refused."""
+    f, c = _calls()[op]
+    plain = _calls()[op][1]
+    negated = torch._neg_view(c[name].neg())
+    assert negated.is_neg() and negated.is_contiguous()
+    c = dict(c, **{name: negated})
+    if name in ("k_pages", "v_pages", "weight"):
+        with pytest.raises(AssertionError):
+            f(**c)
+        return
+    got, want = f(**c), f(**plain)
+    pairs = [(got, want)] if torch.is_tensor(got) else list(zip(got, want)) if got is not None else []
+    pairs += [(c[n], plain[n]) for n in ("k_pages", "v_pages", "weight") if n in c]
+    for a, b in pairs:
+        assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) if a.is_floating_point() else torch.equal(a, b)
+
+
+@pytest.mark.parametrize("op,name", [("attention", "table"), ("append", "table"), ("evict", "table"),
+                                     ("evict", "new_table")])
+def test_negated_tables_are_refused(op, name):
+    f, c = _calls()[op]
+    with pytest.raises(AssertionError):
+        f(**dict(c, **{name: torch._neg_view(c[name].neg())}))
