@@ -306,8 +306,8 @@ int w4_norm_head(const void* x, const void* delta, const void* norm_weight, floa
  *   k, v    [pages, kv_heads, page_size, head_dim] bf16 / fp16, dense, 16-byte aligned;
  *           keys are held rotated
  *   weight  fp32 [pages, kv_heads, page_size], dense: the attention weight each token
- *           has received from every later query of its head's group; NULL where the
- *           caller does not keep it
+ *           has received from every query of its head's group that w4_paged_attention
+ *           has taken since; NULL where the caller does not keep it
  *   table   int32 [rows, width], dense: page of slots i * page_size.. of a row; entries
  *           past a row's tokens are not read.  A page may stand in several rows (a
  *           shared prefix) where weight is NULL and neither row writes to it.

@@ -10,7 +10,8 @@ One layer's cache, shared by all sequences of a batch (``rows``):
   * ``table`` int32 [rows, width]: the page of slots i * page_size.. of a row
     (entries past its tokens are not read);
   * ``weight`` fp32 [pages, kv_heads, page_size], where the cache is to be evicted
-    from: the attention each token has received since it came into the cache.
+    from: the attention each token has received, from the queries of ``paged_attention``
+    alone, since it came into the cache.
 
 A token's *slot* is its place in the cache, its *position* the one its angles are
 taken from; they part once something is evicted.  ``cos`` and ``sin`` are the

@@ -34,11 +34,12 @@ class BatchDecoder:
     ``pages`` pages of ``page_size`` tokens are shared by all rows, at most ``width`` of
     them a row's.  With ``keep`` (and ``recent``) a row that has more than ``keep``
     tokens when ``evict`` is called is cut to its last ``recent`` and, of the others,
-    those with the largest accumulated attention weight.
+    those with the largest accumulated attention weight: from the last ``window`` tokens
+    of its prompt, which stand for what comes next, and from every token decoded since.
     """
 
     def __init__(self, model: LlamaForCausalLM, rows: int, pages: int, width: int, page_size: int = 64,
-                 max_positions: int = 8192, keep: int | None = None, recent: int = 0, top: int = 1):
+                 max_positions: int = 8192, keep: int | None = None, recent: int = 0, top: int = 1, window: int = 32):
         c = model.config
         self.model, self.rows, self.page_size, self.width = model, rows, page_size, width
         self.heads = c.num_attention_heads, c.num_key_value_heads, c.head_dim
@@ -50,7 +51,9 @@ class BatchDecoder:
             raise ValueError("BatchDecoder stands for the model's own attention: a layer has another, or a hook on it")
         if top < 1:
             raise ValueError("the most likely token is the next one: top is at least 1")
-        self.keep, self.recent, self.top = keep, recent, top
+        if window < 1:
+            raise ValueError("a prompt's last token, at least, weighs the ones before it")
+        self.keep, self.recent, self.top, self.window = keep, recent, top, window
         nl, nkv, d = c.num_hidden_layers, c.num_key_value_heads, c.head_dim
         self.k = torch.zeros((nl, pages, nkv, page_size, d), dtype=dtype, device=dev)
         self.v = torch.zeros_like(self.k)
@@ -120,10 +123,18 @@ class BatchDecoder:
         cos, sin = self.cos[:T], self.sin[:T]
         slots = torch.arange(T, dtype=torch.int32, device=dev)
         rows = torch.full_like(slots, row)
+        own = self.table[row:row + 1, :len(self.owned[row])]
 
         def attend(i, q, k, v):
-            paged_append(k, v, self.cos, self.sin, self.k[i], self.v[i], self.table, rows, slots, slots,
-                         None if self.weight is None else self.weight[i])
+            weight = None if self.weight is None else self.weight[i]
+            paged_append(k, v, self.cos, self.sin, self.k[i], self.v[i], self.table, rows, slots, slots, weight)
+            if weight is not None:
+                # the prompt's last queries weigh what they attend to, one after the other (they share the row's
+                # weights); each writes its own key and value again
+                for t in range(max(T - self.window, 0), T):
+                    one = slice(t, t + 1)
+                    paged_attention(q[one], k[one], v[one], self.cos, self.sin, self.k[i], self.v[i], own, slots[one],
+                                    slots[one], weight)
             return llama_ops.attention_prefill(q, k, v, cos, sin, kc, vc, 0, nh, nkv, d)
 
         logits = self._run(self.model.model.embed_tokens(prompt), attend)
