@@ -112,6 +112,8 @@ class BatchDecoder:
         ``ids``.  Returns the log probabilities of the prompt's own tokens 1.. (and of
         the alternatives after each of its tokens)."""
         T, dev = prompt.shape[0], self.ids.device
+        if not 0 <= row < self.rows:
+            raise ValueError(f"row {row} of {self.rows}")
         if self.length[row] >= 0 or T < 1:
             raise ValueError(f"row {row} is taken, or the prompt empty")
         if T > len(self.cos):

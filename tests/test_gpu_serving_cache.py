@@ -65,3 +65,12 @@ def test_a_prompt_weighs_its_tokens(T, window):
         least = early.sort().values[-(keep - recent)]
         assert all((i in kept) == (w > least) for i, w in enumerate(early.tolist()) if abs(w / least - 1) > 1e-4)
     dec.step()  # and goes on
+
+
+@pytest.mark.parametrize("row", [-1, -4, 4])
+def test_rows_that_do_not_exist_are_refused(row):
+    """A negative row is no row of the table: its tokens would go nowhere."""
+    dec = _decoder(_model())
+    with pytest.raises(ValueError):
+        dec.add(row, _prompt(5, 1))
+    assert dec.length == [-1] * 4 and len(dec.free) == 64 and dec.lengths.tolist() == dec.length
