@@ -53,6 +53,8 @@ class BatchDecoder:
             raise ValueError("the most likely token is the next one: top is at least 1")
         if window < 1:
             raise ValueError("a prompt's last token, at least, weighs the ones before it")
+        if keep is not None and not (keep >= 1 and 0 <= recent <= keep):
+            raise ValueError(f"a row is cut to keep >= 1 tokens, 0 to keep of them the last ones: got {keep}, {recent}")
         self.keep, self.recent, self.top, self.window = keep, recent, top, window
         nl, nkv, d = c.num_hidden_layers, c.num_key_value_heads, c.head_dim
         self.k = torch.zeros((nl, pages, nkv, page_size, d), dtype=dtype, device=dev)

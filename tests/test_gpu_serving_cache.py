@@ -74,3 +74,10 @@ def test_rows_that_do_not_exist_are_refused(row):
     with pytest.raises(ValueError):
         dec.add(row, _prompt(5, 1))
     assert dec.length == [-1] * 4 and len(dec.free) == 64 and dec.lengths.tolist() == dec.length
+
+
+@pytest.mark.parametrize("keep,recent", [(0, 0), (-3, 0), (8, 9), (8, -1)])
+def test_budgets_that_cannot_be_kept_are_refused(keep, recent):
+    """When the decoder is made, and not by an eviction that has taken its pages."""
+    with pytest.raises(ValueError):
+        _decoder(_model(), keep=keep, recent=recent)
