@@ -165,22 +165,25 @@ class BatchDecoder:
 
     @torch.no_grad()
     def capture(self) -> None:
-        """Capture the step in a graph; all state is put back afterwards."""
+        """Capture the step in a graph; all state is put back afterwards, also where it fails."""
         state = (self.ids, self.lengths, self.positions)
         kept = [t.clone() for t in state]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side):  # workspaces; idle rows write nothing to the cache
-            self.lengths.fill_(-1)
-            self._step()
-        torch.cuda.current_stream().wait_stream(side)
-        torch.cuda.synchronize()
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=side):
-            self.out = self._step()
-        for t, was in zip(state, kept):
-            t.copy_(was)
-        self.graph = graph
+        try:
+            with torch.cuda.stream(side):  # workspaces; idle rows write nothing to the cache
+                self.lengths.fill_(-1)
+                self._step()
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = self._step()
+        finally:
+            torch.cuda.current_stream().wait_stream(side)
+            for t, was in zip(state, kept):
+                t.copy_(was)
+        self.graph, self.out = graph, out
 
     @torch.no_grad()
     def step(self) -> Step:

@@ -81,3 +81,33 @@ def test_budgets_that_cannot_be_kept_are_refused(keep, recent):
     """When the decoder is made, and not by an eviction that has taken its pages."""
     with pytest.raises(ValueError):
         _decoder(_model(), keep=keep, recent=recent)
+
+
+@pytest.mark.parametrize("at", [0, 1])
+def test_a_capture_that_fails_leaves_the_rows_as_they_were(at, monkeypatch):
+    """In its warm-up, or under capture: lengths, positions and tokens are put back, and
+    the decoder goes on as if it had not been asked."""
+    m = _model()
+    out = []
+    for fail in (False, True):
+        dec = _decoder(m)
+        dec.add(0, _prompt(20, 1))
+        dec.add(2, _prompt(7, 2))
+        dec.step()
+        if fail:
+            step, calls = dec._step, []
+
+            def broken():
+                calls.append(len(calls))
+                if len(calls) == at + 1:
+                    raise MemoryError("none left")
+                return step()
+
+            monkeypatch.setattr(dec, "_step", broken)
+            with pytest.raises(MemoryError):
+                dec.capture()
+            monkeypatch.undo()
+            assert dec.graph is None and dec.lengths.tolist() == dec.length
+        out.append([dec.step().alternatives.top_logprob[[0, 2]].clone() for _ in range(5)])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
