@@ -346,8 +346,10 @@ int w4_paged_append(const w4_paged_cache* cache, int dtype, const void* k, const
 /*
  * Attention of one new token of every row: its key and value are written to slot
  * lengths[b] as by w4_paged_append, then out [rows, num_heads * head_dim] (dense) =
- * softmax(rope(q) K / sqrt(head_dim)) V over slots 0..lengths[b], in fp32 from the
- * cached 16-bit keys and values, rounded once.  With cache->weight every slot's
+ * softmax(rope(q) K / sqrt(head_dim)) V over slots 0..lengths[b], from the cached
+ * 16-bit keys and values, rounded once; fp32 sums, queries and probabilities entering
+ * them with 24 bits (fp16: 22, of numbers down to 2^-38 of a query's largest element
+ * and of a part's largest probability).  With cache->weight every slot's
  * weight grows by the probabilities that the heads of its group gave it (the new
  * slot's is set to them); `scores` is then scratch of rows * num_heads * width *
  * page_size floats, else NULL.  lengths[b] < 0: the row is idle, its out zero and

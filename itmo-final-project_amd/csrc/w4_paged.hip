@@ -314,10 +314,11 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
 // which puts the keys into the tiles' order and transposes the values on reading.  A head's reference follows the
 // running maximum with a lag (Probs; its value cancels in the end), so that most units need no exchange between lanes.
 //
-// Bound by memory where there is enough of it: 131000 slots of 32 / 8 heads of 128 in 91.6 us, 537 MB at 5.9 TB/s; 16
-// rows of 3001 with the weights' scores (203 MB) in 39.8; 32 rows of up to 4000 of 64 in 31.7, 123 MB at 3.9 TB/s,
+// Bound by memory where there is enough of it: 131000 slots of 32 / 8 heads of 128 in 88.3 us, 537 MB at 6.1 TB/s; 16
+// rows of 3001 with the weights' scores (203 MB) in 39.5; 32 rows of up to 4000 of 64 in 32.6, 123 MB at 3.8 TB/s,
 // whose unequal parts leave CUs idle at the end.  A short row is a chain of latencies (lengths, page, tokens, sums,
-// output): 100 slots 7.2 us.
+// output): 100 slots 7.5 us.  bf16 probabilities in three parts instead of two cost 1 to 3% (6 rows of up to 117000 slots
+// of 24 / 1 heads of 64: 33.3 us instead of 31.3).
 template <int DT, int D, int W, int HT>
 __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int KB = 128 / D, UP = 32 * KB, NJ = D / 32, ND = D / 16, VR = 512 / D, NP = Split<DT>::N;
@@ -699,7 +700,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
 // joined (a wide group's by the last part alone would be one CU's traffic with memory).  The others add every
 // slot's probabilities to its weight, from the scores, maxima and sums: the parts of the rows again, four slots
 // a thread.  (In the attention itself the sums are not at hand until all parts are through.)  A chain of latencies, of
-// the parts, their sums, the scores: 5.9 us for 16 rows of 3001 slots of 32 / 8 heads, 9.2 MB; 6.6 for 3 of up to 20000
+// the parts, their sums, the scores: 6.0 us for 16 rows of 3001 slots of 32 / 8 heads, 9.2 MB; 6.7 for 3 of up to 20000
 // of 20 / 2 heads.
 template <int DT, int D>
 __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnArgs a) {
@@ -805,7 +806,9 @@ constexpr int kSelectPlace = 16384;  // early slots that the selection lists its
 //
 // What bounds it is the latency of its steps on the one CU that has the row and head, so the keys are read from
 // memory once and stay in LDS (of more than 32768 early slots, a run at a time in every step).  32768 slots: 20.1 us,
-// of them 4.1 for the keys, 4.0 for the first histogram, 3.3 for the list, 2.8 for the counts; 100000 slots 55.1.
+// of them 4.1 for the keys, 4.0 for the first histogram, 3.3 for the list, 2.8 for the counts; 100000 slots 55.1.  Equal
+// weights are the slowest: all keys fall into one bin, an atomic on one address each, in every histogram (an eviction of
+// 4 x 32768 slots 127 us instead of 54, of 576 slots 13.7 instead of 11.5, of 100000 328 instead of 91).
 //
 // ONCE: no row is longer than LDS holds (a kernel that may have to load again is slower for the others: 32768 slots
 // 21.8 us instead of 20.2, 576 slots 6.2 instead of 5.7).  PLACE: the rows are short enough that the kept slots are
@@ -1213,7 +1216,7 @@ struct PagedAttnPlan {
 // long enough for it: 24 / 1 heads, 10 rows of 107000 slots with weights 109 us instead of 170, 6 of up to 117000
 // 26.7 instead of 49.1; 16 of up to 2000 would take 14.2 instead of 11.1.  So they do where the weights then need no
 // second launch (7 of 15 11.8 us instead of 8.4 and 5.8, 300 of 120 17.7 instead of 15.9 and 12.7).  (Heads of 128
-// have no registers for two tiles.)
+// have no registers for two tiles.)  (Both sides of each with bf16 probabilities in two parts, 1 to 3% faster than three.)
 bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, int64_t units, bool weights,
                      PagedAttnPlan* p) {
   if (rows < 0 || num_heads < 1 || kv_heads < 1 || num_heads % kv_heads) return false;

@@ -13,6 +13,11 @@ One layer's cache, shared by all sequences of a batch (``rows``):
     from: the attention each token has received, from the queries of ``paged_attention``
     alone, since it came into the cache.
 
+Rows may share pages (a common prefix) where there is no ``weight`` and none of them
+writes there.  With ``weight`` every page is one row's alone: the attention of a row
+reads, adds to and writes back its weights with no regard to another's, and
+``paged_append`` sets them to 0.
+
 A token's *slot* is its place in the cache, its *position* the one its angles are
 taken from; they part once something is evicted.  ``cos`` and ``sin`` are the
 tables of all positions, fp32 [positions, head_dim / 2] (``apply_rope`` of

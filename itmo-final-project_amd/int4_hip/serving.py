@@ -24,6 +24,9 @@ from .scoring import TokenLogprobs, token_logprobs
 
 
 class Step(NamedTuple):
+    """Of a captured step these are the graph's own tensors, and ``token`` is always ``ids``:
+    the next ``step`` overwrites them, so what is to be kept is copied before it."""
+
     token: torch.Tensor          # int64 [rows]: the tokens now in ``ids``, idle rows' meaningless
     alternatives: TokenLogprobs  # of every row's logits
 
@@ -36,6 +39,11 @@ class BatchDecoder:
     tokens when ``evict`` is called is cut to its last ``recent`` and, of the others,
     those with the largest accumulated attention weight: from the last ``window`` tokens
     of its prompt, which stand for what comes next, and from every token decoded since.
+
+    The cache holds keys and values in the model's dtype (``decode_step`` of the model
+    keeps them in fp32).  With ``keep`` a step holds rows * heads * width * page_size fp32
+    scores, whatever the rows hold, so ``width`` is best no more than a row may need
+    (of 32 rows of 32 heads 4 MB for every 1024 tokens of it).
     """
 
     def __init__(self, model: LlamaForCausalLM, rows: int, pages: int, width: int, page_size: int = 64,
@@ -112,7 +120,8 @@ class BatchDecoder:
     def add(self, row: int, prompt: torch.Tensor) -> TokenLogprobs:
         """Start a sequence in an idle row with a 1-D prompt; its next token is put in
         ``ids``.  Returns the log probabilities of the prompt's own tokens 1.. (and of
-        the alternatives after each of its tokens)."""
+        the alternatives after each of its tokens), for which it makes all of the
+        prompt's logits at once."""
         T, dev = prompt.shape[0], self.ids.device
         if not 0 <= row < self.rows:
             raise ValueError(f"row {row} of {self.rows}")
