@@ -85,7 +85,7 @@ struct PagedAttnArgs {
   uint16_t* out;  // [rows, nkv * g * D]
   float* scores;  // [rows, nkv * g, width * page_size], of q K / sqrt(D); null without weights
   float* part;    // [items, min(g, tile), D]: outputs of a part, where a row's slots are cut
-  float* stats;   // [items, tile, 2]: its heads' references, in powers of two, and sums relative to them
+  float* stats;   // [items, tile, 2]: its heads' references and sums relative to them
   int* first;     // [rows, nkv * htiles, 2]: index of a row and tile's first part, and how many there are
   unsigned* cnt;  // one arrival counter per row and tile of heads
   float scale;    // 1 / sqrt(D)
@@ -172,14 +172,14 @@ template <int DT> struct Split;
 template <> struct Split<W4_DTYPE_BF16> { static constexpr int N = 3; };  // 8 significant bits each: all 24
 template <> struct Split<W4_DTYPE_FP16> { static constexpr int N = 2; };  // 11 each: 22
 
-// The range of the probabilities, powers of two relative to a head's reference: when it is raised it is put `above`
-// under the largest score, and raised again only once a score passes that by `lag`.  bf16 has fp32's exponents.  fp16
-// ends at 65504, so the largest probability is kept between 2^13 and 2^15: both parts of one 2^25 times smaller are then
-// still numbers, and what is lost of any is 2^-38 of the largest.  (With the largest at 1, the tail of a row that one
-// token dominates by e^17 would be lost, while its sum counts it.)
+// The range of the probabilities: a head's reference is a score, whose own probability is `first` = 2^above, and is raised to the
+// largest one only once that passes it by 2^lag.  bf16 has fp32's exponents.  fp16 ends at 65504, so the largest
+// probability is kept between 2^13 and 2^15: both parts of one 2^25 times smaller are then still numbers, and what is
+// lost of any is 2^-38 of the largest.  (With the largest at 1, the tail of a row that one token dominates by e^17 would
+// be lost, while its sum counts it.)
 template <int DT> struct Probs;
-template <> struct Probs<W4_DTYPE_BF16> { static constexpr float above = 0.f, lag = 8.f; };
-template <> struct Probs<W4_DTYPE_FP16> { static constexpr float above = 13.f, lag = 2.f; };
+template <> struct Probs<W4_DTYPE_BF16> { static constexpr float above = 0.f, first = 1.f, lag = 8.f; };
+template <> struct Probs<W4_DTYPE_FP16> { static constexpr float above = 13.f, first = 8192.f, lag = 2.f; };
 
 // What a head's query is multiplied by before it is split, a power of two.  Its scores carry it until they become
 // exponents (or are stored).  bf16: nothing.  fp16: its largest element gets to 2^13 or more, so that the parts of one 2^38
@@ -252,13 +252,14 @@ __device__ __forceinline__ void rope_chunk(const uint16_t* __restrict__ x, const
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.f : m; }
 
-// Softmax sums and a quad of outputs, relative to 2^M.  A refused part's maximum is NaN and stays.
+// Softmax sums and a quad of outputs, relative to the score M.  (Scores are subtracted before they become exponents: past
+// 2^24 the exponent's own rounding would be powers of two.)  A refused part's reference is NaN and stays.
 struct Share {
   float M = -__builtin_inff(), L = 0.f;
   f32x4 t = {0.f, 0.f, 0.f, 0.f};
   __device__ __forceinline__ void add(float m, float l, const f32x4& x) {
     const float mn = M != M || m != m ? __builtin_nanf("") : fmaxf(M, m), mz = finite_or_zero(mn);
-    const float w0 = __builtin_amdgcn_exp2f(M - mz), w1 = __builtin_amdgcn_exp2f(m - mz);
+    const float w0 = __builtin_amdgcn_exp2f((M - mz) * kLog2e), w1 = __builtin_amdgcn_exp2f((m - mz) * kLog2e);
     L = __builtin_fmaf(w1, l, L * w0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(w1, x[e], t[e] * w0);
@@ -284,8 +285,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-// The probabilities of slots s.. s + 3 added to their weights (the new token's, slot `len`, set); head(g): the maximum
-// (not -inf) and reciprocal sum of a key-value head's query head.
+// The probabilities of slots s.. s + 3 added to their weights (the new token's, slot `len`, set); head(g): the reference
+// (not -inf) of a key-value head's query head, and its own probability.
 template <typename Head>
 __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h, int s, int len, const Head& head) {
   const int64_t cap = a.c.capacity();
@@ -295,7 +296,7 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
     const f32x4 y = *reinterpret_cast<const f32x4*>(sp + g * cap);
     const f32x2 ml = head(g);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) t[e] += __builtin_amdgcn_exp2f(__builtin_fmaf(y[e], kLog2e, -ml[0])) * ml[1];
+    for (int e = 0; e < 4; ++e) t[e] += __builtin_amdgcn_exp2f((y[e] - ml[0]) * kLog2e) * ml[1];
   }
   float* const wp = a.c.weight + a.c.token(b, s, h);
   f32x4 w = *reinterpret_cast<const f32x4*>(wp);
@@ -530,12 +531,11 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kb][t][e]);
         const float log2e = kLog2e * qs[i].back();
-        top *= log2e;
-        if (__ballot(top > m[i] + (P::above + P::lag))) {
-          float mn = fmaxf(top - P::above, m[i]);
+        if (__ballot((top - m[i]) * log2e > P::lag)) {
+          float mn = fmaxf(top, m[i]);
           mn = fmaxf(mn, __shfl_xor(mn, 16));
           mn = fmaxf(mn, __shfl_xor(mn, 32));
-          const float al = __builtin_amdgcn_exp2f(m[i] - finite_or_zero(mn));
+          const float al = __builtin_amdgcn_exp2f((m[i] - finite_or_zero(mn)) * log2e);
           l[i] *= al;
 #pragma unroll
           for (int d = 0; d < ND; ++d)
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
           float p[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3], log2e, -mz));
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3] - mz, log2e, P::above));
             l[i] += p[e];
           }
           u32x4 pf[NP];
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
     if (hd < gh) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(ow + hd * OROW + d * 16 + 4 * c) = o[i][d];
-      if (c == 0) m_s[wv][hd] = m[i], l_s[wv][hd] = l[i];
+      if (c == 0) m_s[wv][hd] = m[i] * qs[i].back(), l_s[wv][hd] = l[i];
     }
   }
   if (lane == 0) bad_s[wv] = bad;
@@ -632,7 +632,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
       x.add(m_s[w][hd], l_s[w][hd],
             *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(kv_s[w]) + hd * OROW + d));
     if (refused) x.M = x.L = __builtin_nanf("");
-    if (d == 0) head_s[hd] = f32x2{finite_or_zero(x.M), 1.f / x.L};
+    if (d == 0) head_s[hd] = f32x2{finite_or_zero(x.M), P::first / x.L};
     if (it.parts == 1)
       *reinterpret_cast<u32x2*>(out + hd * D + d) = x.template out<DT>();
     else
@@ -765,7 +765,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnAr
   if (run == 0) {
     for (int r = 1; r < min(runs, parts); ++r)
       x.add(red_ml[r * a.g + g][0], red_ml[r * a.g + g][1], f32x4{0.f, 0.f, 0.f, 0.f});
-    red[g] = f32x4{finite_or_zero(x.M), 1.f / x.L, 0.f, 0.f};
+    red[g] = f32x4{finite_or_zero(x.M), Probs<DT>::first / x.L, 0.f, 0.f};
   }
   __syncthreads();
   if (red[0][0] != red[0][0]) return;  // a page outside the pool (in all heads alike)

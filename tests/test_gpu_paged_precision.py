@@ -144,3 +144,18 @@ def test_attention_beside_a_key_of_minus_infinity(dtype):
     for i, s in ((0, 3), (7, 60), (13, 0)):
         c["k_pages"][int(c["table"][0, i]), :, s, 5] = -float("inf")
     _run(c, dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("size", [300.0, 3000.0, 9000.0])
+@pytest.mark.parametrize("lens,nh,nkv,d", [([300, 5], 8, 2, 64), ([2000], 20, 2, 128), ([700] * 3, 24, 1, 64)])
+def test_attention_of_huge_scores(dtype, size, lens, nh, nkv, d):
+    """Queries and keys of up to 9000, scores of up to 5 * 10^8 (2^29 as exponents): a score
+    is off by 2^-22 of that, a hundred, the two largest of some hundreds are 10^4 and more apart,
+    and the output is the value of one token."""
+    print(f"[paged attention] {dtype} {lens} {nh}/{nkv}x{d}, elements of {size}", flush=True)
+    c = R.attention_case(lens, nh, nkv, d, 64, dtype, seed=nh + int(size))
+    for name in ("q", "k", "k_pages"):
+        c[name] = c[name].clamp(-4, 4) * size if name != "k_pages" else \
+            torch.where(c[name].isnan(), c[name], c[name].clamp(-4, 4) * size)
+    _run(c, dtype)
