@@ -159,3 +159,10 @@ def test_attention_of_huge_scores(dtype, size, lens, nh, nkv, d):
         c[name] = c[name].clamp(-4, 4) * size if name != "k_pages" else \
             torch.where(c[name].isnan(), c[name], c[name].clamp(-4, 4) * size)
     _run(c, dtype)
+
+
+@pytest.mark.parametrize("size", [1e5, 1e9, 1e15])
+@pytest.mark.parametrize("lens,nh,nkv,d", [([300, 5], 8, 2, 64), ([2000], 20, 2, 128), ([700] * 3, 24, 1, 64)])
+def test_attention_of_scores_that_bf16_alone_has(size, lens, nh, nkv, d):
+    """As above, of 10^11 to 10^31: the two largest are 10^-5 and more of that apart."""
+    test_attention_of_huge_scores(torch.bfloat16, size, lens, nh, nkv, d)
