@@ -172,18 +172,18 @@ template <int DT> struct Split;
 template <> struct Split<W4_DTYPE_BF16> { static constexpr int N = 3; };  // 8 significant bits each: all 24
 template <> struct Split<W4_DTYPE_FP16> { static constexpr int N = 2; };  // 11 each: 22
 
-// The range of the probabilities: a head's reference is a score, whose own probability is `first` = 2^above, and is raised to the
-// largest one only once that passes it by 2^lag.  bf16 has fp32's exponents.  fp16 ends at 65504, so the largest
-// probability is kept between 2^13 and 2^15: both parts of one 2^25 times smaller are then still numbers, and what is
-// lost of any is 2^-38 of the largest.  (With the largest at 1, the tail of a row that one token dominates by e^17 would
-// be lost, while its sum counts it.)
+// The range of the probabilities: a head's reference is a score, whose own probability is `first` = 2^above, and is
+// raised to the largest one only once that passes it by 2^lag.  bf16 has fp32's exponents.  fp16 ends at 65504, so the
+// largest probability is kept between 2^13 and 2^15: both parts of one 2^25 times smaller are then still numbers, and
+// what is lost of any is 2^-38 of the largest.  (With the largest at 1, the tail of a row that one token dominates by
+// e^17 would be lost, while its sum counts it.)
 template <int DT> struct Probs;
 template <> struct Probs<W4_DTYPE_BF16> { static constexpr float above = 0.f, first = 1.f, lag = 8.f; };
 template <> struct Probs<W4_DTYPE_FP16> { static constexpr float above = 13.f, first = 8192.f, lag = 2.f; };
 
 // What a head's query is multiplied by before it is split, a power of two.  Its scores carry it until they become
-// exponents (or are stored).  bf16: nothing.  fp16: its largest element gets to 2^13 or more, so that the parts of one 2^38
-// times smaller are still numbers, whatever the scale of queries and keys.
+// exponents (or are stored).  bf16: nothing.  fp16: its largest element gets to 2^13 or more, so that the parts of one
+// 2^38 times smaller are still numbers, whatever the scale of queries and keys.
 template <int DT> struct QueryScale {
   __device__ __forceinline__ float set(float) { return 1.f; }
   __device__ __forceinline__ float back() const { return 1.f; }
@@ -203,7 +203,8 @@ template <> struct QueryScale<W4_DTYPE_FP16> {
   __device__ __forceinline__ float back() const { return b; }
 };
 
-// QUERY: an infinity or NaN has no small parts.  (A probability is no infinity, and beside a NaN all of its head's are.)
+// QUERY: an infinity or NaN has no small parts.  (A probability is no infinity, and beside a NaN all of its head's
+// are.)
 template <int DT, bool QUERY>
 __device__ __forceinline__ void split8(const float v[8], u32x4* out) {
   float r[8];
@@ -252,8 +253,8 @@ __device__ __forceinline__ void rope_chunk(const uint16_t* __restrict__ x, const
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.f : m; }
 
-// Softmax sums and a quad of outputs, relative to the score M.  (Scores are subtracted before they become exponents: past
-// 2^24 the exponent's own rounding would be powers of two.)  A refused part's reference is NaN and stays.
+// Softmax sums and a quad of outputs, relative to the score M.  (Scores are subtracted before they become exponents:
+// past 2^24 the exponent's own rounding would be powers of two.)  A refused part's reference is NaN and stays.
 struct Share {
   float M = -__builtin_inff(), L = 0.f;
   f32x4 t = {0.f, 0.f, 0.f, 0.f};
@@ -274,8 +275,8 @@ struct Share {
   }
 };
 
-// Between LDS accesses of one wave whose lanes write what others read: the LDS takes a wave's accesses in their order, and
-// the compiler is to leave them in it.  No instruction.
+// Between LDS accesses of one wave whose lanes write what others read: the LDS takes a wave's accesses in their order,
+// and the compiler is to leave them in it.  No instruction.
 __device__ __forceinline__ void wave_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -285,8 +286,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-// The probabilities of slots s.. s + 3 added to their weights (the new token's, slot `len`, set); head(g): the reference
-// (not -inf) of a key-value head's query head, and its own probability.
+// The probabilities of slots s.. s + 3 added to their weights (the new token's, slot `len`, set); head(g): the
+// reference (not -inf) of a key-value head's query head, and its own probability.
 template <typename Head>
 __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h, int s, int len, const Head& head) {
   const int64_t cap = a.c.capacity();
@@ -315,11 +316,11 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
 // which puts the keys into the tiles' order and transposes the values on reading.  A head's reference follows the
 // running maximum with a lag (Probs; its value cancels in the end), so that most units need no exchange between lanes.
 //
-// Bound by memory where there is enough of it: 131000 slots of 32 / 8 heads of 128 in 88.3 us, 537 MB at 6.1 TB/s; 16
-// rows of 3001 with the weights' scores (203 MB) in 39.5; 32 rows of up to 4000 of 64 in 32.6, 123 MB at 3.8 TB/s,
+// Bound by memory where there is enough of it: 131000 slots of 32 / 8 heads of 128 in 90.2 us, 537 MB at 5.9 TB/s; 16
+// rows of 3001 with the weights' scores (203 MB) in 39.4; 32 rows of up to 4000 of 64 in 32.6, 123 MB at 3.8 TB/s,
 // whose unequal parts leave CUs idle at the end.  A short row is a chain of latencies (lengths, page, tokens, sums,
-// output): 100 slots 7.5 us.  bf16 probabilities in three parts instead of two cost 1 to 3% (6 rows of up to 117000 slots
-// of 24 / 1 heads of 64: 33.3 us instead of 31.3).
+// output): 100 slots 7.7 us.  bf16 probabilities in three parts instead of two cost 1 to 3% (6 rows of up to 117000
+// slots of 24 / 1 heads of 64: 33.3 us instead of 31.3), scores subtracted before they are scaled up to 1%.
 template <int DT, int D, int W, int HT>
 __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int KB = 128 / D, UP = 32 * KB, NJ = D / 32, ND = D / 16, VR = 512 / D, NP = Split<DT>::N;
@@ -589,9 +590,9 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
     ids = load_ids(min(u + W, u1 - 1));
   };
   // An infinity would meet the small parts of the other operand as inf * 0 or with the wrong sign, so it is to meet the
-  // leading one alone, whose zeros and signs are the operand's.  Where a head's sums are not finite the part is done again
-  // with keys and values that are not finite left out of the products with the small parts (a query's own have none,
-  // split8).  What is finite keeps its bits.
+  // leading one alone, whose zeros and signs are the operand's.  Where a head's sums are not finite the part is done
+  // again with keys and values that are not finite left out of the products with the small parts (a query's own have
+  // none, split8).  What is finite keeps its bits.
   attend(std::false_type{});
   if (!all_finite()) rewind(), attend(std::true_type{});
 
@@ -700,7 +701,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(PagedAttnArg
 // joined (a wide group's by the last part alone would be one CU's traffic with memory).  The others add every
 // slot's probabilities to its weight, from the scores, maxima and sums: the parts of the rows again, four slots
 // a thread.  (In the attention itself the sums are not at hand until all parts are through.)  A chain of latencies, of
-// the parts, their sums, the scores: 6.0 us for 16 rows of 3001 slots of 32 / 8 heads, 9.2 MB; 6.7 for 3 of up to 20000
+// the parts, their sums, the scores: 6.0 us for 16 rows of 3001 slots of 32 / 8 heads, 9.2 MB; 7.0 for 3 of up to 20000
 // of 20 / 2 heads.
 template <int DT, int D>
 __global__ __launch_bounds__(kPagedThreads) void paged_finish_kernel(PagedAttnArgs a) {
@@ -804,11 +805,11 @@ constexpr int kSelectPlace = 16384;  // early slots that the selection lists its
 // larger and equal keys of every 256 slots are counted, from which a launch that has all of the chip finds the slots'
 // places.
 //
-// What bounds it is the latency of its steps on the one CU that has the row and head, so the keys are read from
-// memory once and stay in LDS (of more than 32768 early slots, a run at a time in every step).  32768 slots: 20.1 us,
-// of them 4.1 for the keys, 4.0 for the first histogram, 3.3 for the list, 2.8 for the counts; 100000 slots 55.1.  Equal
-// weights are the slowest: all keys fall into one bin, an atomic on one address each, in every histogram (an eviction of
-// 4 x 32768 slots 127 us instead of 54, of 576 slots 13.7 instead of 11.5, of 100000 328 instead of 91).
+// What bounds it is the latency of its steps on the one CU that has the row and head, so the keys are read from memory
+// once and stay in LDS (of more than 32768 early slots, a run at a time in every step).  32768 slots: 20.1 us, of them
+// 4.1 for the keys, 4.0 for the first histogram, 3.3 for the list, 2.8 for the counts; 100000 slots 55.1.  Equal
+// weights are the slowest: all keys fall into one bin, an atomic on one address each, in every histogram (an eviction
+// of 4 x 32768 slots 127 us instead of 54, of 576 slots 13.7 instead of 11.5, of 100000 328 instead of 91).
 //
 // ONCE: no row is longer than LDS holds (a kernel that may have to load again is slower for the others: 32768 slots
 // 21.8 us instead of 20.2, 576 slots 6.2 instead of 5.7).  PLACE: the rows are short enough that the kept slots are
@@ -1213,10 +1214,10 @@ struct PagedAttnPlan {
 // instead of 49).
 //
 // More than sixteen query heads a key-value head of 64 share their slots' loads in tiles of 32, where the parts are
-// long enough for it: 24 / 1 heads, 10 rows of 107000 slots with weights 109 us instead of 170, 6 of up to 117000
-// 26.7 instead of 49.1; 16 of up to 2000 would take 14.2 instead of 11.1.  So they do where the weights then need no
-// second launch (7 of 15 11.8 us instead of 8.4 and 5.8, 300 of 120 17.7 instead of 15.9 and 12.7).  (Heads of 128
-// have no registers for two tiles.)  (Both sides of each with bf16 probabilities in two parts, 1 to 3% faster than three.)
+// long enough for it: 24 / 1 heads, 10 rows of 107000 slots with weights 109 us instead of 170, 6 of up to 117000 26.7
+// instead of 49.1; 16 of up to 2000 would take 14.2 instead of 11.1.  So they do where the weights then need no second
+// launch (7 of 15 11.8 us instead of 8.4 and 5.8, 300 of 120 17.7 instead of 15.9 and 12.7).  (Heads of 128 have no
+// registers for two tiles.)  (Both sides of each with bf16 probabilities in two parts, 1 to 3% faster than three.)
 bool paged_attn_plan(int64_t rows, int64_t num_heads, int64_t kv_heads, int64_t head_dim, int64_t units, bool weights,
                      PagedAttnPlan* p) {
   if (rows < 0 || num_heads < 1 || kv_heads < 1 || num_heads % kv_heads) return false;
