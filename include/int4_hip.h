@@ -383,6 +383,90 @@ int w4_paged_evict(const w4_paged_cache* cache, int dtype, const int32_t* length
                    void* stream);
 
 /*
+ * Key-value cache in pages held in 8 bits, of one layer, for a batch of sequences (rows).
+ *   k, v               [pages, kv_heads, page_size, head_dim] codes, dense, 16-byte
+ *                      aligned: int8 (-127..127) or e4m3 (1.4.3 bits, no infinities)
+ *   k_scale, v_scale   fp32 [pages, kv_heads, page_size / block], dense: a code stands for
+ *                      code * scale of its block of `block` slots; keys are held rotated
+ *   table              int32 [rows, width], dense, as in w4_paged_cache: rows may share
+ *                      pages that none of them writes to; entries that no token of a call
+ *                      sees are not read
+ * head_dim 64 or 128; page_size a power of two from 8 to 1024; block one from 8 to 64, at
+ * most a page; width * page_size below 2^30.
+ * No counterpart in the reference (see w4_paged_cache).
+ */
+#define W4_CODE_INT8 0
+#define W4_CODE_E4M3 1
+typedef struct w4_paged8_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* table;
+  int64_t pages;
+  int64_t kv_heads;
+  int64_t page_size;
+  int64_t head_dim;
+  int64_t block;
+  int64_t rows;
+  int64_t width;
+  int32_t code;
+  int32_t reserved;
+} w4_paged8_cache;
+
+/*
+ * Tokens written into the pages: row b's new tokens are offsets[b]..offsets[b + 1] (int32
+ * [rows + 1], not decreasing) of k, v [tokens, kv_heads * head_dim] (bf16 / fp16, row
+ * strides multiples of 8) and go to slots lengths[b].. .  Key t is rotated at positions[t]
+ * (cos, sin: fp32 [angles, head_dim / 2]) in 64 bits and quantised from there.
+ *
+ * With a the largest magnitude among a block's new keys (or values) and Q the largest code
+ * (127, 448): a block whose first slot is written, or whose scale is 0, gets scale
+ * max(a / Q rounded to fp32, 2^-126), 0 if a is 0; another keeps its scale s if a <= Q s,
+ * else takes the smallest s 2^m that does, its codes rounded to what they are at that
+ * scale.  A code is the nearest to value / scale, the even one of two.  A block that an
+ * infinity or NaN comes into has scale NaN until its first slot is written again.
+ *
+ * lengths[b] < 0, tokens of no row, a row whose slots pass the table, pages outside the
+ * pool: nothing written.  A position outside the angles: a key of NaN.  A block is written
+ * by one row of a call only: rows must not share pages that they write to.
+ */
+int w4_paged8_append(const w4_paged8_cache* cache, int dtype, const void* k, const void* v, int64_t stride_k,
+                     int64_t stride_v, int64_t tokens, const int32_t* lengths, const int32_t* offsets,
+                     const int32_t* positions, const float* cos, const float* sin, int64_t angles, void* stream);
+
+/*
+ * Keys (rotated) and values read back into dense rows k, v [tokens, kv_heads * head_dim]
+ * (bf16, fp16 or fp32): tokens offsets[b]..offsets[b + 1] are row b's slots starts[b].. ,
+ * code * scale in fp32, rounded once.  Tokens of no row, and of rows with starts[b] < 0,
+ * are 0; slots past the table or on a page outside the pool NaN.
+ */
+int w4_paged8_read(const w4_paged8_cache* cache, int dtype, const int32_t* starts, const int32_t* offsets,
+                   int64_t tokens, void* k, void* v, void* stream);
+
+/*
+ * Attention of the new tokens of every row: their keys and values are written as by
+ * w4_paged8_append, then out [tokens, num_heads * head_dim] (dense) =
+ * softmax(rope(q) K / sqrt(head_dim)) V, from the cached codes and scales, rounded once;
+ * fp32 sums, queries and probabilities entering them with 24 bits.  The token of slot i
+ * sees slots 0..i or, with window > 0, those past i - window and the first `sinks`.
+ * longest: the most new tokens of any row, 0 if not known; results do not depend on it.
+ * Out is 0 for idle rows (lengths[b] < 0) and tokens of no row, NaN for rows whose slots
+ * pass the table, tokens that see a page outside the pool or have a position outside the
+ * angles, and tokens that see a block with scale NaN or (e4m3) a token with a code of NaN.
+ * lengths is not changed.  num_heads: at most 256 for each key-value head.  workspace: as
+ * for w4a16_gemm, w4_paged8_attention_workspace_bytes long.  Results are bit-identical run
+ * to run.
+ */
+size_t w4_paged8_attention_workspace_bytes(int64_t rows, int64_t tokens, int64_t num_heads, int64_t kv_heads,
+                                           int64_t head_dim);
+int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, const void* q, const void* k, const void* v,
+                        int64_t stride_q, int64_t stride_k, int64_t stride_v, int64_t num_heads, int64_t tokens,
+                        int64_t longest, int64_t window, int64_t sinks, const int32_t* lengths,
+                        const int32_t* offsets, const int32_t* positions, const float* cos, const float* sin,
+                        int64_t angles, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Of every row of logits [rows, vocab] (bf16 / fp16 / fp32, row stride `stride`):
  * logprob [rows] = log softmax at tokens[row] (NaN for a token outside the
  * vocabulary; tokens and logprob may both be NULL), entropy [rows] of the
@@ -396,6 +480,29 @@ size_t w4_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t to
 int w4_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
                       const int64_t* tokens, int64_t top, float* logprob, float* entropy, float* top_logprob,
                       int64_t* top_token, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Drafted tokens verified against the target's probabilities, with given random numbers.
+ * Row b has n = counts[b] drafts (int32; counts NULL: n = drafts) tokens[b, 0..n) of
+ * tokens int64 [rows, drafts].  target [rows, drafts + 1, vocab] has the target's
+ * probabilities after each of them, draft [rows, drafts, vocab] those each was drawn from
+ * (NULL: drafts without a choice, probability 1), both bf16 / fp16 / fp32, in elements of
+ * strides (row, position) with dense vocab.  Draft i is accepted where the ones before are
+ * and accept[b, i] * draft < target at it (fp32 [rows, drafts], uniform in [0, 1)).
+ * accepted int64 [rows]: how many are, r.  token int64 [rows]: the one after them, the
+ * least whose weights up to it pass sample[b] (fp32 [rows]) times their sum; weights are
+ * the target's at r where r = n, else max(target - draft, 0) there or, where that is 0
+ * throughout, the target's.  Products, differences and sums are taken in 64 bits.  A draft
+ * outside the vocabulary is refused.  Negative weights count as 0; where their sum is 0,
+ * infinite or NaN the token is -1.  counts[b] outside 0..drafts: accepted and token -1.
+ * drafts: at most 64.  workspace: as for w4a16_gemm, w4_verify_drafts_workspace_bytes long.
+ */
+size_t w4_verify_drafts_workspace_bytes(int64_t rows, int64_t vocab);
+int w4_verify_drafts(const void* target, const void* draft, int dtype, int64_t rows, int64_t drafts, int64_t vocab,
+                     int64_t target_stride_row, int64_t target_stride, int64_t draft_stride_row,
+                     int64_t draft_stride, const int64_t* tokens, const int32_t* counts, const float* accept,
+                     const float* sample, int64_t* accepted, int64_t* token, void* workspace,
+                     size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

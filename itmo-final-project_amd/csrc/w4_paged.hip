@@ -6,14 +6,11 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "w4_common.hpp"
+#include "w4_paged.hpp"
 
 namespace w4 {
 
 constexpr int kPagedThreads = 256;
-constexpr int kPagedBufFlags = 0x00020000;  // raw buffer: the range is checked in bytes
-constexpr int kPagedCoherentAux = 16;       // sc1: the cache policy of agent-scope atomic loads and stores
-
 struct PagedView {
   uint16_t* k;     // [pages, nkv, S, D]
   uint16_t* v;
@@ -104,7 +101,6 @@ struct AttnItem {
 // many rows of a bounded length (see paged_attn_plan).  Parts have four units of slots at least.
 constexpr int kAttnWaves = 4, kAttnItems = 256, kAttnOneWaveItems = 1024;
 constexpr int kAttnMinUnits = 4;
-constexpr int kPagedCounters = W4_WORKSPACE_COUNTER_BYTES / 4;
 
 // Which item this is, the same in every wave and launch.  The lengths lie on the GPU, so the split is made here:
 // every row is cut into equal parts of at most `per` units of UP slots, per = all units / ITEMS, so that short
@@ -167,11 +163,6 @@ __device__ __forceinline__ bool find_item(const PagedView& c, const int32_t* __r
   return false;
 }
 
-// How an fp32 operand enters 16-bit matrix instructions: as the sum of its roundings.
-template <int DT> struct Split;
-template <> struct Split<W4_DTYPE_BF16> { static constexpr int N = 3; };  // 8 significant bits each: all 24
-template <> struct Split<W4_DTYPE_FP16> { static constexpr int N = 2; };  // 11 each: 22
-
 // The range of the probabilities: a head's reference is a score, whose own probability is `first` = 2^above, and is
 // raised to the largest one only once that passes it by 2^lag.  bf16 has fp32's exponents.  fp16 ends at 65504, so the
 // largest probability is kept between 2^13 and 2^15: both parts of one 2^25 times smaller are then still numbers, and
@@ -202,23 +193,6 @@ template <> struct QueryScale<W4_DTYPE_FP16> {
   }
   __device__ __forceinline__ float back() const { return b; }
 };
-
-// QUERY: an infinity or NaN has no small parts.  (A probability is no infinity, and beside a NaN all of its head's
-// are.)
-template <int DT, bool QUERY>
-__device__ __forceinline__ void split8(const float v[8], u32x4* out) {
-  float r[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = v[e];
-#pragma unroll
-  for (int p = 0; p < Split<DT>::N; ++p) {
-    out[p] = pack8<DT>(r);
-    float t[8];
-    unpack8<DT>(out[p], t);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = QUERY && !(__builtin_fabsf(t[e]) < __builtin_inff()) ? 0.f : r[e] - t[e];
-  }
-}
 
 // Eight elements with zeros in the place of infinities and NaN.
 template <int DT>
@@ -251,39 +225,7 @@ __device__ __forceinline__ void rope_chunk(const uint16_t* __restrict__ x, const
   }
 }
 
-__device__ __forceinline__ float finite_or_zero(float m) { return m == -__builtin_inff() ? 0.f : m; }
-
-// Softmax sums and a quad of outputs, relative to the score M.  (Scores are subtracted before they become exponents:
-// past 2^24 the exponent's own rounding would be powers of two.)  A refused part's reference is NaN and stays.
-struct Share {
-  float M = -__builtin_inff(), L = 0.f;
-  f32x4 t = {0.f, 0.f, 0.f, 0.f};
-  __device__ __forceinline__ void add(float m, float l, const f32x4& x) {
-    const float mn = M != M || m != m ? __builtin_nanf("") : fmaxf(M, m), mz = finite_or_zero(mn);
-    const float w0 = __builtin_amdgcn_exp2f((M - mz) * kLog2e), w1 = __builtin_amdgcn_exp2f((m - mz) * kLog2e);
-    L = __builtin_fmaf(w1, l, L * w0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(w1, x[e], t[e] * w0);
-    M = mn;
-  }
-  template <int DT> __device__ __forceinline__ u32x2 out() const {
-    const float inv = 1.f / L;
-    u32x2 r;
-    r[0] = (uint32_t)float_to_act_bits<DT>(t[0] * inv) | ((uint32_t)float_to_act_bits<DT>(t[1] * inv) << 16);
-    r[1] = (uint32_t)float_to_act_bits<DT>(t[2] * inv) | ((uint32_t)float_to_act_bits<DT>(t[3] * inv) << 16);
-    return r;
-  }
-};
-
-// Between LDS accesses of one wave whose lanes write what others read: the LDS takes a wave's accesses in their order,
-// and the compiler is to leave them in it.  No instruction.
-__device__ __forceinline__ void wave_lds_order() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
 // The probabilities of slots s.. s + 3 added to their weights (the new token's, slot `len`, set); head(g): the

@@ -1,0 +1,1042 @@
+// Key-value cache in pages held in 8 bits (int4_hip/paged8.py): tokens quantised as
+// they are written, read back, and the attention of a few new tokens of every row over
+// them, of all that came before or of a sliding window and a few first tokens.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "w4_paged.hpp"
+
+namespace w4 {
+
+constexpr int kP8Threads = 256;
+
+struct Paged8View {
+  uint8_t* k;       // [pages, nkv, S, D] codes
+  uint8_t* v;
+  float* k_scale;   // [pages, nkv, S / block]
+  float* v_scale;
+  const int32_t* table;  // [rows, width]
+  int64_t pages;
+  int nkv, log2s, log2b, rows, width;
+
+  __device__ __forceinline__ int64_t capacity() const { return (int64_t)width << log2s; }
+  // The page of a slot; -1 where the table or the pool ends before.
+  __device__ __forceinline__ int page(int row, int slot) const {
+    const int at = slot >> log2s;
+    if ((unsigned)at >= (unsigned)width) return -1;
+    const int p = table[(int64_t)row * width + at];
+    return (uint64_t)(int64_t)p < (uint64_t)pages ? p : -1;
+  }
+  // Index of a slot of a page among the pool's tokens, and of its block among the blocks, for one head.
+  __device__ __forceinline__ int64_t token(int page, int head, int slot) const {
+    return (((int64_t)page * nkv + head) << log2s) + (slot & ((1 << log2s) - 1));
+  }
+  __device__ __forceinline__ int64_t block(int page, int head, int slot) const { return token(page, head, slot) >> log2b; }
+};
+
+// The new tokens of every row: tokens offsets[b]..offsets[b + 1] go to slots lengths[b].. .
+struct RowSpan {
+  int len, o0, n;  // n = 0: nothing to do with this row; len < 0: idle; REFUSED: its slots pass the table
+};
+constexpr int kP8Refused = -2;
+__device__ __forceinline__ RowSpan row_span(const Paged8View& c, const int32_t* __restrict__ lengths,
+                                            const int32_t* __restrict__ offsets, int tokens, int r) {
+  RowSpan s{-1, 0, 0};
+  if (r >= c.rows) return s;
+  s.len = max(lengths[r], -1);
+  s.o0 = min(max(offsets[r], 0), tokens);
+  s.n = min(max(offsets[r + 1], s.o0), tokens) - s.o0;
+  if ((int64_t)s.len + s.n > c.capacity()) s.len = kP8Refused;
+  return s;
+}
+
+// ---------------------------------------------------------------- codes
+template <int CT> struct Code;
+template <> struct Code<W4_CODE_INT8> { static constexpr int most = 127; };
+template <> struct Code<W4_CODE_E4M3> { static constexpr int most = 448; };
+
+constexpr double kSmallestScale = 1.1754943508222875e-38;  // 2^-126: scales are normal numbers, or 0
+
+__device__ __forceinline__ double two_to(int e) { return __builtin_bit_cast(double, (uint64_t)(1023 + e) << 52); }
+__device__ __forceinline__ int exponent_of(double y) {  // of a normal number; -1023 of 0
+  return (int)((__builtin_bit_cast(uint64_t, y) >> 52) & 0x7FF) - 1023;
+}
+
+// The code of x / s, to nearest, ties to even.  `inv` is 1 / s: the quotient is taken as x inv, an error of 2^-52, and
+// divided out only where it lies within that of the middle between two codes (values with few bits, as projections
+// are, do lie there).
+template <int CT>
+__device__ __forceinline__ uint32_t encode(double x, double s, double inv) {
+  const double y = x * inv;
+  double up = 1.0;
+  int e = 0;
+  if constexpr (CT == W4_CODE_E4M3) {  // a code is a multiple of 2^(e - 3), subnormal ones of 2^-9
+    e = min(max(exponent_of(y), -6), 8);
+    up = two_to(3 - e);
+  }
+  double t = y * up, n = __builtin_rint(t);
+  if (__builtin_fabs(__builtin_fabs(t - n) - 0.5) < 1e-9) n = __builtin_rint(x / s * up);
+  const int i = (int)n;
+  if constexpr (CT == W4_CODE_INT8) return (uint32_t)min(max(i, -127), 127) & 0xFFu;
+  // eight steps lead from one exponent to the next, so a step count and the exponent add up to the code
+  const int c = min(((e + 7) << 3) + abs(i) - 8, 0x7E);
+  return (uint32_t)c | (__builtin_bit_cast(uint64_t, x) >> 63 ? 0x80u : 0u);
+}
+
+template <int CT>
+__device__ __forceinline__ double decode(uint32_t c) {
+  if constexpr (CT == W4_CODE_INT8) return (double)(int8_t)c;
+  const int e = (int)(c >> 3 & 15), m = (int)(c & 7);
+  const double y = e ? (double)(8 + m) * two_to(e - 10) : (double)m * two_to(-9);
+  return c & 0x80 ? -y : y;
+}
+
+// Codes of a block whose scale has grown by 2^m.
+template <int CT>
+__device__ __forceinline__ u32x2 shrink8(u32x2 w, int m) {
+  const double f = two_to(-min(m, 200));
+  u32x2 r = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t c = w[e >> 2] >> (8 * (e & 3)) & 0xFFu;
+    const uint32_t n = CT == W4_CODE_E4M3 && (c & 0x7F) == 0x7F ? c : encode<CT>(decode<CT>(c) * f, 1.0, 1.0);
+    r[e >> 2] |= n << (8 * (e & 3));
+  }
+  return r;
+}
+
+// Eight codes as bf16, exactly: int8 has 7 bits and a sign, e4m3 4 bits of bf16's exponents.
+template <int CT>
+__device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
+  u32x4 r;
+  if constexpr (CT == W4_CODE_E4M3) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    auto two = [](bf16x2 v) { return __builtin_bit_cast(uint32_t, v); };
+    r[0] = two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+    r[1] = two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+    r[2] = two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+    r[3] = two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = i < 2 ? lo : hi;
+      const float a = (float)(int8_t)(w >> (16 * (i & 1))), b = (float)(int8_t)(w >> (16 * (i & 1) + 8));
+      // (the upper halves of the fp32 numbers, which need no rounding)
+      r[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+    }
+  }
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+// ---------------------------------------------------------------- append
+struct Append8Args {
+  Paged8View c;
+  const uint16_t* k;  // [T, nkv * D], row strides below
+  const uint16_t* v;
+  int64_t stride_k, stride_v, angles;
+  const int32_t *lengths, *offsets, *positions;
+  const float *cos, *sin;  // [angles, D / 2]
+  int tokens;
+};
+
+// Item -> a row and one of its blocks that get new tokens, counted over all rows.
+__device__ __forceinline__ bool find_block(const Append8Args& a, int item, int* row, int* block, RowSpan* span) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int r = 0; r < a.c.rows; r += 64) {
+    const RowSpan s = row_span(a.c, a.lengths, a.offsets, a.tokens, r + lane);
+    const int first = s.len >> a.c.log2b;
+    const int blocks = s.len >= 0 && s.n > 0 ? ((s.len + s.n - 1) >> a.c.log2b) - first + 1 : 0;
+    const int upto = base + wave_scan(blocks);
+    const int end = __builtin_amdgcn_readlane(upto, 63);
+    if (item < end) {
+      const int i = __popcll(__ballot(item >= upto));
+      *row = r + i;
+      span->len = __builtin_amdgcn_readlane(s.len, i);
+      span->o0 = __builtin_amdgcn_readlane(s.o0, i);
+      span->n = __builtin_amdgcn_readlane(s.n, i);
+      *block = (span->len >> a.c.log2b) + item - (__builtin_amdgcn_readlane(upto, i) - __builtin_amdgcn_readlane(blocks, i));
+      return true;
+    }
+    base = end;
+  }
+  return false;
+}
+
+// One workgroup has one block of one row, for as many heads as its 256 threads hold: block * D / 16 threads a head
+// (twice over where they are 512), eight rotary pairs of a key and the sixteen values beside them each.  The rotation
+// and the quotients are taken in 64 bits, where the products of 16-bit numbers and 24-bit angles are exact, so a code
+// is that of the rotated key and not of its rounding.
+//
+// A block's scale is its largest magnitude over the largest code.  Tokens that come into a block that holds some
+// already let its scale grow by a power of two, if they need it: e4m3 codes then stay as they are (but for the
+// smallest), and int8 codes, each rounding at half the step of the next, are never off by more than one step in all.
+template <int DT, int CT, int D>
+__global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a) {
+  constexpr int CH = D / 16;  // threads per token
+  constexpr int MAXIT = 64 * CH / kP8Threads < 1 ? 1 : 64 * CH / kP8Threads;
+  __shared__ unsigned long long top_s[2][kP8Threads / 32];
+  const int tid = threadIdx.x;
+  int row, jb;
+  RowSpan sp;
+  if (!find_block(a, blockIdx.x, &row, &jb, &sp)) return;
+  const int slot0 = jb << a.c.log2b, per = CH << a.c.log2b;
+  const int its = max(per / kP8Threads, 1), units = max(kP8Threads / per, 1);
+  const int unit = its > 1 ? 0 : tid / per, r0 = tid - unit * per;
+  const bool live = (int)blockIdx.y * units + unit < a.c.nkv;
+  const int h = min((int)blockIdx.y * units + unit, a.c.nkv - 1);
+  const int page = a.c.page(row, slot0);
+  if (page < 0) return;  // (uniform)
+  if (tid < 2 * (kP8Threads / 32)) (&top_s[0][0])[tid] = 0;
+  __syncthreads();
+
+  const int d = (r0 % CH) * 8;
+  u32x4 raw[MAXIT][4];
+  bool isnew[MAXIT];
+  int pos[MAXIT];
+  unsigned long long top[2] = {0, 0};
+  auto values = [&](int it, double k1[8], double k2[8], float v1[8], float v2[8]) __attribute__((always_inline)) {
+    float x1[8], x2[8];
+    unpack8<DT>(raw[it][0], x1);
+    unpack8<DT>(raw[it][1], x2);
+    unpack8<DT>(raw[it][2], v1);
+    unpack8<DT>(raw[it][3], v2);
+    const bool there = (uint64_t)(int64_t)pos[it] < (uint64_t)a.angles;
+    const float *cp = a.cos + (there ? (int64_t)pos[it] * (D / 2) + d : 0);
+    const float *sp = a.sin + (there ? (int64_t)pos[it] * (D / 2) + d : 0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const double c = there ? (double)cp[j] : (double)__builtin_nanf(""), s = (double)sp[j];
+      k1[j] = (double)x1[j] * c - (double)x2[j] * s;
+      k2[j] = (double)x2[j] * c + (double)x1[j] * s;
+    }
+  };
+#pragma unroll
+  for (int it = 0; it < MAXIT; ++it) {
+    isnew[it] = false;
+    if (it >= its || !live) continue;
+    const int at = slot0 + (r0 + it * kP8Threads) / CH - sp.len;
+    isnew[it] = at >= 0 && at < sp.n;
+    if (!isnew[it]) continue;
+    const int64_t t = sp.o0 + at;
+    const uint16_t* kp = a.k + t * a.stride_k + h * D + d;
+    const uint16_t* vp = a.v + t * a.stride_v + h * D + d;
+    raw[it][0] = *reinterpret_cast<const u32x4*>(kp);
+    raw[it][1] = *reinterpret_cast<const u32x4*>(kp + D / 2);
+    raw[it][2] = *reinterpret_cast<const u32x4*>(vp);
+    raw[it][3] = *reinterpret_cast<const u32x4*>(vp + D / 2);
+    pos[it] = a.positions[t];
+  }
+#pragma unroll
+  for (int it = 0; it < MAXIT; ++it) {
+    if (!isnew[it]) continue;
+    double k1[8], k2[8];
+    float v1[8], v2[8];
+    values(it, k1, k2, v1, v2);
+    // (as integers their order is that of the magnitudes, a NaN above an infinity above all numbers)
+    auto most = [&](int i, double x) {
+      const unsigned long long u = __builtin_bit_cast(unsigned long long, __builtin_fabs(x));
+      top[i] = u > top[i] ? u : top[i];
+    };
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most(0, k1[j]), most(0, k2[j]), most(1, (double)v1[j]), most(1, (double)v2[j]);
+  }
+  if (top[0]) atomicMax(&top_s[0][unit], top[0]);
+  if (top[1]) atomicMax(&top_s[1][unit], top[1]);
+  __syncthreads();
+
+  const int64_t blk = a.c.block(page, h, slot0);
+  const bool fresh = slot0 >= sp.len;
+  double scale[2], inv[2];
+  int grow[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const double x = __builtin_bit_cast(double, top_s[i][unit]);
+    const double old = fresh ? 0.0 : (double)(i ? a.c.v_scale : a.c.k_scale)[blk];
+    constexpr double Q = Code<CT>::most;
+    grow[i] = 0;
+    if (!(x < __builtin_inf()) || old != old) {
+      scale[i] = __builtin_nan("");
+    } else if (old > 0.0) {
+      if (x > Q * old) {  // the least power of two that will do
+        const double r = x / (Q * old);
+        const int e = exponent_of(r);
+        grow[i] = r > two_to(e) ? e + 1 : e;
+      }
+      scale[i] = old * two_to(grow[i]);
+    } else {
+      scale[i] = x > 0.0 ? fmax((double)(float)(x / Q), kSmallestScale) : 0.0;
+    }
+    inv[i] = scale[i] > 0.0 ? 1.0 / scale[i] : 0.0;  // (also of NaN: its codes are 0)
+  }
+  __syncthreads();  // all have read the scales that are there
+  if (!live) return;
+  if (r0 == 0) {
+    a.c.k_scale[blk] = (float)scale[0];
+    a.c.v_scale[blk] = (float)scale[1];
+  }
+#pragma unroll
+  for (int it = 0; it < MAXIT; ++it) {
+    if (it >= its) continue;
+    const int slot = slot0 + (r0 + it * kP8Threads) / CH;
+    const int64_t at = a.c.token(page, h, slot) * D + d;
+    if (isnew[it]) {
+      double k1[8], k2[8];
+      float v1[8], v2[8];
+      values(it, k1, k2, v1, v2);
+      u32x2 w[4];
+      auto put = [&](int i, u32x2& o, auto& x) __attribute__((always_inline)) {
+        o = u32x2{0u, 0u};
+        if (inv[i] > 0.0)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j >> 2] |= encode<CT>((double)x[j], scale[i], inv[i]) << (8 * (j & 3));
+      };
+      put(0, w[0], k1), put(0, w[1], k2), put(1, w[2], v1), put(1, w[3], v2);
+      *reinterpret_cast<u32x2*>(a.c.k + at) = w[0];
+      *reinterpret_cast<u32x2*>(a.c.k + at + D / 2) = w[1];
+      *reinterpret_cast<u32x2*>(a.c.v + at) = w[2];
+      *reinterpret_cast<u32x2*>(a.c.v + at + D / 2) = w[3];
+    } else if (slot < sp.len) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (grow[i] > 0) {
+          u32x2* const p = reinterpret_cast<u32x2*>((i ? a.c.v : a.c.k) + at);
+          u32x2* const q = reinterpret_cast<u32x2*>((i ? a.c.v : a.c.k) + at + D / 2);
+          *p = shrink8<CT>(*p, grow[i]);
+          *q = shrink8<CT>(*q, grow[i]);
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- read
+struct Read8Args {
+  Paged8View c;
+  const int32_t *starts, *offsets;
+  void *k, *v;  // [tokens, nkv * D]
+  int tokens;
+};
+
+// Sixteen values of a key and of the value beside it a thread.
+template <int CT, int OUT, int D>
+__global__ __launch_bounds__(kP8Threads) void paged8_read_kernel(Read8Args a) {
+  constexpr int CH = D / 16;
+  const int64_t i = (int64_t)blockIdx.x * kP8Threads + threadIdx.x;
+  const int per = a.c.nkv * CH, lane = threadIdx.x & 63;
+  const int64_t t0 = ((int64_t)blockIdx.x * kP8Threads + (threadIdx.x & ~63)) / per;  // the wave's first token
+  int row = 0;
+  for (int r = 0; r < a.c.rows; r += 64) {
+    const int n = __popcll(__ballot(r + lane < a.c.rows && a.offsets[r + lane + 1] <= t0));
+    row += n;
+    if (n < 64) break;
+  }
+  const int64_t t = i / per;
+  if (t >= a.tokens) return;
+  while (row < a.c.rows && a.offsets[row + 1] <= t) ++row;
+  const int r = (int)(i - t * per), h = r / CH, d = (r % CH) * 16;
+  bool zero = row >= a.c.rows, bad = false;
+  u32x4 kw = {0u, 0u, 0u, 0u}, vw = {0u, 0u, 0u, 0u};
+  float ks = 0.f, vs = 0.f;
+  if (!zero) {
+    const int start = a.starts[row];
+    const int64_t o0 = a.offsets[row], slot = start + t - o0;
+    zero = start < 0 || t < o0;
+    if (!zero) {
+      const int page = slot < a.c.capacity() ? a.c.page(row, (int)slot) : -1;
+      bad = page < 0;
+      if (!bad) {
+        const int64_t at = a.c.token(page, h, (int)slot) * D + d, blk = a.c.block(page, h, (int)slot);
+        kw = *reinterpret_cast<const u32x4*>(a.c.k + at);
+        vw = *reinterpret_cast<const u32x4*>(a.c.v + at);
+        ks = a.c.k_scale[blk];
+        vs = a.c.v_scale[blk];
+      }
+    }
+  }
+  if (bad) ks = vs = __builtin_nanf("");
+  const int64_t out = t * ((int64_t)a.c.nkv * D) + h * D + d;
+  auto put = [&](void* to, const u32x4& w, float s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float x[8];
+      unpack8<W4_DTYPE_BF16>(__builtin_bit_cast(u32x4, codes8<CT>(w[2 * g], w[2 * g + 1])), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = zero ? 0.f : x[e] * s;
+      if constexpr (OUT == W4_DTYPE_FP32) {
+        f32x4* const p = reinterpret_cast<f32x4*>(static_cast<float*>(to) + out + 8 * g);
+        p[0] = f32x4{x[0], x[1], x[2], x[3]};
+        p[1] = f32x4{x[4], x[5], x[6], x[7]};
+      } else {
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(to) + out + 8 * g) = pack8<OUT>(x);
+      }
+    }
+  };
+  put(a.k, kw, ks);
+  put(a.v, vw, vs);
+}
+
+// ---------------------------------------------------------------- attention
+struct Attend8Args {
+  Paged8View c;
+  const uint16_t* q;
+  int64_t stride_q, angles;
+  const int32_t *lengths, *offsets, *positions;
+  const float *cos, *sin;
+  uint16_t* out;  // [tokens, nkv * g * D]
+  float* part;    // [split items, 16, D]: outputs of the parts of tiles whose slots are cut
+  float* stats;   // [split items, 16, 2]: their references and sums
+  unsigned* cnt;  // arrival counters of those tiles
+  float scale;    // 1 / sqrt(D)
+  int tokens, g, window, sinks;  // window: 0 for none
+};
+
+// The work of one workgroup: a tile of sixteen (new token, query head) columns of one row and key-value head, and a
+// part of the slots that they see.
+struct Item8 {
+  int b, h, tile, part, parts;
+  int len, o0, n;
+  int first, counter;  // of a tile in several parts: the index of part 0 among such parts, and of the tile among such tiles
+};
+
+constexpr int kP8Waves = 4, kP8Parts = 256, kP8MinUnits = 4;
+
+// Rows are cut into parts of about (all columns' tiles x units of slots) / 256, so that time follows the slots there
+// are and not the table.  Those that are cut have at most 2 * kP8Parts parts in all: each has more units than `per`,
+// and kP8Parts * per are at least all there are.
+template <int UP>
+__device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8* it, int* total) {
+  const int lane = threadIdx.x & 63;
+  auto tiles_of = [&](const RowSpan& s) { return a.c.nkv * (int)(((int64_t)s.n * a.g + 15) / 16); };
+  // units that one tile of a row reads at most, or nearly so
+  auto units_of = [&](const RowSpan& s) {
+    if (s.len < 0 || s.n == 0) return 1;
+    const int all = (s.len + s.n - 1) / UP + 1;
+    if (!a.window) return all;
+    const int64_t span = (int64_t)a.window + min((16 + a.g - 2) / a.g, s.n - 1);
+    return (int)min((int64_t)all, span / UP + 2 + (a.sinks + UP - 1) / UP);
+  };
+  auto span = [&](int r) { return row_span(a.c, a.lengths, a.offsets, a.tokens, r + lane); };
+  const RowSpan s0 = span(0);
+  float all = (float)tiles_of(s0) * (float)units_of(s0);
+  for (int r = 64; r < a.c.rows; r += 64) {
+    const RowSpan s = span(r);
+    all += (float)tiles_of(s) * (float)units_of(s);
+  }
+  all = wave_sum(all);
+  // (rounded up beyond what the sum's own rounding can have taken)
+  const int per = max((int)fminf(ceilf(all * (1.0001f / kP8Parts)), 1e9f), kP8MinUnits);
+  int base = 0, split = 0, counters = 0;
+  for (int r = 0; r < a.c.rows; r += 64) {
+    const RowSpan s = r ? span(r) : s0;
+    const int tiles = tiles_of(s), parts = (units_of(s) + per - 1) / per;
+    const int upto = base + wave_scan(parts * tiles);
+    const int split_to = split + wave_scan(parts > 1 ? parts * tiles : 0);
+    const int counters_to = counters + wave_scan(parts > 1 ? tiles : 0);
+    const int end = __builtin_amdgcn_readlane(upto, 63);
+    if (item < end) {
+      const int i = __popcll(__ballot(item >= upto));
+      auto at = [&](int v) { return __builtin_amdgcn_readlane(v, i); };
+      it->parts = at(parts);
+      const int rem = item - (at(upto) - it->parts * at(tiles)), tile = rem / it->parts;
+      it->b = r + i;
+      it->part = rem - tile * it->parts;
+      it->first = at(split_to) - (at(tiles) - tile) * it->parts;
+      it->counter = at(counters_to) - (at(tiles) - tile);
+      it->len = at(s.len), it->o0 = at(s.o0), it->n = at(s.n);
+      it->tile = tile / a.c.nkv;
+      it->h = tile - it->tile * a.c.nkv;
+      return true;
+    }
+    base = end;
+    split = __builtin_amdgcn_readlane(split_to, 63);
+    counters = __builtin_amdgcn_readlane(counters_to, 63);
+  }
+  *total = base;
+  return false;
+}
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
+
+// A workgroup's four waves take units of UP = 8192 / D slots in turn (16 KB of codes), each its own.
+//
+// Both products are 16x16x32 bf16 matrix instructions, transposed, with the columns (new tokens x query heads of the
+// group) as their columns: S^T = K Q^T, then O^T = V^T P^T.  Codes are bf16 numbers exactly; the scales stay outside:
+// a slot's score is multiplied by its key's, its probability by its value's.  Queries and probabilities enter as the
+// sum of three bf16 numbers, 24 bits, so the result has about fp32's error before its one rounding.
+//
+// Keys come from memory straight into the first product's operand: its inner index may run over a head in any order,
+// so a lane takes 32 (D = 64: 16) bytes in a row of a slot.  A tile's row r is slot 8 (r / 4) + 4 t + r % 4 of its
+// block of 32 (t: the first or second tile), so the scores that a lane holds of a column are those of eight slots in a
+// row, its part of the second product's operand.  Values go through a wave's own LDS, which transposes them on reading.
+template <int DT, int CT, int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args a) {
+  constexpr int UP = 8192 / D, KB = UP / 32, NJ = D / 32, ND = D / 16, NP = Split<W4_DTYPE_BF16>::N;
+  constexpr int KC = D / 64;               // 16-byte loads of a key a lane
+  constexpr int VR = 1024 / D, VC = D / 16;  // rows of values in a load of the wave, 16-byte chunks of a row
+  constexpr int OROW = D + 4;              // floats of an output row in LDS
+  constexpr int WAVE_B = 16 * OROW * 4 > UP * D ? 16 * OROW * 4 : UP * D;
+  constexpr int kThreads = 64 * W;
+  typedef Mfma<W4_DTYPE_BF16> M;
+  __shared__ __attribute__((aligned(16))) uint8_t v_s[W][WAVE_B];
+  __shared__ float m_s[W][16], l_s[W][16];
+  __shared__ unsigned arrived_s;
+
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, c = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nh = a.c.nkv * a.g;
+  Item8 it;
+  int total;
+  if (!find_item8<UP>(a, blockIdx.x, &it, &total)) {
+    // what is left over of the launch (one workgroup at least): tokens of no row
+    const int before = a.c.rows ? min(max(a.offsets[0], 0), a.tokens) : 0;
+    const int after = a.c.rows ? min(max(a.offsets[a.c.rows], before), a.tokens) : 0;
+    const int pads = before + a.tokens - after;
+    for (int64_t i = (int64_t)(blockIdx.x - total) * kThreads + tid; i < (int64_t)pads * (nh * D / 8);
+         i += (int64_t)(gridDim.x - total) * kThreads) {
+      const int64_t p = i / (nh * D / 8), t = p < before ? p : p - before + after;
+      *reinterpret_cast<u32x4*>(a.out + t * (nh * D) + (i - p * (nh * D / 8)) * 8) = u32x4{0u, 0u, 0u, 0u};
+    }
+    return;
+  }
+  const int b = it.b, h = it.h, len = it.len;
+  const int col0 = it.tile * 16, cols = min(it.n * a.g - col0, 16);
+  // where column `col` of the tile goes
+  auto out_at = [&](int col) {
+    const int j = (col0 + col) / a.g;
+    return a.out + ((int64_t)(it.o0 + j) * nh + h * a.g + (col0 + col - j * a.g)) * D;
+  };
+  if (len < 0) {
+    const uint16_t fill = len == kP8Refused ? float_to_act_bits<DT>(__builtin_nanf("")) : 0;
+    for (int i = tid; i < cols * D; i += kThreads) out_at(i / D)[i % D] = fill;
+    return;
+  }
+  // The slots that the tile's columns see: lo..hi of the first's and the last's tokens, and the sinks before.
+  const int first_slot = len + col0 / a.g, last_slot = len + (col0 + cols - 1) / a.g;
+  const int lo = a.window ? max(first_slot - a.window + 1, 0) : 0;
+  const int u_lo = lo / UP, sink_units = a.window ? min((a.sinks + UP - 1) / UP, u_lo) : 0;
+  const int units = sink_units + last_slot / UP - u_lo + 1;
+  auto base_of = [&](int u) { return (u < sink_units ? u : u_lo + u - sink_units) * UP; };
+  const int u0 = (int)((int64_t)it.part * units / it.parts), u1 = (int)((int64_t)(it.part + 1) * units / it.parts);
+
+  u32x4 kr[KB][2][KC], vr[8];
+  float ks[KB], vs[KB];
+  int ids[KB], next_ids[KB];
+  // Lane: the pages of the groups of eight slots that its rows of keys are in.
+  auto load_ids = [&](int u, int id[KB]) __attribute__((always_inline)) {
+    const int base = base_of(u);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int slot = base + kb * 32 + 8 * (l16 >> 2);
+      id[kb] = slot <= last_slot ? a.c.page(b, slot) : -1;
+    }
+  };
+  auto load = [&](int u) __attribute__((always_inline)) {
+    const int base = base_of(u);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int64_t at = a.c.token(max(ids[kb], 0), h, base + kb * 32 + 8 * (l16 >> 2) + (l16 & 3));
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+          kr[kb][t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.c.k + (at + 4 * t) * D + c * (D / 4) + 16 * i));
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {  // (the lane's scores are of group c)
+      const int id = __shfl(ids[kb], 4 * c);
+      const int64_t blk = a.c.block(max(id, 0), h, base + kb * 32 + 8 * c);
+      const float k0 = a.c.k_scale[blk], v0 = a.c.v_scale[blk];
+      ks[kb] = id < 0 ? __builtin_nanf("") : k0;
+      vs[kb] = id < 0 ? __builtin_nanf("") : v0;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      int page;
+      if constexpr (D == 128) {
+        page = __builtin_amdgcn_readlane(ids[i >> 2], 4 * (i & 3));
+      } else {
+        const int p0 = __builtin_amdgcn_readlane(ids[i >> 1], 8 * (i & 1)),
+                  p1 = __builtin_amdgcn_readlane(ids[i >> 1], 8 * (i & 1) + 4);
+        page = lane < 32 ? p0 : p1;
+      }
+      const int64_t at = a.c.token(max(page, 0), h, base + i * VR + lane / VC);
+      vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.c.v + at * D + (lane % VC) * 16));
+    }
+  };
+  // The 16-byte chunk of a row of values lies where it shares no bank with those that are read beside it.
+  auto swizzle = [&](int row) { return D == 128 ? row & 7 : (row >> 2) & 3; };
+  uint8_t* const vw = v_s[wv];
+
+  int u = u0 + wv;
+  if (u < u1) {  // on their way before the query is at hand
+    load_ids(u, ids);
+    load(u);
+    load_ids(min(u + W, u1 - 1), next_ids);
+  }
+
+  // The query of this lane's column; columns past the last copy it and count for nothing.
+  const int col = min(l16, cols - 1), tok = it.o0 + (col0 + col) / a.g;
+  const int mine = len + (col0 + col) / a.g;  // its slot
+  u32x4 qf[NJ][NP];
+  {
+    const int pos = a.positions[tok];
+    const bool there = (uint64_t)(int64_t)pos < (uint64_t)a.angles;
+    const uint16_t* const qp = a.q + tok * a.stride_q + (h * a.g + (col0 + col) % a.g) * D;
+    const float* const cosr = a.cos + (there ? (int64_t)pos * (D / 2) : 0);
+    const float* const sinr = a.sin + (there ? (int64_t)pos * (D / 2) : 0);
+    const float scale = there ? a.scale : __builtin_nanf("");
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int d = c * (D / 4) + 8 * j, da = d & (D / 2 - 1);
+      float x[8], y[8];
+      unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + d), x);
+      unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + (d ^ (D / 2))), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float r1, r2;
+        if (c < 2) rope_pair(x[e], y[e], cosr[da + e], sinr[da + e], &r1, &r2), x[e] = r1 * scale;
+        else rope_pair(y[e], x[e], cosr[da + e], sinr[da + e], &r1, &r2), x[e] = r2 * scale;
+      }
+      split8<W4_DTYPE_BF16, true>(x, qf[j]);
+    }
+  }
+
+  float m = -__builtin_inff(), l = 0.f;  // the column's reference and this lane's share of its sum
+  f32x4 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (; u < u1; u += W) {
+    const int base = base_of(u);
+    f32x4 s[KB][2];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        bf16x8 kf[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          uint32_t k0 = kr[kb][t][j >> 1][2 * (j & 1)], k1 = kr[kb][t][j >> 1][2 * (j & 1) + 1];
+          // (hidden, or the compiler converts where the words are loaded and holds four times as many registers)
+          asm("" : "+v"(k0), "+v"(k1));
+          kf[j] = codes8<CT>(k0, k1);
+        }
+        s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p)  // the small parts first
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) s[kb][t] = M::m16(kf[j], __builtin_bit_cast(bf16x8, qf[j][p]), s[kb][t]);
+      }
+    // e4m3 has a NaN: what a program that is not this one left in the pages.  A token with one counts as NaN, and only
+    // where it is seen.
+    uint32_t nans[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) nans[kb] = 0;
+    if constexpr (CT == W4_CODE_E4M3) {
+      uint32_t any[8], some = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        any[i] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any[i] |= ((vr[i][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+        some |= any[i];
+      }
+      if (__ballot(some != 0)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint64_t hit = __ballot(any[i] != 0);
+#pragma unroll
+          for (int r = 0; r < VR; ++r)
+            if (hit >> (r * VC) & ((1ull << VC) - 1)) nans[(i * VR) / 32] |= 1u << ((i * VR + r) & 31);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t bad = ((vr[i][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+            vr[i][e] &= ~((bad >> 7) * 0xFFu);
+          }
+        }
+      }
+    }
+    wave_lds_order();  // the unit before has been read
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = i * VR + lane / VC;
+      *reinterpret_cast<u32x4*>(vw + row * D + (((lane % VC) ^ swizzle(row)) << 4)) = vr[i];
+    }
+    wave_lds_order();
+    float sk[KB], sv[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) sk[kb] = ks[kb], sv[kb] = vs[kb];
+    if (u + W < u1) {  // the next unit's loads travel under the rest
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) ids[kb] = next_ids[kb];
+      load(u + W);
+      load_ids(min(u + 2 * W, u1 - 1), next_ids);
+    }
+
+    // A slot that a column does not see has score -inf and, whatever is stored there, no share in the output.
+    const bool whole = base + UP - 1 <= first_slot && (!a.window || base > last_slot - a.window || base + UP <= a.sinks);
+    bool odd = false;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) odd = odd || nans[kb] != 0;
+    float top = -__builtin_inff();
+    auto seen = [&](int slot) {
+      return slot <= mine && (!a.window || slot > mine - a.window || slot < a.sinks);
+    };
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float x = s[kb][e >> 2][e & 3] * sk[kb];
+        if (!whole) x = seen(base + kb * 32 + 8 * c + e) ? x : -__builtin_inff();
+        top = fmaxf(top, x);
+        s[kb][e >> 2][e & 3] = x;
+      }
+    // The reference is raised once a score passes it by 8 powers of two; probabilities stay below 1 all the same.
+    if (__ballot((top - m) * kLog2e > 8.f)) {
+      float mn = fmaxf(top, m);
+      mn = fmaxf(mn, __shfl_xor(mn, 16));
+      mn = fmaxf(mn, __shfl_xor(mn, 32));
+      const float al = __builtin_amdgcn_exp2f((m - finite_or_zero(mn)) * kLog2e);
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] *= al;
+      m = mn;
+    }
+    const float mz = finite_or_zero(m);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3] - mz, kLog2e, -8.f));
+        l += p[e];
+        p[e] *= sv[kb];
+      }
+      if (!whole || odd) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (nans[kb] >> (8 * c + e) & 1) p[e] = __builtin_nanf("");
+          if (!seen(base + kb * 32 + 8 * c + e)) p[e] = 0.f;
+        }
+      }
+      u32x4 pf[NP];
+      split8<W4_DTYPE_BF16, false>(p, pf);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const int row = kb * 32 + 8 * c + (l16 >> 1);
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_i32x2)(vw + row * D + ((d ^ swizzle(row)) << 4) + 8 * (l16 & 1)));
+        const bf16x8 vf = codes8<CT>((uint32_t)w[0], (uint32_t)w[1]);
+#pragma unroll
+        for (int q = NP - 1; q >= 0; --q) o[d] = M::m16(vf, __builtin_bit_cast(bf16x8, pf[q]), o[d]);
+      }
+    }
+  }
+
+  // The waves' outputs meet in LDS.
+  wave_lds_order();
+  float* const ow = reinterpret_cast<float*>(vw);
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+#pragma unroll
+  for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(ow + l16 * OROW + d * 16 + 4 * c) = o[d];
+  if (c == 0) m_s[wv][l16] = m, l_s[wv][l16] = l;
+  __syncthreads();
+  constexpr int STRIDE = 16 * D;
+  const int quads = cols * (D / 4);
+  const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(a.part + (int64_t)it.first * STRIDE), (short)0, it.parts * STRIDE * 4, kPagedBufFlags);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.stats + (int64_t)it.first * 32), (short)0,
+                                                                      it.parts * 128, kPagedBufFlags);
+  for (int i = tid; i < quads; i += kThreads) {
+    const int hd = i / (D / 4), d = i % (D / 4) * 4;
+    Share x;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      x.add(m_s[w][hd], l_s[w][hd],
+            *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v_s[w]) + hd * OROW + d));
+    if (it.parts == 1) {
+      *reinterpret_cast<u32x2*>(out_at(hd) + d) = x.template out<DT>();
+    } else {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x.t), rp,
+                                             (uint32_t)(it.part * STRIDE + i * 4) * 4u, 0, kPagedCoherentAux);
+      if (d == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{x.M, x.L}), rs,
+                                              (uint32_t)(it.part * 16 + hd) * 8u, 0, kPagedCoherentAux);
+    }
+  }
+  if (it.parts == 1) return;
+
+  // The last part of a tile to arrive joins them, in their order.
+  __builtin_amdgcn_s_waitcnt(0);  // the stores have reached the level all XCDs share
+  __syncthreads();
+  unsigned* const cnt = a.cnt + it.counter;
+  if (tid == 0) arrived_s = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived_s != (unsigned)(it.parts - 1)) return;
+  if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int runs = max(1, kThreads / quads), run = min(tid / quads, runs);
+  f32x4* const red = reinterpret_cast<f32x4*>(&v_s[0][0]);
+  f32x2* const red_ml = reinterpret_cast<f32x2*>(red + kThreads);
+  for (int i = tid - run * quads; i < quads; i += kThreads) {
+    const int hd = i / (D / 4);
+    Share x;
+    if (run < runs) {
+      for (int p0 = run; p0 < it.parts; p0 += runs * 8) {
+        f32x4 t[8];
+        f32x2 ml[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int p = min(p0 + k * runs, it.parts - 1);
+          t[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                               rp, (uint32_t)(p * STRIDE + i * 4) * 4u, 0, kPagedCoherentAux));
+          ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, (uint32_t)(p * 16 + hd) * 8u, 0,
+                                                                                 kPagedCoherentAux));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (p0 + k * runs < it.parts) x.add(ml[k][0], ml[k][1], t[k]);
+      }
+    }
+    if (runs > 1) {  // (then this is the only go, of all threads)
+      if (run < runs) red[tid] = x.t, red_ml[tid] = f32x2{x.M, x.L};
+      __syncthreads();
+      if (run == 0)
+        for (int r = 1; r < runs; ++r) x.add(red_ml[r * quads + i][0], red_ml[r * quads + i][1], red[r * quads + i]);
+    }
+    if (run == 0) *reinterpret_cast<u32x2*>(out_at(hd) + i % (D / 4) * 4) = x.template out<DT>();
+  }
+}
+
+}  // namespace w4
+
+// ---------------------------------------------------------------- host side
+using namespace w4host;
+
+namespace {
+
+int check_cache8(const w4_paged8_cache* c, const char* what) {
+  if (!c) return fail(W4_ERR_INVALID, "%s: null cache", what);
+  if (c->code != W4_CODE_INT8 && c->code != W4_CODE_E4M3)
+    return fail(W4_ERR_INVALID, "%s: codes must be int8 or e4m3 (got code %d)", what, c->code);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(W4_ERR_UNSUPPORTED, "%s: heads of %lld (64 or 128)", what, (long long)c->head_dim);
+  if (!is_pow2(c->page_size) || c->page_size < 8 || c->page_size > 1024)
+    return fail(W4_ERR_UNSUPPORTED, "%s: pages of %lld tokens (a power of two from 8 to 1024)", what,
+                (long long)c->page_size);
+  if (!is_pow2(c->block) || c->block < 8 || c->block > 64 || c->block > c->page_size)
+    return fail(W4_ERR_UNSUPPORTED, "%s: blocks of %lld tokens (a power of two from 8 to 64, at most a page)", what,
+                (long long)c->block);
+  if (c->pages < 1 || c->pages >= (1ll << 31) || c->kv_heads < 1 || c->kv_heads > 65535 || c->rows < 0 ||
+      c->rows > 65535 || c->width < 1 || c->width > (1ll << 30) || c->width * c->page_size >= (1ll << 30))
+    return fail(W4_ERR_INVALID, "%s: %lld pages, %lld heads, a table of %lld x %lld pages of %lld", what,
+                (long long)c->pages, (long long)c->kv_heads, (long long)c->rows, (long long)c->width,
+                (long long)c->page_size);
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale || (c->rows && !c->table))
+    return fail(W4_ERR_INVALID, "%s: null pointer", what);
+  if (((uintptr_t)c->k | (uintptr_t)c->v) % 16 || ((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) % 4)
+    return fail(W4_ERR_INVALID, "%s: pages must be 16-byte aligned, scales 4-byte", what);
+  return W4_OK;
+}
+
+w4::Paged8View view_of(const w4_paged8_cache* c) {
+  w4::Paged8View v{};
+  v.k = static_cast<uint8_t*>(c->k);
+  v.v = static_cast<uint8_t*>(c->v);
+  v.k_scale = c->k_scale;
+  v.v_scale = c->v_scale;
+  v.table = c->table;
+  v.pages = c->pages;
+  v.nkv = (int)c->kv_heads;
+  v.log2s = ilog2(c->page_size);
+  v.log2b = ilog2(c->block);
+  v.rows = (int)c->rows;
+  v.width = (int)c->width;
+  return v;
+}
+
+bool rows_ok(const void* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0; }
+
+constexpr int64_t kMostTokens = 1 << 24;
+
+// `f(std::integral_constant)` of a runtime choice.
+template <typename F> int by_code(int code, const F& f) {
+  return code == W4_CODE_INT8 ? f(std::integral_constant<int, W4_CODE_INT8>{})
+                              : f(std::integral_constant<int, W4_CODE_E4M3>{});
+}
+template <typename F> int by_head(int64_t d, const F& f) {
+  return d == 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 128>{});
+}
+template <typename F> int by_dtype(int dtype, const F& f) {
+  return dtype == W4_DTYPE_BF16 ? f(std::integral_constant<int, W4_DTYPE_BF16>{})
+                                : f(std::integral_constant<int, W4_DTYPE_FP16>{});
+}
+
+int check_new(const w4_paged8_cache* c, int dtype, const void* k, const void* v, int64_t stride_k, int64_t stride_v,
+              int64_t tokens, const int32_t* lengths, const int32_t* offsets, const int32_t* positions,
+              const float* cos, const float* sin, int64_t angles, const char* what) {
+  if (const int rc = check_cache8(c, what)) return rc;
+  if (dtype != W4_DTYPE_BF16 && dtype != W4_DTYPE_FP16)
+    return fail(W4_ERR_INVALID, "%s: dtype must be bf16 or fp16 (got code %d)", what, dtype);
+  if (tokens < 0 || angles < 1)
+    return fail(W4_ERR_INVALID, "%s: %lld tokens, %lld angles", what, (long long)tokens, (long long)angles);
+  if (tokens > kMostTokens) return fail(W4_ERR_UNSUPPORTED, "%s: %lld tokens in a call", what, (long long)tokens);
+  if (tokens == 0) return W4_OK;
+  if (!k || !v || !positions || !cos || !sin || (c->rows && (!lengths || !offsets)))
+    return fail(W4_ERR_INVALID, "%s: null pointer", what);
+  if (!rows_ok(k, stride_k) || !rows_ok(v, stride_v) || ((uintptr_t)cos | (uintptr_t)sin) % 16)
+    return fail(W4_ERR_INVALID, "%s: operands must be 16-byte aligned, row strides multiples of 8", what);
+  return W4_OK;
+}
+
+int launch_append8(const w4::Append8Args& a, int dtype, int code, int64_t head_dim, hipStream_t st, const char* what) {
+  // blocks that get tokens: at most as many as tokens, and two a row more than whole ones
+  const int64_t block = 1ll << a.c.log2b;
+  const int64_t items = std::min<int64_t>(a.tokens, a.tokens / block + 2 * (int64_t)a.c.rows);
+  if (items == 0) return W4_OK;
+  const int64_t per = block * (head_dim / 16), units = std::max<int64_t>(w4::kP8Threads / per, 1);
+  const dim3 grid((unsigned)items, (unsigned)((a.c.nkv + units - 1) / units));
+  return by_dtype(dtype, [&](auto dt) {
+    return by_code(code, [&](auto ct) {
+      return by_head(head_dim, [&](auto d) {
+        w4::paged8_append_kernel<dt(), ct(), d()><<<grid, w4::kP8Threads, 0, st>>>(a);
+        return check_launch(what);
+      });
+    });
+  });
+}
+
+struct Attend8Plan {
+  int64_t items;
+  size_t stats, part, bytes;
+};
+
+// `tokens` new tokens of `rows` rows are at most this many tiles of sixteen columns; of those that are cut see
+// find_item8.
+Attend8Plan attend8_plan(int64_t rows, int64_t tokens, int64_t num_heads, int64_t kv_heads, int64_t head_dim) {
+  const int64_t g = num_heads / kv_heads;
+  Attend8Plan p;
+  p.items = kv_heads * ((tokens * g + 15 * std::min(rows, tokens)) / 16) + 2 * w4::kP8Parts + 1;
+  p.stats = W4_WORKSPACE_COUNTER_BYTES;
+  p.part = p.stats + 2 * w4::kP8Parts * 16 * 8;
+  p.bytes = p.part + (size_t)(2 * w4::kP8Parts) * 16 * head_dim * 4;
+  return p;
+}
+
+}  // namespace
+
+extern "C" int w4_paged8_append(const w4_paged8_cache* cache, int dtype, const void* k, const void* v, int64_t stride_k,
+                                int64_t stride_v, int64_t tokens, const int32_t* lengths, const int32_t* offsets,
+                                const int32_t* positions, const float* cos, const float* sin, int64_t angles,
+                                void* stream) {
+  clear_error();
+  if (const int rc = check_new(cache, dtype, k, v, stride_k, stride_v, tokens, lengths, offsets, positions, cos, sin,
+                               angles, "w4_paged8_append"))
+    return rc;
+  if (tokens == 0 || cache->rows == 0) return W4_OK;
+  const w4::Append8Args a{view_of(cache), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_k,
+                          stride_v, angles, lengths, offsets, positions, cos, sin, (int)tokens};
+  return launch_append8(a, dtype, cache->code, cache->head_dim, static_cast<hipStream_t>(stream), "w4_paged8_append");
+}
+
+extern "C" int w4_paged8_read(const w4_paged8_cache* cache, int dtype, const int32_t* starts, const int32_t* offsets,
+                              int64_t tokens, void* k, void* v, void* stream) {
+  clear_error();
+  if (const int rc = check_cache8(cache, "w4_paged8_read")) return rc;
+  if (dtype != W4_DTYPE_BF16 && dtype != W4_DTYPE_FP16 && dtype != W4_DTYPE_FP32)
+    return fail(W4_ERR_INVALID, "w4_paged8_read: dtype must be bf16, fp16 or fp32 (got code %d)", dtype);
+  if (tokens < 0) return fail(W4_ERR_INVALID, "w4_paged8_read: %lld tokens", (long long)tokens);
+  const int64_t per = cache->kv_heads * (cache->head_dim / 16);
+  if (tokens > kMostTokens || tokens * per >= (1ll << 32) - w4::kP8Threads)  // HIP refuses launches of 2^32 threads
+    return fail(W4_ERR_UNSUPPORTED, "w4_paged8_read: %lld tokens in a call", (long long)tokens);
+  if (tokens == 0) return W4_OK;
+  if (!k || !v || (cache->rows && (!starts || !offsets))) return fail(W4_ERR_INVALID, "w4_paged8_read: null pointer");
+  if (((uintptr_t)k | (uintptr_t)v) % 16)
+    return fail(W4_ERR_INVALID, "w4_paged8_read: outputs must be 16-byte aligned");
+  const w4::Read8Args a{view_of(cache), starts, offsets, k, v, (int)tokens};
+  const dim3 grid((unsigned)((tokens * per + w4::kP8Threads - 1) / w4::kP8Threads));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return by_code(cache->code, [&](auto ct) {
+    return by_head(cache->head_dim, [&](auto d) {
+      if (dtype == W4_DTYPE_FP32) w4::paged8_read_kernel<ct(), W4_DTYPE_FP32, d()><<<grid, w4::kP8Threads, 0, st>>>(a);
+      else if (dtype == W4_DTYPE_FP16) w4::paged8_read_kernel<ct(), W4_DTYPE_FP16, d()><<<grid, w4::kP8Threads, 0, st>>>(a);
+      else w4::paged8_read_kernel<ct(), W4_DTYPE_BF16, d()><<<grid, w4::kP8Threads, 0, st>>>(a);
+      return check_launch("w4_paged8_read");
+    });
+  });
+}
+
+extern "C" size_t w4_paged8_attention_workspace_bytes(int64_t rows, int64_t tokens, int64_t num_heads, int64_t kv_heads,
+                                                      int64_t head_dim) {
+  if (rows < 0 || tokens < 1 || tokens > kMostTokens || num_heads < 1 || kv_heads < 1 || num_heads % kv_heads) return 0;
+  return attend8_plan(rows, tokens, num_heads, kv_heads, head_dim).bytes;
+}
+
+extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, const void* q, const void* k, const void* v,
+                                   int64_t stride_q, int64_t stride_k, int64_t stride_v, int64_t num_heads,
+                                   int64_t tokens, int64_t longest, int64_t window, int64_t sinks,
+                                   const int32_t* lengths, const int32_t* offsets, const int32_t* positions,
+                                   const float* cos, const float* sin, int64_t angles, void* out, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (const int rc = check_new(cache, dtype, k, v, stride_k, stride_v, tokens, lengths, offsets, positions, cos, sin,
+                               angles, "w4_paged8_attention"))
+    return rc;
+  if (num_heads < 1 || num_heads % cache->kv_heads || num_heads / cache->kv_heads > 256)
+    return fail(W4_ERR_INVALID, "w4_paged8_attention: %lld query heads on %lld key-value heads", (long long)num_heads,
+                (long long)cache->kv_heads);
+  if (window < 0 || sinks < 0 || longest < 0)
+    return fail(W4_ERR_INVALID, "w4_paged8_attention: a window of %lld, %lld first tokens, at most %lld new ones a row",
+                (long long)window, (long long)sinks, (long long)longest);
+  if (tokens == 0) return W4_OK;
+  if (tokens * num_heads >= (1ll << 27))
+    return fail(W4_ERR_UNSUPPORTED, "w4_paged8_attention: %lld tokens of %lld heads", (long long)tokens,
+                (long long)num_heads);
+  if (!q || !out) return fail(W4_ERR_INVALID, "w4_paged8_attention: null pointer");
+  if (!rows_ok(q, stride_q) || (uintptr_t)out % 16)
+    return fail(W4_ERR_INVALID, "w4_paged8_attention: operands must be 16-byte aligned, row strides multiples of 8");
+  const Attend8Plan p = attend8_plan(cache->rows, tokens, num_heads, cache->kv_heads, cache->head_dim);
+  if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 256)
+    return fail(W4_ERR_WORKSPACE, "w4_paged8_attention: needs a 256-byte aligned workspace of %zu bytes (got %zu)",
+                p.bytes, workspace_bytes);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const w4::Paged8View view = view_of(cache);
+  const w4::Append8Args put{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_k, stride_v,
+                            angles, lengths, offsets, positions, cos, sin, (int)tokens};
+  if (const int rc = launch_append8(put, dtype, cache->code, cache->head_dim, st, "w4_paged8_attention (append)"))
+    return rc;
+  const int64_t most = 1 << 30;  // (of slots, which are fewer)
+  char* const ws = static_cast<char*>(workspace);
+  w4::Attend8Args a{};
+  a.c = view;
+  a.q = static_cast<const uint16_t*>(q);
+  a.stride_q = stride_q;
+  a.angles = angles;
+  a.lengths = lengths;
+  a.offsets = offsets;
+  a.positions = positions;
+  a.cos = cos;
+  a.sin = sin;
+  a.out = static_cast<uint16_t*>(out);
+  a.stats = reinterpret_cast<float*>(ws + p.stats);
+  a.part = reinterpret_cast<float*>(ws + p.part);
+  a.cnt = reinterpret_cast<unsigned*>(ws);
+  a.scale = 1.f / sqrtf((float)cache->head_dim);
+  a.tokens = (int)tokens;
+  a.g = (int)(num_heads / cache->kv_heads);
+  a.window = window >= most ? 0 : (int)window;
+  a.sinks = (int)std::min(sinks, most);
+  const dim3 grid((unsigned)p.items);
+  return by_dtype(dtype, [&](auto dt) {
+    return by_code(cache->code, [&](auto ct) {
+      return by_head(cache->head_dim, [&](auto d) {
+        w4::paged8_attention_kernel<dt(), ct(), d(), w4::kP8Waves><<<grid, 64 * w4::kP8Waves, 0, st>>>(a);
+        return check_launch("w4_paged8_attention");
+      });
+    });
+  });
+}

@@ -1,0 +1,257 @@
+// Verification of drafted tokens against the target's probabilities (int4_hip/scoring.py).
+#include <hip/hip_runtime.h>
+
+#include "w4_common.hpp"
+
+namespace w4 {
+
+constexpr int kVerThreads = 256;
+constexpr int kVerMaxDrafts = 64;
+constexpr int kVerMaxParts = 64;
+constexpr int kVerBufFlags = 0x00020000;  // raw buffer: the range is checked in bytes
+constexpr int kVerCoherentAux = 16;       // sc1: the cache policy of agent-scope atomic loads and stores
+constexpr int64_t kVerMaxVocab = 1 << 22;
+
+struct VerifyArgs {
+  const void* target;
+  const void* draft;  // or null
+  const int64_t* tokens;
+  const int32_t* counts;  // or null
+  const float *accept, *sample;
+  int64_t *accepted, *token;
+  unsigned* cnt;  // one arrival counter a row
+  double* sums;   // [rows, parts, 2]: of the differences' weights and of the target's
+  int64_t target_row, target_pos, draft_row, draft_pos;  // strides in elements
+  int drafts, vocab, parts, run;  // run: tokens of a part
+};
+
+template <int DT>
+__device__ __forceinline__ double prob(const void* p, int64_t i) {
+  if constexpr (DT == W4_DTYPE_FP32) return (double)static_cast<const float*>(p)[i];
+  else return (double)act_bits_to_float(static_cast<const uint16_t*>(p)[i], DT);
+}
+
+__device__ __forceinline__ double lane_get(double v, int lane) { return __shfl(v, lane); }
+
+// Inclusive sum over the lanes, each lane's in their order.
+__device__ __forceinline__ double wave_scan64(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double o = __shfl_up(v, d);
+    v = lane >= d ? v + o : v;
+  }
+  return v;
+}
+
+// A row's parts of the vocabulary are a workgroup's each.  Every one of them decides on the drafts (a handful of
+// numbers) and sums its part's weights at the first position that is refused, or past the last; the last part to
+// arrive finds the part that the sample falls into and looks for it there.  The sums are of 64 bits, so that their
+// order, which is fixed, moves no token but one that the sample meets to 2^-50.
+template <int DT>
+__global__ __launch_bounds__(kVerThreads) void verify_kernel(VerifyArgs a) {
+  __shared__ double sum_s[2][kVerThreads / 64];
+  __shared__ double edge_s[2];
+  __shared__ unsigned arrived_s;
+  __shared__ int found_s;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  const int n = a.counts ? a.counts[row] : a.drafts;
+  if ((unsigned)n > (unsigned)a.drafts) {  // (uniform: a.drafts is not negative)
+    if (part == 0 && tid == 0) a.accepted[row] = a.token[row] = -1;
+    return;
+  }
+  bool good = false;
+  if (lane < n) {
+    const int64_t x = a.tokens[(int64_t)row * a.drafts + lane];
+    if ((uint64_t)x < (uint64_t)a.vocab) {
+      const double p = prob<DT>(a.target, row * a.target_row + lane * a.target_pos + x);
+      const double q = a.draft ? prob<DT>(a.draft, row * a.draft_row + lane * a.draft_pos + x) : 1.0;
+      good = (double)a.accept[(int64_t)row * a.drafts + lane] * q < p;
+    }
+  }
+  const uint64_t refused = ~__ballot(good);
+  const int r = min(refused ? __builtin_ctzll(refused) : 64, n);
+  const int64_t tp = row * a.target_row + r * a.target_pos, dp = row * a.draft_row + r * a.draft_pos;
+  // the token that is no choice: the refused draft, where drafts have probability 1
+  const int64_t out = r < n && !a.draft ? a.tokens[(int64_t)row * a.drafts + r] : -1;
+  const bool minus = r < n && a.draft;
+  // (what is not a number stays one, so that the sum shows it)
+  auto weight = [&](int i, double* p) __attribute__((always_inline)) {
+    const double t = prob<DT>(a.target, tp + i);
+    *p = t < 0.0 ? 0.0 : t;
+    const double d = minus ? t - prob<DT>(a.draft, dp + i) : i == out ? t - 1.0 : t;
+    return d < 0.0 ? 0.0 : d;
+  };
+  const int begin = part * a.run, end = min(begin + a.run, a.vocab);
+  double s0 = 0.0, s1 = 0.0;
+#pragma unroll 4
+  for (int i = begin + tid; i < end; i += kVerThreads) {
+    double p;
+    s0 += weight(i, &p);
+    s1 += p;
+  }
+  s0 = lane_get(wave_scan64(s0), 63);
+  s1 = lane_get(wave_scan64(s1), 63);
+  if (lane == 0) sum_s[0][wv] = s0, sum_s[1][wv] = s1;
+  __syncthreads();
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.sums + (int64_t)row * a.parts * 2), (short)0,
+                                                                      a.parts * 16, kVerBufFlags);
+  if (tid == 0) {
+    double t[2] = {0.0, 0.0};
+#pragma unroll
+    for (int w = 0; w < kVerThreads / 64; ++w) t[0] += sum_s[0][w], t[1] += sum_s[1][w];
+    typedef double f64x2 __attribute__((ext_vector_type(2)));
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f64x2{t[0], t[1]}), rs, part * 16u, 0, kVerCoherentAux);
+    __builtin_amdgcn_s_waitcnt(0);  // at the level all XCDs share
+    arrived_s = __hip_atomic_fetch_add(a.cnt + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (arrived_s != (unsigned)(a.parts - 1)) return;
+  if (tid == 0) __hip_atomic_store(a.cnt + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+
+  // Which weights, their sum, and the part where the sample falls: a lane a part.
+  typedef double f64x2 __attribute__((ext_vector_type(2)));
+  const f64x2 mine = lane < a.parts ? __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(rs, lane * 16u, 0, kVerCoherentAux))
+                                    : f64x2{0.0, 0.0};
+  const double u0 = wave_scan64(mine[0]), u1 = wave_scan64(mine[1]);
+  const bool rest = lane_get(u0, 63) != 0.0;  // (also where it is NaN)
+  const double upto = rest ? u0 : u1, own = rest ? mine[0] : mine[1], all = lane_get(upto, 63);
+  if (!(all > 0.0 && all < __builtin_inf())) {
+    if (tid == 0) a.accepted[row] = r, a.token[row] = -1;
+    return;
+  }
+  const double aim = (double)a.sample[row] * all;
+  // (the last with any weight, should the sample's product round up to the whole sum)
+  const uint64_t past = __ballot(upto > aim && own > 0.0), any = __ballot(own > 0.0);
+  const int p = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
+  const double before = p ? lane_get(upto, p - 1) : 0.0;
+  if (tid == 0) found_s = a.vocab;
+  // That part once more, a run of consecutive tokens a thread: the sums up to each, then the token.
+  const int b = p * a.run, e = min(b + a.run, a.vocab), each = (a.run + kVerThreads - 1) / kVerThreads;
+  const int i0 = min(b + tid * each, e), i1 = min(i0 + each, e);
+  double s = 0.0;
+  for (int i = i0; i < i1; ++i) {
+    double t;
+    const double w = weight(i, &t);
+    s += rest ? w : t;
+  }
+  const double scan = wave_scan64(s);
+  if (lane == 63) sum_s[0][wv] = scan;
+  __syncthreads();
+  double from = before;
+  for (int w = 0; w < wv; ++w) from += sum_s[0][w];
+  const double lanes = __shfl_up(scan, 1);  // (of all lanes: one that does not take part gives nothing)
+  from += lane ? lanes : 0.0;
+  int hit = a.vocab, last = -1;
+  for (int i = i0; i < i1; ++i) {
+    double t;
+    const double w = weight(i, &t), x = rest ? w : t;
+    from += x;
+    if (x > 0.0) last = i;
+    if (x > 0.0 && from > aim && hit == a.vocab) hit = i;
+  }
+  if (hit < a.vocab) atomicMin(&found_s, hit);
+  __syncthreads();
+  const int f = found_s;
+  __syncthreads();
+  if (f == a.vocab) {  // rounding: the last token of the part that has any weight
+    if (tid == 0) found_s = -1;
+    __syncthreads();
+    atomicMax(&found_s, last);
+    __syncthreads();
+  }
+  if (tid == 0) a.accepted[row] = r, a.token[row] = found_s;
+}
+
+}  // namespace w4
+
+// ---------------------------------------------------------------- host side
+using namespace w4host;
+
+namespace {
+
+struct VerifyPlan {
+  int parts, run;
+  int64_t slice;  // rows of a launch
+};
+
+// About four workgroups a CU, of 2048 tokens at least.
+VerifyPlan verify_plan(int64_t rows, int64_t vocab) {
+  VerifyPlan p;
+  p.slice = W4_WORKSPACE_COUNTER_BYTES / 4;
+  if (p.slice > rows) p.slice = rows;
+  int64_t parts = (4 * device_cu_count() + p.slice - 1) / p.slice;
+  const int64_t most = (vocab + 2047) / 2048;
+  if (parts > most) parts = most;
+  if (parts > w4::kVerMaxParts) parts = w4::kVerMaxParts;
+  p.run = (int)((vocab + parts - 1) / parts);
+  p.parts = (int)((vocab + p.run - 1) / p.run);
+  return p;
+}
+
+}  // namespace
+
+extern "C" size_t w4_verify_drafts_workspace_bytes(int64_t rows, int64_t vocab) {
+  if (rows < 1 || vocab < 1 || vocab > w4::kVerMaxVocab) return 0;
+  const VerifyPlan p = verify_plan(rows, vocab);
+  return W4_WORKSPACE_COUNTER_BYTES + (size_t)(p.slice * p.parts) * 16;
+}
+
+extern "C" int w4_verify_drafts(const void* target, const void* draft, int dtype, int64_t rows, int64_t drafts,
+                                int64_t vocab, int64_t target_stride_row, int64_t target_stride,
+                                int64_t draft_stride_row, int64_t draft_stride, const int64_t* tokens,
+                                const int32_t* counts, const float* accept, const float* sample, int64_t* accepted,
+                                int64_t* token, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (dtype != W4_DTYPE_BF16 && dtype != W4_DTYPE_FP16 && dtype != W4_DTYPE_FP32)
+    return fail(W4_ERR_INVALID, "w4_verify_drafts: dtype must be bf16, fp16 or fp32 (got code %d)", dtype);
+  if (rows < 0 || drafts < 0 || vocab < 1 || target_stride_row < 0 || target_stride < 0 || draft_stride_row < 0 ||
+      draft_stride < 0)
+    return fail(W4_ERR_INVALID, "w4_verify_drafts: %lld rows of %lld drafts over %lld tokens", (long long)rows,
+                (long long)drafts, (long long)vocab);
+  if (rows >= (1ll << 24) || drafts > w4::kVerMaxDrafts || vocab > w4::kVerMaxVocab)
+    return fail(W4_ERR_UNSUPPORTED, "w4_verify_drafts: %lld rows of %lld drafts (at most %d) over %lld tokens",
+                (long long)rows, (long long)drafts, w4::kVerMaxDrafts, (long long)vocab);
+  if (rows == 0) return W4_OK;
+  if (!target || !sample || !accepted || !token || (drafts && (!tokens || !accept)))
+    return fail(W4_ERR_INVALID, "w4_verify_drafts: null pointer");
+  const uintptr_t align = dtype == W4_DTYPE_FP32 ? 4 : 2;
+  if ((uintptr_t)target % align || (uintptr_t)draft % align)
+    return fail(W4_ERR_INVALID, "w4_verify_drafts: probabilities must be aligned to their size");
+  const size_t need = w4_verify_drafts_workspace_bytes(rows, vocab);
+  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)
+    return fail(W4_ERR_WORKSPACE, "w4_verify_drafts: needs a 256-byte aligned workspace of %zu bytes (got %zu)", need,
+                workspace_bytes);
+  const VerifyPlan p = verify_plan(rows, vocab);
+  const int64_t bytes = (int64_t)align;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  for (int64_t r = 0; r < rows; r += p.slice) {
+    const int64_t n = rows - r < p.slice ? rows - r : p.slice;
+    w4::VerifyArgs a{};
+    a.target = static_cast<const char*>(target) + r * target_stride_row * bytes;
+    a.draft = draft ? static_cast<const char*>(draft) + r * draft_stride_row * bytes : nullptr;
+    a.tokens = tokens ? tokens + r * drafts : nullptr;
+    a.counts = counts ? counts + r : nullptr;
+    a.accept = accept ? accept + r * drafts : nullptr;
+    a.sample = sample + r;
+    a.accepted = accepted + r;
+    a.token = token + r;
+    a.cnt = static_cast<unsigned*>(workspace);
+    a.sums = reinterpret_cast<double*>(static_cast<char*>(workspace) + W4_WORKSPACE_COUNTER_BYTES);
+    a.target_row = target_stride_row;
+    a.target_pos = target_stride;
+    a.draft_row = draft_stride_row;
+    a.draft_pos = draft_stride;
+    a.drafts = (int)drafts;
+    a.vocab = (int)vocab;
+    a.parts = p.parts;
+    a.run = p.run;
+    const dim3 grid((unsigned)(n * p.parts));
+    if (dtype == W4_DTYPE_BF16) w4::verify_kernel<W4_DTYPE_BF16><<<grid, w4::kVerThreads, 0, st>>>(a);
+    else if (dtype == W4_DTYPE_FP16) w4::verify_kernel<W4_DTYPE_FP16><<<grid, w4::kVerThreads, 0, st>>>(a);
+    else w4::verify_kernel<W4_DTYPE_FP32><<<grid, w4::kVerThreads, 0, st>>>(a);
+    if (const int rc = check_launch("w4_verify_drafts")) return rc;
+  }
+  return W4_OK;
+}

@@ -11,8 +11,9 @@ from .quantize import (dequantize_int4, dequantize_int4_ref, quantize_int4, quan
                        quantize_int4_ref, unpack_int4_ref)
 from .gemm import w4a16_matmul, w4a16_matmul_grouped, w16a16_matmul
 from .paged import paged_append, paged_attention, paged_evict
+from .paged8 import paged_append8, paged_attention8, paged_read8
 from .qlinear import Int4Linear, quantize_model_linears
-from .scoring import TokenLogprobs, token_logprobs
+from .scoring import TokenLogprobs, Verified, token_logprobs, verify_drafts
 
 __all__ = [
     "quantize_int4",
@@ -33,4 +34,9 @@ __all__ = [
     "paged_evict",
     "token_logprobs",
     "TokenLogprobs",
+    "paged_append8",
+    "paged_read8",
+    "paged_attention8",
+    "verify_drafts",
+    "Verified",
 ]

@@ -17,6 +17,8 @@ ABI_VERSION = 1
 DTYPE_BF16 = 0
 DTYPE_FP16 = 1
 DTYPE_FP32 = 2
+CODE_INT8 = 0
+CODE_E4M3 = 1
 
 OK = 0
 ERR_INVALID = 1
@@ -83,6 +85,27 @@ class PagedCache(ctypes.Structure):
     ]
 
 
+class Paged8Cache(ctypes.Structure):
+    """Mirror of ``w4_paged8_cache`` (include/int4_hip.h)."""
+
+    _fields_ = [
+        ("k", _c_vp),
+        ("v", _c_vp),
+        ("k_scale", _c_vp),
+        ("v_scale", _c_vp),
+        ("table", _c_vp),
+        ("pages", _c_i64),
+        ("kv_heads", _c_i64),
+        ("page_size", _c_i64),
+        ("head_dim", _c_i64),
+        ("block", _c_i64),
+        ("rows", _c_i64),
+        ("width", _c_i64),
+        ("code", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # symbol -> (restype, argtypes); exactly the functions include/int4_hip.h declares
 SIGNATURES = {
     "w4_abi_version": (_c_int, []),
@@ -119,6 +142,16 @@ SIGNATURES = {
     "w4_token_logprobs_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64]),
     "w4_token_logprobs": (_c_int, [_c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp,
                                    _c_vp, _c_sz, _c_vp]),
+    "w4_paged8_append": (_c_int, [ctypes.POINTER(Paged8Cache), _c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp,
+                                  _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
+    "w4_paged8_read": (_c_int, [ctypes.POINTER(Paged8Cache), _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp]),
+    "w4_paged8_attention_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "w4_paged8_attention": (_c_int, [ctypes.POINTER(Paged8Cache), _c_int, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,
+                                     _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64,
+                                     _c_vp, _c_vp, _c_sz, _c_vp]),
+    "w4_verify_drafts_workspace_bytes": (_c_sz, [_c_i64, _c_i64]),
+    "w4_verify_drafts": (_c_int, [_c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp,
+                                  _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_sz, _c_vp]),
 }
 
 _lock = threading.Lock()

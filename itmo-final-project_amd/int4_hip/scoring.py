@@ -1,5 +1,6 @@
 """Log probabilities of given tokens, the entropy of their distributions and the most
-likely alternatives, in one pass over the logits (csrc/w4_logprobs.hip)."""
+likely alternatives, in one pass over the logits (csrc/w4_logprobs.hip); verification of
+drafted tokens against the target's probabilities (csrc/w4_verify.hip)."""
 from __future__ import annotations
 
 from typing import NamedTuple
@@ -61,3 +62,66 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
     if rc:
         _lib.check(rc, "w4_token_logprobs")
     return TokenLogprobs(logprob, entropy, top_logprob, top_token)
+
+
+class Verified(NamedTuple):
+    accepted: torch.Tensor  # int64 [rows]: how many of a row's drafts are accepted
+    token: torch.Tensor     # int64 [rows]: the token after them
+
+
+MAX_DRAFTS = 64
+
+
+def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, accept: torch.Tensor,
+                  sample: torch.Tensor, counts: torch.Tensor | None = None) -> Verified:
+    """Speculative sampling: which of the drafted ``tokens`` int64 [rows, drafts] (at most 64)
+    stay, and the token that follows, distributed as the target's own samples are.
+
+    ``target`` [rows, drafts + 1, vocab] has the target's probabilities before, between and
+    after the drafts, ``draft`` [rows, drafts, vocab] those that they were drawn from (None:
+    they were no matter of chance, as the greedy choice of a smaller model); both bf16, fp16
+    or fp32.  Draft i stays where the ones before do and ``accept[b, i]`` * draft < target
+    at it.  The next token is drawn with ``sample[b]`` from max(target - draft, 0) at the
+    first that does not stay (from the target where that is 0 throughout, and after the last
+    draft): the least token whose weights up to it pass ``sample[b]`` times their sum.
+    ``accept`` fp32 [rows, drafts] and ``sample`` fp32 [rows] are uniform in [0, 1); with
+    ``counts`` int32 [rows] a row has so many drafts only (outside 0..drafts: none of its
+    results is a number of tokens, both are -1).
+
+    A draft outside the vocabulary does not stay.  Negative weights count as 0; weights whose
+    sum is 0, infinite or NaN have no token: -1.  Products, differences and sums are taken in
+    64 bits.  Launches on the current stream; no part in autograd.
+    """
+    assert target.dtype in DTYPES and target.dim() == 3 and target.is_cuda, (target.dtype, target.shape)
+    assert underived(target, draft, accept, sample), \
+        "verify_drafts has no derivatives: call it under torch.no_grad(), on probabilities without tangents"
+    B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    dev = target.device
+    assert 0 <= K <= MAX_DRAFTS and V >= 1, target.shape
+    assert tokens.dtype == torch.int64 and tokens.shape == (B, K) and tokens.device == dev, (tokens.dtype, tokens.shape)
+    assert accept.dtype == sample.dtype == torch.float32 and accept.shape == (B, K) and sample.shape == (B,)
+    assert accept.device == sample.device == dev
+    target, tokens, accept, sample = (t.resolve_neg() for t in (target, tokens, accept, sample))
+    tokens, accept, sample = tokens.contiguous(), accept.contiguous(), sample.contiguous()
+    if target.stride(2) != 1 and V > 1:
+        target = target.contiguous()
+    if draft is not None:
+        assert draft.dtype == target.dtype and draft.shape == (B, K, V) and draft.device == dev, (draft.dtype, draft.shape)
+        draft = draft.resolve_neg()
+        if draft.stride(2) != 1 and V > 1:
+            draft = draft.contiguous()
+    if counts is not None:
+        assert counts.dtype == torch.int32 and counts.shape == (B,) and counts.device == dev, counts.shape
+        counts = counts.resolve_neg().contiguous()
+    accepted, token = (torch.empty(B, dtype=torch.int64, device=dev) for _ in range(2))
+    lib = _lib.load()
+    nbytes = lib.w4_verify_drafts_workspace_bytes(B, V)
+    at = None if draft is None or K == 0 else draft.data_ptr()
+    rc = _on(dev, lambda st: _with_workspace(dev, st, nbytes, lambda ws, nb: lib.w4_verify_drafts(
+        target.data_ptr(), at, DTYPES[target.dtype], B, K, V, target.stride(0), target.stride(1),
+        0 if at is None else draft.stride(0), 0 if at is None else draft.stride(1), tokens.data_ptr(),
+        None if counts is None else counts.data_ptr(), accept.data_ptr(), sample.data_ptr(), accepted.data_ptr(),
+        token.data_ptr(), ws, nb, st)))
+    if rc:
+        _lib.check(rc, "w4_verify_drafts")
+    return Verified(accepted, token)

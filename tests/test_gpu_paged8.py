@@ -1,0 +1,478 @@
+"""GPU: the operators of the 8-bit paged cache (int4_hip/paged8.py) against a 64-bit
+statement of them on the CPU."""
+import pytest
+import torch
+
+import _paged8_ref as R
+import int4_hip
+from _paged8_ref import CODES, MOST, NAN
+from _synth import randn
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BOTH = [torch.bfloat16, torch.float16]
+CACHE = ("k_pages", "v_pages", "k_scale", "v_scale")
+IDS = {torch.int8: "int8", torch.float8_e4m3fn: "e4m3", torch.bfloat16: "bf16", torch.float16: "fp16"}
+
+
+def ids(x):
+    return IDS.get(x, str(x))
+
+
+def _to(c):
+    return {k: t.to(DEV) if isinstance(t, torch.Tensor) else t for k, t in c.items()}
+
+
+def _call(f, c, *names):
+    return f(*(c[n] for n in names))
+
+
+def _append(c):
+    int4_hip.paged_append8(*(c[n] for n in ("k", "v", "cos", "sin") + CACHE +
+                             ("table", "lengths", "offsets", "positions")))
+
+
+def _same_cache(got, want):
+    """Equal codes (zeros of either sign) and scales, NaN for NaN."""
+    for n in CACHE:
+        a, b = got[n].cpu().float(), want[n].float()
+        assert torch.equal(a.isnan(), b.isnan()), n
+        bad = torch.nan_to_num(a) != torch.nan_to_num(b)
+        assert not bad.any(), (n, bad.nonzero()[:4], a[bad][:4], b[bad][:4])
+
+
+def _check(got, want, mass, reach, dtype, slots, d):
+    """One rounding to the dtype, eps / 2 = half a step; and the fp32 sums before it.
+
+    A score is a sum of d products of rotated queries (two products and their sum each:
+    3 roundings), in 3 d / 32 matrix instructions that round some 32 partial sums each: at most
+    (3 + 3 d) 2^-24 reach, times the scale and 1 / sqrt(d): 2 more.  An exponential: 2^-22 and
+    what its argument's rounding makes, 2^-24 of it, 2 reach at most.  Probabilities times
+    scales enter with 24 bits: 3 roundings; sums over the slots: one a unit of 32 and part.
+    All of it twice, in the sum and in the denominator.
+    """
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()), (got.isnan() != want.isnan()).nonzero()[:5]
+    score = (5 + 3 * d + 2) * 2.0 ** -24 * reach
+    prob = 2 * (score + 2.0 ** -22 + (16 + 3 * slots / 32) * 2.0 ** -24)
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + prob * mass + torch.finfo(dtype).tiny
+    # the nearest number of a dtype to what lies half a step past its largest is infinity
+    past = got.isinf()
+    edge = torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps / 4)
+    assert (torch.sign(got[past]) * want[past] + tol[past] >= edge).all()
+    over = ((got - want).abs() - tol)[~want.isnan() & ~past]
+    assert not over.numel() or over.max().item() <= 0, over.max().item()
+
+
+def _run(c, dtype, **more):
+    """One call on the GPU against the reference; its tensors, updated by both."""
+    g = _to(c)
+    out = int4_hip.paged_attention8(**g, **more)
+    want, mass, reach = R.attention(**c)
+    _same_cache(g, c)
+    assert out.dtype == dtype and out.shape == want.shape
+    _check(out, want, mass, reach, dtype, c["table"].shape[1] * c["k_pages"].shape[2], c["k_pages"].shape[3])
+    return g, out
+
+
+# ---------------------------------------------------------------- append and read
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("dtype", BOTH, ids=ids)
+@pytest.mark.parametrize("nkv,d,S,block", [(2, 64, 16, 8), (3, 128, 64, 64), (1, 64, 64, 32), (5, 128, 32, 16),
+                                           (2, 64, 128, 64), (9, 128, 8, 8)])
+def test_append_is_the_definition(kind, dtype, nkv, d, S, block):
+    """Prompts that begin anywhere, blocks that are full, begun and continued; every code and scale equal."""
+    lens, new = [0, 5, block - 1, block, 2 * block + 3, 0, 7, -1], [1, 2 * block, 1, block + 2, 3, 0, 1, 4]
+    c = R.case(lens, new, nkv, nkv, d, S, block, kind, dtype, seed=nkv)
+    g = _to(c)
+    _append(g)
+    R.append(**c)
+    _same_cache(g, c)
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+def test_append_token_by_token_grows_the_scales(kind):
+    """Values that grow, shrink, vanish and jump: scales double, codes are rounded again, each step as defined."""
+    sizes = [0.0, 1e-3, 1.0, 0.5, 3.0, 2.9, 200.0, 1e-30, 201.0, 6e4, 1e30, 0.0]
+    c = R.case([3], [1], 2, 2, 64, 32, 16, kind, torch.bfloat16, seed=4, width=2, angles=64)
+    c["table"] = torch.tensor([[2, 0]], dtype=torch.int32)
+    g = _to(c)
+    for i, size in enumerate(sizes):
+        for n in ("k", "v"):
+            x = (randn((1, 2 * 64), seed=50 + i) * size).bfloat16()
+            c[n], g[n] = x, x.to(DEV)
+        c["lengths"] = torch.tensor([3 + i], dtype=torch.int32)
+        g["lengths"] = c["lengths"].to(DEV)
+        _append(g)
+        R.append(**c)
+        _same_cache(g, c)
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+def test_append_of_values_between_two_codes(kind):
+    """Values whose quotient by the scale is the middle between two codes exactly: to the even one."""
+    most, nkv, d = MOST[kind], 1, 64
+    scale = 3.0 * 2.0 ** -4
+    steps = [n + 0.5 for n in range(-12, 12)] if kind == torch.int8 else [x * 17 / 16 for x in (1, 2, 4, 8)] + [
+        19 / 16, -21 / 16, 2.0 ** -10, -3 * 2.0 ** -10, 5 * 2.0 ** -10]
+    v = torch.zeros(1, d)
+    v[0, :len(steps)] = torch.tensor(steps) * scale
+    v[0, -1] = most * scale  # 381 or 1344 sixteenths: numbers of fp16
+    c = R.case([0], [1], 1, nkv, d, 16, 16, kind, torch.float16, shift=0)
+    c["v"], c["k"] = v.half(), v.half()  # (position 0 rotates by nothing)
+    assert torch.equal(c["v"].double(), v.double())
+    g = _to(c)
+    _append(g)
+    R.append(**c)
+    assert float(c["v_scale"][int(c["table"][0, 0]), 0, 0]) == scale
+    _same_cache(g, c)
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("dtype", BOTH, ids=ids)
+def test_append_of_numbers_that_are_none_and_of_none(kind, dtype):
+    """Infinities, NaN, zeros and the smallest numbers; a block of NaN until it begins again."""
+    c = R.case([0, 4, 16, 2, 8], [3, 2, 1, 1, 8], 2, 2, 64, 16, 8, kind, dtype, seed=2)
+    c["k"][0, 3] = float("inf")
+    c["v"][1, 70] = NAN
+    c["k"][3], c["v"][3], c["v"][4] = 0, 0, 0
+    c["v"][5] = -0.0
+    c["k"][5] = torch.finfo(dtype).smallest_normal * 2.0 ** -7 * torch.sign(randn((128,), seed=9)).to(dtype)
+    c["v"][6, :64] = torch.finfo(dtype).max
+    c["k"][6, 64:] = torch.finfo(dtype).max
+    c["k_scale"][int(c["table"][3, 0]), 1, 0] = NAN
+    g = _to(c)
+    for _ in range(2):  # written again over itself: nothing changes
+        _append(g)
+        R.append(**c)
+        _same_cache(g, c)
+    c["lengths"][0] = g["lengths"][0] = 0
+    for n in ("k", "v"):
+        c[n] = randn(tuple(c[n].shape), seed=77).to(dtype)
+        g[n] = c[n].to(DEV)
+    _append(g)
+    R.append(**c)
+    _same_cache(g, c)
+    assert not c["k_scale"][int(c["table"][0, 0])].isnan()[:, 0].any()
+
+
+def test_append_leaves_out_what_has_no_place():
+    """Rows that pass their table, pages outside the pool, tokens of no row, positions without angles, idle rows."""
+    c = R.case([5, 29, 8, 3, -1, -7], [4, 3, 9, 1, 2, 1], 2, 2, 64, 16, 8, torch.int8, torch.float16, seed=3, width=2)
+    c["lengths"][1] = 30
+    c["table"][2, 0] = c["k_pages"].shape[0]
+    c["table"][0, 0] = -1
+    c["positions"][16] = len(c["cos"])  # row 3's: a key of NaN
+    for n in ("q", "k", "v"):
+        c[n] = torch.cat((c[n], c[n][:3]))
+    c["positions"] = torch.cat((c["positions"], c["positions"][:3]))
+    g = _to(c)
+    _append(g)
+    R.append(**c)
+    _same_cache(g, c)
+    assert c["k_scale"].isnan().sum() == 2
+    out = int4_hip.paged_attention8(**g)
+    want, mass, reach = R.attention(**c)
+    _check(out, want, mass, reach, torch.float16, 32, 64)
+    assert (out[-3:] == 0).all() and (out[17:20] == 0).all() and out[4:7].isnan().all() and out[16].isnan().all()
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("out", BOTH + [torch.float32], ids=ids)
+@pytest.mark.parametrize("nkv,d,S,block", [(2, 64, 16, 8), (3, 128, 64, 16), (7, 64, 8, 8)])
+def test_read_is_code_times_scale(kind, out, nkv, d, S, block):
+    c = R.case([40, 0, 17, 3, 8, 5], [0] * 6, nkv, nkv, d, S, block, kind, torch.bfloat16, seed=6, width=40 // S + 2)
+    c["table"][3, 0] = -1
+    c["table"][4, 0] = c["k_pages"].shape[0] + 5
+    c["k_scale"][int(c["table"][2, 0]), 0, 0] = NAN
+    starts = torch.tensor([7, 0, 3, 0, 2, -1], dtype=torch.int32)
+    offsets = torch.tensor([2, 35, 35, 49, 52, 58, 60], dtype=torch.int32)
+    c["lengths"] = starts
+    g = _to(c)
+    got = int4_hip.paged_read8(*(g[n] for n in CACHE), g["table"], g["lengths"], offsets.to(DEV), 63, out)
+    want = R.read(*(c[n] for n in CACHE), c["table"], starts, offsets, 63, out)
+    for a, b in zip(got, want):
+        assert a.dtype == out and torch.equal(torch.nan_to_num(a.cpu().float(), nan=7e7), torch.nan_to_num(b.float(), nan=7e7))
+    # past the table
+    starts[2] = (c["table"].shape[1] - 1) * S + 1
+    got = int4_hip.paged_read8(*(g[n] for n in CACHE), g["table"], starts.to(DEV), offsets.to(DEV), 63, out)
+    want = R.read(*(c[n] for n in CACHE), c["table"], starts, offsets, 63, out)
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu().isnan(), b.isnan())
+    assert got[0][35 + S:49].isnan().all()
+
+
+def test_read_after_append_is_near_what_was_written():
+    """Within half a step of the block's scale: a hundred and twenty-seventh of its largest, or a sixteenth of itself."""
+    for kind in CODES:
+        c = _to(R.case([0, 9], [70, 21], 2, 2, 128, 32, 32, kind, torch.bfloat16, seed=8, shift=0))
+        _append(c)
+        k, v = int4_hip.paged_read8(*(c[n] for n in CACHE), c["table"], c["lengths"], c["offsets"], 91, torch.float32)
+        x = c["v"].float()
+        err = (v - x).abs()
+        if kind == torch.int8:
+            assert err.max() <= 0.5001 * x.abs().max() / 127 * 2  # (a block's scale that was there may be larger)
+        else:
+            assert (err <= x.abs() * 2.0 ** -4 + 2.0 ** -10 * x.abs().max() / 448 * 2).all()
+
+
+# ---------------------------------------------------------------- attention
+CASES = [
+    # (lengths, new tokens, heads, kv heads, head_dim, page size, block)
+    ([0], [1], 1, 1, 64, 16, 8),
+    ([1, 0, 63], [1, 1, 1], 4, 2, 64, 8, 8),
+    ([127, 128, 129, 16], [1, 1, 1, 1], 8, 2, 64, 64, 16),
+    ([63, 64, 65, 200], [1, 1, 1, 1], 8, 2, 128, 64, 64),
+    ([5, 100, -1, 31], [1, 1, 1, 1], 6, 1, 128, 16, 16),
+    ([300, 5], [1, 1], 24, 1, 64, 32, 32),
+    ([30, 0, 77, 250], [5, 3, 1, 2], 8, 2, 128, 32, 8),
+    ([0, 9, 60], [70, 33, 0], 4, 2, 64, 16, 8),
+    ([0], [130], 6, 2, 128, 128, 64),
+    ([2, -1, 0, 40], [17, 3, 1, 16], 16, 16, 64, 64, 32),
+    ([10, 20], [9, 7], 33, 1, 64, 16, 16),
+]
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("dtype", BOTH, ids=ids)
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_attention(i, kind, dtype):
+    lens, new, nh, nkv, d, S, block = CASES[i]
+    _run(R.case(lens, new, nh, nkv, d, S, block, kind, dtype, seed=i), dtype)
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (8, 0), (63, 4), (64, 64), (65, 200), (500, 3), (1 << 40, 9)])
+@pytest.mark.parametrize("d,S", [(64, 16), (128, 64)])
+def test_window_and_sinks(window, sinks, d, S, kind):
+    """Windows of one token, as long as a unit, longer than the rows; first tokens inside and outside of them."""
+    c = R.case([0, 3, 150, 420, 260], [1, 7, 1, 3, 40], 4, 2, d, S, 8, kind, torch.float16, seed=window % 97, window=window,
+               sinks=sinks)
+    _run(c, torch.float16)
+
+
+def test_pages_that_nobody_sees_may_be_gone():
+    """Behind the window a table's entries are not read: a program gives those pages back."""
+    c = R.case([700, 300], [2, 1], 4, 2, 64, 16, 16, torch.int8, torch.bfloat16, seed=5, window=100, sinks=20)
+    gone = [list(range(2, (701 - 100) // 16)), list(range(2, (300 - 100) // 16))]
+    for b, entries in enumerate(gone):
+        c["table"][b, entries] = torch.tensor([-1, 1 << 30] * 40, dtype=torch.int32)[:len(entries)]
+    _, out = _run(c, torch.bfloat16)
+    assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("rows", [70, 130, 300])
+def test_many_rows(rows):
+    lens = [(37 * b) % 90 - (b % 11 == 5) * 200 for b in range(rows)]
+    lens = [max(n, -1) for n in lens]
+    new = [(b * 7) % 4 for b in range(rows)]
+    _run(R.case(lens, new, 2, 1, 64, 16, 8, torch.float8_e4m3fn, torch.float16, seed=rows), torch.float16, longest=3)
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("lens,new,nh,nkv,d", [([9000], [1], 4, 1, 64), ([6000, 10, 900], [1, 1, 1], 6, 2, 128),
+                                               ([5000, 100], [3, 60], 8, 2, 64), ([4000], [1], 40, 1, 128)])
+def test_long_rows_are_cut_and_joined(lens, new, nh, nkv, d, kind):
+    c = R.case(lens, new, nh, nkv, d, 64, 32, kind, torch.float16, seed=len(lens))
+    g, out = _run(c, torch.float16)
+    again = int4_hip.paged_attention8(**g)
+    assert torch.equal(out, again)  # the same bits, the cache as it was
+
+
+@pytest.mark.parametrize("dtype", BOTH, ids=ids)
+def test_a_dominant_token_and_scales_of_every_size(dtype):
+    """Rows that one token dominates, blocks whose scales lie 2^40 apart, queries far from 1."""
+    c = R.case([200, 150, 90], [1, 2, 1], 4, 2, 64, 16, 8, torch.int8, dtype, seed=12)
+    c["v_scale"] *= torch.exp2(torch.linspace(-20, 20, c["v_scale"].numel())).view(c["v_scale"].shape)
+    c["k_scale"] *= torch.exp2(torch.linspace(-6, 3, c["k_scale"].numel())).view(c["k_scale"].shape)
+    c["q"][1] *= 8
+    c["q"][2] *= 2.0 ** -10
+    _run(c, dtype)
+
+
+def test_scores_far_from_zero():
+    """Scores of 1e5: differences decide."""
+    c = R.case([60, 33], [1, 1], 2, 1, 64, 16, 8, torch.int8, torch.bfloat16, seed=13)
+    c["q"] *= 2.0 ** 14
+    g = _to(c)
+    out = int4_hip.paged_attention8(**g).float().cpu()
+    want, mass, reach = R.attention(**c)
+    assert out.isfinite().all()
+    # the largest score leads by far more than its error: its value, rounded
+    assert (out - want.float()).abs().max() <= 2.0 ** -7 * want.abs().max()
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+def test_what_lies_where_nobody_looks(kind):
+    """Past a row's tokens and in pages of none: codes of NaN, scales of NaN and infinity; nothing of it comes out."""
+    c = R.case([20, 3, 100], [2, 1, 40], 4, 2, 64, 32, 8, kind, torch.float16, seed=14)
+    if kind == torch.float8_e4m3fn:
+        used = R.case([20, 3, 100], [2, 1, 40], 4, 2, 64, 32, 8, kind, torch.float16, seed=14)
+        for n in ("k_pages", "v_pages"):
+            x = c[n].view(torch.uint8)
+            keep = x.clone()
+            x[:] = 0x7F
+            for b, m in enumerate([22, 4, 140]):
+                for i in range(m):
+                    page = int(c["table"][b, i // 32])
+                    x[page, :, i % 32] = keep[page, :, i % 32]
+        assert used["k_pages"].float().isfinite().all()
+    for n in ("k_scale", "v_scale"):
+        keep = c[n].clone()
+        c[n][:] = NAN
+        c[n][0::2] = float("inf")
+        for b, m in enumerate([22, 4, 140]):
+            for i in range(0, m, 8):
+                page = int(c["table"][b, i // 32])
+                c[n][page, :, i % 32 // 8] = keep[page, :, i % 32 // 8]
+    _, out = _run(c, torch.float16)
+    assert out.isfinite().all()
+
+
+def test_tokens_of_nan_reach_those_that_see_them():
+    """A code of NaN in a key or value, a scale of NaN: NaN for the tokens and heads that see it, no others."""
+    c = R.case([50, 50, 50, 50], [3, 3, 3, 1], 4, 2, 64, 16, 8, torch.float8_e4m3fn, torch.float16, seed=15, window=20,
+               sinks=2)
+    c["k_pages"].view(torch.uint8)[int(c["table"][0, 1]), 0, 15, 7] = 0x7F       # slot 31: seen by the first token alone
+    c["v_pages"].view(torch.uint8)[int(c["table"][1, 2]), 1, 0, 5] = 0xFF        # slot 32: by two
+    c["k_scale"][int(c["table"][2, 1]), 0, 0] = NAN                              # slots 16..23: by none
+    c["v_pages"].view(torch.uint8)[int(c["table"][3, 0]), 1, 1, 60] = 0x7F       # a sink
+    g, out = _run(c, torch.float16)
+    nan = out.view(10, 4, 64).isnan().all(-1).cpu()
+    assert nan[0].tolist() == [True, True, False, False] and not nan[1:3].any()
+    assert nan[3:6, 2:].all(-1).tolist() == [True, True, False] and not nan[6:9].any()
+    assert nan[9].tolist() == [False, False, True, True]
+    assert torch.equal(out.isnan(), out.view(10, 4, 64).isnan().any(-1).repeat_interleave(64, -1).view(10, 256))
+
+
+def test_pages_outside_the_pool_and_rows_past_the_table():
+    c = R.case([40, 40, 31, 5], [4, 4, 2, 1], 4, 2, 64, 16, 16, torch.int8, torch.bfloat16, seed=16, width=3)
+    c["table"][0, 1] = c["k_pages"].shape[0]  # seen by all of row 0
+    c["lengths"][1] = 45                      # 49 slots of 48
+    c["table"][2, 2] = -5                     # slot 32: the second token's own
+    _, out = _run(c, torch.bfloat16)
+    assert out[:8].isnan().all() and out[8].isfinite().all() and out[9].isnan().all() and out[10].isfinite().all()
+
+
+def test_offsets_that_pass_32_bits():
+    """A pool of more than 2^31 codes: pages at its end."""
+    nkv, S, d, P = 2, 64, 128, 140000  # 2.3e9 bytes each
+    c = R.case([150, 70], [2, 1], 4, nkv, d, S, 32, torch.int8, torch.bfloat16, seed=17)
+    n = c["k_pages"].shape[0]
+    big = dict(c)
+    big["table"] = torch.where(c["table"] >= 0, c["table"] + (P - n), c["table"])
+    g = {k: t.to(DEV) if isinstance(t, torch.Tensor) and k not in CACHE else t for k, t in big.items()}
+    for name in CACHE:
+        shape = (P,) + tuple(c[name].shape[1:])
+        g[name] = torch.zeros(shape, dtype=c[name].dtype, device=DEV)
+        g[name][-n:] = c[name].to(DEV)
+    out = int4_hip.paged_attention8(**g)
+    want, mass, reach = R.attention(**c)
+    _check(out, want, mass, reach, torch.bfloat16, 192, d)
+    k, v = int4_hip.paged_read8(*(g[x] for x in CACHE), g["table"], g["lengths"], g["offsets"], 3, torch.float32)
+    wk, wv = R.read(*(c[x] for x in CACHE), c["table"], c["lengths"], c["offsets"], 3, torch.float32)
+    assert torch.equal(k.cpu(), wk) and torch.equal(v.cpu(), wv)
+    _same_cache({x: g[x][-n:] for x in CACHE}, c)
+
+
+def test_strided_and_misaligned_operands():
+    c = R.case([20, 33], [2, 1], 4, 2, 64, 16, 8, torch.int8, torch.float16, seed=18)
+    g = _to(c)
+    for n in ("q", "k", "v"):
+        wide = torch.full((3, g[n].shape[1] + 24), 5.0, dtype=torch.float16, device=DEV)
+        wide[:, 8:-16] = g[n]
+        g[n] = wide[:, 8:-16]
+    odd = torch.empty(3, 257 * 2, dtype=torch.float16, device=DEV)[:, 1:257]
+    odd.copy_(g["q"])
+    g["q"] = odd
+    for n in ("cos", "sin"):
+        wide = torch.zeros(len(g[n]), 33, device=DEV)
+        wide[:, 1:] = g[n]
+        g[n] = wide[:, 1:]
+    for n in ("positions", "lengths"):
+        two = torch.stack((g[n], g[n] - 99), 1)
+        g[n] = two[:, 0]
+    out = int4_hip.paged_attention8(**g)
+    want, mass, reach = R.attention(**c)
+    _check(out, want, mass, reach, torch.float16, 64, 64)
+    _same_cache(g, c)
+
+
+def test_no_tokens_and_no_rows():
+    c = _to(R.case([4, 0], [0, 0], 4, 2, 64, 16, 8, torch.int8, torch.float16))
+    assert int4_hip.paged_attention8(**c).shape == (0, 256)
+    _append(c)
+    k, v = int4_hip.paged_read8(*(c[n] for n in CACHE), c["table"], c["lengths"], c["offsets"], 0)
+    assert k.shape == v.shape == (0, 128)
+    none = dict(_to(R.case([4], [3], 4, 2, 64, 16, 8, torch.int8, torch.float16)))
+    none.update(table=none["table"][:0], lengths=none["lengths"][:0], offsets=none["offsets"][:1])
+    assert (int4_hip.paged_attention8(**none) == 0).all()
+    assert (int4_hip.paged_read8(*(none[n] for n in CACHE), none["table"], none["lengths"], none["offsets"], 2)[0] == 0).all()
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+def test_captured_calls_are_replayed(kind):
+    """A decode step and a few drafts in graphs of one capture stream, replayed between eager calls."""
+    c = R.case([3000, 40, 7], [1, 1, 1], 8, 2, 64, 32, 16, kind, torch.bfloat16, seed=19, width=96)
+    d = R.case([900, 40], [4, 2], 8, 2, 64, 32, 16, kind, torch.bfloat16, seed=20)
+    g, h = _to(c), _to(d)
+    start = {n: g[n].clone() for n in CACHE}
+    graphs, outs = [], []
+    stream = torch.cuda.Stream()
+    for x in (g, h):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(int4_hip.paged_attention8(**x))
+        graphs.append(graph)
+    for n in CACHE:
+        g[n].copy_(start[n])
+    other = _to(R.case([100], [1], 4, 2, 64, 16, 8, kind, torch.float16, seed=1))
+    want, mass, reach = R.attention(**c)
+    want2, mass2, reach2 = R.attention(**d)
+    for _ in range(4):
+        graphs[0].replay()
+        int4_hip.paged_attention8(**other)
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        _check(outs[0], want, mass, reach, torch.bfloat16, 3072, 64)
+        _check(outs[1], want2, mass2, reach2, torch.bfloat16, 928, 64)
+        assert torch.equal(outs[0], int4_hip.paged_attention8(**g))
+        _same_cache(g, c)
+    # the lengths live on the GPU: a replay with others
+    g["lengths"].sub_(5)
+    c["lengths"] -= 5
+    graphs[0].replay()
+    want, mass, reach = R.attention(**c)
+    _check(outs[0], want, mass, reach, torch.bfloat16, 3072, 64)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams have a workspace each."""
+    cases = [_to(R.case([4000 + 100 * i], [1], 8, 1, 64, 64, 32, torch.int8, torch.bfloat16, seed=30 + i)) for i in range(2)]
+    want = [int4_hip.paged_attention8(**c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for s, c, o in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                o.append(int4_hip.paged_attention8(**c))
+    torch.cuda.synchronize()
+    for o, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in o)
+
+
+def test_chunks_and_tokens_make_the_same_cache_as_its_parts_say():
+    """A prompt in chunks, then tokens one by one, attending throughout: as the reference does it."""
+    kind, new = torch.float8_e4m3fn, [20, 13, 1, 1, 4]
+    c = R.case([0], [39], 4, 2, 64, 16, 16, kind, torch.float16, seed=21, shift=0)
+    g, at = _to(c), 0
+    for n in new:
+        one = {k: (t[at:at + n] if k in ("q", "k", "v", "positions") else t) for k, t in c.items()}
+        one.update(lengths=torch.tensor([at], dtype=torch.int32), offsets=torch.tensor([0, n], dtype=torch.int32))
+        h = {k: (g[k] if k in CACHE or k == "table" else t) for k, t in _to(one).items()}
+        out = int4_hip.paged_attention8(**h)
+        want, mass, reach = R.attention(**one)
+        _check(out, want, mass, reach, torch.float16, 48, 64)
+        _same_cache(g, c)
+        at += n
