@@ -450,10 +450,11 @@ int w4_paged8_read(const w4_paged8_cache* cache, int dtype, const int32_t* start
  * softmax(rope(q) K / sqrt(head_dim)) V, from the cached codes and scales, rounded once;
  * fp32 sums, queries and probabilities entering them with 24 bits.  The token of slot i
  * sees slots 0..i or, with window > 0, those past i - window and the first `sinks`.
- * longest: the most new tokens of any row, 0 if not known; results do not depend on it.
- * Out is 0 for idle rows (lengths[b] < 0) and tokens of no row, NaN for rows whose slots
- * pass the table, tokens that see a page outside the pool or have a position outside the
- * angles, and tokens that see a block with scale NaN or (e4m3) a token with a code of NaN.
+ * longest: the most new tokens that a row may have, 0 for any number; at 1 one launch does
+ * it all.  Out is 0 for idle rows (lengths[b] < 0) and tokens of no row, NaN for rows with
+ * more than `longest` tokens or whose slots pass the table (nothing of them is written), tokens that see a page outside the pool or have a position outside the
+ * angles, and tokens that see a block with scale NaN or a key with a code of NaN (e4m3); a
+ * value's code of NaN makes its element NaN.
  * lengths is not changed.  num_heads: at most 256 for each key-value head.  workspace: as
  * for w4a16_gemm, w4_paged8_attention_workspace_bytes long.  Results are bit-identical run
  * to run.

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "w4_paged.hpp"
 
@@ -37,17 +38,17 @@ struct Paged8View {
 
 // The new tokens of every row: tokens offsets[b]..offsets[b + 1] go to slots lengths[b].. .
 struct RowSpan {
-  int len, o0, n;  // n = 0: nothing to do with this row; len < 0: idle; REFUSED: its slots pass the table
+  int len, o0, n;  // n = 0: nothing to do with this row; len < 0: idle, or refused: slots past the table, too many
 };
 constexpr int kP8Refused = -2;
 __device__ __forceinline__ RowSpan row_span(const Paged8View& c, const int32_t* __restrict__ lengths,
-                                            const int32_t* __restrict__ offsets, int tokens, int r) {
+                                            const int32_t* __restrict__ offsets, int tokens, int longest, int r) {
   RowSpan s{-1, 0, 0};
   if (r >= c.rows) return s;
   s.len = max(lengths[r], -1);
   s.o0 = min(max(offsets[r], 0), tokens);
   s.n = min(max(offsets[r + 1], s.o0), tokens) - s.o0;
-  if ((int64_t)s.len + s.n > c.capacity()) s.len = kP8Refused;
+  if ((int64_t)s.len + s.n > c.capacity() || s.n > longest) s.len = s.len < 0 ? -1 : kP8Refused;
   return s;
 }
 
@@ -106,6 +107,22 @@ __device__ __forceinline__ u32x2 shrink8(u32x2 w, int m) {
   return r;
 }
 
+// The scale of a block whose new values reach the magnitude x (of the bits of a double: an infinity or NaN among them
+// is not less than one), with scale `old` (0: it begins), and by how many powers of two it has grown.
+template <int CT>
+__device__ __forceinline__ double block_scale(double x, double old, int* grow) {
+  constexpr double Q = Code<CT>::most;
+  *grow = 0;
+  if (!(x < __builtin_inf()) || old != old) return __builtin_nan("");
+  if (!(old > 0.0)) return x > 0.0 ? fmax((double)(float)(x / Q), kSmallestScale) : 0.0;
+  if (x > Q * old) {  // the least power of two that will do
+    const double r = x / (Q * old);
+    const int e = exponent_of(r);
+    *grow = r > two_to(e) ? e + 1 : e;
+  }
+  return old * two_to(*grow);
+}
+
 // Eight codes as bf16, exactly: int8 has 7 bits and a sign, e4m3 4 bits of bf16's exponents.
 template <int CT>
 __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
@@ -129,6 +146,11 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
+// 1 in every byte that is the NaN of e4m3.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+}
+
 // ---------------------------------------------------------------- append
 struct Append8Args {
   Paged8View c;
@@ -137,7 +159,7 @@ struct Append8Args {
   int64_t stride_k, stride_v, angles;
   const int32_t *lengths, *offsets, *positions;
   const float *cos, *sin;  // [angles, D / 2]
-  int tokens;
+  int tokens, longest;
 };
 
 // Item -> a row and one of its blocks that get new tokens, counted over all rows.
@@ -145,7 +167,7 @@ __device__ __forceinline__ bool find_block(const Append8Args& a, int item, int* 
   const int lane = threadIdx.x & 63;
   int base = 0;
   for (int r = 0; r < a.c.rows; r += 64) {
-    const RowSpan s = row_span(a.c, a.lengths, a.offsets, a.tokens, r + lane);
+    const RowSpan s = row_span(a.c, a.lengths, a.offsets, a.tokens, a.longest, r + lane);
     const int first = s.len >> a.c.log2b;
     const int blocks = s.len >= 0 && s.n > 0 ? ((s.len + s.n - 1) >> a.c.log2b) - first + 1 : 0;
     const int upto = base + wave_scan(blocks);
@@ -252,22 +274,8 @@ __global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a
   int grow[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const double x = __builtin_bit_cast(double, top_s[i][unit]);
     const double old = fresh ? 0.0 : (double)(i ? a.c.v_scale : a.c.k_scale)[blk];
-    constexpr double Q = Code<CT>::most;
-    grow[i] = 0;
-    if (!(x < __builtin_inf()) || old != old) {
-      scale[i] = __builtin_nan("");
-    } else if (old > 0.0) {
-      if (x > Q * old) {  // the least power of two that will do
-        const double r = x / (Q * old);
-        const int e = exponent_of(r);
-        grow[i] = r > two_to(e) ? e + 1 : e;
-      }
-      scale[i] = old * two_to(grow[i]);
-    } else {
-      scale[i] = x > 0.0 ? fmax((double)(float)(x / Q), kSmallestScale) : 0.0;
-    }
+    scale[i] = block_scale<CT>(__builtin_bit_cast(double, top_s[i][unit]), old, &grow[i]);
     inv[i] = scale[i] > 0.0 ? 1.0 / scale[i] : 0.0;  // (also of NaN: its codes are 0)
   }
   __syncthreads();  // all have read the scales that are there
@@ -388,7 +396,9 @@ struct Attend8Args {
   float* stats;   // [split items, 16, 2]: their references and sums
   unsigned* cnt;  // arrival counters of those tiles
   float scale;    // 1 / sqrt(D)
-  int tokens, g, window, sinks;  // window: 0 for none
+  const uint16_t *k, *v;  // PUT: the new tokens', which the attention writes itself
+  int64_t stride_k, stride_v;
+  int tokens, longest, g, window, sinks;  // window: 0 for none
 };
 
 // The work of one workgroup: a tile of sixteen (new token, query head) columns of one row and key-value head, and a
@@ -399,7 +409,9 @@ struct Item8 {
   int first, counter;  // of a tile in several parts: the index of part 0 among such parts, and of the tile among such tiles
 };
 
-constexpr int kP8Waves = 4, kP8Parts = 256, kP8MinUnits = 4;
+constexpr int kP8Unit = 32;  // slots that a wave takes at once
+constexpr int kP8AtOnce = 8;  // parts that a thread of the joining reads together
+constexpr int kP8Waves = 4, kP8Parts = 512, kP8MinUnits = 4;
 
 // Rows are cut into parts of about (all columns' tiles x units of slots) / 256, so that time follows the slots there
 // are and not the table.  Those that are cut have at most 2 * kP8Parts parts in all: each has more units than `per`,
@@ -416,7 +428,7 @@ __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8
     const int64_t span = (int64_t)a.window + min((16 + a.g - 2) / a.g, s.n - 1);
     return (int)min((int64_t)all, span / UP + 2 + (a.sinks + UP - 1) / UP);
   };
-  auto span = [&](int r) { return row_span(a.c, a.lengths, a.offsets, a.tokens, r + lane); };
+  auto span = [&](int r) { return row_span(a.c, a.lengths, a.offsets, a.tokens, a.longest, r + lane); };
   const RowSpan s0 = span(0);
   float all = (float)tiles_of(s0) * (float)units_of(s0);
   for (int r = 64; r < a.c.rows; r += 64) {
@@ -459,7 +471,7 @@ __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
 
-// A workgroup's four waves take units of UP = 8192 / D slots in turn (16 KB of codes), each its own.
+// A workgroup's four waves take units of 64 slots in turn, each its own.
 //
 // Both products are 16x16x32 bf16 matrix instructions, transposed, with the columns (new tokens x query heads of the
 // group) as their columns: S^T = K Q^T, then O^T = V^T P^T.  Codes are bf16 numbers exactly; the scales stay outside:
@@ -467,21 +479,28 @@ typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
 // sum of three bf16 numbers, 24 bits, so the result has about fp32's error before its one rounding.
 //
 // Keys come from memory straight into the first product's operand: its inner index may run over a head in any order,
-// so a lane takes 32 (D = 64: 16) bytes in a row of a slot.  A tile's row r is slot 8 (r / 4) + 4 t + r % 4 of its
+// so a lane takes sixteen bytes in a row of a slot, four lanes 64.  A tile's row r is slot 8 (r / 4) + 4 t + r % 4 of its
 // block of 32 (t: the first or second tile), so the scores that a lane holds of a column are those of eight slots in a
 // row, its part of the second product's operand.  Values go through a wave's own LDS, which transposes them on reading.
-template <int DT, int CT, int D, int W>
-__global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args a) {
-  constexpr int UP = 8192 / D, KB = UP / 32, NJ = D / 32, ND = D / 16, NP = Split<W4_DTYPE_BF16>::N;
+//
+// PUT: no row has more than one new token, a row's and head's columns are one tile, and a block lies in one unit: the
+// wave that takes a row's last unit writes the token (and, where the block's scale grows, its other codes), as
+// paged8_append_kernel does.
+template <int DT, int CT, int D, int W, bool PUT>
+__global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_attention_kernel(Attend8Args a) {
+  constexpr int UP = kP8Unit, KB = UP / 32, NJ = D / 32, ND = D / 16, NP = Split<W4_DTYPE_BF16>::N;
   constexpr int KC = D / 64;               // 16-byte loads of a key a lane
   constexpr int VR = 1024 / D, VC = D / 16;  // rows of values in a load of the wave, 16-byte chunks of a row
+  constexpr int NV = UP / VR;
   constexpr int OROW = D + 4;              // floats of an output row in LDS
   constexpr int WAVE_B = 16 * OROW * 4 > UP * D ? 16 * OROW * 4 : UP * D;
   constexpr int kThreads = 64 * W;
   typedef Mfma<W4_DTYPE_BF16> M;
   __shared__ __attribute__((aligned(16))) uint8_t v_s[W][WAVE_B];
   __shared__ float m_s[W][16], l_s[W][16];
+  __shared__ __attribute__((aligned(16))) uint8_t new_s[2][D];
   __shared__ unsigned arrived_s;
+  static_assert(!PUT || KB == 1, "a block lies in one unit");
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, c = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -520,28 +539,29 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
   auto base_of = [&](int u) { return (u < sink_units ? u : u_lo + u - sink_units) * UP; };
   const int u0 = (int)((int64_t)it.part * units / it.parts), u1 = (int)((int64_t)(it.part + 1) * units / it.parts);
 
-  u32x4 kr[KB][2][KC], vr[8];
+  u32x4 kr[KB][2][KC], vr[NV];
   float ks[KB], vs[KB];
   int ids[KB], next_ids[KB];
-  // Lane: the pages of the groups of eight slots that its rows of keys are in.
+  const int32_t* const table = a.c.table + (int64_t)b * a.c.width;
+  // Lane: the pages of the groups of eight slots that its rows of keys are in, as the table has them.  (Looked at
+  // before they are needed, they would make the wave wait for all the loads before them.)
   auto load_ids = [&](int u, int id[KB]) __attribute__((always_inline)) {
     const int base = base_of(u);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      const int slot = base + kb * 32 + 8 * (l16 >> 2);
-      id[kb] = slot <= last_slot ? a.c.page(b, slot) : -1;
-    }
+    for (int kb = 0; kb < KB; ++kb)
+      id[kb] = table[min(base + kb * 32 + 8 * (l16 >> 2), last_slot) >> a.c.log2s];
   };
   auto load = [&](int u) __attribute__((always_inline)) {
     const int base = base_of(u);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
+      ids[kb] = base + kb * 32 + 8 * (l16 >> 2) <= last_slot && (uint64_t)(int64_t)ids[kb] < (uint64_t)a.c.pages ? ids[kb] : -1;
       const int64_t at = a.c.token(max(ids[kb], 0), h, base + kb * 32 + 8 * (l16 >> 2) + (l16 & 3));
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < KC; ++i)
-          kr[kb][t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.c.k + (at + 4 * t) * D + c * (D / 4) + 16 * i));
+          kr[kb][t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.c.k + (at + 4 * t) * D + 64 * i + 16 * c));
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {  // (the lane's scores are of group c)
@@ -552,7 +572,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
       vs[kb] = id < 0 ? __builtin_nanf("") : v0;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < NV; ++i) {
       int page;
       if constexpr (D == 128) {
         page = __builtin_amdgcn_readlane(ids[i >> 2], 4 * (i & 3));
@@ -566,8 +586,11 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
     }
   };
   // The 16-byte chunk of a row of values lies where it shares no bank with those that are read beside it.
+  // (The same for rows 8, D = 64: 16, apart, so loads and blocks of 32 slots are a constant apart.)
   auto swizzle = [&](int row) { return D == 128 ? row & 7 : (row >> 2) & 3; };
   uint8_t* const vw = v_s[wv];
+  const int put_at = lane / VC * D + (((lane % VC) ^ swizzle(lane / VC)) << 4);
+  const int get_row = 8 * c + (l16 >> 1), get_at = get_row * D + (swizzle(get_row) << 4) + 8 * (l16 & 1);
 
   int u = u0 + wv;
   if (u < u1) {  // on their way before the query is at hand
@@ -587,19 +610,56 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
     const float* const cosr = a.cos + (there ? (int64_t)pos * (D / 2) : 0);
     const float* const sinr = a.sin + (there ? (int64_t)pos * (D / 2) : 0);
     const float scale = there ? a.scale : __builtin_nanf("");
+    // chunk j: elements 64 (j / 2) + 16 c + 8 (j % 2).. ; those that they are rotated with are D / 2 from them, in another
+    // chunk of the lane or (D = 64) another lane's
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const int d = c * (D / 4) + 8 * j, da = d & (D / 2 - 1);
+      const int d = 64 * (j >> 1) + 16 * c + 8 * (j & 1), da = d & (D / 2 - 1);
+      const bool low = D == 128 ? j < 2 : c < 2;
       float x[8], y[8];
       unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + d), x);
       unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + (d ^ (D / 2))), y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float r1, r2;
-        if (c < 2) rope_pair(x[e], y[e], cosr[da + e], sinr[da + e], &r1, &r2), x[e] = r1 * scale;
+        if (low) rope_pair(x[e], y[e], cosr[da + e], sinr[da + e], &r1, &r2), x[e] = r1 * scale;
         else rope_pair(y[e], x[e], cosr[da + e], sinr[da + e], &r1, &r2), x[e] = r2 * scale;
       }
       split8<W4_DTYPE_BF16, true>(x, qf[j]);
+    }
+  }
+
+  // The new token, quantised (the wave that takes the last unit): its codes in LDS, its block's scales.
+  uint32_t new_scale[2];
+  int grow[2];
+  if constexpr (PUT) {
+    if (it.part == it.parts - 1 && wv == (units - 1 - u0) % W) {
+      const int pos = a.positions[it.o0], lane2 = lane & (D / 2 - 1);
+      const bool there = (uint64_t)(int64_t)pos < (uint64_t)a.angles;
+      const uint16_t* const kp = a.k + it.o0 * a.stride_k + h * D;
+      const uint16_t* const vp = a.v + it.o0 * a.stride_v + h * D;
+      const int64_t at = there ? (int64_t)pos * (D / 2) + lane2 : 0;
+      const double cc = there ? (double)a.cos[at] : (double)__builtin_nanf(""), ss = (double)a.sin[at];
+      const double x1 = act_bits_to_float(kp[lane2], DT), x2 = act_bits_to_float(kp[lane2 + D / 2], DT);
+      const double x[2][2] = {{x1 * cc - x2 * ss, x2 * cc + x1 * ss},
+                              {act_bits_to_float(vp[lane2], DT), act_bits_to_float(vp[lane2 + D / 2], DT)}};
+      const int page = a.c.page(b, len);
+      const bool fresh = (len & ((1 << a.c.log2b) - 1)) == 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint64_t y1 = __builtin_bit_cast(uint64_t, __builtin_fabs(x[i][0])),
+                       y2 = __builtin_bit_cast(uint64_t, __builtin_fabs(x[i][1])), y = y1 > y2 ? y1 : y2;
+        const uint32_t hi = wave_umax((uint32_t)(y >> 32));
+        const uint32_t lo = wave_umax((uint32_t)(y >> 32) == hi ? (uint32_t)y : 0u);
+        const double old = fresh || page < 0 ? 0.0 : (double)(i ? a.c.v_scale : a.c.k_scale)[a.c.block(page, h, len)];
+        const double scale = block_scale<CT>(__builtin_bit_cast(double, (uint64_t)hi << 32 | lo), old, &grow[i]);
+        const double inv = scale > 0.0 ? 1.0 / scale : 0.0;
+        grow[i] = __builtin_amdgcn_readfirstlane(grow[i]);
+        new_scale[i] = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, (float)scale));
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          new_s[i][lane2 + e * (D / 2)] = (uint8_t)(inv > 0.0 ? encode<CT>(x[i][e], scale, inv) : 0u);
+      }
     }
   }
 
@@ -610,6 +670,49 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
 
   for (; u < u1; u += W) {
     const int base = base_of(u);
+    if constexpr (PUT) {
+      const int page = u == units - 1 ? a.c.page(b, len) : -1;
+      if (page >= 0) {
+        const int slot0 = len & ~((1 << a.c.log2b) - 1);
+        const int64_t tok0 = a.c.token(page, h, slot0), blk = a.c.block(page, h, len);
+        if (grow[0] > 0 || grow[1] > 0) {
+          for (int i = 0; i < 2; ++i) {
+            if (grow[i] == 0) continue;
+            uint8_t* const p = (i ? a.c.v : a.c.k) + tok0 * D;
+            for (int j = lane * 8; j < (len - slot0) * D; j += 512)
+              *reinterpret_cast<u32x2*>(p + j) = shrink8<CT>(*reinterpret_cast<const u32x2*>(p + j), grow[i]);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // other lanes load what a lane has stored
+          load(u);
+        }
+        wave_lds_order();
+        const int row = len - base;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < KC; ++i) {
+            const u32x4 n = *reinterpret_cast<const u32x4*>(&new_s[0][64 * i + 16 * c]);
+            if (8 * (l16 >> 2) + 4 * t + (l16 & 3) == row) kr[0][t][i] = n;
+          }
+        const u32x4 n = *reinterpret_cast<const u32x4*>(&new_s[1][lane % VC * 16]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * VR + lane / VC == row) vr[i] = n;
+        if ((base + 8 * c) >> a.c.log2b == len >> a.c.log2b) {
+          ks[0] = __builtin_bit_cast(float, new_scale[0]);
+          vs[0] = __builtin_bit_cast(float, new_scale[1]);
+        }
+        if (lane < D / 16) {
+          const int64_t at = a.c.token(page, h, len) * D + lane * 16;
+          *reinterpret_cast<u32x4*>(a.c.k + at) = *reinterpret_cast<const u32x4*>(&new_s[0][lane * 16]);
+          *reinterpret_cast<u32x4*>(a.c.v + at) = *reinterpret_cast<const u32x4*>(&new_s[1][lane * 16]);
+        }
+        if (lane == 0) {
+          a.c.k_scale[blk] = __builtin_bit_cast(float, new_scale[0]);
+          a.c.v_scale[blk] = __builtin_bit_cast(float, new_scale[1]);
+        }
+      }
+    }
     f32x4 s[KB][2];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -629,42 +732,47 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
 #pragma unroll
           for (int j = 0; j < NJ; ++j) s[kb][t] = M::m16(kf[j], __builtin_bit_cast(bf16x8, qf[j][p]), s[kb][t]);
       }
-    // e4m3 has a NaN: what a program that is not this one left in the pages.  A token with one counts as NaN, and only
-    // where it is seen.
-    uint32_t nans[KB];
+    // A slot that a column does not see has score -inf and, whatever is stored there, no share in the output.
+    const bool whole = base + UP - 1 <= first_slot && (!a.window || base > last_slot - a.window || base + UP <= a.sinks);
+    wave_lds_order();  // the unit before has been read
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) nans[kb] = 0;
+    for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4*>(vw + put_at + i * (VR * D)) = vr[i];
+    wave_lds_order();
+    auto seen = [&](int slot) {
+      return slot <= mine && (!a.window || slot > mine - a.window || slot < a.sinks);
+    };
     if constexpr (CT == W4_CODE_E4M3) {
-      uint32_t any[8], some = 0;
+      // e4m3 has a NaN: what a program that is not this one left in the pages.  It must not meet the probability 0 of a
+      // slot that is not seen, so it is taken out here, and what sees it is made NaN by itself.  (Where all is seen, it
+      // does its work.)
+      if (!whole) {
+        uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        any[i] = 0;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) any[i] |= ((vr[i][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-        some |= any[i];
-      }
-      if (__ballot(some != 0)) {
+          for (int e = 0; e < 4; ++e) any |= nan_bytes(vr[i][e]);
+        if (__ballot(any != 0)) {
+          for (int row = 0; row < UP; ++row) {
+            const bool see = seen(base + row);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint64_t hit = __ballot(any[i] != 0);
+            for (int d = 0; d < ND; ++d) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(vw + row * D + ((d ^ swizzle(row)) << 4) + 4 * c);
 #pragma unroll
-          for (int r = 0; r < VR; ++r)
-            if (hit >> (r * VC) & ((1ull << VC) - 1)) nans[(i * VR) / 32] |= 1u << ((i * VR + r) & 31);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t bad = ((vr[i][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-            vr[i][e] &= ~((bad >> 7) * 0xFFu);
+              for (int e = 0; e < 4; ++e)
+                if (see && (w >> (8 * e) & 0x7F) == 0x7F) o[d][e] = __builtin_nanf("");
+            }
           }
+          wave_lds_order();
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vr[i][e] &= ~(nan_bytes(vr[i][e]) * 0xFFu);
+            *reinterpret_cast<u32x4*>(vw + put_at + i * (VR * D)) = vr[i];
+          }
+          wave_lds_order();
         }
       }
     }
-    wave_lds_order();  // the unit before has been read
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = i * VR + lane / VC;
-      *reinterpret_cast<u32x4*>(vw + row * D + (((lane % VC) ^ swizzle(row)) << 4)) = vr[i];
-    }
-    wave_lds_order();
     float sk[KB], sv[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) sk[kb] = ks[kb], sv[kb] = vs[kb];
@@ -675,15 +783,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
       load_ids(min(u + 2 * W, u1 - 1), next_ids);
     }
 
-    // A slot that a column does not see has score -inf and, whatever is stored there, no share in the output.
-    const bool whole = base + UP - 1 <= first_slot && (!a.window || base > last_slot - a.window || base + UP <= a.sinks);
-    bool odd = false;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) odd = odd || nans[kb] != 0;
     float top = -__builtin_inff();
-    auto seen = [&](int slot) {
-      return slot <= mine && (!a.window || slot > mine - a.window || slot < a.sinks);
-    };
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -715,21 +815,13 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
         p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3] - mz, kLog2e, -8.f));
         l += p[e];
         p[e] *= sv[kb];
-      }
-      if (!whole || odd) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (nans[kb] >> (8 * c + e) & 1) p[e] = __builtin_nanf("");
-          if (!seen(base + kb * 32 + 8 * c + e)) p[e] = 0.f;
-        }
+        if (!whole) p[e] = seen(base + kb * 32 + 8 * c + e) ? p[e] : 0.f;
       }
       u32x4 pf[NP];
       split8<W4_DTYPE_BF16, false>(p, pf);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const int row = kb * 32 + 8 * c + (l16 >> 1);
-        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (lds_i32x2)(vw + row * D + ((d ^ swizzle(row)) << 4) + 8 * (l16 & 1)));
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(vw + (get_at ^ (d << 4)) + kb * (32 * D)));
         const bf16x8 vf = codes8<CT>((uint32_t)w[0], (uint32_t)w[1]);
 #pragma unroll
         for (int q = NP - 1; q >= 0; --q) o[d] = M::m16(vf, __builtin_bit_cast(bf16x8, pf[q]), o[d]);
@@ -786,11 +878,11 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
     const int hd = i / (D / 4);
     Share x;
     if (run < runs) {
-      for (int p0 = run; p0 < it.parts; p0 += runs * 8) {
-        f32x4 t[8];
-        f32x2 ml[8];
+      for (int p0 = run; p0 < it.parts; p0 += runs * kP8AtOnce) {
+        f32x4 t[kP8AtOnce];
+        f32x2 ml[kP8AtOnce];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < kP8AtOnce; ++k) {
           const int p = min(p0 + k * runs, it.parts - 1);
           t[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                                rp, (uint32_t)(p * STRIDE + i * 4) * 4u, 0, kPagedCoherentAux));
@@ -798,7 +890,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attention_kernel(Attend8Args
                                                                                  kPagedCoherentAux));
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < kP8AtOnce; ++k)
           if (p0 + k * runs < it.parts) x.add(ml[k][0], ml[k][1], t[k]);
       }
     }
@@ -939,7 +1031,7 @@ extern "C" int w4_paged8_append(const w4_paged8_cache* cache, int dtype, const v
     return rc;
   if (tokens == 0 || cache->rows == 0) return W4_OK;
   const w4::Append8Args a{view_of(cache), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_k,
-                          stride_v, angles, lengths, offsets, positions, cos, sin, (int)tokens};
+                          stride_v, angles, lengths, offsets, positions, cos, sin, (int)tokens, (int)tokens};
   return launch_append8(a, dtype, cache->code, cache->head_dim, static_cast<hipStream_t>(stream), "w4_paged8_append");
 }
 
@@ -1005,10 +1097,14 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
                 p.bytes, workspace_bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const w4::Paged8View view = view_of(cache);
-  const w4::Append8Args put{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_k, stride_v,
-                            angles, lengths, offsets, positions, cos, sin, (int)tokens};
-  if (const int rc = launch_append8(put, dtype, cache->code, cache->head_dim, st, "w4_paged8_attention (append)"))
-    return rc;
+  const int most_new = (int)(longest && longest < tokens ? longest : tokens);
+  const bool put = most_new == 1 && num_heads / cache->kv_heads <= 16 && cache->block <= w4::kP8Unit;
+  if (!put) {
+    const w4::Append8Args p{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_k, stride_v,
+                            angles, lengths, offsets, positions, cos, sin, (int)tokens, most_new};
+    if (const int rc = launch_append8(p, dtype, cache->code, cache->head_dim, st, "w4_paged8_attention (append)"))
+      return rc;
+  }
   const int64_t most = 1 << 30;  // (of slots, which are fewer)
   char* const ws = static_cast<char*>(workspace);
   w4::Attend8Args a{};
@@ -1026,7 +1122,12 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.cnt = reinterpret_cast<unsigned*>(ws);
   a.scale = 1.f / sqrtf((float)cache->head_dim);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.stride_k = stride_k;
+  a.stride_v = stride_v;
   a.tokens = (int)tokens;
+  a.longest = most_new;
   a.g = (int)(num_heads / cache->kv_heads);
   a.window = window >= most ? 0 : (int)window;
   a.sinks = (int)std::min(sinks, most);
@@ -1034,7 +1135,8 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   return by_dtype(dtype, [&](auto dt) {
     return by_code(cache->code, [&](auto ct) {
       return by_head(cache->head_dim, [&](auto d) {
-        w4::paged8_attention_kernel<dt(), ct(), d(), w4::kP8Waves><<<grid, 64 * w4::kP8Waves, 0, st>>>(a);
+        if (put) w4::paged8_attention_kernel<dt(), ct(), d(), w4::kP8Waves, true><<<grid, 64 * w4::kP8Waves, 0, st>>>(a);
+        else w4::paged8_attention_kernel<dt(), ct(), d(), w4::kP8Waves, false><<<grid, 64 * w4::kP8Waves, 0, st>>>(a);
         return check_launch("w4_paged8_attention");
       });
     });

@@ -122,12 +122,12 @@ def paged_attention8(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, tabl
     ``q`` [tokens, heads * head_dim], ``k``, ``v`` [tokens, kv_heads * head_dim]: their
     projections before the rotary embedding, bf16 or fp16.  Keys and values are written as
     by ``paged_append8``; then the token of slot i attends in fp32 to slots 0..i or, with
-    ``window``, to the last ``window`` of them and the first ``sinks``.  ``longest``, the
-    most new tokens of any row where the program knows it, only helps the plan.
-    ``lengths`` is left as it is (all layers of a model share it).
+    ``window``, to the last ``window`` of them and the first ``sinks``.  ``longest`` is
+    the most new tokens that a row may have, where the program knows it: of a decode step, 1,
+    for which one launch writes and attends.  ``lengths`` is left as it is (all layers of a model share it).
 
-    Idle rows and tokens of no row come back 0.  NaN come back: rows whose slots pass the
-    table; tokens that see a page outside the pool or a block of NaN, or whose position is
+    Idle rows and tokens of no row come back 0.  NaN come back: rows with more
+    than ``longest`` tokens or whose slots pass the table (nothing of them is written); tokens that see a page outside the pool or a block of NaN, or whose position is
     outside the tables.
     """
     _no_grad(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale)

@@ -132,7 +132,7 @@ def read(k_pages, v_pages, k_scale, v_scale, table, starts, offsets, tokens, dty
 def attention(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, lengths, offsets, positions, window=None,
               sinks=0, **_):
     """(out, p @ |v|, the largest sum |q||k| / sqrt(d) that a token's head meets) in 64 bits; the cache is updated in
-    place.  A token with a NaN in its key or value is one of NaN."""
+    place."""
     append(k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, lengths, offsets, positions)
     P, nkv, S, d = k_pages.shape
     T, nh = q.shape[0], q.shape[1] // d
@@ -155,11 +155,13 @@ def attention(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, leng
             x = rotate(x, cos[pos], sin[pos]) if 0 <= pos < len(cos) else torch.full_like(x, NAN)
             for h in range(nh):
                 key, val = kk[seen, h // (nh // nkv)], vv[seen, h // (nh // nkv)]
-                if not (key.isfinite().all() and val.isfinite().all() and x[h].isfinite().all()):
+                if not (key.isfinite().all() and x[h].isfinite().all()):
                     out[t, h] = NAN
                     continue
                 p = torch.softmax(key @ x[h] / math.sqrt(d), 0)
-                out[t, h], mass[t, h] = p @ val, p @ val.abs()
+                # (a probability that fp32 cannot have, 2^-118 of the largest with the reference 2^8 behind, is lost: the
+                # tolerance, 2^-21 of the mass or more, is to hold n 2^-110 of the largest value)
+                out[t, h], mass[t, h] = p @ val, p @ val.abs() + len(seen) * 2.0 ** -89 * val.nan_to_num().abs().max()
                 reach[t, h] = (key.abs() @ x[h].abs()).max() / math.sqrt(d)
     return out.flatten(1), mass.flatten(1), reach.expand(-1, -1, d).flatten(1)
 

@@ -251,6 +251,61 @@ def test_window_and_sinks(window, sinks, d, S, kind):
     _run(c, torch.float16)
 
 
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("dtype", BOTH, ids=ids)
+@pytest.mark.parametrize("nh,nkv,d,S,block", [(4, 2, 64, 16, 8), (8, 2, 128, 64, 32), (16, 1, 64, 32, 16), (17, 1, 64, 16, 16),
+                                              (4, 4, 128, 64, 64), (6, 2, 64, 8, 8), (12, 1, 128, 32, 32)])
+def test_steps_of_one_token(nh, nkv, d, S, block, dtype, kind):
+    """Decode steps, known to be of one token a row: values of all sizes come into blocks that are begun, held and
+    full; the same as the reference's, and the same bits as without that knowledge."""
+    lens, sizes = [0, 7, 30, 63, -1, 100, 2000], [1.0, 0.0, 30.0, 29.0, 1e3, 1e-3, float("inf"), 1.0, 1e3, 1e4]
+    c = R.case(lens, [1] * 7, nh, nkv, d, S, block, kind, dtype, seed=nh, width=2064 // S, angles=2100)
+    P, table = R.pages_for([max(n, 0) + 12 for n in lens], S, 1, width=2064 // S)
+    c.update(R.cache(kind, P, nkv, S, d, block, 40), table=table)
+    g = _to(c)
+    for step, size in enumerate(sizes):
+        for n in ("q", "k", "v"):
+            x = randn(tuple(c[n].shape), seed=90 + step).float()
+            x = torch.where(torch.arange(7)[:, None] % 2 == 0, x, x * (1.0 if size == float("inf") else size))
+            if size == float("inf") and n != "q":
+                x[3, 5] = size if n == "k" else NAN
+            c[n] = x.to(dtype)
+            g[n] = c[n].to(DEV)
+        before = {n: g[n].clone() for n in CACHE}
+        out = int4_hip.paged_attention8(**g, longest=1)
+        want, mass, reach = R.attention(**c)
+        _same_cache(g, c)
+        _check(out, want, mass, reach, dtype, 2064, d)
+        two = int4_hip.paged_attention8(**dict(g, **before))
+        assert torch.equal(torch.nan_to_num(out), torch.nan_to_num(two))
+        _same_cache(before, c)
+        live = (c["lengths"] >= 0).int()
+        for n in ("lengths", "positions"):
+            c[n] = c[n] + live
+            g[n] = c[n].to(DEV)
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+def test_one_token_of_long_rows_and_windows(kind):
+    for lens, window in (([9000, 50], None), ([5000, 4999, 3], 700), ([31, 32, 33, 63, 64, 65, 95, 96], 20)):
+        c = R.case(lens, [1] * len(lens), 8, 2, 64, 64, 32, kind, torch.float16, seed=len(lens), window=window, sinks=5)
+        g, out = _run(c, torch.float16, longest=1)
+        assert torch.equal(out, int4_hip.paged_attention8(**g, longest=1))
+
+
+def test_more_tokens_than_the_longest():
+    """A row that has more than it may is refused, its cache left alone; no other is."""
+    for longest in (1, 2):
+        c = R.case([20, 33, 5], [1, 3, 1], 4, 2, 64, 16, 8, torch.int8, torch.float16, seed=3)
+        g = _to(c)
+        out = int4_hip.paged_attention8(**g, longest=longest)
+        c["lengths"][1] = 1 << 20  # past the table: refused by the reference
+        want, mass, reach = R.attention(**c)
+        _check(out, want, mass, reach, torch.float16, 64, 64)
+        assert out[1:4].isnan().all() and not out[[0, 4]].isnan().any()
+        _same_cache(g, c)
+
+
 def test_pages_that_nobody_sees_may_be_gone():
     """Behind the window a table's entries are not read: a program gives those pages back."""
     c = R.case([700, 300], [2, 1], 4, 2, 64, 16, 16, torch.int8, torch.bfloat16, seed=5, window=100, sinks=20)
@@ -338,11 +393,12 @@ def test_tokens_of_nan_reach_those_that_see_them():
     c["k_scale"][int(c["table"][2, 1]), 0, 0] = NAN                              # slots 16..23: by none
     c["v_pages"].view(torch.uint8)[int(c["table"][3, 0]), 1, 1, 60] = 0x7F       # a sink
     g, out = _run(c, torch.float16)
-    nan = out.view(10, 4, 64).isnan().all(-1).cpu()
-    assert nan[0].tolist() == [True, True, False, False] and not nan[1:3].any()
-    assert nan[3:6, 2:].all(-1).tolist() == [True, True, False] and not nan[6:9].any()
-    assert nan[9].tolist() == [False, False, True, True]
-    assert torch.equal(out.isnan(), out.view(10, 4, 64).isnan().any(-1).repeat_interleave(64, -1).view(10, 256))
+    nan = out.view(10, 4, 64).isnan().cpu()
+    every, some = nan.all(-1), nan.any(-1)
+    assert every[0].tolist() == [True, True, False, False] and not some[1:3].any()  # of a key: all elements
+    assert some[3:6, 2:].all(-1).tolist() == [True, True, False] and not some[6:9].any()
+    assert (nan[3:5, 2:].nonzero()[:, 2] == 5).all() and not some[3:6, :2].any()     # of a value: its own
+    assert some[9].tolist() == [False, False, True, True] and (nan[9].nonzero()[:, 1] == 60).all()
 
 
 def test_pages_outside_the_pool_and_rows_past_the_table():
@@ -419,10 +475,10 @@ def test_captured_calls_are_replayed(kind):
     start = {n: g[n].clone() for n in CACHE}
     graphs, outs = [], []
     stream = torch.cuda.Stream()
-    for x in (g, h):
+    for x, longest in ((g, 1), (h, None)):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
-            outs.append(int4_hip.paged_attention8(**x))
+            outs.append(int4_hip.paged_attention8(**x, longest=longest))
         graphs.append(graph)
     for n in CACHE:
         g[n].copy_(start[n])
