@@ -46,6 +46,12 @@ struct Api {
   decltype(&w4_paged_evict) paged_evict;
   decltype(&w4_token_logprobs_workspace_bytes) token_logprobs_workspace_bytes;
   decltype(&w4_token_logprobs) token_logprobs;
+  decltype(&w4_paged8_append) paged8_append;
+  decltype(&w4_paged8_read) paged8_read;
+  decltype(&w4_paged8_attention_workspace_bytes) paged8_attention_workspace_bytes;
+  decltype(&w4_paged8_attention) paged8_attention;
+  decltype(&w4_verify_drafts_workspace_bytes) verify_drafts_workspace_bytes;
+  decltype(&w4_verify_drafts) verify_drafts;
 };
 Api api{};
 PyObject* py_workspace = nullptr;  // (device index, stream, bytes) -> (address, bytes)
@@ -577,6 +583,187 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The 8-bit cache of plain, dense tensors (k_pages, v_pages, k_scale, v_scale, table); false: not plain.
+bool cache8_of(PyObject* const* o, w4_paged8_cache* c) {
+  const at::Tensor* t[5];
+  for (int i = 0; i < 5; ++i) {
+    t[i] = plain(o[i]);
+    if (!t[i] || t[i]->device() != t[0]->device() || !t[i]->is_contiguous() || tracked(t[i])) return false;
+  }
+  const at::Tensor &k = *t[0], &ks = *t[2], &table = *t[4];
+  const at::ScalarType type = k.scalar_type();
+  if ((type != at::kChar && type != at::kFloat8_e4m3fn) || k.dim() != 4 || t[1]->scalar_type() != type ||
+      t[1]->sizes() != k.sizes() || ks.scalar_type() != at::kFloat || t[3]->scalar_type() != at::kFloat ||
+      ks.dim() != 3 || t[3]->sizes() != ks.sizes() || ks.size(0) != k.size(0) || ks.size(1) != k.size(1) ||
+      ks.size(2) < 1 || table.scalar_type() != at::kInt || table.dim() != 2 || table.size(1) < 1)
+    return false;
+  const int64_t S = k.size(2), d = k.size(3), block = S / ks.size(2);
+  if ((d != 64 && d != 128) || S < 8 || S > 1024 || (S & (S - 1)) != 0 || block * ks.size(2) != S || block < 8 ||
+      block > 64 || (block & (block - 1)) != 0)
+    return false;
+  *c = w4_paged8_cache{k.mutable_data_ptr(),
+                       t[1]->mutable_data_ptr(),
+                       static_cast<float*>(ks.mutable_data_ptr()),
+                       static_cast<float*>(t[3]->mutable_data_ptr()),
+                       ints(&table),
+                       k.size(0),
+                       k.size(1),
+                       S,
+                       d,
+                       block,
+                       table.size(0),
+                       table.size(1),
+                       type == at::kChar ? W4_CODE_INT8 : W4_CODE_E4M3,
+                       0};
+  return current(k.device());
+}
+
+// The operands of new tokens (k, v, cos, sin) and (lengths, offsets, positions); false: not plain, or not fitting.
+bool new_fit(const at::Tensor* const kv[4], const at::Tensor* const at3[3], const w4_paged8_cache& c, c10::Device dev) {
+  const at::Tensor* k = kv[0];
+  if (!k || k->dim() != 2 || act_code(k->scalar_type()) < 0 || k->device() != dev) return false;
+  const int64_t T = k->size(0), width = c.kv_heads * c.head_dim;
+  return rows_fit(k, T, width, *k) && rows_fit(kv[1], T, width, *k) && angles_fit(kv[2], kv[3], c.head_dim, dev) &&
+         index_fit(at3[0], c.rows, dev) && index_fit(at3[1], c.rows + 1, dev) && index_fit(at3[2], T, dev);
+}
+
+// (k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, lengths, offsets, positions) -> True
+PyObject* paged_append8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  w4_paged8_cache c;
+  if (n != 12 || !api.paged8_append || !quiet() || !cache8_of(args + 4, &c)) Py_RETURN_NONE;
+  const c10::Device dev = THPVariable_Unpack(args[4]).device();
+  const at::Tensor* const kv[4] = {plain(args[0]), plain(args[1]), plain(args[2]), plain(args[3])};
+  const at::Tensor* const at3[3] = {plain(args[9]), plain(args[10]), plain(args[11])};
+  if (!new_fit(kv, at3, c, dev)) Py_RETURN_NONE;
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.paged8_append(&c, act_code(kv[0]->scalar_type()), kv[0]->const_data_ptr(), kv[1]->const_data_ptr(),
+                         kv[0]->stride(0), kv[1]->stride(0), kv[0]->size(0), ints(at3[0]), ints(at3[1]), ints(at3[2]),
+                         floats(kv[2]), floats(kv[3]), kv[2]->size(0), stream);
+  Py_END_ALLOW_THREADS
+  if (!check(rc, "w4_paged8_append")) return nullptr;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (k_pages, v_pages, k_scale, v_scale, table, starts, offsets, tokens, dtype) -> (k, v)
+PyObject* paged_read8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  w4_paged8_cache c;
+  if (n != 9 || !api.paged8_read || !quiet() || !THPDtype_Check(args[8]) || !cache8_of(args, &c)) Py_RETURN_NONE;
+  const c10::Device dev = THPVariable_Unpack(args[0]).device();
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(args[8])->scalar_type;
+  const int dt = type == at::kFloat ? W4_DTYPE_FP32 : act_code(type);
+  const int64_t T = count_arg(args[7]);
+  const at::Tensor *starts = plain(args[5]), *offsets = plain(args[6]);
+  if (dt < 0 || T < 0 || T > (1 << 24) || !index_fit(starts, c.rows, dev) || !index_fit(offsets, c.rows + 1, dev))
+    Py_RETURN_NONE;
+  at::Tensor k = empty({T, c.kv_heads * c.head_dim}, type, dev), v = empty({T, c.kv_heads * c.head_dim}, type, dev);
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.paged8_read(&c, dt, ints(starts), ints(offsets), T, k.mutable_data_ptr(), v.mutable_data_ptr(), stream);
+  Py_END_ALLOW_THREADS
+  if (!check(rc, "w4_paged8_read")) return nullptr;
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, lengths, offsets, positions, longest or None,
+// window or None, sinks) -> out
+PyObject* paged_attention8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  w4_paged8_cache c;
+  if (n != 16 || !api.paged8_attention || !quiet() || !cache8_of(args + 5, &c)) Py_RETURN_NONE;
+  const c10::Device dev = THPVariable_Unpack(args[5]).device();
+  const at::Tensor* q = plain(args[0]);
+  const at::Tensor* const kv[4] = {plain(args[1]), plain(args[2]), plain(args[3]), plain(args[4])};
+  const at::Tensor* const at3[3] = {plain(args[10]), plain(args[11]), plain(args[12])};
+  const int64_t longest = args[13] == Py_None ? 0 : count_arg(args[13]);
+  const int64_t window = args[14] == Py_None ? 0 : count_arg(args[14]), sinks = count_arg(args[15]);
+  if (!q || q->dim() != 2 || longest < 0 || sinks < 0 || window < (args[14] == Py_None ? 0 : 1) || !new_fit(kv, at3, c, dev))
+    Py_RETURN_NONE;
+  const at::Tensor& k = *kv[0];
+  const int64_t T = k.size(0), width = c.kv_heads * c.head_dim;
+  if (T < 1 || T > (1 << 24) || q->size(1) < 1 || q->size(1) % width != 0 || !rows_fit(q, T, q->size(1), k))
+    Py_RETURN_NONE;
+  const int64_t heads = q->size(1) / c.head_dim;
+  at::Tensor out = empty({T, q->size(1)}, k.scalar_type(), dev);
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  void* ws;
+  size_t ws_bytes;
+  if (!workspace(dev, stream, api.paged8_attention_workspace_bytes(c.rows, T, heads, c.kv_heads, c.head_dim), &ws, &ws_bytes))
+    return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.paged8_attention(&c, act_code(k.scalar_type()), q->const_data_ptr(), k.const_data_ptr(),
+                            kv[1]->const_data_ptr(), q->stride(0), k.stride(0), kv[1]->stride(0), heads, T, longest,
+                            window, sinks, ints(at3[0]), ints(at3[1]), ints(at3[2]), floats(kv[2]), floats(kv[3]),
+                            kv[2]->size(0), out.mutable_data_ptr(), ws, ws_bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (!check(rc, "w4_paged8_attention")) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// (target, draft or None, tokens, accept, sample, counts or None) -> (accepted, token)
+PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !api.verify_drafts || !quiet()) Py_RETURN_NONE;
+  const at::Tensor* p = plain(args[0]);
+  if (!p || p->dim() != 3 || tracked(p)) Py_RETURN_NONE;
+  const int dt = p->scalar_type() == at::kFloat ? W4_DTYPE_FP32 : act_code(p->scalar_type());
+  const int64_t B = p->size(0), K = p->size(1) - 1, V = p->size(2);
+  const c10::Device dev = p->device();
+  if (dt < 0 || B < 1 || K < 0 || K > 64 || V < 1 || p->stride(2) != 1 || !current(dev)) Py_RETURN_NONE;
+  const at::Tensor* d = args[1] == Py_None ? nullptr : plain(args[1]);
+  if (args[1] != Py_None && (!d || d->dim() != 3 || d->scalar_type() != p->scalar_type() || d->size(0) != B ||
+                             d->size(1) != K || d->size(2) != V || d->device() != dev || d->stride(2) != 1 || tracked(d)))
+    Py_RETURN_NONE;
+  const at::Tensor *x = plain(args[2]), *u = plain(args[3]), *r = plain(args[4]);
+  const at::Tensor* counts = args[5] == Py_None ? nullptr : plain(args[5]);
+  auto grid = [&](const at::Tensor* t, at::ScalarType type) {
+    return t && t->scalar_type() == type && t->dim() == 2 && t->size(0) == B && t->size(1) == K && t->device() == dev &&
+           t->is_contiguous() && !tracked(t);
+  };
+  if (!grid(x, at::kLong) || !grid(u, at::kFloat) || !r || r->scalar_type() != at::kFloat || r->dim() != 1 ||
+      r->size(0) != B || r->device() != dev || !r->is_contiguous() || tracked(r) ||
+      (args[5] != Py_None && !index_fit(counts, B, dev)))
+    Py_RETURN_NONE;
+  at::Tensor accepted = empty({B}, at::kLong, dev), token = empty({B}, at::kLong, dev);
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  void* ws;
+  size_t ws_bytes;
+  if (!workspace(dev, stream, api.verify_drafts_workspace_bytes(B, V), &ws, &ws_bytes)) return nullptr;
+  if (K == 0) d = nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.verify_drafts(p->const_data_ptr(), d ? d->const_data_ptr() : nullptr, dt, B, K, V, p->stride(0), p->stride(1),
+                         d ? d->stride(0) : 0, d ? d->stride(1) : 0, static_cast<const int64_t*>(x->const_data_ptr()),
+                         counts ? ints(counts) : nullptr, floats(u), floats(r),
+                         static_cast<int64_t*>(accepted.mutable_data_ptr()),
+                         static_cast<int64_t*>(token.mutable_data_ptr()), ws, ws_bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (!check(rc, "w4_verify_drafts")) return nullptr;
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(accepted)), THPVariable_Wrap(std::move(token)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (addresses of the 8-bit cache's and the verification's C-ABI functions in Api's order)
+PyObject* init_paged8(PyObject*, PyObject* args) {
+  unsigned long long p[6];
+  if (!PyArg_ParseTuple(args, "(KKKKKK)", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5])) return nullptr;
+  api.paged8_append = reinterpret_cast<decltype(api.paged8_append)>(p[0]);
+  api.paged8_read = reinterpret_cast<decltype(api.paged8_read)>(p[1]);
+  api.paged8_attention_workspace_bytes = reinterpret_cast<decltype(api.paged8_attention_workspace_bytes)>(p[2]);
+  api.paged8_attention = reinterpret_cast<decltype(api.paged8_attention)>(p[3]);
+  api.verify_drafts_workspace_bytes = reinterpret_cast<decltype(api.verify_drafts_workspace_bytes)>(p[4]);
+  api.verify_drafts = reinterpret_cast<decltype(api.verify_drafts)>(p[5]);
+  Py_RETURN_NONE;
+}
+
 // (addresses of the paged cache's and the log probabilities' C-ABI functions in Api's order)
 PyObject* init_paged(PyObject*, PyObject* args) {
   unsigned long long p[7];
@@ -619,6 +806,11 @@ PyMethodDef methods[] = {{"init", init, METH_VARARGS, nullptr},
                          W4_FAST(paged_attention),
                          W4_FAST(paged_evict),
                          W4_FAST(token_logprobs),
+                         {"init_paged8", init_paged8, METH_VARARGS, nullptr},
+                         W4_FAST(paged_append8),
+                         W4_FAST(paged_read8),
+                         W4_FAST(paged_attention8),
+                         W4_FAST(verify_drafts),
                          W4_FAST(matmul),
                          W4_FAST(matmul_grouped),
                          W4_FAST(quantize),

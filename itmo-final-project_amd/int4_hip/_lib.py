@@ -184,6 +184,9 @@ def _load_ext(lib, workspace=None):
              "w4_paged_evict_scratch_words", "w4_paged_evict", "w4_token_logprobs_workspace_bytes",
              "w4_token_logprobs")
     _int4_torch.init_paged(tuple(ctypes.cast(getattr(lib, n), _c_vp).value for n in names))
+    names = ("w4_paged8_append", "w4_paged8_read", "w4_paged8_attention_workspace_bytes", "w4_paged8_attention",
+             "w4_verify_drafts_workspace_bytes", "w4_verify_drafts")
+    _int4_torch.init_paged8(tuple(ctypes.cast(getattr(lib, n), _c_vp).value for n in names))
     return _int4_torch
 
 

@@ -79,6 +79,9 @@ def paged_append8(k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, len
     Idle rows, rows whose slots pass the table, tokens of no row and pages outside the pool
     are left out; a position outside the tables makes a key of NaN.
     """
+    if _lib.ext is not None and _lib.ext.paged_append8(k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, lengths,
+                                                       offsets, positions):
+        return  # plain operands: the same call without Python's share of its cost
     _no_grad(k, v, cos, sin, k_pages, v_pages, k_scale, v_scale)
     c = _cache(k_pages, v_pages, k_scale, v_scale, table)
     dev = k_pages.device
@@ -100,6 +103,10 @@ def paged_read8(k_pages, v_pages, k_scale, v_scale, table, starts, offsets, toke
     Tokens of no row and of rows with ``starts[b] < 0`` are 0; slots past the table or on a
     page outside the pool are NaN.
     """
+    if _lib.ext is not None:
+        kv = _lib.ext.paged_read8(k_pages, v_pages, k_scale, v_scale, table, starts, offsets, tokens, dtype)
+        if kv is not None:
+            return kv
     _no_grad(k_pages, v_pages, k_scale, v_scale)
     c = _cache(k_pages, v_pages, k_scale, v_scale, table)
     dev = k_pages.device
@@ -124,12 +131,19 @@ def paged_attention8(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, tabl
     by ``paged_append8``; then the token of slot i attends in fp32 to slots 0..i or, with
     ``window``, to the last ``window`` of them and the first ``sinks``.  ``longest`` is
     the most new tokens that a row may have, where the program knows it: of a decode step, 1,
-    for which one launch writes and attends.  ``lengths`` is left as it is (all layers of a model share it).
+    for which one launch writes and attends.  ``lengths`` is left as it is (all layers of a
+    model share it).
 
     Idle rows and tokens of no row come back 0.  NaN come back: rows with more
-    than ``longest`` tokens or whose slots pass the table (nothing of them is written); tokens that see a page outside the pool or a block of NaN, or whose position is
-    outside the tables.
+    than ``longest`` tokens or whose slots pass the table (nothing of them is written);
+    tokens that see a page outside the pool or a block of NaN, or whose position is outside
+    the tables.
     """
+    if _lib.ext is not None:
+        out = _lib.ext.paged_attention8(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, lengths, offsets,
+                                        positions, longest, window, sinks)
+        if out is not None:
+            return out
     _no_grad(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale)
     c = _cache(k_pages, v_pages, k_scale, v_scale, table)
     dev, T = k_pages.device, q.shape[0]

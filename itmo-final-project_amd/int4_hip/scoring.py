@@ -92,6 +92,10 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     sum is 0, infinite or NaN have no token: -1.  Products, differences and sums are taken in
     64 bits.  Launches on the current stream; no part in autograd.
     """
+    if _lib.ext is not None:
+        r = _lib.ext.verify_drafts(target, draft, tokens, accept, sample, counts)
+        if r is not None:
+            return Verified(*r)
     assert target.dtype in DTYPES and target.dim() == 3 and target.is_cuda, (target.dtype, target.shape)
     assert underived(target, draft, accept, sample), \
         "verify_drafts has no derivatives: call it under torch.no_grad(), on probabilities without tangents"
