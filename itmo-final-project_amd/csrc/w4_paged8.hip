@@ -186,10 +186,30 @@ __device__ __forceinline__ bool find_block(const Append8Args& a, int item, int* 
   return false;
 }
 
+// The code of x / s by its quotient y in 32 bits, off by less than `off`; false where another could be meant.
+template <int CT>
+__device__ __forceinline__ bool quick_code(float y, float off, uint32_t* code) {
+  if constexpr (CT == W4_CODE_INT8) {
+    const float n = __builtin_rintf(y);
+    *code = (uint32_t)(int)fminf(fmaxf(n, -127.f), 127.f) & 0xFFu;
+    return !(__builtin_fabsf(__builtin_fabsf(y - n) - 0.5f) < off);
+  } else {
+    const uint32_t b = __builtin_bit_cast(uint32_t, y);
+    *code = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fminf(fmaxf(y, -448.f), 448.f), 0.f, 0, false) & 0xFFu;
+    // the middle between the two codes around it: the first bit that is rounded away, alone
+    const float middle = __builtin_bit_cast(float, (b & 0xFFF00000u) | 0x00080000u), size = __builtin_fabsf(y);
+    return y == 0.f || (size >= 0.015625f && !(__builtin_fabsf(y - middle) < off));  // (else: subnormal codes)
+  }
+}
+
 // One workgroup has one block of one row, for as many heads as its 256 threads hold: block * D / 16 threads a head
-// (twice over where they are 512), eight rotary pairs of a key and the sixteen values beside them each.  The rotation
-// and the quotients are taken in 64 bits, where the products of 16-bit numbers and 24-bit angles are exact, so a code
-// is that of the rotated key and not of its rounding.
+// (twice over where they are 512), eight rotary pairs of a key and the sixteen values beside them each.
+//
+// A code is that of the rotated key in 64 bits, where the products of 16-bit numbers and 24-bit angles are exact, and
+// not of a rounding of it.  Nearly all are found in 32 bits: a rotation's error there is under 2^-22 of the block's
+// largest magnitude (its pair is no longer than 1.42 of that, each product and the sum rounded by 2^-24), and a
+// quotient that lies further from the middle between two codes than that is rounded the same way.  The others, and the
+// keys that may be the largest, are taken in 64 bits.
 //
 // A block's scale is its largest magnitude over the largest code.  Tokens that come into a block that holds some
 // already let its scale grow by a power of two, if they need it: e4m3 codes then stay as they are (but for the
@@ -198,7 +218,9 @@ template <int DT, int CT, int D>
 __global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a) {
   constexpr int CH = D / 16;  // threads per token
   constexpr int MAXIT = 64 * CH / kP8Threads < 1 ? 1 : 64 * CH / kP8Threads;
-  __shared__ unsigned long long top_s[2][kP8Threads / 32];
+  constexpr int UNITS = kP8Threads / 32;
+  __shared__ unsigned near_s[2][UNITS];
+  __shared__ unsigned long long top_s[UNITS];
   const int tid = threadIdx.x;
   int row, jb;
   RowSpan sp;
@@ -210,62 +232,70 @@ __global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a
   const int h = min((int)blockIdx.y * units + unit, a.c.nkv - 1);
   const int page = a.c.page(row, slot0);
   if (page < 0) return;  // (uniform)
-  if (tid < 2 * (kP8Threads / 32)) (&top_s[0][0])[tid] = 0;
+  if (tid < UNITS) near_s[0][tid] = near_s[1][tid] = 0, top_s[tid] = 0;
   __syncthreads();
 
   const int d = (r0 % CH) * 8;
-  u32x4 raw[MAXIT][4];
+  float x[MAXIT][4][8];  // the key's pairs, rotated, and the values beside them
   bool isnew[MAXIT];
-  int pos[MAXIT];
-  unsigned long long top[2] = {0, 0};
-  auto values = [&](int it, double k1[8], double k2[8], float v1[8], float v2[8]) __attribute__((always_inline)) {
-    float x1[8], x2[8];
-    unpack8<DT>(raw[it][0], x1);
-    unpack8<DT>(raw[it][1], x2);
-    unpack8<DT>(raw[it][2], v1);
-    unpack8<DT>(raw[it][3], v2);
-    const bool there = (uint64_t)(int64_t)pos[it] < (uint64_t)a.angles;
-    const float *cp = a.cos + (there ? (int64_t)pos[it] * (D / 2) + d : 0);
-    const float *sp = a.sin + (there ? (int64_t)pos[it] * (D / 2) + d : 0);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double c = there ? (double)cp[j] : (double)__builtin_nanf(""), s = (double)sp[j];
-      k1[j] = (double)x1[j] * c - (double)x2[j] * s;
-      k2[j] = (double)x2[j] * c + (double)x1[j] * s;
-    }
-  };
+  const uint16_t *kp[MAXIT], *vp[MAXIT];
+  int64_t angle[MAXIT];  // of the position's row in the tables; -1: it has none
+  unsigned near[2] = {0, 0};
 #pragma unroll
   for (int it = 0; it < MAXIT; ++it) {
-    isnew[it] = false;
-    if (it >= its || !live) continue;
     const int at = slot0 + (r0 + it * kP8Threads) / CH - sp.len;
-    isnew[it] = at >= 0 && at < sp.n;
+    isnew[it] = it < its && live && at >= 0 && at < sp.n;
     if (!isnew[it]) continue;
     const int64_t t = sp.o0 + at;
-    const uint16_t* kp = a.k + t * a.stride_k + h * D + d;
-    const uint16_t* vp = a.v + t * a.stride_v + h * D + d;
-    raw[it][0] = *reinterpret_cast<const u32x4*>(kp);
-    raw[it][1] = *reinterpret_cast<const u32x4*>(kp + D / 2);
-    raw[it][2] = *reinterpret_cast<const u32x4*>(vp);
-    raw[it][3] = *reinterpret_cast<const u32x4*>(vp + D / 2);
-    pos[it] = a.positions[t];
+    const int pos = a.positions[t];
+    kp[it] = a.k + t * a.stride_k + h * D + d;
+    vp[it] = a.v + t * a.stride_v + h * D + d;
+    unpack8<DT>(*reinterpret_cast<const u32x4*>(kp[it]), x[it][0]);
+    unpack8<DT>(*reinterpret_cast<const u32x4*>(kp[it] + D / 2), x[it][1]);
+    unpack8<DT>(*reinterpret_cast<const u32x4*>(vp[it]), x[it][2]);
+    unpack8<DT>(*reinterpret_cast<const u32x4*>(vp[it] + D / 2), x[it][3]);
+    angle[it] = (uint64_t)(int64_t)pos < (uint64_t)a.angles ? (int64_t)pos * (D / 2) + d : -1;
+    const float* const cosp = a.cos + max(angle[it], (int64_t)0);
+    const float* const sinp = a.sin + max(angle[it], (int64_t)0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float c = angle[it] < 0 ? __builtin_nanf("") : cosp[j], s = sinp[j], x1 = x[it][0][j], x2 = x[it][1][j];
+      x[it][0][j] = x1 * c - x2 * s;
+      x[it][1][j] = x2 * c + x1 * s;
+    }
+    // (as integers their order is that of the magnitudes, a NaN above an infinity above all numbers)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        near[q >> 1] = max(near[q >> 1], __builtin_bit_cast(uint32_t, x[it][q][j]) & 0x7FFFFFFFu);
   }
+  // Element j of a thread's sixteen of a key, in 64 bits.
+  auto key = [&](int it, int j) {
+    const int i = j & 7;
+    const double x1 = act_bits_to_float(kp[it][i], DT), x2 = act_bits_to_float(kp[it][i + D / 2], DT);
+    if (angle[it] < 0) return (double)__builtin_nanf("");
+    const double c = a.cos[angle[it] + i], s = a.sin[angle[it] + i];
+    return j < 8 ? x1 * c - x2 * s : x2 * c + x1 * s;
+  };
+  if (near[0]) atomicMax(&near_s[0][unit], near[0]);
+  if (near[1]) atomicMax(&near_s[1][unit], near[1]);
+  __syncthreads();
+  const float reach = __builtin_bit_cast(float, near_s[0][unit]), least = reach * (1.f - 0x1p-20f);
+  const bool wild = !(reach < __builtin_inff());  // past 32 bits, or no number: all in 64
+  unsigned long long top = 0;
 #pragma unroll
   for (int it = 0; it < MAXIT; ++it) {
     if (!isnew[it]) continue;
-    double k1[8], k2[8];
-    float v1[8], v2[8];
-    values(it, k1, k2, v1, v2);
-    // (as integers their order is that of the magnitudes, a NaN above an infinity above all numbers)
-    auto most = [&](int i, double x) {
-      const unsigned long long u = __builtin_bit_cast(unsigned long long, __builtin_fabs(x));
-      top[i] = u > top[i] ? u : top[i];
-    };
+    unsigned some = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most(0, k1[j]), most(0, k2[j]), most(1, (double)v1[j]), most(1, (double)v2[j]);
+    for (int j = 0; j < 16; ++j) some |= wild || __builtin_fabsf(x[it][j >> 3][j & 7]) >= least ? 1u << j : 0u;
+    for (; some; some &= some - 1) {
+      const unsigned long long u = __builtin_bit_cast(unsigned long long, __builtin_fabs(key(it, __builtin_ctz(some))));
+      top = u > top ? u : top;
+    }
   }
-  if (top[0]) atomicMax(&top_s[0][unit], top[0]);
-  if (top[1]) atomicMax(&top_s[1][unit], top[1]);
+  if (top) atomicMax(&top_s[unit], top);
   __syncthreads();
 
   const int64_t blk = a.c.block(page, h, slot0);
@@ -274,8 +304,9 @@ __global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a
   int grow[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
+    const double most = i ? (double)__builtin_bit_cast(float, near_s[1][unit]) : __builtin_bit_cast(double, top_s[unit]);
     const double old = fresh ? 0.0 : (double)(i ? a.c.v_scale : a.c.k_scale)[blk];
-    scale[i] = block_scale<CT>(__builtin_bit_cast(double, top_s[i][unit]), old, &grow[i]);
+    scale[i] = block_scale<CT>(most, old, &grow[i]);
     inv[i] = scale[i] > 0.0 ? 1.0 / scale[i] : 0.0;  // (also of NaN: its codes are 0)
   }
   __syncthreads();  // all have read the scales that are there
@@ -290,29 +321,39 @@ __global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a
     const int slot = slot0 + (r0 + it * kP8Threads) / CH;
     const int64_t at = a.c.token(page, h, slot) * D + d;
     if (isnew[it]) {
-      double k1[8], k2[8];
-      float v1[8], v2[8];
-      values(it, k1, k2, v1, v2);
-      u32x2 w[4];
-      auto put = [&](int i, u32x2& o, auto& x) __attribute__((always_inline)) {
-        o = u32x2{0u, 0u};
-        if (inv[i] > 0.0)
+      // (the quotient's own roundings add 2^-22 of it)
+      constexpr float off = Code<CT>::most * 0x1p-20f;
+      unsigned left[2] = {0, 0};
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j >> 2] |= encode<CT>((double)x[j], scale[i], inv[i]) << (8 * (j & 3));
-      };
-      put(0, w[0], k1), put(0, w[1], k2), put(1, w[2], v1), put(1, w[3], v2);
-      *reinterpret_cast<u32x2*>(a.c.k + at) = w[0];
-      *reinterpret_cast<u32x2*>(a.c.k + at + D / 2) = w[1];
-      *reinterpret_cast<u32x2*>(a.c.v + at) = w[2];
-      *reinterpret_cast<u32x2*>(a.c.v + at + D / 2) = w[3];
+      for (int q = 0; q < 4; ++q) {
+        const int i = q >> 1;
+        u32x2 w = {0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t n;
+          if (!quick_code<CT>(x[it][q][j] * (float)inv[i], off, &n)) left[i] |= 1u << ((q & 1) * 8 + j);
+          w[j >> 2] |= n << (8 * (j & 3));
+        }
+        if (!(inv[i] > 0.0)) w = u32x2{0u, 0u};
+        *reinterpret_cast<u32x2*>((i ? a.c.v : a.c.k) + at + (q & 1) * (D / 2)) = w;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        unsigned some = !(inv[i] > 0.0) ? 0u : i == 0 && wild ? 0xFFFFu : left[i];
+        for (; some; some &= some - 1) {
+          const int j = __builtin_ctz(some), e = (j & 7) + (j >> 3) * (D / 2);
+          const double y = i ? (double)act_bits_to_float(vp[it][e], DT) : key(it, j);
+          (i ? a.c.v : a.c.k)[at + e] = (uint8_t)encode<CT>(y, scale[i], inv[i]);
+        }
+      }
     } else if (slot < sp.len) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (grow[i] > 0) {
-          u32x2* const p = reinterpret_cast<u32x2*>((i ? a.c.v : a.c.k) + at);
-          u32x2* const q = reinterpret_cast<u32x2*>((i ? a.c.v : a.c.k) + at + D / 2);
-          *p = shrink8<CT>(*p, grow[i]);
-          *q = shrink8<CT>(*q, grow[i]);
+          for (int e = 0; e < 2; ++e) {
+            u32x2* const p = reinterpret_cast<u32x2*>((i ? a.c.v : a.c.k) + at + e * (D / 2));
+            *p = shrink8<CT>(*p, grow[i]);
+          }
         }
     }
   }

@@ -33,25 +33,55 @@ __device__ __forceinline__ double prob(const void* p, int64_t i) {
 
 __device__ __forceinline__ double lane_get(double v, int lane) { return __shfl(v, lane); }
 
-// Inclusive sum over the lanes, each lane's in their order.
+// Inclusive sum over the lanes (as wave_scan of integers: a lane with none before it adds 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_scan64(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double o = __shfl_up(v, d);
-    v = lane >= d ? v + o : v;
-  }
+  v += dpp_or_zero<0x111, 0xF>(v);  // shifted right by 1, 2, 4, 8 in rows of 16
+  v += dpp_or_zero<0x112, 0xF>(v);
+  v += dpp_or_zero<0x114, 0xF>(v);
+  v += dpp_or_zero<0x118, 0xF>(v);
+  v += dpp_or_zero<0x142, 0xA>(v);  // rows 1, 3 take the last lane before them
+  v += dpp_or_zero<0x143, 0xC>(v);  // rows 2, 3 take lane 31
   return v;
 }
 
-// A row's parts of the vocabulary are a workgroup's each.  Every one of them decides on the drafts (a handful of
-// numbers) and sums its part's weights at the first position that is refused, or past the last; the last part to
-// arrive finds the part that the sample falls into and looks for it there.  The sums are of 64 bits, so that their
-// order, which is fixed, moves no token but one that the sample meets to 2^-50.
+// Eight probabilities in a row (rows need not start on 16 bytes: a vocabulary may be odd), as far as there are any.
+template <int DT>
+__device__ __forceinline__ void probs8(const void* p, int64_t i, int n, double out[8]) {
+  if (n >= 8) {
+    if constexpr (DT == W4_DTYPE_FP32) {
+      typedef f32x4 vec __attribute__((aligned(4)));
+      const float* const q = static_cast<const float*>(p) + i;
+      const f32x4 a = *reinterpret_cast<const vec*>(q), b = *reinterpret_cast<const vec*>(q + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = (double)a[e], out[e + 4] = (double)b[e];
+    } else {
+      typedef u32x4 vec __attribute__((aligned(2)));
+      float x[8];
+      unpack8<DT>(*reinterpret_cast<const vec*>(static_cast<const uint16_t*>(p) + i), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = (double)x[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = e < n ? prob<DT>(p, i + e) : 0.0;
+  }
+}
+
+// A row's parts of the vocabulary are a workgroup's each, eight tokens in a row a thread (more than once of vocabularies
+// past 131072).  Every one of them decides on the drafts (a handful of numbers) and sums its part's weights at the first
+// position that is refused, or past the last; the last part to arrive finds the part that the sample falls into and looks
+// for it there.  The sums are of 64 bits, so that their order, which is fixed, moves no token but one that the sample
+// meets to 2^-50.
 template <int DT>
 __global__ __launch_bounds__(kVerThreads) void verify_kernel(VerifyArgs a) {
   __shared__ double sum_s[2][kVerThreads / 64];
-  __shared__ double edge_s[2];
   __shared__ unsigned arrived_s;
   __shared__ int found_s;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -76,20 +106,31 @@ __global__ __launch_bounds__(kVerThreads) void verify_kernel(VerifyArgs a) {
   // the token that is no choice: the refused draft, where drafts have probability 1
   const int64_t out = r < n && !a.draft ? a.tokens[(int64_t)row * a.drafts + r] : -1;
   const bool minus = r < n && a.draft;
-  // (what is not a number stays one, so that the sum shows it)
-  auto weight = [&](int i, double* p) __attribute__((always_inline)) {
-    const double t = prob<DT>(a.target, tp + i);
-    *p = t < 0.0 ? 0.0 : t;
-    const double d = minus ? t - prob<DT>(a.draft, dp + i) : i == out ? t - 1.0 : t;
-    return d < 0.0 ? 0.0 : d;
-  };
   const int begin = part * a.run, end = min(begin + a.run, a.vocab);
+  // The weights of tokens i.. i + 7 below `to`: of what is left of the target, and the target's own.  (What is not a
+  // number stays one, so that the sum shows it.)
+  auto weights = [&](int i, int to, double w[8], double p[8]) __attribute__((always_inline)) {
+    double d[8];
+    probs8<DT>(a.target, tp + i, to - i, p);
+    if (minus) {
+      probs8<DT>(a.draft, dp + i, to - i, d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = i + e == out ? 1.0 : 0.0;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const double x = p[e] - d[e];
+      w[e] = x < 0.0 ? 0.0 : x;
+      p[e] = p[e] < 0.0 ? 0.0 : p[e];
+    }
+  };
   double s0 = 0.0, s1 = 0.0;
-#pragma unroll 4
-  for (int i = begin + tid; i < end; i += kVerThreads) {
-    double p;
-    s0 += weight(i, &p);
-    s1 += p;
+  for (int i = begin + tid * 8; i < end; i += kVerThreads * 8) {
+    double w[8], p[8];
+    weights(i, end, w, p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s0 += w[e], s1 += p[e];
   }
   s0 = lane_get(wave_scan64(s0), 63);
   s1 = lane_get(wave_scan64(s1), 63);
@@ -127,29 +168,39 @@ __global__ __launch_bounds__(kVerThreads) void verify_kernel(VerifyArgs a) {
   const int p = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
   const double before = p ? lane_get(upto, p - 1) : 0.0;
   if (tid == 0) found_s = a.vocab;
-  // That part once more, a run of consecutive tokens a thread: the sums up to each, then the token.
-  const int b = p * a.run, e = min(b + a.run, a.vocab), each = (a.run + kVerThreads - 1) / kVerThreads;
-  const int i0 = min(b + tid * each, e), i1 = min(i0 + each, e);
-  double s = 0.0;
-  for (int i = i0; i < i1; ++i) {
-    double t;
-    const double w = weight(i, &t);
-    s += rest ? w : t;
-  }
-  const double scan = wave_scan64(s);
-  if (lane == 63) sum_s[0][wv] = scan;
-  __syncthreads();
-  double from = before;
-  for (int w = 0; w < wv; ++w) from += sum_s[0][w];
-  const double lanes = __shfl_up(scan, 1);  // (of all lanes: one that does not take part gives nothing)
-  from += lane ? lanes : 0.0;
+  // That part once more, in runs of consecutive tokens: the sums up to each thread's eight, then the token.
+  const int b = p * a.run, e = min(b + a.run, a.vocab);
   int hit = a.vocab, last = -1;
-  for (int i = i0; i < i1; ++i) {
-    double t;
-    const double w = weight(i, &t), x = rest ? w : t;
-    from += x;
-    if (x > 0.0) last = i;
-    if (x > 0.0 && from > aim && hit == a.vocab) hit = i;
+  double from = before;
+  for (int i0 = b; i0 < e; i0 += kVerThreads * 8) {
+    const int i = i0 + tid * 8;
+    double w[8], t[8], s = 0.0;
+    weights(min(i, e), e, w, t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (!rest) w[k] = t[k];
+      s += w[k];
+    }
+    const double scan = wave_scan64(s);
+    if (i0 != b) __syncthreads();  // the sums before have been read
+    if (lane == 63) sum_s[0][wv] = scan;
+    __syncthreads();
+    double x = from;
+#pragma unroll
+    for (int k = 0; k < kVerThreads / 64; ++k) {
+      x += k < wv ? sum_s[0][k] : 0.0;
+      from += sum_s[0][k];
+    }
+    const double lanes = __shfl_up(scan, 1);  // (of all lanes: one that does not take part gives nothing)
+    x += lane ? lanes : 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      x += w[k];
+      if (w[k] > 0.0) {
+        last = i + k;
+        if (x > aim) hit = min(hit, i + k);
+      }
+    }
   }
   if (hit < a.vocab) atomicMin(&found_s, hit);
   __syncthreads();
@@ -176,16 +227,13 @@ struct VerifyPlan {
   int64_t slice;  // rows of a launch
 };
 
-// About four workgroups a CU, of 2048 tokens at least.
+// Parts of 2048 tokens, or of a multiple of that where there would be more of them than lanes.
 VerifyPlan verify_plan(int64_t rows, int64_t vocab) {
   VerifyPlan p;
   p.slice = W4_WORKSPACE_COUNTER_BYTES / 4;
   if (p.slice > rows) p.slice = rows;
-  int64_t parts = (4 * device_cu_count() + p.slice - 1) / p.slice;
-  const int64_t most = (vocab + 2047) / 2048;
-  if (parts > most) parts = most;
-  if (parts > w4::kVerMaxParts) parts = w4::kVerMaxParts;
-  p.run = (int)((vocab + parts - 1) / parts);
+  const int64_t once = 8 * w4::kVerThreads;
+  p.run = (int)(((vocab + w4::kVerMaxParts - 1) / w4::kVerMaxParts + once - 1) / once * once);
   p.parts = (int)((vocab + p.run - 1) / p.run);
   return p;
 }

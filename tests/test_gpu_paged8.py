@@ -532,3 +532,40 @@ def test_chunks_and_tokens_make_the_same_cache_as_its_parts_say():
         _check(out, want, mass, reach, torch.float16, 48, 64)
         _same_cache(g, c)
         at += n
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("dtype", BOTH, ids=ids)
+def test_codes_of_many_tokens(kind, dtype):
+    """Against the definition on the GPU in 64 bits: enough values that some lie next to every kind of border, of
+    magnitudes that reach the subnormal codes, pairs that nearly cancel, and what 32 bits cannot hold."""
+    T, nkv, d, S, block = 3000, 4, 128, 64, 32
+    c = _to(R.case([0], [T], nkv, nkv, d, S, block, kind, dtype, seed=23, shift=5))
+    g = torch.Generator(DEV).manual_seed(3)
+    for n in ("k", "v"):
+        x = torch.randn((T, nkv * d), device=DEV, generator=g) * torch.exp(4 * torch.randn((T, nkv * d), device=DEV, generator=g))
+        c[n] = x.clamp(-6e4, 6e4).to(dtype)
+    if dtype == torch.bfloat16:
+        c["k"][40] = 3e38
+    c["k"][100:132], c["v"][100:132] = 1.0, 0.75  # (equal magnitudes, rotated)
+    pos = c["positions"].long()
+    x = c["k"].double().view(T, nkv, d)
+    h, co, si = d // 2, c["cos"].double()[pos][:, None], c["sin"].double()[pos][:, None]
+    key = torch.cat((x[..., :h] * co - x[..., h:] * si, x[..., h:] * co + x[..., :h] * si), -1)
+    _append(c)
+    k, v = int4_hip.paged_read8(*(c[n] for n in CACHE), c["table"], c["lengths"], c["offsets"], T, torch.float32)
+    pages = c["table"][0].long()
+    grid = torch.tensor(R._TABLE[kind][0], device=DEV, dtype=torch.float64)
+    codes = torch.tensor(R._TABLE[kind][1], device=DEV)
+    for got, x, scales in ((k, key, c["k_scale"]), (v, c["v"].double().view(T, nkv, d), c["v_scale"])):
+        s = scales[pages].transpose(1, 2).flatten(0, 1)[:-(-T // block)]
+        a = torch.nn.functional.pad(x, (0, 0, 0, 0, 0, -T % block)).view(-1, block, nkv, d).abs().amax((1, 3))
+        most = torch.full_like(a, MOST[kind])
+        want = (a / most).float().clamp(min=R.TINY)
+        assert torch.equal(s, torch.where(a > 0, want, 0.0))
+        y = x / s.double().repeat_interleave(block, 0)[:T, :, None]
+        i = torch.searchsorted(grid, y.contiguous()).clamp(1, len(grid) - 1)
+        lo, hi = grid[i - 1], grid[i]
+        up = (hi - y < y - lo) | ((hi - y == y - lo) & (codes[i] % 2 == 0))
+        q = torch.where(up, hi, lo)
+        assert torch.equal(got.view(T, nkv, d), (q * s.double().repeat_interleave(block, 0)[:T, :, None]).float())
