@@ -93,18 +93,18 @@ __device__ __forceinline__ double decode(uint32_t c) {
   return c & 0x80 ? -y : y;
 }
 
-// Codes of a block whose scale has grown by 2^m.
+// Eight codes of a block whose scale has grown by 2^m.  (Seldom: a loop, to be small.)
 template <int CT>
 __device__ __forceinline__ u32x2 shrink8(u32x2 w, int m) {
   const double f = two_to(-min(m, 200));
-  u32x2 r = {0u, 0u};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t c = w[e >> 2] >> (8 * (e & 3)) & 0xFFu;
+  uint64_t from = __builtin_bit_cast(uint64_t, w), r = 0;
+#pragma unroll 1
+  for (int e = 0; e < 64; e += 8) {
+    const uint32_t c = (uint32_t)(from >> e) & 0xFFu;
     const uint32_t n = CT == W4_CODE_E4M3 && (c & 0x7F) == 0x7F ? c : encode<CT>(decode<CT>(c) * f, 1.0, 1.0);
-    r[e >> 2] |= n << (8 * (e & 3));
+    r |= (uint64_t)n << e;
   }
-  return r;
+  return __builtin_bit_cast(u32x2, r);
 }
 
 // The scale of a block whose new values reach the magnitude x (of the bits of a double: an infinity or NaN among them
@@ -159,7 +159,7 @@ struct Append8Args {
   int64_t stride_k, stride_v, angles;
   const int32_t *lengths, *offsets, *positions;
   const float *cos, *sin;  // [angles, D / 2]
-  int tokens, longest;
+  int tokens, longest, heads;  // heads of a workgroup
 };
 
 // Item -> a row and one of its blocks that get new tokens, counted over all rows.
@@ -186,65 +186,89 @@ __device__ __forceinline__ bool find_block(const Append8Args& a, int item, int* 
   return false;
 }
 
-// The code of x / s by its quotient y in 32 bits, off by less than `off`; false where another could be meant.
+// The codes of a number that 32 bits hold to 2^-24, by quotients in 32 bits that are a little larger and smaller, by
+// more than they may be off: in the lowest bytes of *c and of the result, which are equal but next to the middle of two.
 template <int CT>
-__device__ __forceinline__ bool quick_code(float y, float off, uint32_t* code) {
+__device__ __forceinline__ uint32_t two_codes(float x, float more, float less, uint32_t* c) {
   if constexpr (CT == W4_CODE_INT8) {
-    const float n = __builtin_rintf(y);
-    *code = (uint32_t)(int)fminf(fmaxf(n, -127.f), 127.f) & 0xFFu;
-    return !(__builtin_fabsf(__builtin_fabsf(y - n) - 0.5f) < off);
+    // a number this large has no bits below 1: its lowest eight are the rounded quotient's
+    *c = __builtin_bit_cast(uint32_t, __builtin_fmaf(x, more, 12582912.f));
+    return __builtin_bit_cast(uint32_t, __builtin_fmaf(x, less, 12582912.f));
   } else {
-    const uint32_t b = __builtin_bit_cast(uint32_t, y);
-    *code = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fminf(fmaxf(y, -448.f), 448.f), 0.f, 0, false) & 0xFFu;
-    // the middle between the two codes around it: the first bit that is rounded away, alone
-    const float middle = __builtin_bit_cast(float, (b & 0xFFF00000u) | 0x00080000u), size = __builtin_fabsf(y);
-    return y == 0.f || (size >= 0.015625f && !(__builtin_fabsf(y - middle) < off));  // (else: subnormal codes)
+    *c = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x * more, x * less, 0, false);
+    return *c >> 8;
   }
+}
+constexpr float kMore = 1.f + 0x1p-21f, kLess = 1.f - 0x1p-21f;
+// Eight codes; *odd is set where one could be another.
+template <int CT>
+__device__ __forceinline__ u32x2 quick_codes(const float x[8], float inv, uint32_t* odd) {
+  uint32_t c[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t other = two_codes<CT>(x[e], inv * kMore, inv * kLess, &c[e]);
+    *odd |= (c[e] ^ other) & 0xFFu;
+  }
+  auto four = [&](int e) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[e + 3], c[e + 2], 0x0C0C0400u),
+                                 __builtin_amdgcn_perm(c[e + 1], c[e], 0x0C0C0400u), 0x05040100u);
+  };
+  return u32x2{four(0), four(4)};
+}
+// Which of the eight.
+template <int CT>
+__device__ __forceinline__ unsigned odd_ones(const float x[8], float inv) {
+  unsigned some = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    uint32_t c;
+    const uint32_t other = two_codes<CT>(x[e], inv * kMore, inv * kLess, &c);
+    some |= (c ^ other) & 0xFFu ? 1u << e : 0u;
+  }
+  return some;
 }
 
 // One workgroup has one block of one row, for as many heads as its 256 threads hold: block * D / 16 threads a head
-// (twice over where they are 512), eight rotary pairs of a key and the sixteen values beside them each.
+// (ITS = 2: twice over, of 512), eight rotary pairs of a key and the sixteen values beside them each.
 //
-// A code is that of the rotated key in 64 bits, where the products of 16-bit numbers and 24-bit angles are exact, and
-// not of a rounding of it.  Nearly all are found in 32 bits: a rotation's error there is under 2^-22 of the block's
-// largest magnitude (its pair is no longer than 1.42 of that, each product and the sum rounded by 2^-24), and a
-// quotient that lies further from the middle between two codes than that is rounded the same way.  The others, and the
-// keys that may be the largest, are taken in 64 bits.
+// Keys are rotated in 64 bits, where the products of 16-bit numbers and 24-bit angles are exact, so a code is that of
+// the rotated key and not of a rounding of it.  The quotients are taken in 32 bits, which finds nearly all codes; a
+// thread with one that lies next to the middle between two codes takes its own again in 64.
 //
 // A block's scale is its largest magnitude over the largest code.  Tokens that come into a block that holds some
 // already let its scale grow by a power of two, if they need it: e4m3 codes then stay as they are (but for the
 // smallest), and int8 codes, each rounding at half the step of the next, are never off by more than one step in all.
-template <int DT, int CT, int D>
-__global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a) {
+template <int DT, int CT, int D, int ITS>
+__global__ __launch_bounds__(kP8Threads, ITS > 1 ? 3 : 5) void paged8_append_kernel(Append8Args a) {
   constexpr int CH = D / 16;  // threads per token
-  constexpr int MAXIT = 64 * CH / kP8Threads < 1 ? 1 : 64 * CH / kP8Threads;
   constexpr int UNITS = kP8Threads / 32;
-  __shared__ unsigned near_s[2][UNITS];
-  __shared__ unsigned long long top_s[UNITS];
+  __shared__ unsigned long long top_s[2][UNITS];
   const int tid = threadIdx.x;
   int row, jb;
   RowSpan sp;
-  if (!find_block(a, blockIdx.x, &row, &jb, &sp)) return;
+  const int groups = (a.c.nkv + a.heads - 1) / a.heads, go = blockIdx.x;
+  if (!find_block(a, go / groups, &row, &jb, &sp)) return;
   const int slot0 = jb << a.c.log2b, per = CH << a.c.log2b;
-  const int its = max(per / kP8Threads, 1), units = max(kP8Threads / per, 1);
-  const int unit = its > 1 ? 0 : tid / per, r0 = tid - unit * per;
-  const bool live = (int)blockIdx.y * units + unit < a.c.nkv;
-  const int h = min((int)blockIdx.y * units + unit, a.c.nkv - 1);
+  const int units = ITS > 1 ? 1 : kP8Threads / per, unit = ITS > 1 ? 0 : tid / per, r0 = tid - unit * per;
+  const bool live = go % groups * units + unit < a.c.nkv;
+  const int h = min(go % groups * units + unit, a.c.nkv - 1);
   const int page = a.c.page(row, slot0);
   if (page < 0) return;  // (uniform)
-  if (tid < UNITS) near_s[0][tid] = near_s[1][tid] = 0, top_s[tid] = 0;
+  if (tid < 2 * UNITS) (&top_s[0][0])[tid] = 0;
   __syncthreads();
 
   const int d = (r0 % CH) * 8;
-  float x[MAXIT][4][8];  // the key's pairs, rotated, and the values beside them
-  bool isnew[MAXIT];
-  const uint16_t *kp[MAXIT], *vp[MAXIT];
-  int64_t angle[MAXIT];  // of the position's row in the tables; -1: it has none
-  unsigned near[2] = {0, 0};
+  float x[ITS][4][8];  // the key's pairs, rotated, and the values beside them
+  bool isnew[ITS];
+  const uint16_t *kp[ITS], *vp[ITS];
+  int64_t angle[ITS];  // of the position's row in the tables; -1: it has none
+  // the largest magnitudes (as integers their order is that of the numbers, a NaN above an infinity above them all)
+  uint64_t top = 0;
+  uint32_t top_v = 0;
 #pragma unroll
-  for (int it = 0; it < MAXIT; ++it) {
+  for (int it = 0; it < ITS; ++it) {
     const int at = slot0 + (r0 + it * kP8Threads) / CH - sp.len;
-    isnew[it] = it < its && live && at >= 0 && at < sp.n;
+    isnew[it] = live && at >= 0 && at < sp.n;
     if (!isnew[it]) continue;
     const int64_t t = sp.o0 + at;
     const int pos = a.positions[t];
@@ -255,56 +279,56 @@ __global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a
     unpack8<DT>(*reinterpret_cast<const u32x4*>(vp[it]), x[it][2]);
     unpack8<DT>(*reinterpret_cast<const u32x4*>(vp[it] + D / 2), x[it][3]);
     angle[it] = (uint64_t)(int64_t)pos < (uint64_t)a.angles ? (int64_t)pos * (D / 2) + d : -1;
-    const float* const cosp = a.cos + max(angle[it], (int64_t)0);
-    const float* const sinp = a.sin + max(angle[it], (int64_t)0);
+    const f32x4* const cosp = reinterpret_cast<const f32x4*>(a.cos + max(angle[it], (int64_t)0));
+    const f32x4* const sinp = reinterpret_cast<const f32x4*>(a.sin + max(angle[it], (int64_t)0));
+    const f32x4 cs[2] = {cosp[0], cosp[1]}, sn[2] = {sinp[0], sinp[1]};
+    double most = 0.0;
+    float none = angle[it] < 0 ? __builtin_nanf("") : 0.f;  // NaN where a key is no number
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float c = angle[it] < 0 ? __builtin_nanf("") : cosp[j], s = sinp[j], x1 = x[it][0][j], x2 = x[it][1][j];
-      x[it][0][j] = x1 * c - x2 * s;
-      x[it][1][j] = x2 * c + x1 * s;
+      const double c = (double)cs[j >> 2][j & 3], s = (double)sn[j >> 2][j & 3];
+      const double x1 = (double)x[it][0][j], x2 = (double)x[it][1][j];
+      const double y1 = x1 * c - x2 * s, y2 = x2 * c + x1 * s;
+      most = fmax(most, fmax(__builtin_fabs(y1), __builtin_fabs(y2)));
+      x[it][0][j] = (float)y1;
+      x[it][1][j] = (float)y2;
+      none = __builtin_fmaf(x[it][0][j], 0.f, none);
+      none = __builtin_fmaf(x[it][1][j], 0.f, none);
     }
-    // (as integers their order is that of the magnitudes, a NaN above an infinity above all numbers)
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
+    // (a maximum leaves a NaN out; an infinity may be a number that 32 bits do not hold)
+    if (none != 0.f) {
+      bool wrong = angle[it] < 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        near[q >> 1] = max(near[q >> 1], __builtin_bit_cast(uint32_t, x[it][q][j]) & 0x7FFFFFFFu);
+        wrong = wrong || x[it][0][j] != x[it][0][j] || x[it][1][j] != x[it][1][j];
+      if (wrong) most = __builtin_nan("");
+    }
+    const uint64_t bits = __builtin_bit_cast(uint64_t, most) & ~(1ull << 63);
+    top = bits > top ? bits : top;
+#pragma unroll
+    for (int q = 2; q < 4; ++q)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top_v = max(top_v, __builtin_bit_cast(uint32_t, x[it][q][j]) & 0x7FFFFFFFu);
   }
   // Element j of a thread's sixteen of a key, in 64 bits.
   auto key = [&](int it, int j) {
     const int i = j & 7;
     const double x1 = act_bits_to_float(kp[it][i], DT), x2 = act_bits_to_float(kp[it][i + D / 2], DT);
-    if (angle[it] < 0) return (double)__builtin_nanf("");
     const double c = a.cos[angle[it] + i], s = a.sin[angle[it] + i];
     return j < 8 ? x1 * c - x2 * s : x2 * c + x1 * s;
   };
-  if (near[0]) atomicMax(&near_s[0][unit], near[0]);
-  if (near[1]) atomicMax(&near_s[1][unit], near[1]);
-  __syncthreads();
-  const float reach = __builtin_bit_cast(float, near_s[0][unit]), least = reach * (1.f - 0x1p-20f);
-  const bool wild = !(reach < __builtin_inff());  // past 32 bits, or no number: all in 64
-  unsigned long long top = 0;
-#pragma unroll
-  for (int it = 0; it < MAXIT; ++it) {
-    if (!isnew[it]) continue;
-    unsigned some = 0;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) some |= wild || __builtin_fabsf(x[it][j >> 3][j & 7]) >= least ? 1u << j : 0u;
-    for (; some; some &= some - 1) {
-      const unsigned long long u = __builtin_bit_cast(unsigned long long, __builtin_fabs(key(it, __builtin_ctz(some))));
-      top = u > top ? u : top;
-    }
-  }
-  if (top) atomicMax(&top_s[unit], top);
+  if (top) atomicMax(&top_s[0][unit], (unsigned long long)top);
+  if (top_v) atomicMax(&top_s[1][unit], (unsigned long long)top_v);
   __syncthreads();
 
-  const int64_t blk = a.c.block(page, h, slot0);
   const bool fresh = slot0 >= sp.len;
+  const int64_t blk = a.c.block(page, h, slot0);
   double scale[2], inv[2];
   int grow[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const double most = i ? (double)__builtin_bit_cast(float, near_s[1][unit]) : __builtin_bit_cast(double, top_s[unit]);
+    const double most = i ? (double)__builtin_bit_cast(float, (uint32_t)top_s[1][unit])
+                          : __builtin_bit_cast(double, (uint64_t)top_s[0][unit]);
     const double old = fresh ? 0.0 : (double)(i ? a.c.v_scale : a.c.k_scale)[blk];
     scale[i] = block_scale<CT>(most, old, &grow[i]);
     inv[i] = scale[i] > 0.0 ? 1.0 / scale[i] : 0.0;  // (also of NaN: its codes are 0)
@@ -316,34 +340,30 @@ __global__ __launch_bounds__(kP8Threads) void paged8_append_kernel(Append8Args a
     a.c.v_scale[blk] = (float)scale[1];
   }
 #pragma unroll
-  for (int it = 0; it < MAXIT; ++it) {
-    if (it >= its) continue;
+  for (int it = 0; it < ITS; ++it) {
     const int slot = slot0 + (r0 + it * kP8Threads) / CH;
     const int64_t at = a.c.token(page, h, slot) * D + d;
     if (isnew[it]) {
-      // (the quotient's own roundings add 2^-22 of it)
-      constexpr float off = Code<CT>::most * 0x1p-20f;
-      unsigned left[2] = {0, 0};
+      uint32_t odd[2] = {0, 0};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int i = q >> 1;
-        u32x2 w = {0u, 0u};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t n;
-          if (!quick_code<CT>(x[it][q][j] * (float)inv[i], off, &n)) left[i] |= 1u << ((q & 1) * 8 + j);
-          w[j >> 2] |= n << (8 * (j & 3));
-        }
+        u32x2 w = quick_codes<CT>(x[it][q], (float)inv[i], &odd[i]);
         if (!(inv[i] > 0.0)) w = u32x2{0u, 0u};
         *reinterpret_cast<u32x2*>((i ? a.c.v : a.c.k) + at + (q & 1) * (D / 2)) = w;
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        unsigned some = !(inv[i] > 0.0) ? 0u : i == 0 && wild ? 0xFFFFu : left[i];
-        for (; some; some &= some - 1) {
-          const int j = __builtin_ctz(some), e = (j & 7) + (j >> 3) * (D / 2);
-          const double y = i ? (double)act_bits_to_float(vp[it][e], DT) : key(it, j);
-          (i ? a.c.v : a.c.k)[at + e] = (uint8_t)encode<CT>(y, scale[i], inv[i]);
+        // (also where 32 bits are short of exponents)
+        const double u = inv[i];
+        const bool all = u > 0x1p100 || u < 0x1p-100;
+        if (u > 0.0 && (odd[i] || all)) {
+          unsigned some = all ? 0xFFFFu : odd_ones<CT>(x[it][2 * i], (float)u) | odd_ones<CT>(x[it][2 * i + 1], (float)u) << 8;
+          for (; some; some &= some - 1) {
+            const int j = __builtin_ctz(some), e = (j & 7) + (j >> 3) * (D / 2);
+            const double y = i ? (double)act_bits_to_float(vp[it][e], DT) : key(it, j);
+            (i ? a.c.v : a.c.k)[at + e] = (uint8_t)encode<CT>(y, scale[i], u);
+          }
         }
       }
     } else if (slot < sp.len) {
@@ -660,11 +680,15 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
       float x[8], y[8];
       unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + d), x);
       unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + (d ^ (D / 2))), y);
+      const f32x4* const cp = reinterpret_cast<const f32x4*>(cosr + da);
+      const f32x4* const sp = reinterpret_cast<const f32x4*>(sinr + da);
+      const f32x4 cs[2] = {cp[0], cp[1]}, sn[2] = {sp[0], sp[1]};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
+        const float cc = cs[e >> 2][e & 3], ss = sn[e >> 2][e & 3];
         float r1, r2;
-        if (low) rope_pair(x[e], y[e], cosr[da + e], sinr[da + e], &r1, &r2), x[e] = r1 * scale;
-        else rope_pair(y[e], x[e], cosr[da + e], sinr[da + e], &r1, &r2), x[e] = r2 * scale;
+        if (low) rope_pair(x[e], y[e], cc, ss, &r1, &r2), x[e] = r1 * scale;
+        else rope_pair(y[e], x[e], cc, ss, &r1, &r2), x[e] = r2 * scale;
       }
       split8<W4_DTYPE_BF16, true>(x, qf[j]);
     }
@@ -1026,17 +1050,22 @@ int check_new(const w4_paged8_cache* c, int dtype, const void* k, const void* v,
   return W4_OK;
 }
 
-int launch_append8(const w4::Append8Args& a, int dtype, int code, int64_t head_dim, hipStream_t st, const char* what) {
+int launch_append8(w4::Append8Args a, int dtype, int code, int64_t head_dim, hipStream_t st, const char* what) {
   // blocks that get tokens: at most as many as tokens, and two a row more than whole ones
   const int64_t block = 1ll << a.c.log2b;
   const int64_t items = std::min<int64_t>(a.tokens, a.tokens / block + 2 * (int64_t)a.c.rows);
   if (items == 0) return W4_OK;
   const int64_t per = block * (head_dim / 16), units = std::max<int64_t>(w4::kP8Threads / per, 1);
-  const dim3 grid((unsigned)items, (unsigned)((a.c.nkv + units - 1) / units));
+  const int64_t groups = items * ((a.c.nkv + units - 1) / units);
+  if (groups > 0xFFFFFFFFll / w4::kP8Threads)  // HIP refuses launches of 2^32 threads and more
+    return fail(W4_ERR_UNSUPPORTED, "%s: %d tokens of %d heads", what, a.tokens, a.c.nkv);
+  a.heads = (int)units;
+  const dim3 grid((unsigned)groups);
   return by_dtype(dtype, [&](auto dt) {
     return by_code(code, [&](auto ct) {
       return by_head(head_dim, [&](auto d) {
-        w4::paged8_append_kernel<dt(), ct(), d()><<<grid, w4::kP8Threads, 0, st>>>(a);
+        if (per <= w4::kP8Threads) w4::paged8_append_kernel<dt(), ct(), d(), 1><<<grid, w4::kP8Threads, 0, st>>>(a);
+        else if constexpr (d() == 128) w4::paged8_append_kernel<dt(), ct(), d(), 2><<<grid, w4::kP8Threads, 0, st>>>(a);
         return check_launch(what);
       });
     });
@@ -1072,7 +1101,7 @@ extern "C" int w4_paged8_append(const w4_paged8_cache* cache, int dtype, const v
     return rc;
   if (tokens == 0 || cache->rows == 0) return W4_OK;
   const w4::Append8Args a{view_of(cache), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_k,
-                          stride_v, angles, lengths, offsets, positions, cos, sin, (int)tokens, (int)tokens};
+                          stride_v, angles, lengths, offsets, positions, cos, sin, (int)tokens, (int)tokens, 0};
   return launch_append8(a, dtype, cache->code, cache->head_dim, static_cast<hipStream_t>(stream), "w4_paged8_append");
 }
 
@@ -1142,7 +1171,7 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   const bool put = most_new == 1 && num_heads / cache->kv_heads <= 16 && cache->block <= w4::kP8Unit;
   if (!put) {
     const w4::Append8Args p{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_k, stride_v,
-                            angles, lengths, offsets, positions, cos, sin, (int)tokens, most_new};
+                            angles, lengths, offsets, positions, cos, sin, (int)tokens, most_new, 0};
     if (const int rc = launch_append8(p, dtype, cache->code, cache->head_dim, st, "w4_paged8_attention (append)"))
       return rc;
   }

@@ -51,28 +51,45 @@ __device__ __forceinline__ double wave_scan64(double v) {
   return v;
 }
 
-// Eight probabilities in a row (rows need not start on 16 bytes: a vocabulary may be odd), as far as there are any.
-template <int DT>
-__device__ __forceinline__ void probs8(const void* p, int64_t i, int n, double out[8]) {
-  if (n >= 8) {
+// Eight probabilities in a row as they are stored (rows need not start on 16 bytes: a vocabulary may be odd), zeros
+// where there are fewer.
+template <int DT> struct Eight {
+  u32x4 v[DT == W4_DTYPE_FP32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, int64_t i, int n) {
     if constexpr (DT == W4_DTYPE_FP32) {
-      typedef f32x4 vec __attribute__((aligned(4)));
-      const float* const q = static_cast<const float*>(p) + i;
-      const f32x4 a = *reinterpret_cast<const vec*>(q), b = *reinterpret_cast<const vec*>(q + 4);
+      typedef u32x4 vec __attribute__((aligned(4)));
+      const uint32_t* const q = static_cast<const uint32_t*>(p) + i;
+      if (n >= 8) {
+        v[0] = *reinterpret_cast<const vec*>(q);
+        v[1] = *reinterpret_cast<const vec*>(q + 4);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = (double)a[e], out[e + 4] = (double)b[e];
+        for (int e = 0; e < 8; ++e) v[e >> 2][e & 3] = e < n ? q[e] : 0u;
+      }
     } else {
       typedef u32x4 vec __attribute__((aligned(2)));
-      float x[8];
-      unpack8<DT>(*reinterpret_cast<const vec*>(static_cast<const uint16_t*>(p) + i), x);
+      const uint16_t* const q = static_cast<const uint16_t*>(p) + i;
+      if (n >= 8) {
+        v[0] = *reinterpret_cast<const vec*>(q);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = (double)x[e];
+        for (int e = 0; e < 4; ++e)
+          v[0][e] = (2 * e < n ? (uint32_t)q[2 * e] : 0u) | (2 * e + 1 < n ? (uint32_t)q[2 * e + 1] << 16 : 0u);
+      }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = e < n ? prob<DT>(p, i + e) : 0.0;
   }
-}
+  __device__ __forceinline__ void values(double out[8]) const {
+    float x[8];
+    if constexpr (DT == W4_DTYPE_FP32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(float, (uint32_t)v[e >> 2][e & 3]);
+    } else {
+      unpack8<DT>(v[0], x);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = (double)x[e];
+  }
+};
 
 // A row's parts of the vocabulary are a workgroup's each, eight tokens in a row a thread (more than once of vocabularies
 // past 131072).  Every one of them decides on the drafts (a handful of numbers) and sums its part's weights at the first
@@ -80,7 +97,7 @@ __device__ __forceinline__ void probs8(const void* p, int64_t i, int n, double o
 // for it there.  The sums are of 64 bits, so that their order, which is fixed, moves no token but one that the sample
 // meets to 2^-50.
 template <int DT>
-__global__ __launch_bounds__(kVerThreads) void verify_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kVerThreads, 5) void verify_kernel(VerifyArgs a) {
   __shared__ double sum_s[2][kVerThreads / 64];
   __shared__ unsigned arrived_s;
   __shared__ int found_s;
@@ -107,13 +124,17 @@ __global__ __launch_bounds__(kVerThreads) void verify_kernel(VerifyArgs a) {
   const int64_t out = r < n && !a.draft ? a.tokens[(int64_t)row * a.drafts + r] : -1;
   const bool minus = r < n && a.draft;
   const int begin = part * a.run, end = min(begin + a.run, a.vocab);
-  // The weights of tokens i.. i + 7 below `to`: of what is left of the target, and the target's own.  (What is not a
+  // Tokens i.. i + 7 below `to`, and their weights: of what is left of the target, and the target's own.  (What is not a
   // number stays one, so that the sum shows it.)
-  auto weights = [&](int i, int to, double w[8], double p[8]) __attribute__((always_inline)) {
+  auto load = [&](int i, int to, Eight<DT>& p, Eight<DT>& q) __attribute__((always_inline)) {
+    p.load(a.target, tp + i, to - i);
+    if (minus) q.load(a.draft, dp + i, to - i);
+  };
+  auto weights = [&](int i, const Eight<DT>& pr, const Eight<DT>& qr, double w[8], double p[8]) __attribute__((always_inline)) {
     double d[8];
-    probs8<DT>(a.target, tp + i, to - i, p);
+    pr.values(p);
     if (minus) {
-      probs8<DT>(a.draft, dp + i, to - i, d);
+      qr.values(d);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = i + e == out ? 1.0 : 0.0;
@@ -125,12 +146,25 @@ __global__ __launch_bounds__(kVerThreads) void verify_kernel(VerifyArgs a) {
       p[e] = p[e] < 0.0 ? 0.0 : p[e];
     }
   };
+  constexpr int ONCE = kVerThreads * 8;
   double s0 = 0.0, s1 = 0.0;
-  for (int i = begin + tid * 8; i < end; i += kVerThreads * 8) {
+  auto sum = [&](int i, const Eight<DT>& pr, const Eight<DT>& qr) __attribute__((always_inline)) {
     double w[8], p[8];
-    weights(i, end, w, p);
+    weights(i, pr, qr, w, p);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s0 += w[e], s1 += p[e];
+  };
+  int i = begin + tid * 8;
+  Eight<DT> p0, q0, p1, q1;
+  for (; i + ONCE + 8 <= end; i += 2 * ONCE) {  // two goes' loads travel together
+    load(i, end, p0, q0);
+    load(i + ONCE, end, p1, q1);
+    sum(i, p0, q0);
+    sum(i + ONCE, p1, q1);
+  }
+  for (; i < end; i += ONCE) {
+    load(i, end, p0, q0);
+    sum(i, p0, q0);
   }
   s0 = lane_get(wave_scan64(s0), 63);
   s1 = lane_get(wave_scan64(s1), 63);
@@ -175,7 +209,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_kernel(VerifyArgs a) {
   for (int i0 = b; i0 < e; i0 += kVerThreads * 8) {
     const int i = i0 + tid * 8;
     double w[8], t[8], s = 0.0;
-    weights(min(i, e), e, w, t);
+    load(min(i, e), e, p0, q0);
+    weights(i, p0, q0, w, t);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (!rest) w[k] = t[k];
@@ -227,13 +262,16 @@ struct VerifyPlan {
   int64_t slice;  // rows of a launch
 };
 
-// Parts of 2048 tokens, or of a multiple of that where there would be more of them than lanes.
+// Parts of 2048 tokens, or of a multiple of that where there would be more of them than lanes, or more workgroups than
+// the chip holds (five a CU): each begins with three loads that wait for one another.
 VerifyPlan verify_plan(int64_t rows, int64_t vocab) {
   VerifyPlan p;
   p.slice = W4_WORKSPACE_COUNTER_BYTES / 4;
   if (p.slice > rows) p.slice = rows;
   const int64_t once = 8 * w4::kVerThreads;
-  p.run = (int)(((vocab + w4::kVerMaxParts - 1) / w4::kVerMaxParts + once - 1) / once * once);
+  int64_t parts = 5 * device_cu_count() / p.slice;
+  parts = parts < 1 ? 1 : parts > w4::kVerMaxParts ? w4::kVerMaxParts : parts;
+  p.run = (int)(((vocab + parts - 1) / parts + once - 1) / once * once);
   p.parts = (int)((vocab + p.run - 1) / p.run);
   return p;
 }

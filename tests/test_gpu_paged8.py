@@ -548,6 +548,9 @@ def test_codes_of_many_tokens(kind, dtype):
     if dtype == torch.bfloat16:
         c["k"][40] = 3e38
     c["k"][100:132], c["v"][100:132] = 1.0, 0.75  # (equal magnitudes, rotated)
+    tiny = torch.finfo(dtype).smallest_normal * 2.0 ** -3  # subnormal numbers, and in bf16 the smallest scale
+    for n in ("k", "v"):
+        c[n][320:400] = (torch.randn((80, nkv * d), device=DEV, generator=g) * tiny).to(dtype)
     pos = c["positions"].long()
     x = c["k"].double().view(T, nkv, d)
     h, co, si = d // 2, c["cos"].double()[pos][:, None], c["sin"].double()[pos][:, None]
