@@ -8,7 +8,12 @@ output product, the norm and the MLP; the logits go to ``token_logprobs``, whose
 likely token is the next one.  It is captured in a HIP graph: slots, lengths, positions
 and the page table live on the GPU.
 
+The cache may be held in 8 bits (``paged8.py``).  Its rows may see a sliding window and a
+few first tokens only, whose other pages go back to the pool, and several drafted tokens
+of every row may go through the model at once and be verified (``verify``).
+
     python -m int4_hip.serving --batch 32 --prompt-len 512 --new-tokens 64
+    python -m int4_hip.serving --batch 8 --cache e4m3 --window 256 --sinks 4 --drafts 3
 """
 from __future__ import annotations
 
@@ -20,7 +25,8 @@ import torch
 from . import llama_ops
 from .llama import (Attention, LlamaConfig, LlamaForCausalLM, _add_norm, _all_int4, _grouped, _plain, rope_inv_freq)
 from .paged import paged_append, paged_attention, paged_evict
-from .scoring import TokenLogprobs, token_logprobs
+from .paged8 import CODES, paged_attention8
+from .scoring import TokenLogprobs, Verified, token_logprobs, verify_drafts
 
 
 class Step(NamedTuple):
@@ -44,10 +50,17 @@ class BatchDecoder:
     keeps them in fp32).  With ``keep`` a step holds rows * heads * width * page_size fp32
     scores, whatever the rows hold, so ``width`` is best no more than a row may need
     (of 32 rows of 32 heads 4 MB for every 1024 tokens of it).
+
+    ``cache``: ``torch.int8`` or ``torch.float8_e4m3fn`` holds it in 8 bits, with a scale for
+    every ``block`` tokens of a page and head; a prompt attends to its keys and values as
+    they are held.  Such a cache is not evicted from; with ``sees`` every token attends to the
+    last ``sees`` tokens and the first ``sinks`` alone, and pages that no token will see
+    again are given back.
     """
 
     def __init__(self, model: LlamaForCausalLM, rows: int, pages: int, width: int, page_size: int = 64,
-                 max_positions: int = 8192, keep: int | None = None, recent: int = 0, top: int = 1, window: int = 32):
+                 max_positions: int = 8192, keep: int | None = None, recent: int = 0, top: int = 1, window: int = 32,
+                 cache: torch.dtype | None = None, block: int = 32, sees: int | None = None, sinks: int = 0):
         c = model.config
         self.model, self.rows, self.page_size, self.width = model, rows, page_size, width
         self.heads = c.num_attention_heads, c.num_key_value_heads, c.head_dim
@@ -63,10 +76,23 @@ class BatchDecoder:
             raise ValueError("a prompt's last token, at least, weighs the ones before it")
         if keep is not None and not (keep >= 1 and 0 <= recent <= keep):
             raise ValueError(f"a row is cut to keep >= 1 tokens, 0 to keep of them the last ones: got {keep}, {recent}")
+        if cache is not None and (cache not in CODES or block not in (8, 16, 32, 64) or page_size % block):
+            raise ValueError("a cache of int8 or float8_e4m3fn, blocks of 8, 16, 32 or 64 tokens that fill a page: got "
+                             f"{cache}, {block} of {page_size}")
+        if cache is not None and keep is not None:
+            raise ValueError("a cache of 8 bits is not evicted from")
+        if (cache is None and (sees is not None or sinks)) or (sees is not None and sees < 1) or sinks < 0:
+            raise ValueError(f"a cache of 8 bits may be seen by sees >= 1 last and sinks >= 0 first tokens: got {sees}, "
+                             f"{sinks}")
         self.keep, self.recent, self.top, self.window = keep, recent, top, window
+        self.sees, self.sinks = sees, sinks
         nl, nkv, d = c.num_hidden_layers, c.num_key_value_heads, c.head_dim
-        self.k = torch.zeros((nl, pages, nkv, page_size, d), dtype=dtype, device=dev)
+        self.k = torch.zeros((nl, pages, nkv, page_size, d), dtype=cache or dtype, device=dev)
         self.v = torch.zeros_like(self.k)
+        self.scales = None
+        if cache is not None:
+            self.scales = torch.zeros((2, nl, pages, nkv, page_size // block), device=dev)
+            self.each = torch.arange(rows + 1, dtype=torch.int32, device=dev)  # offsets of a token a row
         self.weight = torch.zeros((nl, pages, nkv, page_size), device=dev) if keep is not None else None
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.full((rows,), -1, dtype=torch.int32, device=dev)
@@ -76,7 +102,7 @@ class BatchDecoder:
         self.cos, self.sin = ang.cos(), ang.sin()
         # the host's copy: what a row holds is known without asking the GPU
         self.free = list(range(pages))
-        self.owned: list[list[int]] = [[] for _ in range(rows)]
+        self.owned: list[list[int | None]] = [[] for _ in range(rows)]  # None: given back
         self.length = [-1] * rows
         self.position = [0] * rows
         self.graph = None
@@ -97,13 +123,32 @@ class BatchDecoder:
 
     def release(self, row: int) -> None:
         """Forget a sequence; the row is idle."""
-        self.free += self.owned[row]
+        self.free += [page for page in self.owned[row] if page is not None]
         self.owned[row], self.length[row] = [], -1
         self.lengths[row] = -1
+
+    def _give_back(self, row: int) -> None:
+        """Pages that no token will see again: behind the window of the row's next one, and no sink in them."""
+        if self.sees is None:
+            return
+        S, own = self.page_size, self.owned[row]
+        for i in range(-(-self.sinks // S), min(len(own), (self.length[row] - self.sees + 1) // S)):
+            if own[i] is not None:
+                self.free.append(own[i])
+                own[i] = None
+                self.table[row, i] = -1
 
     # -------------------------------------------------------------- the model
     def _linears(self, x, mods):
         return _grouped(x, mods) if _all_int4(mods) else [m(x) for m in mods]
+
+    def _attend8(self, table, lengths, offsets, positions, longest):
+        """The attention of new tokens of the rows of ``table`` over a cache in 8 bits, for ``_run``."""
+        def attend(i, q, k, v):
+            return paged_attention8(q, k, v, self.cos, self.sin, self.k[i], self.v[i], self.scales[0, i],
+                                    self.scales[1, i], table, lengths, offsets, positions, longest=longest,
+                                    window=self.sees, sinks=self.sinks)
+        return attend
 
     def _run(self, x, attend) -> torch.Tensor:
         """Logits of the rows ``x`` [n, hidden]; ``attend(i, q, k, v)``: the attention of layer i."""
@@ -137,6 +182,9 @@ class BatchDecoder:
         slots = torch.arange(T, dtype=torch.int32, device=dev)
         rows = torch.full_like(slots, row)
         own = self.table[row:row + 1, :len(self.owned[row])]
+        if self.scales is not None:
+            one = torch.tensor([0, T], dtype=torch.int32, device=dev)
+            attend8 = self._attend8(own.contiguous(), one[:1], one, slots, T)
 
         def attend(i, q, k, v):
             weight = None if self.weight is None else self.weight[i]
@@ -150,13 +198,14 @@ class BatchDecoder:
                                     slots[one], weight)
             return llama_ops.attention_prefill(q, k, v, cos, sin, kc, vc, 0, nh, nkv, d)
 
-        logits = self._run(self.model.model.embed_tokens(prompt), attend)
+        logits = self._run(self.model.model.embed_tokens(prompt), attend if self.scales is None else attend8)
         given = torch.cat([prompt[1:].to(torch.int64), torch.zeros(1, dtype=torch.int64, device=dev)])
         r = token_logprobs(logits, given, top=self.top)
         self.ids[row] = r.top_token[-1, 0]
         self.length[row], self.position[row] = T, T
         self.lengths[row] = T
         self.positions[row] = T
+        self._give_back(row)
         return TokenLogprobs(r.logprob[:-1], r.entropy, r.top_logprob, r.top_token)
 
     def _step(self) -> Step:
@@ -164,6 +213,8 @@ class BatchDecoder:
             return paged_attention(q, k, v, self.cos, self.sin, self.k[i], self.v[i], self.table, self.lengths,
                                    self.positions, None if self.weight is None else self.weight[i])
 
+        if self.scales is not None:
+            attend = self._attend8(self.table, self.lengths, self.each, self.positions, 1)
         logits = self._run(self.model.model.embed_tokens(self.ids), attend)
         r = token_logprobs(logits, None, top=self.top)
         live = (self.lengths >= 0).to(torch.int32)
@@ -212,7 +263,50 @@ class BatchDecoder:
             if n >= 0:
                 self.length[row] += 1
                 self.position[row] += 1
+                self._give_back(row)
         return out
+
+    @torch.no_grad()
+    def verify(self, drafts: torch.Tensor, accept: torch.Tensor, sample: torch.Tensor,
+               draft: torch.Tensor | None = None, temperature: float = 1.0) -> Verified:
+        """A step of several tokens: every live row's token in ``ids`` and its ``drafts`` int64
+        [rows, K] go through the model together; those that ``verify_drafts`` accepts stay in
+        the cache, and the token after them is put in ``ids``.  ``accept`` fp32 [rows, K] and
+        ``sample`` fp32 [rows] are the random numbers, ``draft`` [rows, K, vocab] fp32 the
+        probabilities the drafts were drawn with (None: no matter of chance).  The target's
+        are the softmax of its logits over ``temperature``.
+
+        Waits for the GPU: what the rows hold is known to the host.  Refused drafts leave no
+        trace but the scale of the block that they came into.
+        """
+        if self.scales is None:
+            raise ValueError("drafts are verified over a cache of 8 bits")
+        if drafts.dim() != 2 or drafts.shape[0] != self.rows or not temperature > 0:
+            raise ValueError(f"drafts of {self.rows} rows and a temperature above 0: got {tuple(drafts.shape)}, {temperature}")
+        K = drafts.shape[1]
+        for row, n in enumerate(self.length):
+            if n >= 0:
+                if self.position[row] + K >= len(self.cos):
+                    raise RuntimeError(f"row {row} is past the {len(self.cos)} positions")
+                self._reserve(row, n + K + 1)
+        tokens = torch.cat((self.ids[:, None], drafts), 1)
+        positions = self.positions[:, None] + torch.arange(K + 1, dtype=torch.int32, device=self.ids.device)
+        attend = self._attend8(self.table, self.lengths, self.each * (K + 1), positions.flatten(), K + 1)
+        # (a draft outside the vocabulary is refused; until then it is some token of it)
+        embed = self.model.model.embed_tokens
+        logits = self._run(embed(tokens.flatten().clamp(0, embed.num_embeddings - 1)), attend)
+        target = torch.softmax(logits.float() / temperature, -1).view(self.rows, K + 1, -1)
+        r = verify_drafts(target, draft, drafts, accept, sample)
+        step = torch.where(self.lengths >= 0, r.accepted + 1, 0).to(torch.int32)
+        self.lengths += step
+        self.positions += step
+        self.ids.copy_(r.token.clamp(min=0))  # (-1: of logits that are no numbers)
+        for row, n in enumerate(step.tolist()):
+            if self.length[row] >= 0:
+                self.length[row] += n
+                self.position[row] += n
+                self._give_back(row)
+        return r
 
     @torch.no_grad()
     def evict(self) -> list[int]:
@@ -240,11 +334,22 @@ class BatchDecoder:
         return over
 
 
+def looked_up(history: list[int], drafts: int) -> list[int]:
+    """Drafts without a model: what followed the last token where it stood before (the last
+    token itself, where it did not, and where that ends)."""
+    last = history[-1]
+    at = next((i for i in range(len(history) - 2, -1, -1) if history[i] == last), len(history))
+    got = history[at + 1:at + 1 + drafts]
+    return got + [last] * (drafts - len(got))
+
+
 @torch.no_grad()
 def run(batch: int = 32, prompt_len: int = 512, new_tokens: int = 64, group_size: int = 128, seed: int = 0,
-        keep: int | None = None, recent: int = 0, top: int = 5, cfg: LlamaConfig | None = None) -> dict:
+        keep: int | None = None, recent: int = 0, top: int = 5, cfg: LlamaConfig | None = None,
+        cache: torch.dtype | None = None, sees: int | None = None, sinks: int = 0, drafts: int = 0) -> dict:
     """Batched decoding of the random-init W4 model on ragged prompts: prompts put into
-    the pages, then ``new_tokens`` graph-replayed steps, evicting every 64 if ``keep``."""
+    the pages, then ``new_tokens`` graph-replayed steps, evicting every 64 if ``keep``; with
+    ``drafts`` (and a ``cache`` of 8 bits) steps that verify so many looked-up tokens a row."""
     from .qlinear import quantize_model_linears
 
     dev = torch.device("cuda")
@@ -255,19 +360,39 @@ def run(batch: int = 32, prompt_len: int = 512, new_tokens: int = 64, group_size
     model = model.to(torch.bfloat16).eval()
     quantize_model_linears(model, group_size, skip=("lm_head",))
     S = 64
-    width = -(-(prompt_len + new_tokens + 1) // S)
+    most = prompt_len + new_tokens * (drafts + 1) + 1
+    width = -(-most // S)
     dec = BatchDecoder(model, batch, pages=batch * width * (2 if keep is not None else 1), width=width, page_size=S,
-                       max_positions=prompt_len + new_tokens + 1, keep=keep, recent=recent, top=top)
+                       max_positions=most, keep=keep, recent=recent, top=top, cache=cache, sees=sees, sinks=sinks)
     g = torch.Generator(device=dev).manual_seed(seed + 1)
-    scored = 0.0
+    scored, prompts = 0.0, []
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     for row in range(batch):
         n = max(2, prompt_len * (row + 1) // batch)
-        r = dec.add(row, torch.randint(0, cfg.vocab_size, (n,), device=dev, generator=g))
+        prompts.append(torch.randint(0, cfg.vocab_size, (n,), device=dev, generator=g))
+        r = dec.add(row, prompts[-1])
         scored += r.logprob.mean()
     torch.cuda.synchronize()
     prompt_s = time.perf_counter() - t0
+    result = {"batch": batch, "prompt_len": prompt_len, "new_tokens": new_tokens, "group_size": group_size, "keep": keep,
+              "recent": recent, "cache": str(cache or torch.bfloat16), "sees": sees, "sinks": sinks, "drafts": drafts,
+              "prompt_s": prompt_s, "prompt_mean_logprob": float(scored) / batch,
+              "data": "synthetic (seeded random weights and prompts)"}
+    if drafts:
+        history = [p.tolist() + [t] for p, t in zip(prompts, dec.ids.tolist())]
+        torch.cuda.synchronize()
+        t0, made = time.perf_counter(), 0
+        for _ in range(new_tokens):
+            guess = torch.tensor([looked_up(h, drafts) for h in history], device=dev)
+            r = dec.verify(guess, torch.rand((batch, drafts), device=dev, generator=g),
+                           torch.rand(batch, device=dev, generator=g))
+            for h, d, n, t in zip(history, guess.tolist(), r.accepted.tolist(), r.token.tolist()):
+                h += d[:n] + [t]
+                made += n + 1
+        s = time.perf_counter() - t0
+        return {**result, "decode_ms_per_step": s / new_tokens * 1e3, "decode_tokens_per_s": made / s,
+                "accepted_per_step": made / (new_tokens * batch) - 1}
     dec.capture()
     evicted = 0
     dec.step()
@@ -279,12 +404,8 @@ def run(batch: int = 32, prompt_len: int = 512, new_tokens: int = 64, group_size
             evicted += len(dec.evict())
     torch.cuda.synchronize()
     s = time.perf_counter() - t0
-    return {"batch": batch, "prompt_len": prompt_len, "new_tokens": new_tokens, "group_size": group_size, "keep": keep,
-            "recent": recent, "rows_evicted": evicted, "prompt_s": prompt_s,
-            "prompt_mean_logprob": float(scored) / batch, "decode_ms_per_step": s / (new_tokens - 1) * 1e3,
-            "decode_tokens_per_s": batch * (new_tokens - 1) / s,
-            "last_entropy": float(out.alternatives.entropy.mean()),
-            "data": "synthetic (seeded random weights and prompts)"}
+    return {**result, "rows_evicted": evicted, "decode_ms_per_step": s / (new_tokens - 1) * 1e3,
+            "decode_tokens_per_s": batch * (new_tokens - 1) / s, "last_entropy": float(out.alternatives.entropy.mean())}
 
 
 if __name__ == "__main__":
@@ -297,5 +418,11 @@ if __name__ == "__main__":
     ap.add_argument("--group-size", type=int, default=128)
     ap.add_argument("--keep", type=int, default=None, help="tokens a row is cut to every 64 steps")
     ap.add_argument("--recent", type=int, default=0, help="of them, the last ones that always stay")
+    ap.add_argument("--cache", choices=["int8", "e4m3"], default=None, help="hold the cache in 8 bits")
+    ap.add_argument("--window", type=int, default=None, help="last tokens that a token sees, of a cache in 8 bits")
+    ap.add_argument("--sinks", type=int, default=0, help="first tokens that stay visible beside them")
+    ap.add_argument("--drafts", type=int, default=0, help="tokens a row that a step looks up and verifies")
     a = ap.parse_args()
-    print(json.dumps(run(a.batch, a.prompt_len, a.new_tokens, a.group_size, keep=a.keep, recent=a.recent)))
+    cache = {None: None, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}[a.cache]
+    print(json.dumps(run(a.batch, a.prompt_len, a.new_tokens, a.group_size, keep=a.keep, recent=a.recent, cache=cache,
+                         sees=a.window, sinks=a.sinks, drafts=a.drafts)))
