@@ -460,6 +460,7 @@ struct Attend8Args {
   const uint16_t *k, *v;  // PUT: the new tokens', which the attention writes itself
   int64_t stride_k, stride_v;
   int tokens, longest, g, window, sinks;  // window: 0 for none
+  int many;  // rows of so many new tokens and more are paged8_prompt_kernel's
 };
 
 // The work of one workgroup: a tile of sixteen (new token, query head) columns of one row and key-value head, and a
@@ -480,7 +481,7 @@ constexpr int kP8Waves = 4, kP8Parts = 512, kP8MinUnits = 4;
 template <int UP>
 __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8* it, int* total) {
   const int lane = threadIdx.x & 63;
-  auto tiles_of = [&](const RowSpan& s) { return a.c.nkv * (int)(((int64_t)s.n * a.g + 15) / 16); };
+  auto tiles_of = [&](const RowSpan& s) { return s.n < a.many ? a.c.nkv * (int)(((int64_t)s.n * a.g + 15) / 16) : 0; };
   // units that one tile of a row reads at most, or nearly so
   auto units_of = [&](const RowSpan& s) {
     if (s.len < 0 || s.n == 0) return 1;
@@ -530,7 +531,9 @@ __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8
 }
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
 // A workgroup's four waves take units of 64 slots in turn, each its own.
 //
@@ -969,6 +972,282 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
   }
 }
 
+// ---------------------------------------------------------------- attention of rows with many new tokens
+constexpr int kPromptCols = 64, kPromptUnit = 64;
+
+// A workgroup has 64 columns of a row and key-value head, sixteen a wave, and all the slots that they see, 64 at once:
+// the four waves turn the codes into bf16 in LDS together, once, and multiply from there.  Otherwise as
+// paged8_attention_kernel, whose waves share their columns and not the slots: that spreads a few columns over the chip,
+// but converts every code for sixteen columns alone.
+template <int DT, int CT, int D>
+__global__ __launch_bounds__(256, 2) void paged8_prompt_kernel(Attend8Args a) {
+  constexpr int UP = kPromptUnit, KB = UP / 32, NJ = D / 32, ND = D / 16, NP = Split<W4_DTYPE_BF16>::N;
+  constexpr int KROW = D + 8;               // halfwords of a key row in LDS: sixteen rows on different banks
+  constexpr int VROW = D == 64 ? 72 : 144;  // of a value row: four rows of 32 bytes on different banks
+  constexpr int CH = D / 16, NC = UP * CH / 256;  // chunks of 16 codes of a slot, and of a thread
+  typedef Mfma<W4_DTYPE_BF16> M;
+  __shared__ __attribute__((aligned(16))) uint16_t k_s[2][UP * KROW], v_s[2][UP * VROW];
+  __shared__ float ks_s[2][UP / 8], vs_s[2][UP / 8];
+  __shared__ uint16_t nan_s[2][CT == W4_CODE_E4M3 ? UP * CH : 1];
+  __shared__ int odd_s[2];  // the unit there, where it has codes of NaN
+
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, c = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nh = a.c.nkv * a.g;
+  // The row and the tile of its columns, a head's tiles beside another head's; the last ones, which see most, first.
+  RowSpan sp;
+  int b = 0, tile = 0, h = 0;
+  for (int r = 0, base = 0;; r += 64) {
+    if (r >= a.c.rows) return;
+    const RowSpan s = row_span(a.c, a.lengths, a.offsets, a.tokens, a.longest, r + lane);
+    const int tiles = s.n >= a.many ? (int)(((int64_t)s.n * a.g + kPromptCols - 1) / kPromptCols) * a.c.nkv : 0;
+    const int upto = base + wave_scan(tiles), item = blockIdx.x;
+    const int end = __builtin_amdgcn_readlane(upto, 63);
+    if (item < end) {
+      const int i = __popcll(__ballot(item >= upto));
+      b = r + i;
+      sp.len = __builtin_amdgcn_readlane(s.len, i);
+      sp.o0 = __builtin_amdgcn_readlane(s.o0, i);
+      sp.n = __builtin_amdgcn_readlane(s.n, i);
+      const int left = __builtin_amdgcn_readlane(upto, i) - 1 - item;
+      tile = left / a.c.nkv;
+      h = left - tile * a.c.nkv;
+      break;
+    }
+    base = end;
+  }
+  const int len = sp.len, col0 = tile * kPromptCols, cols = min(sp.n * a.g - col0, kPromptCols);
+  auto out_at = [&](int col) {
+    const int j = (col0 + col) / a.g;
+    return a.out + ((int64_t)(sp.o0 + j) * nh + h * a.g + (col0 + col - j * a.g)) * D;
+  };
+  if (len < 0) {
+    const uint16_t fill = len == kP8Refused ? float_to_act_bits<DT>(__builtin_nanf("")) : 0;
+    for (int i = tid; i < cols * D; i += 256) out_at(i / D)[i % D] = fill;
+    return;
+  }
+  const int first_slot = len + col0 / a.g, last_slot = len + (col0 + cols - 1) / a.g;
+  const int lo = a.window ? max(first_slot - a.window + 1, 0) : 0;
+  const int u_lo = lo / UP, sink_units = a.window ? min((int)(((int64_t)a.sinks + UP - 1) / UP), u_lo) : 0;
+  const int units = sink_units + last_slot / UP - u_lo + 1;
+  auto base_of = [&](int u) { return (u < sink_units ? u : u_lo + u - sink_units) * UP; };
+  // this wave's columns (past the tile's last: copies of it that count for nothing)
+  const int wcol = min(wv * 16, cols - 1);
+  const int w_first = len + (col0 + wcol) / a.g, w_last = len + (col0 + min(wv * 16 + 15, cols - 1)) / a.g;
+
+  // A thread's chunks of a unit: chunk tid + 256 i is chunk % CH of slot / CH.
+  const int32_t* const table = a.c.table + (int64_t)b * a.c.width;
+  u32x4 kr[NC], vr[NC];
+  float sr = 0.f;
+  int ids[NC], sid = 0;
+  auto load_ids = [&](int u) __attribute__((always_inline)) {
+    const int base = base_of(u);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) ids[i] = table[min(base + (tid + 256 * i) / CH, last_slot) >> a.c.log2s];
+    sid = table[min(base + 8 * (tid & 7), last_slot) >> a.c.log2s];
+  };
+  auto valid = [&](int id, int slot) {
+    return slot <= last_slot && (uint64_t)(int64_t)id < (uint64_t)a.c.pages ? id : -1;
+  };
+  auto load = [&](int u) __attribute__((always_inline)) {
+    const int base = base_of(u);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int slot = base + (tid + 256 * i) / CH;
+      const int64_t at = a.c.token(max(valid(ids[i], slot), 0), h, slot) * D + tid % CH * 16;
+      kr[i] = *reinterpret_cast<const u32x4*>(a.c.k + at);
+      vr[i] = *reinterpret_cast<const u32x4*>(a.c.v + at);
+    }
+    if (tid < 16) {  // keys' scales of the unit's groups of eight slots, then values'
+      const int slot = base + 8 * (tid & 7), id = valid(sid, slot);
+      const float x = (tid < 8 ? a.c.k_scale : a.c.v_scale)[a.c.block(max(id, 0), h, slot)];
+      sr = id < 0 ? __builtin_nanf("") : x;
+    }
+  };
+  auto stage = [&](int u) __attribute__((always_inline)) {
+    const int buf = u & 1;
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int slot = (tid + 256 * i) / CH, ch = tid % CH;
+      const int row = (slot & 32) + ((slot >> 2) & 1) * 16 + ((slot >> 3) & 3) * 4 + (slot & 3);
+      if constexpr (CT == W4_CODE_E4M3) {
+        // NaN of e4m3, what a program that is not this one left in the pages, must not meet the probability 0 of a slot
+        // that is not seen: it is taken out, and what sees it is made NaN by itself.
+        uint32_t bad[4], any = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= bad[e] = nan_bytes(vr[i][e]);
+        uint32_t bits = 0;
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            vr[i][e] &= ~(bad[e] * 0xFFu);
+            bits |= (bad[e] & 1 | bad[e] >> 7 & 2 | bad[e] >> 14 & 4 | bad[e] >> 21 & 8) << (4 * e);
+          }
+          some = true;
+        }
+        nan_s[buf][tid + 256 * i] = (uint16_t)bits;
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        *reinterpret_cast<bf16x8*>(&k_s[buf][row * KROW + ch * 16 + 8 * g]) = codes8<CT>(kr[i][2 * g], kr[i][2 * g + 1]);
+        *reinterpret_cast<bf16x8*>(&v_s[buf][slot * VROW + ch * 16 + 8 * g]) = codes8<CT>(vr[i][2 * g], vr[i][2 * g + 1]);
+      }
+    }
+    if (tid < 8) ks_s[buf][tid] = sr;
+    else if (tid < 16) vs_s[buf][tid - 8] = sr;
+    if (CT == W4_CODE_E4M3 && some) odd_s[buf] = u;
+  };
+
+  if (tid < 2) odd_s[tid] = -1;
+  load_ids(0);
+  load(0);
+  load_ids(min(1, units - 1));
+
+  const int col = min(wv * 16 + l16, cols - 1), tok = sp.o0 + (col0 + col) / a.g, mine = len + (col0 + col) / a.g;
+  u32x4 qf[NJ][NP];
+  {
+    const int pos = a.positions[tok];
+    const bool there = (uint64_t)(int64_t)pos < (uint64_t)a.angles;
+    const uint16_t* const qp = a.q + tok * a.stride_q + (h * a.g + (col0 + col) % a.g) * D;
+    const float* const cosr = a.cos + (there ? (int64_t)pos * (D / 2) : 0);
+    const float* const sinr = a.sin + (there ? (int64_t)pos * (D / 2) : 0);
+    const float scale = there ? a.scale : __builtin_nanf("");
+#pragma unroll
+    for (int j = 0; j < NJ / 2; ++j) {
+      const int d = 32 * j + 8 * c;
+      float x[8], y[8];
+      unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + d), x);
+      unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + d + D / 2), y);
+      const f32x4* const cp = reinterpret_cast<const f32x4*>(cosr + d);
+      const f32x4* const sp4 = reinterpret_cast<const f32x4*>(sinr + d);
+      const f32x4 cs[2] = {cp[0], cp[1]}, sn[2] = {sp4[0], sp4[1]};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float r1, r2;
+        rope_pair(x[e], y[e], cs[e >> 2][e & 3], sn[e >> 2][e & 3], &r1, &r2);
+        x[e] = r1 * scale, y[e] = r2 * scale;
+      }
+      split8<W4_DTYPE_BF16, true>(x, qf[j]);
+      split8<W4_DTYPE_BF16, true>(y, qf[j + NJ / 2]);
+    }
+  }
+  __syncthreads();
+  stage(0);
+  __syncthreads();
+
+  float m = -__builtin_inff(), l = 0.f;
+  f32x4 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto seen = [&](int slot) { return slot <= mine && (!a.window || slot > mine - a.window || slot < a.sinks); };
+  for (int u = 0; u < units; ++u) {
+    const int base = base_of(u), buf = u & 1;
+    if (u + 1 < units) {  // the next unit's loads travel under this one's products
+      load(u + 1);
+      load_ids(min(u + 2, units - 1));
+    }
+    // (a wave none of whose columns sees any of it waits)
+    if (base <= w_last && (!a.window || base + UP - 1 > w_first - a.window || base < a.sinks)) {
+      const bool whole = base + UP - 1 <= w_first && (!a.window || base > w_last - a.window || base + UP <= a.sinks);
+      f32x4 s[KB][2];
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const float sk = ks_s[buf][4 * kb + c];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint16_t* const at = &k_s[buf][(kb * 32 + t * 16 + l16) * KROW + 8 * c];
+          bf16x8 kf[NJ];
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const bf16x8*>(at + 32 * j);
+          s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) s[kb][t] = M::m16(kf[j], __builtin_bit_cast(bf16x8, qf[j][p]), s[kb][t]);
+          s[kb][t] *= sk;
+        }
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x = s[kb][e >> 2][e & 3];
+          if (!whole) x = seen(base + kb * 32 + 8 * c + e) ? x : -__builtin_inff();
+          top = fmaxf(top, x);
+          s[kb][e >> 2][e & 3] = x;
+        }
+      if (__ballot((top - m) * kLog2e > 8.f)) {
+        float mn = fmaxf(top, m);
+        mn = fmaxf(mn, __shfl_xor(mn, 16));
+        mn = fmaxf(mn, __shfl_xor(mn, 32));
+        const float al = __builtin_amdgcn_exp2f((m - finite_or_zero(mn)) * kLog2e);
+        l *= al;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][e] *= al;
+        m = mn;
+      }
+      const float mz = finite_or_zero(m);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const float sv = vs_s[buf][4 * kb + c];
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3] - mz, kLog2e, -8.f));
+          l += p[e];
+          p[e] *= sv;
+          if (!whole) p[e] = seen(base + kb * 32 + 8 * c + e) ? p[e] : 0.f;
+        }
+        u32x4 pf[NP];
+        split8<W4_DTYPE_BF16, false>(p, pf);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const uint16_t* at = &v_s[buf][(kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3)];
+          const s16x4 vl = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+          const s16x4 vh = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * VROW));
+          const u32x2 lw = __builtin_bit_cast(u32x2, vl), hw = __builtin_bit_cast(u32x2, vh);
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{lw[0], lw[1], hw[0], hw[1]});
+#pragma unroll
+          for (int q = NP - 1; q >= 0; --q) o[d] = M::m16(vf, __builtin_bit_cast(bf16x8, pf[q]), o[d]);
+        }
+      }
+      if (CT == W4_CODE_E4M3 && odd_s[buf] == u) {
+        for (int row = 0; row < UP; ++row) {
+          const bool see = seen(base + row);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            const uint32_t bits = nan_s[buf][row * CH + d] >> (4 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (see && bits >> e & 1) o[d][e] = __builtin_nanf("");
+          }
+        }
+      }
+    }
+    if (u + 1 < units) {
+      stage(u + 1);  // (what was there was read before the last barrier)
+      __syncthreads();
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (wv * 16 + l16 < cols) {
+    const float inv = 1.f / l;
+    uint16_t* const out = out_at(wv * 16 + l16) + 4 * c;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      u32x2 w;
+      w[0] = (uint32_t)float_to_act_bits<DT>(o[d][0] * inv) | ((uint32_t)float_to_act_bits<DT>(o[d][1] * inv) << 16);
+      w[1] = (uint32_t)float_to_act_bits<DT>(o[d][2] * inv) | ((uint32_t)float_to_act_bits<DT>(o[d][3] * inv) << 16);
+      *reinterpret_cast<u32x2*>(out + 16 * d) = w;
+    }
+  }
+}
+
 }  // namespace w4
 
 // ---------------------------------------------------------------- host side
@@ -1201,10 +1480,20 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   a.g = (int)(num_heads / cache->kv_heads);
   a.window = window >= most ? 0 : (int)window;
   a.sinks = (int)std::min(sinks, most);
+  // Rows with this many columns in all fill the chip with whole tiles of them, whatever else there is.
+  constexpr int64_t kManyColumns = 9600;
+  const int64_t many = (kManyColumns + num_heads - 1) / num_heads;
+  a.many = most_new >= many ? (int)many : INT32_MAX;
+  const int64_t wide = tokens / many;  // such rows, at most
   const dim3 grid((unsigned)p.items);
+  const dim3 prompt((unsigned)(a.c.nkv * ((tokens * a.g + (w4::kPromptCols - 1) * wide) / w4::kPromptCols)));
   return by_dtype(dtype, [&](auto dt) {
     return by_code(cache->code, [&](auto ct) {
       return by_head(cache->head_dim, [&](auto d) {
+        if (most_new >= many) {
+          w4::paged8_prompt_kernel<dt(), ct(), d()><<<prompt, 256, 0, st>>>(a);
+          if (const int rc = check_launch("w4_paged8_attention (prompts)")) return rc;
+        }
         if (put) w4::paged8_attention_kernel<dt(), ct(), d(), w4::kP8Waves, true><<<grid, 64 * w4::kP8Waves, 0, st>>>(a);
         else w4::paged8_attention_kernel<dt(), ct(), d(), w4::kP8Waves, false><<<grid, 64 * w4::kP8Waves, 0, st>>>(a);
         return check_launch("w4_paged8_attention");

@@ -572,3 +572,78 @@ def test_codes_of_many_tokens(kind, dtype):
         up = (hi - y < y - lo) | ((hi - y == y - lo) & (codes[i] % 2 == 0))
         q = torch.where(up, hi, lo)
         assert torch.equal(got.view(T, nkv, d), (q * s.double().repeat_interleave(block, 0)[:T, :, None]).float())
+
+
+# ---------------------------------------------------------------- rows of many new tokens (9600 columns of all heads)
+PROMPTS = [
+    # (lengths, new tokens, heads, kv heads, head_dim, page size, block, window, sinks)
+    ([0], [160], 64, 2, 64, 16, 8, None, 0),
+    ([0, 5, 40, 0], [151, 1, 150, 3], 64, 2, 64, 64, 64, None, 0),
+    ([70, 0], [150, 150], 64, 4, 128, 32, 16, None, 0),
+    ([130], [205], 48, 16, 64, 64, 32, 50, 0),
+    ([300, 64], [170, 160], 60, 1, 128, 64, 32, 70, 5),
+    ([63], [151], 64, 8, 64, 8, 8, 1, 130),
+]
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("dtype", BOTH, ids=ids)
+@pytest.mark.parametrize("i", range(len(PROMPTS)))
+def test_prompts(i, dtype, kind):
+    lens, new, nh, nkv, d, S, block, window, sinks = PROMPTS[i]
+    c = R.case(lens, new, nh, nkv, d, S, block, kind, dtype, seed=70 + i, window=window, sinks=sinks)
+    g, out = _run(c, dtype, longest=max(new))
+    assert torch.equal(out, int4_hip.paged_attention8(**g))  # the same bits
+
+
+def test_prompts_that_are_no_rows():
+    """Idle and refused rows of many tokens, tokens of none, pages outside the pool, positions without angles."""
+    c = R.case([4, -1, 0, 9, 2], [150, 151, 152, 153, 2], 64, 2, 64, 16, 8, torch.int8, torch.float16, seed=80)
+    c["lengths"][2] = 1000
+    c["table"][3, 5] = -1
+    c["positions"][140] = -3
+    for n in ("q", "k", "v"):
+        c[n] = torch.cat((c[n], c[n][:70]))
+    c["positions"] = torch.cat((c["positions"], c["positions"][:70]))
+    _, out = _run(c, torch.float16)
+    assert (out[150:301] == 0).all() and out[301:453].isnan().all() and (out[-70:] == 0).all()
+    few = int4_hip.paged_attention8(**_to(c), longest=100)  # all rows but the last have more
+    live = torch.arange(678) >= 606
+    live[150:301] = True
+    assert few[~live.to(DEV)].isnan().all() and (few[150:301] == 0).all() and not few[606:608].isnan().any()
+
+
+def test_prompts_beside_codes_of_nan():
+    """Where nobody looks, and where some do."""
+    lens, new = [40, 10], [150, 160]
+    c = R.case(lens, new, 64, 2, 64, 32, 8, torch.float8_e4m3fn, torch.float16, seed=81, window=60, sinks=2)
+    for n in ("k_pages", "v_pages"):
+        x = c[n].view(torch.uint8)
+        keep = x.clone()
+        x[:] = 0x7F
+        for b, m in enumerate(lens):
+            for i in range(m + new[b]):
+                page = int(c["table"][b, i // 32])
+                x[page, :, i % 32] = keep[page, :, i % 32]
+    _, out = _run({k: t.clone() if isinstance(t, torch.Tensor) else t for k, t in c.items()}, torch.float16)
+    assert out.isfinite().all()
+    c["v_pages"].view(torch.uint8)[int(c["table"][0, 0]), 0, 20, 33] = 0xFF  # slot 20: seen up to slot 79
+    c["k_pages"].view(torch.uint8)[int(c["table"][1, 0]), 1, 1, 3] = 0x7F    # a sink
+    _, out = _run(c, torch.float16)
+    nan = out.view(310, 2, 32, 64).isnan().cpu()
+    assert nan[:40, 0, :, 33].all() and not nan[40:150, 0].any() and nan[150:, 1].all() and not nan[150:, 0].any()
+
+
+def test_prompts_in_a_graph():
+    c = R.case([50, 7], [150, 1], 64, 2, 64, 32, 16, torch.int8, torch.bfloat16, seed=82)
+    g = _to(c)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = int4_hip.paged_attention8(**g, longest=150)
+    want, mass, reach = R.attention(**c)
+    for _ in range(3):
+        graph.replay()
+        eager = int4_hip.paged_attention8(**g)
+        torch.cuda.synchronize()
+        _check(out, want, mass, reach, torch.bfloat16, 224, 64)
+        assert torch.equal(out, eager)
