@@ -535,6 +535,14 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
+// Which of the slots from.. from + 7 the token of slot `mine` sees, a bit each.
+__device__ __forceinline__ uint32_t seen8(int from, int mine, int window, int sinks) {
+  auto below = [&](int slot) { return (1u << min(max(max(slot, 0) - from, 0), 8)) - 1u; };  // those before it
+  uint32_t v = below(mine + 1);
+  if (window) v &= ~below(mine - window + 1) | below(sinks);
+  return v;
+}
+
 // A workgroup's four waves take units of 64 slots in turn, each its own.
 //
 // Both products are 16x16x32 bf16 matrix instructions, transposed, with the columns (new tokens x query heads of the
@@ -806,9 +814,6 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
 #pragma unroll
     for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4*>(vw + put_at + i * (VR * D)) = vr[i];
     wave_lds_order();
-    auto seen = [&](int slot) {
-      return slot <= mine && (!a.window || slot > mine - a.window || slot < a.sinks);
-    };
     if constexpr (CT == W4_CODE_E4M3) {
       // e4m3 has a NaN: what a program that is not this one left in the pages.  It must not meet the probability 0 of a
       // slot that is not seen, so it is taken out here, and what sees it is made NaN by itself.  (Where all is seen, it
@@ -821,7 +826,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
           for (int e = 0; e < 4; ++e) any |= nan_bytes(vr[i][e]);
         if (__ballot(any != 0)) {
           for (int row = 0; row < UP; ++row) {
-            const bool see = seen(base + row);
+            const bool see = seen8(base + row, mine, a.window, a.sinks) & 1;
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
               const uint32_t w = *reinterpret_cast<const uint32_t*>(vw + row * D + ((d ^ swizzle(row)) << 4) + 4 * c);
@@ -851,16 +856,25 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
       load_ids(min(u + 2 * W, u1 - 1), next_ids);
     }
 
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[kb][t] *= sk[kb];
+    if (!whole) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const uint32_t sight = seen8(base + kb * 32 + 8 * c, mine, a.window, a.sinks);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[kb][e >> 2][e & 3] = sight >> e & 1 ? s[kb][e >> 2][e & 3] : -__builtin_inff();
+        // (a scale that is NaN is no matter of a token that sees none of its slots)
+        sv[kb] = sight ? sv[kb] : 0.f;
+      }
+    }
     float top = -__builtin_inff();
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float x = s[kb][e >> 2][e & 3] * sk[kb];
-        if (!whole) x = seen(base + kb * 32 + 8 * c + e) ? x : -__builtin_inff();
-        top = fmaxf(top, x);
-        s[kb][e >> 2][e & 3] = x;
-      }
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, s[kb][e >> 2][e & 3]);
     // The reference is raised once a score passes it by 8 powers of two; probabilities stay below 1 all the same.
     if (__ballot((top - m) * kLog2e > 8.f)) {
       float mn = fmaxf(top, m);
@@ -883,7 +897,6 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
         p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3] - mz, kLog2e, -8.f));
         l += p[e];
         p[e] *= sv[kb];
-        if (!whole) p[e] = seen(base + kb * 32 + 8 * c + e) ? p[e] : 0.f;
       }
       u32x4 pf[NP];
       split8<W4_DTYPE_BF16, false>(p, pf);
@@ -980,7 +993,7 @@ constexpr int kPromptCols = 64, kPromptUnit = 64;
 // paged8_attention_kernel, whose waves share their columns and not the slots: that spreads a few columns over the chip,
 // but converts every code for sixteen columns alone.
 template <int DT, int CT, int D>
-__global__ __launch_bounds__(256, 2) void paged8_prompt_kernel(Attend8Args a) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Attend8Args a) {
   constexpr int UP = kPromptUnit, KB = UP / 32, NJ = D / 32, ND = D / 16, NP = Split<W4_DTYPE_BF16>::N;
   constexpr int KROW = D + 8;               // halfwords of a key row in LDS: sixteen rows on different banks
   constexpr int VROW = D == 64 ? 72 : 144;  // of a value row: four rows of 32 bytes on different banks
@@ -1140,7 +1153,6 @@ __global__ __launch_bounds__(256, 2) void paged8_prompt_kernel(Attend8Args a) {
   f32x4 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto seen = [&](int slot) { return slot <= mine && (!a.window || slot > mine - a.window || slot < a.sinks); };
   for (int u = 0; u < units; ++u) {
     const int base = base_of(u), buf = u & 1;
     if (u + 1 < units) {  // the next unit's loads travel under this one's products
@@ -1151,33 +1163,44 @@ __global__ __launch_bounds__(256, 2) void paged8_prompt_kernel(Attend8Args a) {
     if (base <= w_last && (!a.window || base + UP - 1 > w_first - a.window || base < a.sinks)) {
       const bool whole = base + UP - 1 <= w_first && (!a.window || base > w_last - a.window || base + UP <= a.sinks);
       f32x4 s[KB][2];
-      float top = -__builtin_inff();
+      float sv[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const float sk = ks_s[buf][4 * kb + c];
+        sv[kb] = vs_s[buf][4 * kb + c];
+        bf16x8 kf[2][NJ];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const uint16_t* const at = &k_s[buf][(kb * 32 + t * 16 + l16) * KROW + 8 * c];
-          bf16x8 kf[NJ];
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) kf[j] = *reinterpret_cast<const bf16x8*>(at + 32 * j);
+          for (int j = 0; j < NJ; ++j)
+            kf[t][j] = *reinterpret_cast<const bf16x8*>(&k_s[buf][(kb * 32 + t * 16 + l16) * KROW + 8 * c + 32 * j]);
           s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll
-          for (int p = NP - 1; p >= 0; --p)
+        for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) s[kb][t] = M::m16(kf[j], __builtin_bit_cast(bf16x8, qf[j][p]), s[kb][t]);
-          s[kb][t] *= sk;
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[kb][t] = M::m16(kf[t][j], __builtin_bit_cast(bf16x8, qf[j][p]), s[kb][t]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[kb][t] *= sk;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const uint32_t sight = seen8(base + kb * 32 + 8 * c, mine, a.window, a.sinks);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            s[kb][e >> 2][e & 3] = sight >> e & 1 ? s[kb][e >> 2][e & 3] : -__builtin_inff();
+          // (a scale that is NaN is no matter of a token that sees none of its slots)
+          sv[kb] = sight ? sv[kb] : 0.f;
         }
       }
+      float top = -__builtin_inff();
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float x = s[kb][e >> 2][e & 3];
-          if (!whole) x = seen(base + kb * 32 + 8 * c + e) ? x : -__builtin_inff();
-          top = fmaxf(top, x);
-          s[kb][e >> 2][e & 3] = x;
-        }
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, s[kb][e >> 2][e & 3]);
       if (__ballot((top - m) * kLog2e > 8.f)) {
         float mn = fmaxf(top, m);
         mn = fmaxf(mn, __shfl_xor(mn, 16));
@@ -1193,31 +1216,32 @@ __global__ __launch_bounds__(256, 2) void paged8_prompt_kernel(Attend8Args a) {
       const float mz = finite_or_zero(m);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const float sv = vs_s[buf][4 * kb + c];
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3] - mz, kLog2e, -8.f));
           l += p[e];
-          p[e] *= sv;
-          if (!whole) p[e] = seen(base + kb * 32 + 8 * c + e) ? p[e] : 0.f;
+          p[e] *= sv[kb];
         }
         u32x4 pf[NP];
         split8<W4_DTYPE_BF16, false>(p, pf);
+        bf16x8 vf[ND];
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           const uint16_t* at = &v_s[buf][(kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3)];
           const s16x4 vl = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
           const s16x4 vh = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * VROW));
           const u32x2 lw = __builtin_bit_cast(u32x2, vl), hw = __builtin_bit_cast(u32x2, vh);
-          const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{lw[0], lw[1], hw[0], hw[1]});
-#pragma unroll
-          for (int q = NP - 1; q >= 0; --q) o[d] = M::m16(vf, __builtin_bit_cast(bf16x8, pf[q]), o[d]);
+          vf[d] = __builtin_bit_cast(bf16x8, u32x4{lw[0], lw[1], hw[0], hw[1]});
         }
+#pragma unroll
+        for (int q = NP - 1; q >= 0; --q)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[d] = M::m16(vf[d], __builtin_bit_cast(bf16x8, pf[q]), o[d]);
       }
       if (CT == W4_CODE_E4M3 && odd_s[buf] == u) {
         for (int row = 0; row < UP; ++row) {
-          const bool see = seen(base + row);
+          const bool see = seen8(base + row, mine, a.window, a.sinks) & 1;
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
             const uint32_t bits = nan_s[buf][row * CH + d] >> (4 * c);
@@ -1485,7 +1509,9 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   const int64_t many = (kManyColumns + num_heads - 1) / num_heads;
   a.many = most_new >= many ? (int)many : INT32_MAX;
   const int64_t wide = tokens / many;  // such rows, at most
-  const dim3 grid((unsigned)p.items);
+  // (and the others' tokens)
+  const int64_t rest = most_new >= many ? std::min(tokens, cache->rows * (many - 1)) : tokens;
+  const dim3 grid((unsigned)attend8_plan(cache->rows, rest, num_heads, cache->kv_heads, cache->head_dim).items);
   const dim3 prompt((unsigned)(a.c.nkv * ((tokens * a.g + (w4::kPromptCols - 1) * wide) / w4::kPromptCols)));
   return by_dtype(dtype, [&](auto dt) {
     return by_code(cache->code, [&](auto ct) {
