@@ -475,8 +475,8 @@ constexpr int kP8Unit = 32;  // slots that a wave takes at once
 constexpr int kP8AtOnce = 8;  // parts that a thread of the joining reads together
 constexpr int kP8Waves = 4, kP8Parts = 512, kP8MinUnits = 4;
 
-// Rows are cut into parts of about (all columns' tiles x units of slots) / 256, so that time follows the slots there
-// are and not the table.  Those that are cut have at most 2 * kP8Parts parts in all: each has more units than `per`,
+// Rows are cut into parts of about (all columns' tiles x units of slots) / kP8Parts, so that time follows the slots
+// there are and not the table.  Those that are cut have at most 2 * kP8Parts parts in all: each has more units than `per`,
 // and kP8Parts * per are at least all there are.
 template <int UP>
 __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8* it, int* total) {
@@ -535,6 +535,79 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
+// Eight codes, which fp16 holds exactly.
+template <int CT>
+__device__ __forceinline__ f16x8 codes8h(uint32_t lo, uint32_t hi) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  f16x2 r[4];
+  if constexpr (CT == W4_CODE_E4M3) {
+    r[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+    r[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+    r[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+    r[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  } else {
+    // below the exponent of 1024 a byte is 1024 + the code + 128
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = (i < 2 ? lo : hi) ^ 0x80808080u;
+      const uint32_t b = __builtin_amdgcn_perm(0x64646464u, w, i & 1 ? 0x04030402u : 0x04010400u);
+      r[i] = __builtin_bit_cast(f16x2, b) - (f16x2){(_Float16)1152.f, (_Float16)1152.f};
+    }
+  }
+  return __builtin_bit_cast(f16x8, (u32x4){__builtin_bit_cast(uint32_t, r[0]), __builtin_bit_cast(uint32_t, r[1]),
+                                           __builtin_bit_cast(uint32_t, r[2]), __builtin_bit_cast(uint32_t, r[3])});
+}
+
+// Numbers below 2^16 as the sums of two of fp16: within 2^-24 of themselves, or 2^-25 where they are below 1/2.
+__device__ __forceinline__ void halves8(const float x[8], f16x8 out[2]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  f16x2 h[4], r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), f16x2);
+    r[i] = __builtin_convertvector((f32x2{x[2 * i] - (float)h[i][0], x[2 * i + 1] - (float)h[i][1]}), f16x2);
+  }
+  __builtin_memcpy(&out[0], h, 16);
+  __builtin_memcpy(&out[1], r, 16);
+}
+
+// The power of two (2^-115.. 2^126) that takes numbers up to `most` below 2^to and above 2^(to - 2).
+__device__ __forceinline__ float raise_to(float most, int to) {
+  const int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23 & 0xFF) - 127;  // most < 2^(e + 1)
+  return __builtin_bit_cast(float, (uint32_t)(min(max(to - 1 - e, -115), 126) + 127) << 23);
+}
+__device__ __forceinline__ float inverse_power(float f) {  // of such a power
+  return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, f));
+}
+
+// A column's rotated query, of which a lane has some elements, in two parts of fp16; the factor it is short of.  One
+// that holds an infinity or NaN is NaN.
+template <int NJ>
+__device__ __forceinline__ float query_parts(const float (*x)[8], f16x8 (*qf)[2]) {
+  float top = 0.f;
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      top = fmaxf(top, __builtin_fabsf(x[j][e]));
+      odd |= !(__builtin_fabsf(x[j][e]) < __builtin_inff());
+    }
+  if (odd) top = __builtin_inff();
+  top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const float f = raise_to(top, 15);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[j][e] * f;
+    halves8(y, qf[j]);
+  }
+  return top < __builtin_inff() ? inverse_power(f) : __builtin_nanf("");
+}
+
 // Which of the slots from.. from + 7 the token of slot `mine` sees, a bit each.
 __device__ __forceinline__ uint32_t seen8(int from, int mine, int window, int sinks) {
   auto below = [&](int slot) { return (1u << min(max(max(slot, 0) - from, 0), 8)) - 1u; };  // those before it
@@ -543,12 +616,17 @@ __device__ __forceinline__ uint32_t seen8(int from, int mine, int window, int si
   return v;
 }
 
-// A workgroup's four waves take units of 64 slots in turn, each its own.
+// A workgroup's four waves take units of 32 slots in turn, each its own.
 //
-// Both products are 16x16x32 bf16 matrix instructions, transposed, with the columns (new tokens x query heads of the
-// group) as their columns: S^T = K Q^T, then O^T = V^T P^T.  Codes are bf16 numbers exactly; the scales stay outside:
-// a slot's score is multiplied by its key's, its probability by its value's.  Queries and probabilities enter as the
-// sum of three bf16 numbers, 24 bits, so the result has about fp32's error before its one rounding.
+// Both products are 16x16x32 fp16 matrix instructions, transposed, with the columns (new tokens x query heads of the
+// group) as their columns: S^T = K Q^T, then O^T = V^T P^T.  Codes are fp16 numbers exactly; the scales stay outside: a
+// slot's score is multiplied by its key's, its probability by its value's, which makes its weight.  Queries and weights
+// enter as the sum of two fp16 numbers, so within 2^-24 of themselves, about fp32's error, as long as they are not far
+// below the largest of their column: a power of two takes a column's queries below 2^15 and its weights below 2^15, and
+// the smallest step of fp16 is then 2^-38 of the largest query and 2^-35 (2^-40 at best) of the largest weight.  The
+// weights' power follows the largest so far: it changes with the softmax's reference, and when a weight passes 2^15.
+// (Three bf16 numbers each hold any size and cost half as many matrix instructions again and twice the other ones: 32
+// rows of up to 4000 slots 29.3 us instead of 26.8, 131000 slots 63 instead of 58, a window 25 instead of 21.)
 //
 // Keys come from memory straight into the first product's operand: its inner index may run over a head in any order,
 // so a lane takes sixteen bytes in a row of a slot, four lanes 64.  A tile's row r is slot 8 (r / 4) + 4 t + r % 4 of its
@@ -560,14 +638,14 @@ __device__ __forceinline__ uint32_t seen8(int from, int mine, int window, int si
 // paged8_append_kernel does.
 template <int DT, int CT, int D, int W, bool PUT>
 __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_attention_kernel(Attend8Args a) {
-  constexpr int UP = kP8Unit, KB = UP / 32, NJ = D / 32, ND = D / 16, NP = Split<W4_DTYPE_BF16>::N;
+  constexpr int UP = kP8Unit, KB = UP / 32, NJ = D / 32, ND = D / 16;
   constexpr int KC = D / 64;               // 16-byte loads of a key a lane
   constexpr int VR = 1024 / D, VC = D / 16;  // rows of values in a load of the wave, 16-byte chunks of a row
   constexpr int NV = UP / VR;
   constexpr int OROW = D + 4;              // floats of an output row in LDS
   constexpr int WAVE_B = 16 * OROW * 4 > UP * D ? 16 * OROW * 4 : UP * D;
   constexpr int kThreads = 64 * W;
-  typedef Mfma<W4_DTYPE_BF16> M;
+  typedef Mfma<W4_DTYPE_FP16> M;
   __shared__ __attribute__((aligned(16))) uint8_t v_s[W][WAVE_B];
   __shared__ float m_s[W][16], l_s[W][16];
   __shared__ __attribute__((aligned(16))) uint8_t new_s[2][D];
@@ -674,8 +752,10 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
   // The query of this lane's column; columns past the last copy it and count for nothing.
   const int col = min(l16, cols - 1), tok = it.o0 + (col0 + col) / a.g;
   const int mine = len + (col0 + col) / a.g;  // its slot
-  u32x4 qf[NJ][NP];
+  f16x8 qf[NJ][2];
+  float q_short;
   {
+    float xs[NJ][8];
     const int pos = a.positions[tok];
     const bool there = (uint64_t)(int64_t)pos < (uint64_t)a.angles;
     const uint16_t* const qp = a.q + tok * a.stride_q + (h * a.g + (col0 + col) % a.g) * D;
@@ -686,9 +766,10 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
     // chunk of the lane or (D = 64) another lane's
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
+      float* const x = xs[j];
       const int d = 64 * (j >> 1) + 16 * c + 8 * (j & 1), da = d & (D / 2 - 1);
       const bool low = D == 128 ? j < 2 : c < 2;
-      float x[8], y[8];
+      float y[8];
       unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + d), x);
       unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + (d ^ (D / 2))), y);
       const f32x4* const cp = reinterpret_cast<const f32x4*>(cosr + da);
@@ -701,8 +782,8 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
         if (low) rope_pair(x[e], y[e], cc, ss, &r1, &r2), x[e] = r1 * scale;
         else rope_pair(y[e], x[e], cc, ss, &r1, &r2), x[e] = r2 * scale;
       }
-      split8<W4_DTYPE_BF16, true>(x, qf[j]);
     }
+    q_short = query_parts<NJ>(xs, qf);
   }
 
   // The new token, quantised (the wave that takes the last unit): its codes in LDS, its block's scales.
@@ -740,6 +821,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
   }
 
   float m = -__builtin_inff(), l = 0.f;  // the column's reference and this lane's share of its sum
+  float heavy = 0.f, lift = 1.f;         // the largest of this lane's weights, what the column's are multiplied by
   f32x4 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -794,19 +876,19 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        bf16x8 kf[NJ];
+        f16x8 kf[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           uint32_t k0 = kr[kb][t][j >> 1][2 * (j & 1)], k1 = kr[kb][t][j >> 1][2 * (j & 1) + 1];
           // (hidden, or the compiler converts where the words are loaded and holds four times as many registers)
           asm("" : "+v"(k0), "+v"(k1));
-          kf[j] = codes8<CT>(k0, k1);
+          kf[j] = codes8h<CT>(k0, k1);
         }
         s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int p = NP - 1; p >= 0; --p)  // the small parts first
+        for (int p = 1; p >= 0; --p)  // the small parts first
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) s[kb][t] = M::m16(kf[j], __builtin_bit_cast(bf16x8, qf[j][p]), s[kb][t]);
+          for (int j = 0; j < NJ; ++j) s[kb][t] = M::m16(kf[j], qf[j][p], s[kb][t]);
       }
     // A slot that a column does not see has score -inf and, whatever is stored there, no share in the output.
     const bool whole = base + UP - 1 <= first_slot && (!a.window || base > last_slot - a.window || base + UP <= a.sinks);
@@ -848,7 +930,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
     }
     float sk[KB], sv[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) sk[kb] = ks[kb], sv[kb] = vs[kb];
+    for (int kb = 0; kb < KB; ++kb) sk[kb] = ks[kb] * q_short, sv[kb] = vs[kb];
     if (u + W < u1) {  // the next unit's loads travel under the rest
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) ids[kb] = next_ids[kb];
@@ -870,42 +952,57 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
         sv[kb] = sight ? sv[kb] : 0.f;
       }
     }
-    float top = -__builtin_inff();
+    float top = -__builtin_inff(), top_kb[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < KB; ++kb) {
+      top_kb[kb] = s[kb][0][0];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, s[kb][e >> 2][e & 3]);
-    // The reference is raised once a score passes it by 8 powers of two; probabilities stay below 1 all the same.
+      for (int e = 1; e < 8; ++e) top_kb[kb] = fmaxf(top_kb[kb], s[kb][e >> 2][e & 3]);
+      top = fmaxf(top, top_kb[kb]);
+    }
+    // A column's reference is raised once a score passes it by 8 powers of two; probabilities are 2^6 at most.
+    float al = 1.f;
     if (__ballot((top - m) * kLog2e > 8.f)) {
-      float mn = fmaxf(top, m);
-      mn = fmaxf(mn, __shfl_xor(mn, 16));
+      float mn = fmaxf(top, __shfl_xor(top, 16));
       mn = fmaxf(mn, __shfl_xor(mn, 32));
-      const float al = __builtin_amdgcn_exp2f((m - finite_or_zero(mn)) * kLog2e);
+      mn = (mn - m) * kLog2e > 8.f ? mn : m;
+      al = __builtin_amdgcn_exp2f((m - finite_or_zero(mn)) * kLog2e);
       l *= al;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[d][e] *= al;
+      heavy *= al;
       m = mn;
     }
     const float mz = finite_or_zero(m);
+    auto prob = [&](float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x - mz, kLog2e, -2.f)); };    // The largest of eight slots' weights with one scale is that of their largest score.
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) heavy = fmaxf(heavy, prob(top_kb[kb]) * sv[kb]);
+    if (__ballot(al < 1.f || heavy * lift > 0x1p15f)) {
+      heavy = fmaxf(heavy, __shfl_xor(heavy, 16));
+      heavy = fmaxf(heavy, __shfl_xor(heavy, 32));
+      const float to = al < 1.f || heavy * lift > 0x1p15f ? raise_to(heavy, 12) : lift;
+      const float by = al * fminf(to * inverse_power(lift), 0x1p127f);
+      lift = to;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] *= by;
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3] - mz, kLog2e, -8.f));
+        p[e] = prob(s[kb][e >> 2][e & 3]);
         l += p[e];
-        p[e] *= sv[kb];
+        p[e] = p[e] * sv[kb] * lift;
       }
-      u32x4 pf[NP];
-      split8<W4_DTYPE_BF16, false>(p, pf);
+      f16x8 pf[2];
+      halves8(p, pf);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(vw + (get_at ^ (d << 4)) + kb * (32 * D)));
-        const bf16x8 vf = codes8<CT>((uint32_t)w[0], (uint32_t)w[1]);
+        const f16x8 vf = codes8h<CT>((uint32_t)w[0], (uint32_t)w[1]);
 #pragma unroll
-        for (int q = NP - 1; q >= 0; --q) o[d] = M::m16(vf, __builtin_bit_cast(bf16x8, pf[q]), o[d]);
+        for (int q = 1; q >= 0; --q) o[d] = M::m16(vf, pf[q], o[d]);
       }
     }
   }
@@ -916,8 +1013,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
 #pragma unroll
-  for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(ow + l16 * OROW + d * 16 + 4 * c) = o[d];
-  if (c == 0) m_s[wv][l16] = m, l_s[wv][l16] = l;
+  for (int d = 0; d < ND; ++d)
+    *reinterpret_cast<f32x4*>(ow + l16 * OROW + d * 16 + 4 * c) = o[d] * (0x1p-6f * inverse_power(lift));
+  if (c == 0) m_s[wv][l16] = m, l_s[wv][l16] = 0x1p-6f * l;
   __syncthreads();
   constexpr int STRIDE = 16 * D;
   const int quads = cols * (D / 4);
@@ -989,16 +1087,16 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
 constexpr int kPromptCols = 64, kPromptUnit = 64;
 
 // A workgroup has 64 columns of a row and key-value head, sixteen a wave, and all the slots that they see, 64 at once:
-// the four waves turn the codes into bf16 in LDS together, once, and multiply from there.  Otherwise as
+// the four waves turn the codes into fp16 in LDS together, once, and multiply from there.  Otherwise as
 // paged8_attention_kernel, whose waves share their columns and not the slots: that spreads a few columns over the chip,
 // but converts every code for sixteen columns alone.
 template <int DT, int CT, int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Attend8Args a) {
-  constexpr int UP = kPromptUnit, KB = UP / 32, NJ = D / 32, ND = D / 16, NP = Split<W4_DTYPE_BF16>::N;
+  constexpr int UP = kPromptUnit, KB = UP / 32, NJ = D / 32, ND = D / 16;
   constexpr int KROW = D + 8;               // halfwords of a key row in LDS: sixteen rows on different banks
   constexpr int VROW = D == 64 ? 72 : 144;  // of a value row: four rows of 32 bytes on different banks
   constexpr int CH = D / 16, NC = UP * CH / 256;  // chunks of 16 codes of a slot, and of a thread
-  typedef Mfma<W4_DTYPE_BF16> M;
+  typedef Mfma<W4_DTYPE_FP16> M;
   __shared__ __attribute__((aligned(16))) uint16_t k_s[2][UP * KROW], v_s[2][UP * VROW];
   __shared__ float ks_s[2][UP / 8], vs_s[2][UP / 8];
   __shared__ uint16_t nan_s[2][CT == W4_CODE_E4M3 ? UP * CH : 1];
@@ -1103,8 +1201,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
       }
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        *reinterpret_cast<bf16x8*>(&k_s[buf][row * KROW + ch * 16 + 8 * g]) = codes8<CT>(kr[i][2 * g], kr[i][2 * g + 1]);
-        *reinterpret_cast<bf16x8*>(&v_s[buf][slot * VROW + ch * 16 + 8 * g]) = codes8<CT>(vr[i][2 * g], vr[i][2 * g + 1]);
+        *reinterpret_cast<f16x8*>(&k_s[buf][row * KROW + ch * 16 + 8 * g]) = codes8h<CT>(kr[i][2 * g], kr[i][2 * g + 1]);
+        *reinterpret_cast<f16x8*>(&v_s[buf][slot * VROW + ch * 16 + 8 * g]) = codes8h<CT>(vr[i][2 * g], vr[i][2 * g + 1]);
       }
     }
     if (tid < 8) ks_s[buf][tid] = sr;
@@ -1118,8 +1216,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
   load_ids(min(1, units - 1));
 
   const int col = min(wv * 16 + l16, cols - 1), tok = sp.o0 + (col0 + col) / a.g, mine = len + (col0 + col) / a.g;
-  u32x4 qf[NJ][NP];
+  f16x8 qf[NJ][2];
+  float q_short;
   {
+    float xs[NJ][8];
     const int pos = a.positions[tok];
     const bool there = (uint64_t)(int64_t)pos < (uint64_t)a.angles;
     const uint16_t* const qp = a.q + tok * a.stride_q + (h * a.g + (col0 + col) % a.g) * D;
@@ -1129,7 +1229,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
 #pragma unroll
     for (int j = 0; j < NJ / 2; ++j) {
       const int d = 32 * j + 8 * c;
-      float x[8], y[8];
+      float *const x = xs[j], *const y = xs[j + NJ / 2];
       unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + d), x);
       unpack8<DT>(*reinterpret_cast<const u32x4*>(qp + d + D / 2), y);
       const f32x4* const cp = reinterpret_cast<const f32x4*>(cosr + d);
@@ -1141,15 +1241,14 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
         rope_pair(x[e], y[e], cs[e >> 2][e & 3], sn[e >> 2][e & 3], &r1, &r2);
         x[e] = r1 * scale, y[e] = r2 * scale;
       }
-      split8<W4_DTYPE_BF16, true>(x, qf[j]);
-      split8<W4_DTYPE_BF16, true>(y, qf[j + NJ / 2]);
     }
+    q_short = query_parts<NJ>(xs, qf);
   }
   __syncthreads();
   stage(0);
   __syncthreads();
 
-  float m = -__builtin_inff(), l = 0.f;
+  float m = -__builtin_inff(), l = 0.f, heavy = 0.f, lift = 1.f;  // as there
   f32x4 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1166,22 +1265,22 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
       float sv[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const float sk = ks_s[buf][4 * kb + c];
+        const float sk = ks_s[buf][4 * kb + c] * q_short;
         sv[kb] = vs_s[buf][4 * kb + c];
-        bf16x8 kf[2][NJ];
+        f16x8 kf[2][NJ];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
           for (int j = 0; j < NJ; ++j)
-            kf[t][j] = *reinterpret_cast<const bf16x8*>(&k_s[buf][(kb * 32 + t * 16 + l16) * KROW + 8 * c + 32 * j]);
+            kf[t][j] = *reinterpret_cast<const f16x8*>(&k_s[buf][(kb * 32 + t * 16 + l16) * KROW + 8 * c + 32 * j]);
           s[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
 #pragma unroll
-        for (int p = NP - 1; p >= 0; --p)
+        for (int p = 1; p >= 0; --p)  // the small parts first
 #pragma unroll
           for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) s[kb][t] = M::m16(kf[t][j], __builtin_bit_cast(bf16x8, qf[j][p]), s[kb][t]);
+            for (int t = 0; t < 2; ++t) s[kb][t] = M::m16(kf[t][j], qf[j][p], s[kb][t]);
 #pragma unroll
         for (int t = 0; t < 2; ++t) s[kb][t] *= sk;
       }
@@ -1196,48 +1295,63 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
           sv[kb] = sight ? sv[kb] : 0.f;
         }
       }
-      float top = -__builtin_inff();
+      float top = -__builtin_inff(), top_kb[KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+      for (int kb = 0; kb < KB; ++kb) {
+        top_kb[kb] = s[kb][0][0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, s[kb][e >> 2][e & 3]);
+        for (int e = 1; e < 8; ++e) top_kb[kb] = fmaxf(top_kb[kb], s[kb][e >> 2][e & 3]);
+        top = fmaxf(top, top_kb[kb]);
+      }
+      float al = 1.f;
       if (__ballot((top - m) * kLog2e > 8.f)) {
-        float mn = fmaxf(top, m);
-        mn = fmaxf(mn, __shfl_xor(mn, 16));
+        float mn = fmaxf(top, __shfl_xor(top, 16));
         mn = fmaxf(mn, __shfl_xor(mn, 32));
-        const float al = __builtin_amdgcn_exp2f((m - finite_or_zero(mn)) * kLog2e);
+        mn = (mn - m) * kLog2e > 8.f ? mn : m;
+        al = __builtin_amdgcn_exp2f((m - finite_or_zero(mn)) * kLog2e);
         l *= al;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[d][e] *= al;
+        heavy *= al;
         m = mn;
       }
       const float mz = finite_or_zero(m);
+      auto prob = [&](float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x - mz, kLog2e, -2.f)); };
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) heavy = fmaxf(heavy, prob(top_kb[kb]) * sv[kb]);
+      if (__ballot(al < 1.f || heavy * lift > 0x1p15f)) {
+        heavy = fmaxf(heavy, __shfl_xor(heavy, 16));
+        heavy = fmaxf(heavy, __shfl_xor(heavy, 32));
+        const float to = al < 1.f || heavy * lift > 0x1p15f ? raise_to(heavy, 12) : lift;
+        const float by = al * fminf(to * inverse_power(lift), 0x1p127f);
+        lift = to;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][e] *= by;
+      }
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e >> 2][e & 3] - mz, kLog2e, -8.f));
+          p[e] = prob(s[kb][e >> 2][e & 3]);
           l += p[e];
-          p[e] *= sv[kb];
+          p[e] = p[e] * sv[kb] * lift;
         }
-        u32x4 pf[NP];
-        split8<W4_DTYPE_BF16, false>(p, pf);
-        bf16x8 vf[ND];
+        f16x8 pf[2];
+        halves8(p, pf);
+        f16x8 vf[ND];
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           const uint16_t* at = &v_s[buf][(kb * 32 + 8 * c + (l16 >> 2)) * VROW + d * 16 + 4 * (l16 & 3)];
           const s16x4 vl = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
           const s16x4 vh = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * VROW));
           const u32x2 lw = __builtin_bit_cast(u32x2, vl), hw = __builtin_bit_cast(u32x2, vh);
-          vf[d] = __builtin_bit_cast(bf16x8, u32x4{lw[0], lw[1], hw[0], hw[1]});
+          vf[d] = __builtin_bit_cast(f16x8, u32x4{lw[0], lw[1], hw[0], hw[1]});
         }
 #pragma unroll
-        for (int q = NP - 1; q >= 0; --q)
+        for (int q = 1; q >= 0; --q)
 #pragma unroll
-          for (int d = 0; d < ND; ++d) o[d] = M::m16(vf[d], __builtin_bit_cast(bf16x8, pf[q]), o[d]);
+          for (int d = 0; d < ND; ++d) o[d] = M::m16(vf[d], pf[q], o[d]);
       }
       if (CT == W4_CODE_E4M3 && odd_s[buf] == u) {
         for (int row = 0; row < UP; ++row) {
@@ -1260,13 +1374,13 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   if (wv * 16 + l16 < cols) {
-    const float inv = 1.f / l;
+    const float inv = 1.f / l, down = inverse_power(lift);
     uint16_t* const out = out_at(wv * 16 + l16) + 4 * c;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       u32x2 w;
-      w[0] = (uint32_t)float_to_act_bits<DT>(o[d][0] * inv) | ((uint32_t)float_to_act_bits<DT>(o[d][1] * inv) << 16);
-      w[1] = (uint32_t)float_to_act_bits<DT>(o[d][2] * inv) | ((uint32_t)float_to_act_bits<DT>(o[d][3] * inv) << 16);
+      w[0] = (uint32_t)float_to_act_bits<DT>(o[d][0] * inv * down) | ((uint32_t)float_to_act_bits<DT>(o[d][1] * inv * down) << 16);
+      w[1] = (uint32_t)float_to_act_bits<DT>(o[d][2] * inv * down) | ((uint32_t)float_to_act_bits<DT>(o[d][3] * inv * down) << 16);
       *reinterpret_cast<u32x2*>(out + 16 * d) = w;
     }
   }

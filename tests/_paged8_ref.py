@@ -146,6 +146,7 @@ def attention(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, leng
             out[o0:o1] = NAN
             continue
         kk, vv = (values(x, s, table[b], n + o1 - o0) for x, s in ((k_pages, k_scale), (v_pages, v_scale)))
+        scale = values(torch.ones_like(v_pages), v_scale, table[b], n + o1 - o0)[..., 0]
         for t in range(o0, o1):
             i = n + t - o0
             j = torch.arange(i + 1)
@@ -161,7 +162,14 @@ def attention(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, leng
                 p = torch.softmax(key @ x[h] / math.sqrt(d), 0)
                 # (a probability that fp32 cannot have, 2^-118 of the largest with the reference 2^8 behind, is lost: the
                 # tolerance, 2^-21 of the mass or more, is to hold n 2^-110 of the largest value)
-                out[t, h], mass[t, h] = p @ val, p @ val.abs() + len(seen) * 2.0 ** -89 * val.nan_to_num().abs().max()
+                # (weights, probability times scale, enter as two numbers of 11 bits each, whose smallest step is 2^-24:
+                # with the column's largest raised past 2^10, they are within 2^-35 of the largest at worst, 2^-14 of
+                # that 2^-21)
+                step = scale[seen, h // (nh // nkv)]
+                sums = (val / step[:, None]).nan_to_num().abs().sum(0)
+                out[t, h] = p @ val
+                mass[t, h] = (p @ val.abs() + len(seen) * 2.0 ** -89 * val.nan_to_num().abs().max()
+                              + 2.0 ** -14 * (p * step).nan_to_num().max() * sums)
                 reach[t, h] = (key.abs() @ x[h].abs()).max() / math.sqrt(d)
     return out.flatten(1), mass.flatten(1), reach.expand(-1, -1, d).flatten(1)
 

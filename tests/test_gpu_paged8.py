@@ -647,3 +647,44 @@ def test_prompts_in_a_graph():
         torch.cuda.synchronize()
         _check(out, want, mass, reach, torch.bfloat16, 224, 64)
         assert torch.equal(out, eager)
+
+
+# ---------------------------------------------------------------- numbers of every size
+FAR = [([200, 150, 90], [1, 2, 1], 4, 2, 64, 16, 8), ([700, 300], [1, 1], 6, 1, 128, 32, 16),
+       ([40, 9], [152, 3], 64, 2, 64, 32, 8), ([60], [76], 128, 2, 128, 64, 16)]
+
+
+@pytest.mark.parametrize("lens,new,nh,nkv,d,S,block", FAR)
+def test_scales_in_any_order(lens, new, nh, nkv, d, S, block):
+    """Value scales up to 2^60 apart from one block to the next: what is large often has next to no probability."""
+    c = R.case(lens, new, nh, nkv, d, S, block, torch.int8, torch.bfloat16, seed=91)
+    c["v_scale"] *= torch.exp2(30 * torch.sin(torch.arange(c["v_scale"].numel()) * 1.7)).view(c["v_scale"].shape)
+    c["q"] *= 4
+    _run(c, torch.bfloat16, longest=max(new))
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("lens,new,nh,nkv,d,S,block", FAR)
+def test_the_largest_and_the_smallest_numbers(lens, new, nh, nkv, d, S, block, kind):
+    """Queries of 2^100 on keys of 2^-100 and the other way round, values of 2^120 and of 2^-110."""
+    for up, there in ((100, 120), (-100, -110)):
+        c = R.case(lens, new, nh, nkv, d, S, block, kind, torch.bfloat16, seed=92)
+        c["q"] *= 2.0 ** up
+        c["k"] *= 2.0 ** -up
+        c["v"] *= 2.0 ** there
+        most = MOST[kind]
+        c["k_scale"] = torch.full_like(c["k_scale"], 2.0 ** -up / most)
+        c["v_scale"] = torch.full_like(c["v_scale"], 2.0 ** there / most)
+        _run(c, torch.bfloat16, longest=max(new))
+
+
+@pytest.mark.parametrize("lens,new,nh,nkv,d,S,block", FAR)
+def test_queries_that_are_no_numbers(lens, new, nh, nkv, d, S, block):
+    """An infinity or NaN in a head's query makes that head's output NaN, and no other's."""
+    c = R.case(lens, new, nh, nkv, d, S, block, torch.int8, torch.bfloat16, seed=93)
+    c["q"][0, 5] = float("inf")
+    c["q"][0, d + 1] = float("nan")
+    c["q"][-1, -1] = float("-inf")
+    _, out = _run(c, torch.bfloat16, longest=max(new))
+    nan = out.view(-1, nh, d).isnan().all(-1)
+    assert nan[0, :2].all() and nan[-1, -1] and nan.sum() == 3
