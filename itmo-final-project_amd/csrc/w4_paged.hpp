@@ -39,12 +39,14 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -__builti
 
 // Softmax sums and a quad of outputs, relative to the score M.  (Scores are subtracted before they become exponents:
 // past 2^24 the exponent's own rounding would be powers of two.)  A refused part's reference is NaN and stays.
-struct Share {
+template <bool LOG2>  // scores are exponents of 2 already
+struct ShareOf {
+  static __device__ __forceinline__ float weight(float d) { return __builtin_amdgcn_exp2f(LOG2 ? d : d * kLog2e); }
   float M = -__builtin_inff(), L = 0.f;
   f32x4 t = {0.f, 0.f, 0.f, 0.f};
   __device__ __forceinline__ void add(float m, float l, const f32x4& x) {
     const float mn = M != M || m != m ? __builtin_nanf("") : fmaxf(M, m), mz = finite_or_zero(mn);
-    const float w0 = __builtin_amdgcn_exp2f((M - mz) * kLog2e), w1 = __builtin_amdgcn_exp2f((m - mz) * kLog2e);
+    const float w0 = weight(M - mz), w1 = weight(m - mz);
     L = __builtin_fmaf(w1, l, L * w0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(w1, x[e], t[e] * w0);
@@ -58,6 +60,7 @@ struct Share {
     return r;
   }
 };
+typedef ShareOf<false> Share;
 
 // Between LDS accesses of one wave whose lanes write what others read: the LDS takes a wave's accesses in their order,
 // and the compiler is to leave them in it.  No instruction.

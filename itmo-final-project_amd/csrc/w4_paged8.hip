@@ -535,6 +535,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
+typedef ShareOf<true> Share8;
+
 // Eight codes, which fp16 holds exactly.
 template <int CT>
 __device__ __forceinline__ f16x8 codes8h(uint32_t lo, uint32_t hi) {
@@ -581,8 +583,8 @@ __device__ __forceinline__ float inverse_power(float f) {  // of such a power
   return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, f));
 }
 
-// A column's rotated query, of which a lane has some elements, in two parts of fp16; the factor it is short of.  One
-// that holds an infinity or NaN is NaN.
+// A column's rotated query, of which a lane has some elements, in two parts of fp16; the factor it is short of,
+// times log2(e).  One that holds an infinity or NaN is NaN.
 template <int NJ>
 __device__ __forceinline__ float query_parts(const float (*x)[8], f16x8 (*qf)[2]) {
   float top = 0.f;
@@ -605,7 +607,7 @@ __device__ __forceinline__ float query_parts(const float (*x)[8], f16x8 (*qf)[2]
     for (int e = 0; e < 8; ++e) y[e] = x[j][e] * f;
     halves8(y, qf[j]);
   }
-  return top < __builtin_inff() ? inverse_power(f) : __builtin_nanf("");
+  return top < __builtin_inff() ? kLog2e * inverse_power(f) : __builtin_nanf("");
 }
 
 // Which of the slots from.. from + 7 the token of slot `mine` sees, a bit each.
@@ -960,19 +962,21 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
       for (int e = 1; e < 8; ++e) top_kb[kb] = fmaxf(top_kb[kb], s[kb][e >> 2][e & 3]);
       top = fmaxf(top, top_kb[kb]);
     }
-    // A column's reference is raised once a score passes it by 8 powers of two; probabilities are 2^6 at most.
+    // Scores are exponents of 2.  A column's reference is raised, to 2 above its largest score so far, once a score passes
+    // it by 6: probabilities are 2^6 at most.
     float al = 1.f;
-    if (__ballot((top - m) * kLog2e > 8.f)) {
+    if (__ballot(top - m > 6.f)) {
       float mn = fmaxf(top, __shfl_xor(top, 16));
       mn = fmaxf(mn, __shfl_xor(mn, 32));
-      mn = (mn - m) * kLog2e > 8.f ? mn : m;
-      al = __builtin_amdgcn_exp2f((m - finite_or_zero(mn)) * kLog2e);
+      mn = mn - m > 6.f ? mn + 2.f : m;
+      al = __builtin_amdgcn_exp2f(m - finite_or_zero(mn));
       l *= al;
       heavy *= al;
       m = mn;
     }
     const float mz = finite_or_zero(m);
-    auto prob = [&](float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x - mz, kLog2e, -2.f)); };    // The largest of eight slots' weights with one scale is that of their largest score.
+    auto prob = [&](float x) { return __builtin_amdgcn_exp2f(x - mz); };
+    // The largest of eight slots' weights with one scale is that of their largest score.
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) heavy = fmaxf(heavy, prob(top_kb[kb]) * sv[kb]);
     if (__ballot(al < 1.f || heavy * lift > 0x1p15f)) {
@@ -1025,7 +1029,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
                                                                       it.parts * 128, kPagedBufFlags);
   for (int i = tid; i < quads; i += kThreads) {
     const int hd = i / (D / 4), d = i % (D / 4) * 4;
-    Share x;
+    Share8 x;
 #pragma unroll
     for (int w = 0; w < W; ++w)
       x.add(m_s[w][hd], l_s[w][hd],
@@ -1055,7 +1059,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
   f32x2* const red_ml = reinterpret_cast<f32x2*>(red + kThreads);
   for (int i = tid - run * quads; i < quads; i += kThreads) {
     const int hd = i / (D / 4);
-    Share x;
+    Share8 x;
     if (run < runs) {
       for (int p0 = run; p0 < it.parts; p0 += runs * kP8AtOnce) {
         f32x4 t[kP8AtOnce];
@@ -1157,6 +1161,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
     for (int i = 0; i < NC; ++i) ids[i] = table[min(base + (tid + 256 * i) / CH, last_slot) >> a.c.log2s];
     sid = table[min(base + 8 * (tid & 7), last_slot) >> a.c.log2s];
   };
+  // whether columns of these tokens, from the first to the last, all see a whole unit
+  auto all_see = [&](int base, int first, int last) {
+    return base + UP - 1 <= first && (!a.window || base > last - a.window || base + UP <= a.sinks);
+  };
   auto valid = [&](int id, int slot) {
     return slot <= last_slot && (uint64_t)(int64_t)id < (uint64_t)a.c.pages ? id : -1;
   };
@@ -1182,7 +1190,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
     for (int i = 0; i < NC; ++i) {
       const int slot = (tid + 256 * i) / CH, ch = tid % CH;
       const int row = (slot & 32) + ((slot >> 2) & 1) * 16 + ((slot >> 3) & 3) * 4 + (slot & 3);
-      if constexpr (CT == W4_CODE_E4M3) {
+      if (CT == W4_CODE_E4M3 && !all_see(base_of(u), first_slot, last_slot)) {
         // NaN of e4m3, what a program that is not this one left in the pages, must not meet the probability 0 of a slot
         // that is not seen: it is taken out, and what sees it is made NaN by itself.
         uint32_t bad[4], any = 0;
@@ -1260,7 +1268,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
     }
     // (a wave none of whose columns sees any of it waits)
     if (base <= w_last && (!a.window || base + UP - 1 > w_first - a.window || base < a.sinks)) {
-      const bool whole = base + UP - 1 <= w_first && (!a.window || base > w_last - a.window || base + UP <= a.sinks);
+      const bool whole = all_see(base, w_first, w_last);
       f32x4 s[KB][2];
       float sv[KB];
 #pragma unroll
@@ -1304,17 +1312,17 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Att
         top = fmaxf(top, top_kb[kb]);
       }
       float al = 1.f;
-      if (__ballot((top - m) * kLog2e > 8.f)) {
+      if (__ballot(top - m > 6.f)) {
         float mn = fmaxf(top, __shfl_xor(top, 16));
         mn = fmaxf(mn, __shfl_xor(mn, 32));
-        mn = (mn - m) * kLog2e > 8.f ? mn : m;
-        al = __builtin_amdgcn_exp2f((m - finite_or_zero(mn)) * kLog2e);
+        mn = mn - m > 6.f ? mn + 2.f : m;
+        al = __builtin_amdgcn_exp2f(m - finite_or_zero(mn));
         l *= al;
         heavy *= al;
         m = mn;
       }
       const float mz = finite_or_zero(m);
-      auto prob = [&](float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x - mz, kLog2e, -2.f)); };
+      auto prob = [&](float x) { return __builtin_amdgcn_exp2f(x - mz); };
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) heavy = fmaxf(heavy, prob(top_kb[kb]) * sv[kb]);
       if (__ballot(al < 1.f || heavy * lift > 0x1p15f)) {
