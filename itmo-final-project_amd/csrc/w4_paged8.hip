@@ -473,12 +473,15 @@ struct Item8 {
 
 constexpr int kP8Unit = 32;  // slots that a wave takes at once
 constexpr int kP8AtOnce = 8;  // parts that a thread of the joining reads together
-constexpr int kP8Waves = 4, kP8Parts = 512, kP8MinUnits = 4;
+constexpr int kP8Waves = 4, kP8MinUnits = 4;
+// As many parts as workgroups that are at work together: four a CU have heads of 64, two those of 128.  (512 and 768:
+// 32 ragged rows of 64 26.0 and 24.8 us; 131000 slots of 128 57 and 76, drafts 24 and 28.)
+constexpr int p8_parts(int d) { return d == 64 ? 768 : 512; }
 
-// Rows are cut into parts of about (all columns' tiles x units of slots) / kP8Parts, so that time follows the slots
-// there are and not the table.  Those that are cut have at most 2 * kP8Parts parts in all: each has more units than `per`,
-// and kP8Parts * per are at least all there are.
-template <int UP>
+// Rows are cut into parts of about (all columns' tiles x units of slots) / PARTS, so that time follows the slots there
+// are and not the table.  Those that are cut have at most 2 * PARTS parts in all: each has more units than `per`, and
+// PARTS * per are at least all there are.
+template <int UP, int PARTS>
 __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8* it, int* total) {
   const int lane = threadIdx.x & 63;
   auto tiles_of = [&](const RowSpan& s) { return s.n < a.many ? a.c.nkv * (int)(((int64_t)s.n * a.g + 15) / 16) : 0; };
@@ -499,7 +502,7 @@ __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8
   }
   all = wave_sum(all);
   // (rounded up beyond what the sum's own rounding can have taken)
-  const int per = max((int)fminf(ceilf(all * (1.0001f / kP8Parts)), 1e9f), kP8MinUnits);
+  const int per = max((int)fminf(ceilf(all * (1.0001f / PARTS)), 1e9f), kP8MinUnits);
   int base = 0, split = 0, counters = 0;
   for (int r = 0; r < a.c.rows; r += 64) {
     const RowSpan s = r ? span(r) : s0;
@@ -659,7 +662,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
   const int nh = a.c.nkv * a.g;
   Item8 it;
   int total;
-  if (!find_item8<UP>(a, blockIdx.x, &it, &total)) {
+  if (!find_item8<UP, p8_parts(D)>(a, blockIdx.x, &it, &total)) {
     // what is left over of the launch (one workgroup at least): tokens of no row
     const int before = a.c.rows ? min(max(a.offsets[0], 0), a.tokens) : 0;
     const int after = a.c.rows ? min(max(a.offsets[a.c.rows], before), a.tokens) : 0;
@@ -1506,11 +1509,12 @@ struct Attend8Plan {
 // find_item8.
 Attend8Plan attend8_plan(int64_t rows, int64_t tokens, int64_t num_heads, int64_t kv_heads, int64_t head_dim) {
   const int64_t g = num_heads / kv_heads;
+  const int64_t split = 2 * w4::p8_parts((int)head_dim);
   Attend8Plan p;
-  p.items = kv_heads * ((tokens * g + 15 * std::min(rows, tokens)) / 16) + 2 * w4::kP8Parts + 1;
+  p.items = kv_heads * ((tokens * g + 15 * std::min(rows, tokens)) / 16) + split + 1;
   p.stats = W4_WORKSPACE_COUNTER_BYTES;
-  p.part = p.stats + 2 * w4::kP8Parts * 16 * 8;
-  p.bytes = p.part + (size_t)(2 * w4::kP8Parts) * 16 * head_dim * 4;
+  p.part = p.stats + split * 16 * 8;
+  p.bytes = p.part + (size_t)split * 16 * head_dim * 4;
   return p;
 }
 
