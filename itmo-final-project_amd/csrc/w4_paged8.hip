@@ -366,7 +366,7 @@ __global__ __launch_bounds__(kP8Threads, ITS > 1 ? 3 : 5) void paged8_append_ker
           }
         }
       }
-    } else if (slot < sp.len) {
+    } else {  // all codes of the block, also those behind the row's last token
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (grow[i] > 0) {
@@ -842,7 +842,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_atte
           for (int i = 0; i < 2; ++i) {
             if (grow[i] == 0) continue;
             uint8_t* const p = (i ? a.c.v : a.c.k) + tok0 * D;
-            for (int j = lane * 8; j < (len - slot0) * D; j += 512)
+            for (int j = lane * 8; j < D << a.c.log2b; j += 512)
               *reinterpret_cast<u32x2*>(p + j) = shrink8<CT>(*reinterpret_cast<const u32x2*>(p + j), grow[i]);
           }
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // other lanes load what a lane has stored

@@ -23,8 +23,9 @@ rotated).
 
 A block's scale is its largest magnitude over the largest code (127, 448).  It starts with
 the block's first slot; tokens that come later let it grow by a power of two if they need
-it, which leaves e4m3 codes as they are (but for the smallest) and costs int8 codes one step
-in all.  Tokens written over (drafts that were refused) leave the scale where it is.  A
+it.  All other codes of the block are then divided by that power (those behind the row's
+last token too), which keeps e4m3 codes exactly (but for the smallest) and costs int8 codes
+one step in all.  Tokens written over (drafts that were refused) leave the scale where it is.  A
 block that an infinity or NaN comes into reads as NaN until its first slot is written again.
 
 The functions launch on the current stream and never synchronise, so lengths, offsets,

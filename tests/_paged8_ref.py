@@ -92,10 +92,10 @@ def append(k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, lengths, o
                         while a > MOST[kind] * s:
                             s *= 2
                         if s > old:
-                            was = pages[page, h, at:at + lo - j * block].double()
+                            was = pages[page, h, at:at + block].double()  # (what is new is written over)
                             new = quantise(was * old, s, kind)
                             new = torch.where(was.isnan(), was, new)
-                            pages[page, h, at:at + lo - j * block] = new.float().to(kind)
+                            pages[page, h, at:at + block] = new.float().to(kind)
                     else:
                         s = max(float(torch.tensor(a / MOST[kind], dtype=torch.float64).float()), TINY) if a > 0 else 0.0
                     scales[page, h, at // block] = s
