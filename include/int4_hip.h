@@ -438,7 +438,7 @@ int w4_paged8_append(const w4_paged8_cache* cache, int dtype, const void* k, con
 /*
  * Keys (rotated) and values read back into dense rows k, v [tokens, kv_heads * head_dim]
  * (bf16, fp16 or fp32): tokens offsets[b]..offsets[b + 1] are row b's slots starts[b].. ,
- * code * scale in fp32, rounded once.  Tokens of no row, and of rows with starts[b] < 0,
+ * code * scale, rounded to the outputs' type.  Tokens of no row, and of rows with starts[b] < 0,
  * are 0; slots past the table or on a page outside the pool NaN.
  */
 int w4_paged8_read(const w4_paged8_cache* cache, int dtype, const int32_t* starts, const int32_t* offsets,

@@ -255,6 +255,10 @@ __global__ __launch_bounds__(kP8Threads, ITS > 1 ? 3 : 5) void paged8_append_ker
   const int page = a.c.page(row, slot0);
   if (page < 0) return;  // (uniform)
   if (tid < 2 * UNITS) (&top_s[0][0])[tid] = 0;
+  const bool fresh = slot0 >= sp.len;
+  const int64_t blk = a.c.block(page, h, slot0);
+  float there[2] = {0.f, 0.f};  // (read before the barriers, written behind them)
+  if (!fresh) there[0] = a.c.k_scale[blk], there[1] = a.c.v_scale[blk];
   __syncthreads();
 
   const int d = (r0 % CH) * 8;
@@ -321,19 +325,15 @@ __global__ __launch_bounds__(kP8Threads, ITS > 1 ? 3 : 5) void paged8_append_ker
   if (top_v) atomicMax(&top_s[1][unit], (unsigned long long)top_v);
   __syncthreads();
 
-  const bool fresh = slot0 >= sp.len;
-  const int64_t blk = a.c.block(page, h, slot0);
   double scale[2], inv[2];
   int grow[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const double most = i ? (double)__builtin_bit_cast(float, (uint32_t)top_s[1][unit])
                           : __builtin_bit_cast(double, (uint64_t)top_s[0][unit]);
-    const double old = fresh ? 0.0 : (double)(i ? a.c.v_scale : a.c.k_scale)[blk];
-    scale[i] = block_scale<CT>(most, old, &grow[i]);
+    scale[i] = block_scale<CT>(most, (double)there[i], &grow[i]);
     inv[i] = scale[i] > 0.0 ? 1.0 / scale[i] : 0.0;  // (also of NaN: its codes are 0)
   }
-  __syncthreads();  // all have read the scales that are there
   if (!live) return;
   if (r0 == 0) {
     a.c.k_scale[blk] = (float)scale[0];
