@@ -495,18 +495,22 @@ __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8
   };
   auto span = [&](int r) { return row_span(a.c, a.lengths, a.offsets, a.tokens, a.longest, r + lane); };
   const RowSpan s0 = span(0);
-  float all = (float)tiles_of(s0) * (float)units_of(s0);
+  float all = (float)tiles_of(s0) * (float)units_of(s0), news = (float)s0.n;
   for (int r = 64; r < a.c.rows; r += 64) {
     const RowSpan s = span(r);
     all += (float)tiles_of(s) * (float)units_of(s);
+    news += (float)s.n;
   }
   all = wave_sum(all);
+  // Rows that overlap (offsets that decrease) may need more workgroups than there are: none of them is cut, or parts
+  // would wait for others that never come, and their counter be left for the next call.
+  const bool overlap = wave_sum(news) > (float)a.tokens;
   // (rounded up beyond what the sum's own rounding can have taken)
-  const int per = max((int)fminf(ceilf(all * (1.0001f / PARTS)), 1e9f), kP8MinUnits);
+  const int per = overlap ? INT32_MAX : max((int)fminf(ceilf(all * (1.0001f / PARTS)), 1e9f), kP8MinUnits);
   int base = 0, split = 0, counters = 0;
   for (int r = 0; r < a.c.rows; r += 64) {
     const RowSpan s = r ? span(r) : s0;
-    const int tiles = tiles_of(s), parts = (units_of(s) + per - 1) / per;
+    const int tiles = tiles_of(s), parts = 1 + (units_of(s) - 1) / per;
     const int upto = base + wave_scan(parts * tiles);
     const int split_to = split + wave_scan(parts > 1 ? parts * tiles : 0);
     const int counters_to = counters + wave_scan(parts > 1 ? tiles : 0);

@@ -688,3 +688,22 @@ def test_queries_that_are_no_numbers(lens, new, nh, nkv, d, S, block):
     _, out = _run(c, torch.bfloat16, longest=max(new))
     nan = out.view(-1, nh, d).isnan().all(-1)
     assert nan[0, :2].all() and nan[-1, -1] and nan.sum() == 3
+
+
+def test_offsets_that_decrease():
+    """Rows that overlap need more tiles than the tokens are: no sense, but the call after it is as before."""
+    lens = [0] * 101 + [20000]
+    c = _to(R.case([20000], [1], 8, 2, 64, 64, 8, torch.int8, torch.float16, seed=94))
+    want = int4_hip.paged_attention8(**c)
+    bad = dict(c)
+    T = 65
+    for n in ("q", "k", "v", "positions"):
+        bad[n] = c[n].expand(T, *c[n].shape[1:]).contiguous()
+    bad["offsets"] = torch.tensor([0, 64] * 51 + [65], dtype=torch.int32, device=DEV)
+    bad["lengths"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    bad["table"] = c["table"].expand(len(lens), -1).contiguous()
+    for n in CACHE:
+        bad[n] = c[n].clone()
+    int4_hip.paged_attention8(**bad)
+    for _ in range(2):
+        assert torch.equal(int4_hip.paged_attention8(**c), want)
