@@ -238,6 +238,11 @@ __device__ __forceinline__ unsigned odd_ones(const float x[8], float inv) {
 // A block's scale is its largest magnitude over the largest code.  Tokens that come into a block that holds some
 // already let its scale grow by a power of two, if they need it: e4m3 codes then stay as they are (but for the
 // smallest), and int8 codes, each rounding at half the step of the next, are never off by more than one step in all.
+//
+// What bounds it: 7999 tokens of 8 x 128 (49 MB) take 18.5 us, 2.6 TB/s, of which two thirds go to the vector
+// instructions: the rotation in 64 bits and two quotients a code (50 us with every code in 64 bits, 31 where a thread with
+// one doubtful code took all of its own again).  32 tokens take 6.2 us, a chain of dependent loads: lengths and offsets,
+// page and position, angles and the block's scale.
 template <int DT, int CT, int D, int ITS>
 __global__ __launch_bounds__(kP8Threads, ITS > 1 ? 3 : 5) void paged8_append_kernel(Append8Args a) {
   constexpr int CH = D / 16;  // threads per token
@@ -387,7 +392,8 @@ struct Read8Args {
   int tokens;
 };
 
-// Sixteen values of a key and of the value beside it a thread.
+// Sixteen values of a key and of the value beside it a thread.  Bound by HBM: 60000 tokens of 8 x 128 to fp16 (369 MB)
+// take 79 us, 4.7 TB/s (a large copy: 4.9); 300 tokens 3.5 us, a launch and three dependent loads.
 template <int CT, int OUT, int D>
 __global__ __launch_bounds__(kP8Threads) void paged8_read_kernel(Read8Args a) {
   constexpr int CH = D / 16;
@@ -644,7 +650,14 @@ __device__ __forceinline__ uint32_t seen8(int from, int mine, int window, int si
 //
 // PUT: no row has more than one new token, a row's and head's columns are one tile, and a block lies in one unit: the
 // wave that takes a row's last unit writes the token (and, where the block's scale grows, its other codes), as
-// paged8_append_kernel does.
+// paged8_append_kernel does.  That saves a launch: 100 slots 9.2 us a call instead of 11.8, 32 rows of up to 4000 32
+// instead of 38, one of 131000 57.6 instead of 59.8.
+//
+// What bounds it: one row of 131000 slots of 8 x 128 (268 MB) takes 56 us, 4.8 TB/s, HBM.  32 rows of up to 4000 slots of
+// 8 x 64 (62 MB) take 24.2 us, 24 windows of 128-wide heads (49 MB) 20.4: of either, the vector instructions (conversion of
+// codes, softmax, weights in two parts) take about half the cycles of a busy CU and the matrix instructions a twelfth, and
+// 7 us go before the first and after the last unit.  Five drafts of four query heads are 20 columns, two tiles, each of
+// which converts all codes: 16 rows of 3001 slots 23.8 us.  100 slots: 7.9 us of dependent loads.
 template <int DT, int CT, int D, int W, bool PUT>
 __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_attention_kernel(Attend8Args a) {
   constexpr int UP = kP8Unit, KB = UP / 32, NJ = D / 32, ND = D / 16;
@@ -1101,6 +1114,12 @@ constexpr int kPromptCols = 64, kPromptUnit = 64;
 // the four waves turn the codes into fp16 in LDS together, once, and multiply from there.  Otherwise as
 // paged8_attention_kernel, whose waves share their columns and not the slots: that spreads a few columns over the chip,
 // but converts every code for sixteen columns alone.
+//
+// What bounds it: 2000 tokens of 32 / 8 x 64 (16.4 GFLOP) take 59 us, 0.28 PFLOP/s (in two parts each, 0.56; a large
+// product reaches 1.18): of a busy CU's cycles the vector instructions take 0.7, the LDS 0.4 and the matrix
+// instructions 0.3.  (Without LDS conversion, sixteen columns a workgroup: 110 us.  Masks tested slot by slot: 86
+// instead of 79 at that time.  Two workgroups a CU instead of four: 95 against 86.  Every second unit in one half of eight
+// waves: 64 against 60.  The order of tiles turned round in every second 256: 60.4 against 59.9.)
 template <int DT, int CT, int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged8_prompt_kernel(Attend8Args a) {
   constexpr int UP = kPromptUnit, KB = UP / 32, NJ = D / 32, ND = D / 16;
@@ -1634,19 +1653,23 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   a.g = (int)(num_heads / cache->kv_heads);
   a.window = window >= most ? 0 : (int)window;
   a.sinks = (int)std::min(sinks, most);
-  // Rows with this many columns in all fill the chip with whole tiles of them, whatever else there is.
-  constexpr int64_t kManyColumns = 9600;
+  // Calls of so many columns fill the chip with tiles of 64 of them and all their slots.  (Times of both ways, us, tiles
+  // of 64 first, 32 heads of 64 on 8: 600 tokens 30 and 23, after 4000 slots 122 and 88; 900 37 and 35, after 1500 68 and
+  // 71; 1200 43 and 42, after 1500 81 and 89; 2000 64 and 80, after 6000 308 and 380; four rows of 450 34 and 40.)  Rows of
+  // fewer than 150 tokens of 64 heads are cut among them all the same.
+  constexpr int64_t kAllColumns = 36864, kManyColumns = 9600;
   const int64_t many = (kManyColumns + num_heads - 1) / num_heads;
-  a.many = most_new >= many ? (int)many : INT32_MAX;
+  const bool prompts = tokens * num_heads >= kAllColumns && most_new >= many;
+  a.many = prompts ? (int)many : INT32_MAX;
   const int64_t wide = tokens / many;  // such rows, at most
   // (and the others' tokens)
-  const int64_t rest = most_new >= many ? std::min(tokens, cache->rows * (many - 1)) : tokens;
+  const int64_t rest = prompts ? std::min(tokens, cache->rows * (many - 1)) : tokens;
   const dim3 grid((unsigned)attend8_plan(cache->rows, rest, num_heads, cache->kv_heads, cache->head_dim).items);
   const dim3 prompt((unsigned)(a.c.nkv * ((tokens * a.g + (w4::kPromptCols - 1) * wide) / w4::kPromptCols)));
   return by_dtype(dtype, [&](auto dt) {
     return by_code(cache->code, [&](auto ct) {
       return by_head(cache->head_dim, [&](auto d) {
-        if (most_new >= many) {
+        if (prompts) {
           w4::paged8_prompt_kernel<dt(), ct(), d()><<<prompt, 256, 0, st>>>(a);
           if (const int rc = check_launch("w4_paged8_attention (prompts)")) return rc;
         }

@@ -154,23 +154,21 @@ def attention(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, table, leng
             pos = int(positions[t])
             x = q[t].double().view(nh, d)
             x = rotate(x, cos[pos], sin[pos]) if 0 <= pos < len(cos) else torch.full_like(x, NAN)
-            for h in range(nh):
-                key, val = kk[seen, h // (nh // nkv)], vv[seen, h // (nh // nkv)]
-                if not (key.isfinite().all() and x[h].isfinite().all()):
-                    out[t, h] = NAN
-                    continue
-                p = torch.softmax(key @ x[h] / math.sqrt(d), 0)
+            for h in range(nkv):
+                key, val, heads = kk[seen, h], vv[seen, h], slice(h * nh // nkv, (h + 1) * nh // nkv)
+                p = torch.softmax(key @ x[heads].T / math.sqrt(d), 0).T
                 # (a probability that fp32 cannot have, 2^-118 of the largest with the reference 2^8 behind, is lost: the
                 # tolerance, 2^-21 of the mass or more, is to hold n 2^-110 of the largest value)
                 # (weights, probability times scale, enter as two numbers of 11 bits each, whose smallest step is 2^-24:
                 # with the column's largest raised past 2^10, they are within 2^-35 of the largest at worst, 2^-14 of
                 # that 2^-21)
-                step = scale[seen, h // (nh // nkv)]
+                step = scale[seen, h]
                 sums = (val / step[:, None]).nan_to_num().abs().sum(0)
-                out[t, h] = p @ val
-                mass[t, h] = (p @ val.abs() + len(seen) * 2.0 ** -89 * val.nan_to_num().abs().max()
-                              + 2.0 ** -14 * (p * step).nan_to_num().max() * sums)
-                reach[t, h] = (key.abs() @ x[h].abs()).max() / math.sqrt(d)
+                out[t, heads] = p @ val
+                mass[t, heads] = (p @ val.abs() + len(seen) * 2.0 ** -89 * val.nan_to_num().abs().max()
+                                  + 2.0 ** -14 * (p * step).nan_to_num().amax(1, True) * sums)
+                reach[t, heads] = (x[heads].abs() @ key.abs().T).amax(1, True) / math.sqrt(d)
+                out[t, heads][~x[heads].isfinite().all(1) | ~key.isfinite().all()] = NAN
     return out.flatten(1), mass.flatten(1), reach.expand(-1, -1, d).flatten(1)
 
 

@@ -574,7 +574,8 @@ def test_codes_of_many_tokens(kind, dtype):
         assert torch.equal(got.view(T, nkv, d), (q * s.double().repeat_interleave(block, 0)[:T, :, None]).float())
 
 
-# ---------------------------------------------------------------- rows of many new tokens (9600 columns of all heads)
+# ---------------------------------------------------------------- rows of many new tokens (9600 columns, token and head,
+# and more, in calls of 36864 and more)
 PROMPTS = [
     # (lengths, new tokens, heads, kv heads, head_dim, page size, block, window, sinks)
     ([0], [160], 64, 2, 64, 16, 8, None, 0),
@@ -583,6 +584,12 @@ PROMPTS = [
     ([130], [205], 48, 16, 64, 64, 32, 50, 0),
     ([300, 64], [170, 160], 60, 1, 128, 64, 32, 70, 5),
     ([63], [151], 64, 8, 64, 8, 8, 1, 130),
+    ([0], [160], 256, 2, 64, 16, 8, None, 0),
+    ([0, 5, 40, 0], [151, 1, 150, 3], 256, 2, 64, 64, 64, None, 0),
+    ([70, 0], [150, 150], 256, 4, 128, 32, 16, None, 0),
+    ([130], [205], 192, 16, 64, 64, 32, 50, 0),
+    ([300, 64], [170, 160], 180, 1, 128, 64, 32, 70, 5),
+    ([63], [151], 256, 8, 64, 8, 8, 1, 130),
 ]
 
 
@@ -616,7 +623,7 @@ def test_prompts_that_are_no_rows():
 def test_prompts_beside_codes_of_nan():
     """Where nobody looks, and where some do."""
     lens, new = [40, 10], [150, 160]
-    c = R.case(lens, new, 64, 2, 64, 32, 8, torch.float8_e4m3fn, torch.float16, seed=81, window=60, sinks=2)
+    c = R.case(lens, new, 128, 2, 64, 32, 8, torch.float8_e4m3fn, torch.float16, seed=81, window=60, sinks=2)
     for n in ("k_pages", "v_pages"):
         x = c[n].view(torch.uint8)
         keep = x.clone()
@@ -630,12 +637,12 @@ def test_prompts_beside_codes_of_nan():
     c["v_pages"].view(torch.uint8)[int(c["table"][0, 0]), 0, 20, 33] = 0xFF  # slot 20: seen up to slot 79
     c["k_pages"].view(torch.uint8)[int(c["table"][1, 0]), 1, 1, 3] = 0x7F    # a sink
     _, out = _run(c, torch.float16)
-    nan = out.view(310, 2, 32, 64).isnan().cpu()
+    nan = out.view(310, 2, 64, 64).isnan().cpu()
     assert nan[:40, 0, :, 33].all() and not nan[40:150, 0].any() and nan[150:, 1].all() and not nan[150:, 0].any()
 
 
 def test_prompts_in_a_graph():
-    c = R.case([50, 7], [150, 1], 64, 2, 64, 32, 16, torch.int8, torch.bfloat16, seed=82)
+    c = R.case([50, 7], [150, 1], 256, 2, 64, 32, 16, torch.int8, torch.bfloat16, seed=82)
     g = _to(c)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
@@ -651,7 +658,7 @@ def test_prompts_in_a_graph():
 
 # ---------------------------------------------------------------- numbers of every size
 FAR = [([200, 150, 90], [1, 2, 1], 4, 2, 64, 16, 8), ([700, 300], [1, 1], 6, 1, 128, 32, 16),
-       ([40, 9], [152, 3], 64, 2, 64, 32, 8), ([60], [76], 128, 2, 128, 64, 16)]
+       ([40, 9], [152, 3], 256, 2, 64, 32, 8), ([60], [76], 512, 2, 128, 64, 16)]
 
 
 @pytest.mark.parametrize("lens,new,nh,nkv,d,S,block", FAR)
