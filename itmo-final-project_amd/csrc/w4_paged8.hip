@@ -480,6 +480,10 @@ struct Item8 {
 constexpr int kP8Unit = 32;  // slots that a wave takes at once
 constexpr int kP8AtOnce = 8;  // parts that a thread of the joining reads together
 constexpr int kP8Waves = 4, kP8MinUnits = 4;
+// A part takes time with its units, the joining of a tile with its parts, eight at once: parts of sqrt(units / 2) units at
+// least keep the two alike.  (Without: one row of 60000 slots of 20 / 2 heads of 128 84 us, with 39, one of 131000 of 6 / 1
+// 89 and 41; 4000 of 8 / 2 of 64 10.2 and 11.0.  Of sqrt(units / 5): 46.5, 41, 10.8; sqrt(1.5 units): 40.5, 47.6, 12.3.)
+constexpr float kP8Join = 0.5f;
 // As many parts as workgroups that are at work together: four a CU have heads of 64, two those of 128.  (512 and 768:
 // 32 ragged rows of 64 26.0 and 24.8 us; 131000 slots of 128 57 and 76, drafts 24 and 28.)
 constexpr int p8_parts(int d) { return d == 64 ? 768 : 512; }
@@ -516,7 +520,8 @@ __device__ __forceinline__ bool find_item8(const Attend8Args& a, int item, Item8
   int base = 0, split = 0, counters = 0;
   for (int r = 0; r < a.c.rows; r += 64) {
     const RowSpan s = r ? span(r) : s0;
-    const int tiles = tiles_of(s), parts = 1 + (units_of(s) - 1) / per;
+    const int tiles = tiles_of(s), units = units_of(s);
+    const int parts = 1 + (units - 1) / max(per, (int)__builtin_amdgcn_sqrtf((float)units * kP8Join));
     const int upto = base + wave_scan(parts * tiles);
     const int split_to = split + wave_scan(parts > 1 ? parts * tiles : 0);
     const int counters_to = counters + wave_scan(parts > 1 ? tiles : 0);
@@ -657,7 +662,7 @@ __device__ __forceinline__ uint32_t seen8(int from, int mine, int window, int si
 // 8 x 64 (62 MB) take 24.2 us, 24 windows of 128-wide heads (49 MB) 20.4: of either, the vector instructions (conversion of
 // codes, softmax, weights in two parts) take about half the cycles of a busy CU and the matrix instructions a twelfth, and
 // 7 us go before the first and after the last unit.  Five drafts of four query heads are 20 columns, two tiles, each of
-// which converts all codes: 16 rows of 3001 slots 23.8 us.  100 slots: 7.9 us of dependent loads.
+// which converts all codes: 16 rows of 3001 slots with one to five drafts 23.8 us.  100 slots: 7.9 us of dependent loads.
 template <int DT, int CT, int D, int W, bool PUT>
 __global__ __launch_bounds__(64 * W, D == 64 ? 4 : PUT ? 2 : 3) void paged8_attention_kernel(Attend8Args a) {
   constexpr int UP = kP8Unit, KB = UP / 32, NJ = D / 32, ND = D / 16;
