@@ -239,7 +239,7 @@ __device__ __forceinline__ unsigned odd_ones(const float x[8], float inv) {
 // already let its scale grow by a power of two, if they need it: e4m3 codes then stay as they are (but for the
 // smallest), and int8 codes, each rounding at half the step of the next, are never off by more than one step in all.
 //
-// What bounds it: 7999 tokens of 8 x 128 (49 MB) take 18.5 us, 2.6 TB/s, of which two thirds go to the vector
+// What bounds it: 7999 tokens of 8 x 128 (49 MB) take 18.9 us, 2.6 TB/s, of which two thirds go to the vector
 // instructions: the rotation in 64 bits and two quotients a code (50 us with every code in 64 bits, 31 where a thread with
 // one doubtful code took all of its own again).  32 tokens take 6.2 us, a chain of dependent loads: lengths and offsets,
 // page and position, angles and the block's scale.
