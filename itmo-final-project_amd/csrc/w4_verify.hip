@@ -267,7 +267,8 @@ struct VerifyPlan {
 };
 
 // Parts of 2048 tokens, or of a multiple of that where there would be more of them than lanes, or more workgroups than
-// the chip holds (five a CU): each begins with three loads that wait for one another.
+// the chip holds (five a CU): each begins with three loads that wait for one another.  (48 rows with two a CU
+// 21.8 us, five 20.0, ten 22.8; one row in 63 parts 7.6, in sixteen 11.6.)
 VerifyPlan verify_plan(int64_t rows, int64_t vocab) {
   VerifyPlan p;
   p.slice = W4_WORKSPACE_COUNTER_BYTES / 4;
