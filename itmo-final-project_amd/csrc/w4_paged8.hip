@@ -1664,7 +1664,8 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   // fewer than 150 tokens of 64 heads are cut among them all the same.
   constexpr int64_t kAllColumns = 36864, kManyColumns = 9600;
   const int64_t many = (kManyColumns + num_heads - 1) / num_heads;
-  const bool prompts = tokens * num_heads >= kAllColumns && most_new >= many;
+  // (Not where the attention writes: a single token of 9600 heads and more is a prompt by its columns, and nobody's to write.)
+  const bool prompts = !put && tokens * num_heads >= kAllColumns && most_new >= many;
   a.many = prompts ? (int)many : INT32_MAX;
   const int64_t wide = tokens / many;  // such rows, at most
   // (and the others' tokens)

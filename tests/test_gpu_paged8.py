@@ -714,3 +714,12 @@ def test_offsets_that_decrease():
     int4_hip.paged_attention8(**bad)
     for _ in range(2):
         assert torch.equal(int4_hip.paged_attention8(**c), want)
+
+
+@pytest.mark.parametrize("kind", CODES, ids=ids)
+@pytest.mark.parametrize("longest", [1, None])
+def test_one_token_of_thousands_of_heads(kind, longest):
+    """Decode steps whose single tokens are 9600 columns each, as many as a prompt's rows begin with: written and
+    attended to, whether the call knows that a row has one token (one launch) or not (the prompts' kernel)."""
+    c = R.case([5, 0, 17, -1, 40], [1] * 5, 9600, 600, 64, 8, 8, kind, torch.float16, seed=95)
+    _run(c, torch.float16, longest=longest)
