@@ -72,6 +72,22 @@ class Verified(NamedTuple):
 MAX_DRAFTS = 64
 
 
+def drafts_fit(shape, dtype, dev, draft, tokens, accept, sample, counts=None) -> None:
+    """Asserts what ``verify_drafts`` needs beside target probabilities of ``shape``, ``dtype`` and
+    device ``dev``, so that a caller can ask before it computes them."""
+    B, K, V = shape[0], shape[1] - 1, shape[2]
+    assert underived(draft, accept, sample), \
+        "verify_drafts has no derivatives: call it under torch.no_grad(), on probabilities without tangents"
+    assert 0 <= K <= MAX_DRAFTS and V >= 1, shape
+    assert tokens.dtype == torch.int64 and tokens.shape == (B, K) and tokens.device == dev, (tokens.dtype, tokens.shape)
+    assert accept.dtype == sample.dtype == torch.float32 and accept.shape == (B, K) and sample.shape == (B,)
+    assert accept.device == sample.device == dev
+    if draft is not None:
+        assert draft.dtype == dtype and draft.shape == (B, K, V) and draft.device == dev, (draft.dtype, draft.shape)
+    if counts is not None:
+        assert counts.dtype == torch.int32 and counts.shape == (B,) and counts.device == dev, counts.shape
+
+
 def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, accept: torch.Tensor,
                   sample: torch.Tensor, counts: torch.Tensor | None = None) -> Verified:
     """Speculative sampling: which of the drafted ``tokens`` int64 [rows, drafts] (at most 64)
@@ -97,25 +113,20 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
         if r is not None:
             return Verified(*r)
     assert target.dtype in DTYPES and target.dim() == 3 and target.is_cuda, (target.dtype, target.shape)
-    assert underived(target, draft, accept, sample), \
+    assert underived(target), \
         "verify_drafts has no derivatives: call it under torch.no_grad(), on probabilities without tangents"
     B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
     dev = target.device
-    assert 0 <= K <= MAX_DRAFTS and V >= 1, target.shape
-    assert tokens.dtype == torch.int64 and tokens.shape == (B, K) and tokens.device == dev, (tokens.dtype, tokens.shape)
-    assert accept.dtype == sample.dtype == torch.float32 and accept.shape == (B, K) and sample.shape == (B,)
-    assert accept.device == sample.device == dev
+    drafts_fit(target.shape, target.dtype, dev, draft, tokens, accept, sample, counts)
     target, tokens, accept, sample = (t.resolve_neg() for t in (target, tokens, accept, sample))
     tokens, accept, sample = tokens.contiguous(), accept.contiguous(), sample.contiguous()
     if target.stride(2) != 1 and V > 1:
         target = target.contiguous()
     if draft is not None:
-        assert draft.dtype == target.dtype and draft.shape == (B, K, V) and draft.device == dev, (draft.dtype, draft.shape)
         draft = draft.resolve_neg()
         if draft.stride(2) != 1 and V > 1:
             draft = draft.contiguous()
     if counts is not None:
-        assert counts.dtype == torch.int32 and counts.shape == (B,) and counts.device == dev, counts.shape
         counts = counts.resolve_neg().contiguous()
     accepted, token = (torch.empty(B, dtype=torch.int64, device=dev) for _ in range(2))
     lib = _lib.load()

@@ -26,7 +26,7 @@ from . import llama_ops
 from .llama import (Attention, LlamaConfig, LlamaForCausalLM, _add_norm, _all_int4, _grouped, _plain, rope_inv_freq)
 from .paged import paged_append, paged_attention, paged_evict
 from .paged8 import CODES, paged_attention8
-from .scoring import TokenLogprobs, Verified, token_logprobs, verify_drafts
+from .scoring import TokenLogprobs, Verified, drafts_fit, token_logprobs, verify_drafts
 
 
 class Step(NamedTuple):
@@ -284,6 +284,9 @@ class BatchDecoder:
         if drafts.dim() != 2 or drafts.shape[0] != self.rows or not temperature > 0:
             raise ValueError(f"drafts of {self.rows} rows and a temperature above 0: got {tuple(drafts.shape)}, {temperature}")
         K = drafts.shape[1]
+        # (before anything of them is in the cache)
+        drafts_fit((self.rows, K + 1, self.model.config.vocab_size), torch.float32, self.ids.device, draft, drafts, accept,
+                   sample)
         for row, n in enumerate(self.length):
             if n >= 0:
                 if self.position[row] + K >= len(self.cos):

@@ -168,6 +168,33 @@ def test_refusals():
     assert dec.length[0] == 18 and dec.evict() == []
 
 
+def _state(dec):
+    return [dec.k.view(torch.uint8).clone(), dec.v.view(torch.uint8).clone(), dec.scales.clone(), dec.table.clone(),
+            dec.lengths.clone(), dec.positions.clone(), dec.ids.clone(), list(dec.free), [list(o) for o in dec.owned],
+            list(dec.length), list(dec.position)]
+
+
+def test_drafts_that_cannot_be_verified_leave_everything():
+    """What the verification would refuse is refused before the drafts are in the cache."""
+    m = _model()
+    dec = _decoder(m, cache=torch.int8, block=8)
+    dec.add(0, _prompt(15, 1))
+    dec.add(2, _prompt(6, 2))
+    was = _state(dec)
+    x, many = (torch.zeros((4, k), dtype=torch.int64, device=DEV) for k in (2, 65))
+    ok = dict(drafts=x, accept=x.float(), sample=x[:, 0].float())
+    for bad in (dict(drafts=x.int()), dict(drafts=x.cpu()), dict(accept=x[:, :1].float()), dict(accept=x.double()),
+                dict(accept=x.float().cpu()), dict(sample=x.float()), dict(sample=x[:, 0].half()),
+                dict(sample=x[:3, 0].float()), dict(draft=torch.zeros(4, 2, CFG.vocab_size - 1, device=DEV)),
+                dict(draft=torch.zeros(4, 3, CFG.vocab_size, device=DEV)),
+                dict(draft=torch.zeros(4, 2, CFG.vocab_size, device=DEV, dtype=torch.bfloat16)),
+                dict(draft=torch.zeros(4, 2, CFG.vocab_size)), dict(drafts=many, accept=many.float())):
+        with pytest.raises((AssertionError, ValueError)):
+            dec.verify(**{**ok, **bad})
+        for a, b in zip(was, _state(dec)):
+            assert torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b
+
+
 def test_looked_up():
     assert looked_up([1, 2, 3, 4, 2], 3) == [3, 4, 2] and looked_up([5], 2) == [5, 5]
     assert looked_up([1, 2, 2], 2) == [2, 2] and looked_up([9, 1, 9, 4, 9], 1) == [4]
