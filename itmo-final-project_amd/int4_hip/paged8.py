@@ -25,8 +25,10 @@ A block's scale is its largest magnitude over the largest code (127, 448).  It s
 the block's first slot; tokens that come later let it grow by a power of two if they need
 it.  All other codes of the block are then divided by that power (those behind the row's
 last token too), which keeps e4m3 codes exactly (but for the smallest) and costs int8 codes
-one step in all.  Tokens written over (drafts that were refused) leave the scale where it is.  A
-block that an infinity or NaN comes into reads as NaN until its first slot is written again.
+one step in all.  Tokens written over (drafts that were refused) leave the scale where it is
+and the other codes divided; who wants neither keeps the block and puts it back
+(``BatchDecoder.verify``).  A block that an infinity or NaN comes into reads as NaN until its
+first slot is written again.
 
 The functions launch on the current stream and never synchronise, so lengths, offsets,
 pages and positions, which live on the GPU, are checked there: what is out of range is

@@ -25,7 +25,7 @@ import torch
 from . import llama_ops
 from .llama import (Attention, LlamaConfig, LlamaForCausalLM, _add_norm, _all_int4, _grouped, _plain, rope_inv_freq)
 from .paged import paged_append, paged_attention, paged_evict
-from .paged8 import CODES, paged_attention8
+from .paged8 import CODES, paged_append8, paged_attention8
 from .scoring import TokenLogprobs, Verified, drafts_fit, token_logprobs, verify_drafts
 
 
@@ -138,13 +138,50 @@ class BatchDecoder:
                 own[i] = None
                 self.table[row, i] = -1
 
+    def _begun(self):
+        """The blocks of a cache in 8 bits that the next tokens come into beside others, as they are: what to call to
+        put them back."""
+        S, n = self.page_size, self.scales.shape[-1]
+        block = S // n
+        at = [(self.owned[row][m // S], m % S // block) for row, m in enumerate(self.length) if m >= 0 and m % block]
+        page, part = torch.tensor(at, dtype=torch.int64).view(-1, 2).T.to(self.k.device)
+        # [..., pages, kv_heads, blocks of a page, words of a block]
+        views = [t.view(torch.int64).view(*t.shape[:3], n, -1) for t in (self.k, self.v)] + [self.scales[..., None]]
+        kept = [t[..., page, :, part, :] for t in views]
+
+        def put_back():
+            for t, was in zip(views, kept):
+                t[..., page, :, part, :] = was
+        return put_back
+
+    def _write_again(self, new, starts, step, positions):
+        """The first ``step`` of every row's tokens, which begin at ``starts`` of the keys and values ``new`` of the
+        layers.  Layers are rows of one call; a row's other tokens are an idle row's behind it."""
+        rows, T, P = self.rows, new[0][0].shape[0], self.k.shape[1]
+        most = max(65535 // (2 * rows), 1)  # an operator has as many rows
+        for i in range(0, len(new), most):
+            n = min(most, len(new) - i)
+            k, v = (torch.cat([kv[j] for kv in new[i:i + n]]) for j in range(2))
+            layer = torch.arange(n, dtype=torch.int32, device=step.device)[:, None]
+            real = torch.arange(2, dtype=torch.int32, device=step.device) == 0
+            # (entries of no page are those of slots that no token goes to)
+            table = self.table[:, None] + (layer * P)[:, None, None].expand(n, rows, 2, 1)
+            lengths = torch.where(real, self.lengths[:, None], -1).expand(n, rows, 2).flatten()
+            offsets = starts[:-1, None] + torch.where(real, 0, step[:, None]) + (layer * T)[..., None]
+            kp, vp, ks, vs = (t[i:i + n].flatten(0, 1) for t in (self.k, self.v, *self.scales))
+            paged_append8(k, v, self.cos, self.sin, kp, vp, ks, vs, table.flatten(0, 2), lengths,
+                          torch.cat((offsets.flatten(), torch.full_like(starts[:1], n * T))), positions.repeat(n))
+
     # -------------------------------------------------------------- the model
     def _linears(self, x, mods):
         return _grouped(x, mods) if _all_int4(mods) else [m(x) for m in mods]
 
-    def _attend8(self, table, lengths, offsets, positions, longest):
-        """The attention of new tokens of the rows of ``table`` over a cache in 8 bits, for ``_run``."""
+    def _attend8(self, table, lengths, offsets, positions, longest, new=None):
+        """The attention of new tokens of the rows of ``table`` over a cache in 8 bits, for ``_run``; their keys and
+        values of every layer are put into the list ``new``."""
         def attend(i, q, k, v):
+            if new is not None:
+                new.append((k, v))
             return paged_attention8(q, k, v, self.cos, self.sin, self.k[i], self.v[i], self.scales[0, i],
                                     self.scales[1, i], table, lengths, offsets, positions, longest=longest,
                                     window=self.sees, sinks=self.sinks)
@@ -277,7 +314,11 @@ class BatchDecoder:
         are the softmax of its logits over ``temperature``.
 
         Waits for the GPU: what the rows hold is known to the host.  Refused drafts leave no
-        trace but the scale of the block that they came into.
+        trace: where there are any, the blocks they came into are put back and the accepted
+        tokens written to them once more.  (In the step itself all its tokens see the cache
+        with the drafts in it: a draft far larger than the tokens of its block costs their
+        codes bits there.)  A row whose probabilities are no numbers has the token -1 and is
+        as it was before, whatever ``accepted`` says.
         """
         if self.scales is None:
             raise ValueError("drafts are verified over a cache of 8 bits")
@@ -293,18 +334,24 @@ class BatchDecoder:
                     raise RuntimeError(f"row {row} is past the {len(self.cos)} positions")
                 self._reserve(row, n + K + 1)
         tokens = torch.cat((self.ids[:, None], drafts), 1)
-        positions = self.positions[:, None] + torch.arange(K + 1, dtype=torch.int32, device=self.ids.device)
-        attend = self._attend8(self.table, self.lengths, self.each * (K + 1), positions.flatten(), K + 1)
+        positions = (self.positions[:, None] + torch.arange(K + 1, dtype=torch.int32, device=self.ids.device)).flatten()
+        put_back, new, starts = self._begun(), [], self.each * (K + 1)
+        attend = self._attend8(self.table, self.lengths, starts, positions, K + 1, new)
         # (a draft outside the vocabulary is refused; until then it is some token of it)
         embed = self.model.model.embed_tokens
         logits = self._run(embed(tokens.flatten().clamp(0, embed.num_embeddings - 1)), attend)
         target = torch.softmax(logits.float() / temperature, -1).view(self.rows, K + 1, -1)
         r = verify_drafts(target, draft, drafts, accept, sample)
-        step = torch.where(self.lengths >= 0, r.accepted + 1, 0).to(torch.int32)
+        good = (self.lengths >= 0) & (r.token >= 0)
+        step = torch.where(good, r.accepted + 1, 0).to(torch.int32)
+        steps = step.tolist()
+        if any(m >= 0 and n <= K for m, n in zip(self.length, steps)):
+            put_back()
+            self._write_again(new, starts, step, positions)
         self.lengths += step
         self.positions += step
-        self.ids.copy_(r.token.clamp(min=0))  # (-1: of logits that are no numbers)
-        for row, n in enumerate(step.tolist()):
+        self.ids.copy_(torch.where(good, r.token, self.ids))
+        for row, n in enumerate(steps):
             if self.length[row] >= 0:
                 self.length[row] += n
                 self.position[row] += n
@@ -391,8 +438,9 @@ def run(batch: int = 32, prompt_len: int = 512, new_tokens: int = 64, group_size
             r = dec.verify(guess, torch.rand((batch, drafts), device=dev, generator=g),
                            torch.rand(batch, device=dev, generator=g))
             for h, d, n, t in zip(history, guess.tolist(), r.accepted.tolist(), r.token.tolist()):
-                h += d[:n] + [t]
-                made += n + 1
+                if t >= 0:
+                    h += d[:n] + [t]
+                    made += n + 1
         s = time.perf_counter() - t0
         return {**result, "decode_ms_per_step": s / new_tokens * 1e3, "decode_tokens_per_s": made / s,
                 "accepted_per_step": made / (new_tokens * batch) - 1}

@@ -6,7 +6,7 @@ import torch
 import _paged8_ref as R
 import int4_hip.serving as serving
 from int4_hip.llama import LlamaConfig
-from int4_hip.paged8 import paged_attention8 as int4_attention
+from int4_hip.paged8 import paged_append8, paged_attention8 as int4_attention, paged_read8
 from int4_hip.scoring import verify_drafts as int4_verify
 from int4_hip.serving import BatchDecoder, looked_up, run
 from test_gpu_serving import CFG, DEV, _decoder, _model, _prompt
@@ -193,6 +193,74 @@ def test_drafts_that_cannot_be_verified_leave_everything():
             dec.verify(**{**ok, **bad})
         for a, b in zip(was, _state(dec)):
             assert torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b
+
+
+@pytest.mark.parametrize("kind", CODES)
+def test_refused_drafts_leave_no_trace(kind, monkeypatch):
+    """Drafts whose keys and values are far larger than those of the tokens before them, or infinite: once they are
+    refused, the cache is what the accepted tokens alone make of it, bit for bit."""
+    m = _model()
+    dec = _decoder(m, cache=kind, block=8)
+    for row, n in enumerate((5, 40, 17)):
+        dec.add(row, _prompt(n, n))
+    dec.ids[3] = 1
+    was, K, made = _state(dec), 4, []
+
+    def loud(q, k, v, *a, **kw):
+        made.append((k.clone(), v.clone()))
+        k, v = k.clone(), v.clone()
+        for x in (k, v):
+            x.view(4, 5, -1)[:, 1:] *= 512.0
+        v.view(4, 5, -1)[2, 3] = float("inf")
+        return int4_attention(q, k, v, *a, **kw)
+
+    monkeypatch.setattr(serving, "paged_attention8", loud)
+    one = torch.ones((4, K), device=DEV)  # 1 * 1 is not below any probability: refused
+    r = dec.verify(torch.full((4, K), 11, device=DEV), one, one[:, 0] / 2)
+    assert r.accepted.tolist()[:2] == [0, 0] and (r.token[:2] >= 0).all() and r.token[2] == -1
+    # what is no number has no next token, and the row is as it was
+    assert dec.length == [6, 41, 17, -1] == dec.lengths.tolist() and dec.position[:3] == [6, 41, 17]
+    assert dec.ids[:2].tolist() == r.token[:2].tolist() and dec.ids[2] == was[6][2]
+    lengths = torch.tensor([5, 40, -1, -1], dtype=torch.int32, device=DEV)
+    starts = torch.zeros(4, dtype=torch.int32, device=DEV)
+    offsets = torch.tensor([0, 6, 47, 64, 64], dtype=torch.int32, device=DEV)
+    for i, (k, v) in enumerate(made):
+        old = [was[0][i].view(kind), was[1][i].view(kind), was[2][0, i], was[2][1, i]]
+        one = [x[::5].contiguous() for x in (k, v)]
+        paged_append8(*one, dec.cos, dec.sin, *old, dec.table, lengths, dec.each, was[5])
+        new = [dec.k[i], dec.v[i], dec.scales[0, i], dec.scales[1, i]]
+        for a, b in zip(paged_read8(*old, dec.table, starts, offsets, 64, torch.float32),
+                        paged_read8(*new, dec.table, starts, offsets, 64, torch.float32)):
+            assert a.isfinite().all() and torch.equal(a, b), i
+    monkeypatch.setattr(serving, "paged_attention8", int4_attention)
+    assert dec.step().alternatives.top_logprob[:3].isfinite().all()
+
+
+def test_accepted_drafts_beside_refused_ones(monkeypatch):
+    """Rows that keep none, some and all of their drafts: each slot's values are within its own codes' steps of the
+    keys and values that came, whatever was refused behind it."""
+    m = _model()
+    dec = _decoder(m, cache=torch.int8, block=16, rows=4)
+    for row, n in enumerate((3, 14, 29, 7)):
+        dec.add(row, _prompt(n, n))
+    lengths, made = list(dec.length), []
+
+    def seen(q, k, v, *a, **kw):
+        made.append(v.clone())
+        return int4_attention(q, k, v, *a, **kw)
+
+    monkeypatch.setattr(serving, "paged_attention8", seen)
+    keep = torch.tensor([[0., 0, 0], [0, 1, 1], [0, 0, 1], [1, 1, 1]], device=DEV)
+    r = dec.verify(torch.full((4, 3), 11, device=DEV), keep, torch.full((4,), 0.5, device=DEV))
+    assert r.accepted.tolist() == [3, 1, 2, 0]
+    assert dec.length == [n + a + 1 for n, a in zip(lengths, (3, 1, 2, 0))]
+    at = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    offsets = torch.tensor([0, 4, 6, 9, 10], dtype=torch.int32, device=DEV)
+    take = torch.tensor([0, 1, 2, 3, 4, 5, 8, 9, 10, 12], device=DEV)
+    for i, v in enumerate(made):
+        got = paged_read8(dec.k[i], dec.v[i], dec.scales[0, i], dec.scales[1, i], dec.table, at, offsets, 10, torch.float32)[1]
+        # half a step of the largest code's block (its scale may be twice what its values need)
+        assert (got - v[take].float()).abs().max() <= dec.scales[1, i].max() * 0.5001
 
 
 def test_looked_up():
