@@ -1626,6 +1626,24 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   const w4::Paged8View view = view_of(cache);
   const int most_new = (int)(longest && longest < tokens ? longest : tokens);
   const bool put = most_new == 1 && num_heads / cache->kv_heads <= 16 && cache->block <= w4::kP8Unit;
+  // Calls of so many columns fill the chip with tiles of 64 of them and all their slots.  (Times of both ways, us, tiles
+  // of 64 first, 32 heads of 64 on 8: 600 tokens 30 and 23, after 4000 slots 122 and 88; 900 37 and 35, after 1500 68 and
+  // 71; 1200 43 and 42, after 1500 81 and 89; 2000 64 and 80, after 6000 308 and 380; four rows of 450 34 and 40.)  Rows of
+  // fewer than 150 tokens of 64 heads are cut among them all the same.
+  constexpr int64_t kAllColumns = 36864, kManyColumns = 9600;
+  const int64_t many = (kManyColumns + num_heads - 1) / num_heads;
+  // (Not where the attention writes: a single token of 9600 heads and more is a prompt by its columns, and nobody's to write.)
+  const bool prompts = !put && tokens * num_heads >= kAllColumns && most_new >= many;
+  const int64_t wide = tokens / many;  // such rows, at most
+  // (and the others' tokens)
+  const int64_t rest = prompts ? std::min(tokens, cache->rows * (many - 1)) : tokens;
+  const int64_t items = attend8_plan(cache->rows, rest, num_heads, cache->kv_heads, cache->head_dim).items;
+  const int64_t prompt_items =
+      cache->kv_heads * ((tokens * (num_heads / cache->kv_heads) + (w4::kPromptCols - 1) * wide) / w4::kPromptCols);
+  if (std::max(items, prompts ? prompt_items : 0) > 0xFFFFFFFFll / 256)  // HIP refuses launches of 2^32 threads and more
+    return fail(W4_ERR_UNSUPPORTED, "w4_paged8_attention: %lld tokens of %lld heads", (long long)tokens,
+                (long long)num_heads);
+  static_assert(64 * w4::kP8Waves == 256, "threads of a workgroup");
   if (!put) {
     const w4::Append8Args p{view, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_k, stride_v,
                             angles, lengths, offsets, positions, cos, sin, (int)tokens, most_new, 0};
@@ -1658,20 +1676,8 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   a.g = (int)(num_heads / cache->kv_heads);
   a.window = window >= most ? 0 : (int)window;
   a.sinks = (int)std::min(sinks, most);
-  // Calls of so many columns fill the chip with tiles of 64 of them and all their slots.  (Times of both ways, us, tiles
-  // of 64 first, 32 heads of 64 on 8: 600 tokens 30 and 23, after 4000 slots 122 and 88; 900 37 and 35, after 1500 68 and
-  // 71; 1200 43 and 42, after 1500 81 and 89; 2000 64 and 80, after 6000 308 and 380; four rows of 450 34 and 40.)  Rows of
-  // fewer than 150 tokens of 64 heads are cut among them all the same.
-  constexpr int64_t kAllColumns = 36864, kManyColumns = 9600;
-  const int64_t many = (kManyColumns + num_heads - 1) / num_heads;
-  // (Not where the attention writes: a single token of 9600 heads and more is a prompt by its columns, and nobody's to write.)
-  const bool prompts = !put && tokens * num_heads >= kAllColumns && most_new >= many;
   a.many = prompts ? (int)many : INT32_MAX;
-  const int64_t wide = tokens / many;  // such rows, at most
-  // (and the others' tokens)
-  const int64_t rest = prompts ? std::min(tokens, cache->rows * (many - 1)) : tokens;
-  const dim3 grid((unsigned)attend8_plan(cache->rows, rest, num_heads, cache->kv_heads, cache->head_dim).items);
-  const dim3 prompt((unsigned)(a.c.nkv * ((tokens * a.g + (w4::kPromptCols - 1) * wide) / w4::kPromptCols)));
+  const dim3 grid((unsigned)items), prompt((unsigned)prompt_items);
   return by_dtype(dtype, [&](auto dt) {
     return by_code(cache->code, [&](auto ct) {
       return by_head(cache->head_dim, [&](auto d) {

@@ -87,6 +87,15 @@ def test_c_abi_rejects_bad_arguments(lib):
         assert lib.w4_paged8_attention_workspace_bytes(*bad) == 0
 
 
+def test_calls_of_more_threads_than_a_launch_has_are_refused(lib):
+    """2^24 workgroups of 256: known before anything is written."""
+    big = dict(kv_heads=4096, rows=4096, page_size=8, block=8)
+    for longest in (0, 1):
+        assert _attention(lib, _cache(**big), tokens=4096, heads=4096, longest=longest, stride=4096 * 64,
+                          stride_q=4096 * 64) == _lib.ERR_UNSUPPORTED, longest
+        assert b"4096 tokens" in lib.w4_last_error()
+
+
 def _verify(lib, target=FAKE, draft=FAKE, dtype=2, rows=2, drafts=3, vocab=100, strides=(400, 100, 300, 100), tokens=FAKE,
             accept=FAKE, sample=FAKE, ws=(FAKE, 1 << 30)):
     return lib.w4_verify_drafts(target, draft, dtype, rows, drafts, vocab, *strides, tokens, FAKE, accept, sample, FAKE,
