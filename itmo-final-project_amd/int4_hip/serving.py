@@ -213,15 +213,16 @@ class BatchDecoder:
             raise ValueError(f"{T} tokens are more than the {len(self.cos)} positions")
         self._reserve(row, T)
         nh, nkv, d = self.heads
-        kc = torch.empty((nkv, d, T), device=dev)
-        vc = torch.empty((nkv, T, d), device=dev)
-        cos, sin = self.cos[:T], self.sin[:T]
         slots = torch.arange(T, dtype=torch.int32, device=dev)
-        rows = torch.full_like(slots, row)
         own = self.table[row:row + 1, :len(self.owned[row])]
         if self.scales is not None:
             one = torch.tensor([0, T], dtype=torch.int32, device=dev)
             attend8 = self._attend8(own.contiguous(), one[:1], one, slots, T)
+        else:
+            kc = torch.empty((nkv, d, T), device=dev)
+            vc = torch.empty((nkv, T, d), device=dev)
+            cos, sin = self.cos[:T], self.sin[:T]
+            rows = torch.full_like(slots, row)
 
         def attend(i, q, k, v):
             weight = None if self.weight is None else self.weight[i]

@@ -268,6 +268,16 @@ def test_looked_up():
     assert looked_up([1, 2, 2], 2) == [2, 2] and looked_up([9, 1, 9, 4, 9], 1) == [4]
 
 
+def test_prompts_make_no_other_cache(monkeypatch):
+    """A prompt's keys and values go into the pages and nowhere else."""
+    m = _model()
+    dec = _decoder(m, cache=torch.int8, block=8)
+    shapes, empty = [], torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: (shapes.append(a), empty(*a, **kw))[1])
+    dec.add(0, _prompt(50, 1))
+    assert not [a for a in shapes if a and tuple(a[0] if isinstance(a[0], (tuple, list)) else a) in ((2, 64, 50), (2, 50, 64))]
+
+
 def test_run_command():
     cfg = LlamaConfig(vocab_size=500, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
                       num_key_value_heads=2, head_dim=64)
