@@ -424,8 +424,9 @@ typedef struct w4_paged8_cache {
  * (127, 448): a block whose first slot is written, or whose scale is 0, gets scale
  * max(a / Q rounded to fp32, 2^-126), 0 if a is 0; another keeps its scale s if a <= Q s,
  * else takes the smallest s 2^m that does, all its other codes rounded to what they are at
- * that scale (those behind the row's last token too).  A code is the nearest to value / scale, the even one of two.  A block that an
- * infinity or NaN comes into has scale NaN until its first slot is written again.
+ * that scale (those behind the row's last token too).  A code is the nearest to value /
+ * scale, the even one of two.  A block that an infinity or NaN comes into has scale NaN until
+ * its first slot is written again.
  *
  * lengths[b] < 0, tokens of no row, a row whose slots pass the table, pages outside the
  * pool: nothing written.  A position outside the angles: a key of NaN.  A block is written
@@ -448,15 +449,18 @@ int w4_paged8_read(const w4_paged8_cache* cache, int dtype, const int32_t* start
  * Attention of the new tokens of every row: their keys and values are written as by
  * w4_paged8_append, then out [tokens, num_heads * head_dim] (dense) =
  * softmax(rope(q) K / sqrt(head_dim)) V, from the cached codes and scales, rounded once;
- * fp32 sums, queries and probabilities times scales entering them with 22 to 24 bits, to
- * 2^-38 and 2^-35 of their head's largest.  The token of slot i
- * sees slots 0..i or, with window > 0, those past i - window and the first `sinks`.
- * longest: the most new tokens that a row may have, 0 for any number; at 1 one launch does
- * it all.  Out is 0 for idle rows (lengths[b] < 0) and tokens of no row, NaN for rows with
+ * fp32 sums, queries and probabilities times scales entering them within 2^-23 of
+ * themselves, those far below their head's largest to 2^-38 and 2^-35 of that.  The token
+ * of slot i sees slots 0..i or, with window > 0, those past i - window and the first
+ * `sinks`.  longest: the most new tokens that a row may have, 0 for any number; at 1 one
+ * launch does it all where block is at most 32 and a key-value head has at most 16 query
+ * heads.  Out is 0 for idle rows (lengths[b] < 0) and tokens of no row, NaN for rows with
  * more than `longest` tokens or whose slots pass the table (nothing of them is written),
- * tokens that see a page outside the pool or have a position outside the angles, and tokens that see a block with scale NaN or a key with a code of NaN (e4m3); a
- * value's code of NaN makes its element NaN.
- * lengths is not changed.  num_heads: at most 256 for each key-value head.  workspace: as
+ * tokens that see a page outside the pool or have a position outside the angles, and
+ * tokens that see a block with scale NaN or a key with a code of NaN (e4m3); a value's code
+ * of NaN makes its element NaN.  lengths is not changed.  num_heads: at most 256 for each
+ * key-value head.  Calls that need launches of 2^24 workgroups and more (16 columns of a
+ * token and query head each, of one row and key-value head) are refused.  workspace: as
  * for w4a16_gemm, w4_paged8_attention_workspace_bytes long.  Results are bit-identical run
  * to run.
  */

@@ -239,10 +239,11 @@ __device__ __forceinline__ unsigned odd_ones(const float x[8], float inv) {
 // already let its scale grow by a power of two, if they need it: e4m3 codes then stay as they are (but for the
 // smallest), and int8 codes, each rounding at half the step of the next, are never off by more than one step in all.
 //
-// What bounds it: 7999 tokens of 8 x 128 (49 MB) take 18.9 us, 2.6 TB/s, of which two thirds go to the vector
-// instructions: the rotation in 64 bits and two quotients a code (50 us with every code in 64 bits, 31 where a thread with
-// one doubtful code took all of its own again).  32 tokens take 6.2 us, a chain of dependent loads: lengths and offsets,
-// page and position, angles and the block's scale.
+// What bounds it: 7999 tokens of 8 x 128 (37 MB in, 16.5 out) take 18.9 us.  66 MB come in: a block's heads are eight
+// workgroups, on eight XCDs, each of which fetches the angles (4.1 MB) into its own L2; so 83 MB pass at 4.4 TB/s.  Two
+// thirds of a busy CU's cycles go to the vector instructions, the rotation in 64 bits and two quotients a code (50 us with
+// every code in 64 bits, 31 where a thread with one doubtful code took all of its own again).  32 tokens take 6.2 us, a
+// chain of dependent loads: lengths and offsets, page and position, angles and the block's scale.
 template <int DT, int CT, int D, int ITS>
 __global__ __launch_bounds__(kP8Threads, ITS > 1 ? 3 : 5) void paged8_append_kernel(Append8Args a) {
   constexpr int CH = D / 16;  // threads per token
@@ -484,8 +485,8 @@ constexpr int kP8Waves = 4, kP8MinUnits = 4;
 // least keep the two alike.  (Without: one row of 60000 slots of 20 / 2 heads of 128 84 us, with 39, one of 131000 of 6 / 1
 // 89 and 41; 4000 of 8 / 2 of 64 10.2 and 11.0.  Of sqrt(units / 5): 46.5, 41, 10.8; sqrt(1.5 units): 40.5, 47.6, 12.3.)
 constexpr float kP8Join = 0.5f;
-// As many parts as workgroups that are at work together: four a CU have heads of 64, two those of 128.  (512 and 768:
-// 32 ragged rows of 64 26.0 and 24.8 us; 131000 slots of 128 57 and 76, drafts 24 and 28.)
+// Three parts a CU with heads of 64, two with those of 128, as measured.  (512 and 768: 32 ragged rows of 64 26.0 and 24.8
+// us; 131000 slots of 128 57 and 76, drafts 24 and 28.)
 constexpr int p8_parts(int d) { return d == 64 ? 768 : 512; }
 
 // Rows are cut into parts of about (all columns' tiles x units of slots) / PARTS, so that time follows the slots there
@@ -578,7 +579,8 @@ __device__ __forceinline__ f16x8 codes8h(uint32_t lo, uint32_t hi) {
                                            __builtin_bit_cast(uint32_t, r[2]), __builtin_bit_cast(uint32_t, r[3])});
 }
 
-// Numbers below 2^16 as the sums of two of fp16: within 2^-24 of themselves, or 2^-25 where they are below 1/2.
+// Numbers below 2^16 as the sums of two of fp16, each with 11 bits and a sign of its own: three in four exactly, the others
+// within 2^-23 of themselves (the last of 24 bits); to 2^-25 where they are so small that fp16 has no smaller step.
 __device__ __forceinline__ void halves8(const float x[8], f16x8 out[2]) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -641,9 +643,9 @@ __device__ __forceinline__ uint32_t seen8(int from, int mine, int window, int si
 // Both products are 16x16x32 fp16 matrix instructions, transposed, with the columns (new tokens x query heads of the
 // group) as their columns: S^T = K Q^T, then O^T = V^T P^T.  Codes are fp16 numbers exactly; the scales stay outside: a
 // slot's score is multiplied by its key's, its probability by its value's, which makes its weight.  Queries and weights
-// enter as the sum of two fp16 numbers, so within 2^-24 of themselves, about fp32's error, as long as they are not far
-// below the largest of their column: a power of two takes a column's queries below 2^15 and its weights below 2^15, and
-// the smallest step of fp16 is then 2^-38 of the largest query and 2^-35 (2^-40 at best) of the largest weight.  The
+// enter as the sum of two fp16 numbers, so within 2^-23 of themselves, twice fp32's own rounding at most, as long as they
+// are not far below the largest of their column: a power of two takes a column's queries and weights below 2^15, and what
+// is far below is then off by 2^-38 of the largest query at most, by 2^-35 (2^-40 at best) of the largest weight.  The
 // weights' power follows the largest so far: it changes with the softmax's reference, and when a weight passes 2^15.
 // (Three bf16 numbers each hold any size and cost half as many matrix instructions again and twice the other ones: 32
 // rows of up to 4000 slots 29.3 us instead of 26.8, 131000 slots 63 instead of 58, a window 25 instead of 21.)
@@ -655,8 +657,8 @@ __device__ __forceinline__ uint32_t seen8(int from, int mine, int window, int si
 //
 // PUT: no row has more than one new token, a row's and head's columns are one tile, and a block lies in one unit: the
 // wave that takes a row's last unit writes the token (and, where the block's scale grows, its other codes), as
-// paged8_append_kernel does.  That saves a launch: 100 slots 9.2 us a call instead of 11.8, 32 rows of up to 4000 32
-// instead of 38, one of 131000 57.6 instead of 59.8.
+// paged8_append_kernel does.  That saves a launch: 100 slots 9.0 us a call instead of 12.4, 32 rows of up to 4000 24.7
+// instead of 28.3, one of 131000 56.8 instead of 58.9.
 //
 // What bounds it: one row of 131000 slots of 8 x 128 (268 MB) takes 56 us, 4.8 TB/s, HBM.  32 rows of up to 4000 slots of
 // 8 x 64 (62 MB) take 24.2 us, 24 windows of 128-wide heads (49 MB) 20.4: of either, the vector instructions (conversion of
@@ -1626,10 +1628,17 @@ extern "C" int w4_paged8_attention(const w4_paged8_cache* cache, int dtype, cons
   const w4::Paged8View view = view_of(cache);
   const int most_new = (int)(longest && longest < tokens ? longest : tokens);
   const bool put = most_new == 1 && num_heads / cache->kv_heads <= 16 && cache->block <= w4::kP8Unit;
-  // Calls of so many columns fill the chip with tiles of 64 of them and all their slots.  (Times of both ways, us, tiles
-  // of 64 first, 32 heads of 64 on 8: 600 tokens 30 and 23, after 4000 slots 122 and 88; 900 37 and 35, after 1500 68 and
-  // 71; 1200 43 and 42, after 1500 81 and 89; 2000 64 and 80, after 6000 308 and 380; four rows of 450 34 and 40.)  Rows of
-  // fewer than 150 tokens of 64 heads are cut among them all the same.
+  // Calls of so many columns fill the chip with tiles of 64 of them and all their slots.  Times of both ways, us, tiles of
+  // 64 first, of one row of new tokens on an empty cache / after 2000 slots / after 8000:
+  //   columns  32 / 8 x 64                32 / 8 x 128               24 / 1 x 64                20 / 2 x 128
+  //   19200    31 25 / 77 63 / 231 169    36 32 / 103 85 / 321 243   33 26 / 75 60 / 224 158    45 39 / 109 91 / 327 252
+  //   36864    43 40 / 99 97 / 285 269    55 60 / 173 156 / 533 487  51 48 / 99 103 / 288 279   76 83 / 199 190 / 557 536
+  //   64000    65 83 / 145 178 / 386 482  106 135 / 249 321 / 676 932  80 100 / 155 196 / 399 492
+  //   and of 20 / 2 x 128 146 193 / 295 391 / 712 993.
+  // Four rows of 150 tokens of 64 heads after 100000 slots: 3191 and 3795 (heads of 64), 7270 and 8221 (of 128).  Rows of
+  // fewer than 150 tokens of 64 heads are cut among them all the same.  One long row whose tokens are few and that passes
+  // by the others' columns is slower for it: 150 tokens of 64 heads after 100000 slots beside 460 single ones 2242 and
+  // 1137, after 2000 131 and 106; the lengths are on the GPU, so the rule cannot know.
   constexpr int64_t kAllColumns = 36864, kManyColumns = 9600;
   const int64_t many = (kManyColumns + num_heads - 1) / num_heads;
   // (Not where the attention writes: a single token of 9600 heads and more is a prompt by its columns, and nobody's to write.)

@@ -1,7 +1,8 @@
 """Key-value cache in pages held in 8 bits, for batches of sequences: tokens quantised as
 they are written, read back, and the attention of a few new tokens of every row over
-them (csrc/w4_paged8.hip).  It holds about twice the tokens of ``paged.py``'s cache and is
-read in about half the time.
+them (csrc/w4_paged8.hip).  It holds about twice the tokens of ``paged.py``'s cache; a decode
+step's attention takes 0.6 to 0.75 of the time (56 us instead of 88 over 131000 slots of 8
+heads of 128, 23 instead of 32 over 32 ragged rows of up to 4000 of 8 heads of 64).
 
 One layer's cache, shared by all sequences of a batch (``rows``):
 
@@ -133,8 +134,9 @@ def paged_attention8(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, tabl
     projections before the rotary embedding, bf16 or fp16.  Keys and values are written as
     by ``paged_append8``; then the token of slot i attends in fp32 to slots 0..i or, with
     ``window``, to the last ``window`` of them and the first ``sinks``.  ``longest`` is
-    the most new tokens that a row may have, where the program knows it: of a decode step, 1,
-    for which one launch writes and attends.  ``lengths`` is left as it is (all layers of a
+    the most new tokens that a row may have, where the program knows it (None or 0: any
+    number): of a decode step, 1, for which one launch writes and attends where blocks have
+    at most 32 slots and a key head at most 16 query heads.  ``lengths`` is left as it is (all layers of a
     model share it).
 
     Idle rows and tokens of no row come back 0.  NaN come back: rows with more
