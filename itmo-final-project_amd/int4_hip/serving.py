@@ -340,9 +340,13 @@ class BatchDecoder:
         attend = self._attend8(self.table, self.lengths, starts, positions, K + 1, new)
         # (a draft outside the vocabulary is refused; until then it is some token of it)
         embed = self.model.model.embed_tokens
-        logits = self._run(embed(tokens.flatten().clamp(0, embed.num_embeddings - 1)), attend)
-        target = torch.softmax(logits.float() / temperature, -1).view(self.rows, K + 1, -1)
-        r = verify_drafts(target, draft, drafts, accept, sample)
+        try:
+            logits = self._run(embed(tokens.flatten().clamp(0, embed.num_embeddings - 1)), attend)
+            target = torch.softmax(logits.float() / temperature, -1).view(self.rows, K + 1, -1)
+            r = verify_drafts(target, draft, drafts, accept, sample)
+        except BaseException:  # (of memory, for one)
+            put_back()
+            raise
         good = (self.lengths >= 0) & (r.token >= 0)
         step = torch.where(good, r.accepted + 1, 0).to(torch.int32)
         steps = step.tolist()

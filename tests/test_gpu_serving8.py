@@ -236,6 +236,35 @@ def test_refused_drafts_leave_no_trace(kind, monkeypatch):
     assert dec.step().alternatives.top_logprob[:3].isfinite().all()
 
 
+def test_a_verification_that_fails_leaves_the_tokens_as_they_were(monkeypatch):
+    """An error behind the model (memory for the probabilities, for one), when the drafts are in the cache already."""
+    m = _model()
+    dec = _decoder(m, cache=torch.int8, block=8)
+    for row, n in enumerate((5, 40, 17)):
+        dec.add(row, _prompt(n, n))
+    starts = torch.zeros(4, dtype=torch.int32, device=DEV)
+    offsets = torch.tensor([0, 5, 45, 62, 62], dtype=torch.int32, device=DEV)
+
+    def held():
+        return [x for i in range(3) for x in paged_read8(dec.k[i], dec.v[i], dec.scales[0, i], dec.scales[1, i], dec.table,
+                                                         starts, offsets, 62, torch.float32)]
+
+    def loud(q, k, v, *a, **kw):
+        return int4_attention(q, k * 512, v * 512, *a, **kw)
+
+    def fails(*a):
+        raise torch.OutOfMemoryError("none left")
+
+    was = held(), dec.lengths.clone(), dec.ids.clone(), list(dec.length)
+    monkeypatch.setattr(serving, "paged_attention8", loud)
+    monkeypatch.setattr(serving, "verify_drafts", fails)
+    x = torch.zeros((4, 2), dtype=torch.int64, device=DEV)
+    with pytest.raises(torch.OutOfMemoryError):
+        dec.verify(x, x.float(), x[:, 0].float())
+    assert all(torch.equal(a, b) for a, b in zip(was[0], held()))
+    assert torch.equal(was[1], dec.lengths) and torch.equal(was[2], dec.ids) and was[3] == dec.length
+
+
 def test_accepted_drafts_beside_refused_ones(monkeypatch):
     """Rows that keep none, some and all of their drafts: each slot's values are within its own codes' steps of the
     keys and values that came, whatever was refused behind it."""
